@@ -258,6 +258,95 @@ int rqmv_attention_rope(const float* qkv, const float* rope_table, void* k_cache
                         int q_heads, int kv_heads, int head_dim, int max_ctx, void* workspace, size_t workspace_bytes,
                         float* out, void* stream);
 
+/* Paged serving: one step of several sequences over caches cut into pages.
+ * They stand beside the decode-step helpers above (one sequence, one
+ * contiguous cache): rqmv_paged_plan makes the step's tables from the
+ * requests' lengths, rqmv_qk_norm_rope puts the projected queries and keys
+ * through their norms and the rotation and stores keys and values,
+ * rqmv_paged_attention attends, rqmv_sample picks the next tokens. No
+ * counterpart in the reference, which runs one sequence's positions
+ * (recipe.rs:21314-21470). All pointers inside the structs are device
+ * pointers, read when the work runs, so a captured step replays with the
+ * lengths it then finds; every launch is sized by the structs' counts alone.
+ *
+ * rqmv_paged_cache: one layer's keys and values, fp16, each
+ * [blocks][kv_heads][block_size][head_dim], 16-byte aligned; block_size is 16,
+ * 32, 64, 128 or 256, head_dim 64, 128 or 256, and blocks * block_size stays
+ * below 2^31. Slot b * block_size + i is row i of block b (in every kv head).
+ *
+ * rqmv_paged_batch: `seqs` sequences (1..8192) with at most `tokens` (1..2^20)
+ * new tokens among them. The new tokens of sequence s are rows q_start[s] ..
+ * q_start[s + 1] - 1 (q_start holds seqs + 1 entries, never decreasing, from
+ * 0; rows from q_start[seqs] on belong to no sequence and are padding), the
+ * last of its kv_len[s] positions. Its position p lies in block
+ * block_table[s * table_stride + p / block_size] at row p % block_size, for p
+ * < max_blocks * block_size; a table entry outside 0..blocks-1 is an absent
+ * page, whose positions are never attended to. positions and slots hold each
+ * row's position and slot (-1: none). Each call names the fields it reads;
+ * the others may be NULL. */
+typedef struct {
+    void* k;
+    void* v;
+    int64_t blocks;
+    int block_size;
+    int kv_heads;
+    int head_dim;
+} rqmv_paged_cache;
+
+typedef struct {
+    int* q_start;
+    int* kv_len;
+    int* block_table;
+    int64_t table_stride;
+    int max_blocks;
+    int seqs;
+    int tokens;
+    int* positions;
+    int* slots;
+} rqmv_paged_batch;
+
+/* What a plan's *status holds: 0, or a sum of these. */
+enum {
+    RQMV_PLAN_LENGTH = 1, /* a negative length, or more positions than max_blocks pages hold */
+    RQMV_PLAN_TOKENS = 2, /* more new tokens than the batch's `tokens` rows */
+    RQMV_PLAN_POOL = 4    /* the pool has too few free blocks, or *free_head is outside 0..free_count */
+};
+
+/* The tables of a step from the requests' lengths: sequence s has
+ * cached_len[s] positions in its pages and takes new_len[s] more (either may be
+ * 0). Blocks that it needs beyond ceil(cached_len / block_size) come from the
+ * pool, free_list[*free_head ..], in the order of the sequences, and are written
+ * into its row of block_table; *free_head_out is *free_head plus the blocks
+ * taken. Writes q_start, kv_len (cached + new), the new table entries, and
+ * positions and slots of all `tokens` rows (padding rows: position 0, slot -1;
+ * a row whose block id is outside the cache: slot -1). Of the cache it reads
+ * blocks and block_size alone. All or nothing: unless *status becomes 0, q_start
+ * is all 0, kv_len is cached_len, every row is padding, and the table and the
+ * pool stay as they were. kv_len may be cached_len itself, and free_head_out
+ * free_head (a captured step that continues); other buffers must not overlap.
+ * One launch, two above 2048 rows. */
+int rqmv_paged_plan(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, const int* cached_len,
+                    const int* new_len, const int* free_list, int free_count, const int* free_head, int* free_head_out,
+                    int* status, void* stream);
+
+/* Per row (token) t of the batch's `tokens`: the q and k heads of
+ * qkv + t * ld ([q | k | v] heads of head_dim, x_dtype) are normalised, each
+ * head by itself, x / sqrt(mean(x^2) + eps) * weight, with q_norm and k_norm
+ * (fp32, head_dim values; both or neither, NULL: no norm), then rotated (NeoX
+ * pairs (i, i + rot_dim / 2) of the first rot_dim dims by row positions[t] of
+ * rope_table, a rqmv_rope_table of head_dim = rot_dim; positions outside
+ * 0..rope_rows-1 take the nearest row). The queries go to q_out + t * ldq
+ * (q_dtype), and the rotated keys and the values, rounded to fp16, to the
+ * cache at slots[t] (nothing is stored where it is outside the cache's slots;
+ * stored slots are to be distinct). rot_dim is a multiple of 8 up to head_dim;
+ * rows and pointers are 16-byte aligned (norms and table too); q_out is qkv
+ * itself (same dtype, ldq = ld) or spans none of its memory. Arithmetic is
+ * fp32. One launch. Reads tokens, positions and slots of the batch. */
+int rqmv_qk_norm_rope(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, const void* qkv, int x_dtype,
+                      int64_t ld, int q_heads, const float* q_norm, const float* k_norm, float eps,
+                      const float* rope_table, int rot_dim, int rope_rows, void* q_out, int q_dtype, int64_t ldq,
+                      void* stream);
+
 /* out[i] = silu(gate_up[i]) * gate_up[n + i]. */
 int rqmv_silu_mul(const float* gate_up, int n, float* out, void* stream);
 

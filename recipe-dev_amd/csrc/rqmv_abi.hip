@@ -1,4 +1,5 @@
 // C-ABI entry points of librqmv (declared in include/rqmv.h).
+#include <stdint.h>
 #include <stdlib.h>
 
 #include <memory>
@@ -13,6 +14,7 @@
 #include "decode.h"
 #include "gguf.h"
 #include "moe.h"
+#include "paged.h"
 #include "repack.h"
 #include "requant.h"
 
@@ -248,6 +250,59 @@ int matvec_rows(const rqmv_weight* w, int64_t first_row, int64_t rows, const voi
         done += mb;
     }
     return RQMV_OK;
+}
+
+// Checks of the paged serving structs (what a call launches is sized by these
+// counts; the arrays' contents are checked by the kernels).
+constexpr int kPagedMaxTokens = 1 << 20;
+constexpr int kPagedMaxHeads = 1024;
+constexpr int64_t kPagedMaxStride = int64_t(1) << 40;
+
+int check_paged_blocks(const rqmv_paged_cache* c, const char* what, int* shift) {
+    if (!c) return fail(RQMV_EINVAL, std::string(what) + ": cache is NULL");
+    int s = 4;
+    while (s < 8 && (1 << s) != c->block_size) ++s;
+    if ((1 << s) != c->block_size)
+        return fail(RQMV_EINVAL, std::string(what) + ": block_size must be 16, 32, 64, 128 or 256");
+    if (c->blocks <= 0 || c->blocks > (INT32_MAX >> s))
+        return fail(RQMV_EINVAL, std::string(what) + ": blocks must be positive and blocks * block_size below 2^31");
+    *shift = s;
+    return RQMV_OK;
+}
+
+int check_paged_cache(const rqmv_paged_cache* c, const char* what, rq::PagedCache* out) {
+    int shift = 0;
+    const int rc = check_paged_blocks(c, what, &shift);
+    if (rc != RQMV_OK) return rc;
+    if (!c->k || !c->v || (((uintptr_t)c->k | (uintptr_t)c->v) & 15))
+        return fail(RQMV_EINVAL, std::string(what) + ": the caches must be 16-byte aligned, not NULL");
+    if (c->kv_heads <= 0 || (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256))
+        return fail(RQMV_EINVAL, std::string(what) + ": kv_heads must be positive and head_dim 64, 128 or 256");
+    out->k = static_cast<__half*>(c->k);
+    out->v = static_cast<__half*>(c->v);
+    out->blocks = (int)c->blocks;
+    out->block_shift = shift;
+    out->kv_heads = c->kv_heads;
+    out->head_dim = c->head_dim;
+    return RQMV_OK;
+}
+
+int check_paged_batch(const rqmv_paged_batch* b, const char* what) {
+    if (!b) return fail(RQMV_EINVAL, std::string(what) + ": batch is NULL");
+    if (b->seqs < 1 || b->seqs > rq::kPagedMaxSeqs || b->tokens < 1 || b->tokens > kPagedMaxTokens)
+        return fail(RQMV_EINVAL, std::string(what) + ": seqs must be 1..8192 and tokens 1..2^20");
+    return RQMV_OK;
+}
+
+int check_paged_table(const rqmv_paged_batch* b, const char* what) {
+    if (b->max_blocks < 1 || (b->seqs > 1 && (b->table_stride < b->max_blocks || b->table_stride > kPagedMaxStride)))
+        return fail(RQMV_EINVAL, std::string(what) + ": max_blocks must be positive and at most table_stride");
+    return RQMV_OK;
+}
+
+rq::PagedBatch paged_batch(const rqmv_paged_batch* b) {
+    return rq::PagedBatch{b->q_start,    b->kv_len, b->block_table, b->table_stride, b->max_blocks,
+                          b->seqs,       b->tokens, b->positions,   b->slots};
 }
 
 }  // namespace
@@ -749,6 +804,71 @@ int rqmv_attention_rope(const float* qkv, const float* rope_table, void* k_cache
                                              kv_heads, head_dim, max_ctx, workspace, out,
                                              static_cast<hipStream_t>(stream));
     return e == hipSuccess ? RQMV_OK : hip_fail(e, "attention_rope launch");
+}
+
+// ---------------------------------------------------------- paged serving ----
+
+int rqmv_paged_plan(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, const int* cached_len,
+                    const int* new_len, const int* free_list, int free_count, const int* free_head, int* free_head_out,
+                    int* status, void* stream) {
+    int shift = 0;
+    int rc = check_paged_blocks(cache, "paged_plan", &shift);
+    if (rc == RQMV_OK) rc = check_paged_batch(batch, "paged_plan");
+    if (rc != RQMV_OK) return rc;
+    if (!batch->q_start || !batch->kv_len || !batch->block_table || !batch->positions || !batch->slots || !cached_len ||
+        !new_len || !free_head || !free_head_out || !status || free_count < 0 || (!free_list && free_count > 0))
+        return fail(RQMV_EINVAL, "paged_plan: bad arguments");
+    rc = check_paged_table(batch, "paged_plan");
+    if (rc != RQMV_OK) return rc;
+    hipError_t e = rq::launch_paged_plan(paged_batch(batch), (int)cache->blocks, shift, cached_len, new_len, free_list,
+                                         free_count, free_head, free_head_out, status, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? RQMV_OK : hip_fail(e, "paged_plan launch");
+}
+
+int rqmv_qk_norm_rope(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, const void* qkv, int x_dtype,
+                      int64_t ld, int q_heads, const float* q_norm, const float* k_norm, float eps,
+                      const float* rope_table, int rot_dim, int rope_rows, void* q_out, int q_dtype, int64_t ldq,
+                      void* stream) {
+    rq::PagedCache c;
+    int rc = check_paged_cache(cache, "qk_norm_rope", &c);
+    if (rc == RQMV_OK) rc = check_paged_batch(batch, "qk_norm_rope");
+    if (rc != RQMV_OK) return rc;
+    if (!batch->positions || !batch->slots || !qkv || !rope_table || !q_out || q_heads <= 0 || rope_rows <= 0 ||
+        !q_norm != !k_norm || (q_norm && !(eps >= 0.f)))
+        return fail(RQMV_EINVAL, "qk_norm_rope: bad arguments");
+    if ((x_dtype != RQMV_DTYPE_F16 && x_dtype != RQMV_DTYPE_F32) || (q_dtype != RQMV_DTYPE_F16 && q_dtype != RQMV_DTYPE_F32))
+        return fail(RQMV_EINVAL, "qk_norm_rope: dtypes must be F16 or F32");
+    if (q_heads > kPagedMaxHeads || c.kv_heads > kPagedMaxHeads)
+        return fail(RQMV_EINVAL, "qk_norm_rope: at most 1024 heads of a kind");
+    if (rot_dim <= 0 || rot_dim % 8 || rot_dim > c.head_dim)
+        return fail(RQMV_EINVAL, "qk_norm_rope: rot_dim must be a multiple of 8 up to head_dim");
+    const int64_t xs = x_dtype == RQMV_DTYPE_F16 ? 2 : 4, qs = q_dtype == RQMV_DTYPE_F16 ? 2 : 4;
+    const int64_t xrow = (int64_t)(q_heads + 2 * c.kv_heads) * c.head_dim, qrow = (int64_t)q_heads * c.head_dim;
+    const int64_t t1 = batch->tokens - 1;
+    if (t1 && (ld < xrow || ldq < qrow || ld > kPagedMaxStride || ldq > kPagedMaxStride || ld * xs % 16 || ldq * qs % 16))
+        return fail(RQMV_EINVAL, "qk_norm_rope: ld or ldq is too small, too large or no multiple of 16 bytes");
+    if (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)rope_table) & 15)
+        return fail(RQMV_EINVAL, "qk_norm_rope: qkv, q_out, the norms and the table must be 16-byte aligned");
+    const uintptr_t x0 = (uintptr_t)qkv, x1 = x0 + (uintptr_t)((t1 ? t1 * ld : 0) + xrow) * xs;
+    const uintptr_t q0 = (uintptr_t)q_out, q1 = q0 + (uintptr_t)((t1 ? t1 * ldq : 0) + qrow) * qs;
+    const bool same = q0 == x0 && x_dtype == q_dtype && (!t1 || ld == ldq);
+    if (!same && q0 < x1 && x0 < q1)
+        return fail(RQMV_EINVAL, "qk_norm_rope: q_out must be qkv itself or lie outside it");
+    rq::QkNormRope p;
+    p.qkv = qkv;
+    p.ld = ld;
+    p.q_heads = q_heads;
+    p.q_norm = q_norm;
+    p.k_norm = k_norm;
+    p.eps = eps;
+    p.rope = reinterpret_cast<const float2*>(rope_table);
+    p.rot_dim = rot_dim;
+    p.rope_rows = rope_rows;
+    p.q_out = q_out;
+    p.ldq = ldq;
+    hipError_t e = rq::launch_qk_norm_rope(paged_batch(batch), c, p, x_dtype == RQMV_DTYPE_F16,
+                                           q_dtype == RQMV_DTYPE_F16, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? RQMV_OK : hip_fail(e, "qk_norm_rope launch");
 }
 
 int rqmv_silu_mul(const float* gate_up, int n, float* out, void* stream) {

@@ -95,6 +95,10 @@ class _Lib:
         L.rqmv_rope_table.argtypes = [c_void_p, c_int, c_double, c_int, c_void_p]
         L.rqmv_attention_rope.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                           c_void_p, c_size_t, c_void_p, c_void_p]
+        L.rqmv_paged_plan.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                      c_void_p, c_void_p]
+        L.rqmv_qk_norm_rope.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p,
+                                        c_float, c_void_p, c_int, c_int, c_void_p, c_int, c_int64, c_void_p]
         L.rqmv_glu_weight_create.argtypes = [c_int, c_int64, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]
         L.rqmv_matvec_fused.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
         L.rqmv_layout_bytes.argtypes = [c_int, c_int64, c_int64, POINTER(c_size_t)]
@@ -652,6 +656,84 @@ def advance(pos: DeviceBuffer, stream: Stream | None = None):
 def embed_row(table: DeviceBuffer, rows: int, n: int, token: DeviceBuffer, out: DeviceBuffer,
               stream: Stream | None = None):
     _check(lib().lib.rqmv_embed_row(table.ptr, rows, n, token.ptr, out.ptr, _sh(stream)), "rqmv_embed_row")
+
+
+# -------------------------------------------------------- paged serving ----
+# One step of several sequences over caches cut into pages: the step's tables,
+# the queries and keys, attention, the next tokens.
+
+PLAN_LENGTH, PLAN_TOKENS, PLAN_POOL = 1, 2, 4  # what a plan's status holds
+
+
+def _p(buf):
+    return buf.ptr if buf is not None else None
+
+
+class _CacheStruct(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("blocks", c_int64), ("block_size", c_int), ("kv_heads", c_int),
+                ("head_dim", c_int)]
+
+
+class _BatchStruct(ctypes.Structure):
+    _fields_ = [("q_start", c_void_p), ("kv_len", c_void_p), ("block_table", c_void_p), ("table_stride", c_int64),
+                ("max_blocks", c_int), ("seqs", c_int), ("tokens", c_int), ("positions", c_void_p),
+                ("slots", c_void_p)]
+
+
+class PagedCache:
+    """One layer's keys and values in pages (rqmv_paged_cache): k and v are fp16
+    [blocks, kv_heads, block_size, head_dim] on the device."""
+
+    def __init__(self, k, v, blocks: int, block_size: int, kv_heads: int, head_dim: int):
+        self.k, self.v = k, v
+        self.blocks, self.block_size, self.kv_heads, self.head_dim = blocks, block_size, kv_heads, head_dim
+        self.struct = _CacheStruct(_p(k), _p(v), blocks, block_size, kv_heads, head_dim)
+
+    @classmethod
+    def allocate(cls, blocks: int, block_size: int, kv_heads: int, head_dim: int) -> "PagedCache":
+        nbytes = 2 * blocks * block_size * kv_heads * head_dim
+        return cls(DeviceBuffer(nbytes), DeviceBuffer(nbytes), blocks, block_size, kv_heads, head_dim)
+
+
+class PagedBatch:
+    """The tables of one step (rqmv_paged_batch): `seqs` sequences with at most
+    `tokens` new tokens. Buffers are int32 on the device; those that a call does
+    not read may be None. table_stride (default max_blocks) is in entries."""
+
+    def __init__(self, seqs: int, tokens: int, max_blocks: int, q_start=None, kv_len=None, block_table=None,
+                 positions=None, slots=None, table_stride: int | None = None):
+        self.seqs, self.tokens, self.max_blocks = seqs, tokens, max_blocks
+        self.q_start, self.kv_len, self.block_table = q_start, kv_len, block_table
+        self.positions, self.slots = positions, slots
+        self.struct = _BatchStruct(_p(q_start), _p(kv_len), _p(block_table), table_stride or max_blocks, max_blocks,
+                                   seqs, tokens, _p(positions), _p(slots))
+
+    @classmethod
+    def allocate(cls, seqs: int, tokens: int, max_blocks: int) -> "PagedBatch":
+        """A batch with buffers of its own for rqmv_paged_plan to fill; the table starts without pages."""
+        table = DeviceBuffer.from_array(np.full(seqs * max_blocks, -1, np.int32))
+        return cls(seqs, tokens, max_blocks, DeviceBuffer(4 * seqs + 4), DeviceBuffer(4 * seqs), table,
+                   DeviceBuffer(4 * tokens), DeviceBuffer(4 * tokens))
+
+
+def paged_plan(batch: PagedBatch, cache: PagedCache, cached_len, new_len, free_list, free_count: int, free_head,
+               free_head_out, status, stream: Stream | None = None):
+    """Block tables, starts, positions and slots from the requests' lengths
+    (rqmv_paged_plan); `status` (int32 on the device) says whether the step fits."""
+    _check(lib().lib.rqmv_paged_plan(byref(batch.struct), byref(cache.struct), cached_len.ptr, new_len.ptr,
+                                     _p(free_list), free_count, free_head.ptr, free_head_out.ptr, status.ptr,
+                                     _sh(stream)), "rqmv_paged_plan")
+
+
+def qk_norm_rope(batch: PagedBatch, cache: PagedCache, qkv, x_dtype: int, ld: int, q_heads: int, table, rope_rows: int,
+                 q_out, q_dtype: int, ldq: int, q_norm=None, k_norm=None, eps: float = 1e-6,
+                 rot_dim: int | None = None, stream: Stream | None = None):
+    """Per-head norms and rotation of queries and keys, the append to the paged
+    cache (rqmv_qk_norm_rope); rot_dim defaults to the whole head."""
+    _check(lib().lib.rqmv_qk_norm_rope(byref(batch.struct), byref(cache.struct), qkv.ptr, x_dtype, ld, q_heads,
+                                       _p(q_norm), _p(k_norm), eps, table.ptr,
+                                       cache.head_dim if rot_dim is None else rot_dim, rope_rows, q_out.ptr, q_dtype,
+                                       ldq, _sh(stream)), "rqmv_qk_norm_rope")
 
 
 # ------------------------------------------------------- fused products ----

@@ -1,0 +1,103 @@
+"""What the paged serving entry points refuse, before anything is launched (no
+GPU needed: every call here returns RQMV_EINVAL from its checks)."""
+import numpy as np
+import pytest
+
+import rqmv
+
+
+class At:
+    """Stands for a device address; nothing is read through it."""
+
+    def __init__(self, ptr=1 << 20, nbytes=1 << 30):
+        self.ptr, self.nbytes = ptr, nbytes
+
+
+A = At()
+
+
+def batch(seqs=2, tokens=4, max_blocks=3, stride=None, **none):
+    names = ("q_start", "kv_len", "block_table", "positions", "slots")
+    return rqmv.PagedBatch(seqs, tokens, max_blocks, table_stride=stride,
+                           **{n: none.get(n, A) for n in names})
+
+
+def cache(blocks=10, block=16, kv=2, hd=64, k=A, v=A):
+    return rqmv.PagedCache(k, v, blocks, block, kv, hd)
+
+
+BAD_CACHES = [dict(block=8), dict(block=48), dict(block=512), dict(block=0), dict(blocks=0), dict(blocks=-1),
+              dict(blocks=1 << 27)]
+BAD_BATCHES = [dict(seqs=0), dict(seqs=8193), dict(tokens=0), dict(tokens=(1 << 20) + 1)]
+BAD_TABLES = [dict(max_blocks=0), dict(max_blocks=5, stride=4), dict(stride=1 << 41)]
+
+
+def refused(call, *args, **kw):
+    with pytest.raises(rqmv.RqmvError, match=r"\(-1\)"):
+        call(*args, **kw)
+
+
+def plan(b=None, c=None, **kw):
+    a = dict(cached_len=A, new_len=A, free_list=A, free_count=3, free_head=A, free_head_out=A, status=A)
+    a.update(kw)
+    rqmv.paged_plan(b or batch(), c or cache(), **a)
+
+
+@pytest.mark.parametrize("kw", BAD_CACHES)
+def test_plan_refuses_caches(kw):
+    refused(plan, c=cache(**kw))
+
+
+@pytest.mark.parametrize("kw", BAD_BATCHES + BAD_TABLES)
+def test_plan_refuses_batches(kw):
+    refused(plan, b=batch(**kw))
+
+
+@pytest.mark.parametrize("name", ["q_start", "kv_len", "block_table", "positions", "slots"])
+def test_plan_refuses_missing_tables(name):
+    refused(plan, b=batch(**{name: None}))
+
+
+@pytest.mark.parametrize("kw", [dict(cached_len=At(None)), dict(new_len=At(None)), dict(free_head=At(None)),
+                                dict(free_head_out=At(None)), dict(status=At(None)), dict(free_list=None),
+                                dict(free_count=-1)])
+def test_plan_refuses_arguments(kw):
+    refused(plan, **kw)
+
+
+def qk(b=None, c=None, **kw):
+    a = dict(qkv=At(1 << 24), x_dtype=0, ld=512, q_heads=4, table=A, rope_rows=8, q_out=At(1 << 30), q_dtype=0, ldq=256)
+    a.update(kw)
+    rqmv.qk_norm_rope(b or batch(), c or cache(), **a)
+
+
+@pytest.mark.parametrize("kw", BAD_CACHES + [dict(kv=0), dict(kv=1025), dict(hd=32), dict(hd=96), dict(k=None),
+                                             dict(v=None), dict(k=At(8)), dict(v=At(24))])
+def test_qk_norm_rope_refuses_caches(kw):
+    refused(qk, c=cache(**kw))
+
+
+@pytest.mark.parametrize("kw", BAD_BATCHES + [dict(positions=None), dict(slots=None)])
+def test_qk_norm_rope_refuses_batches(kw):
+    refused(qk, b=batch(**kw))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(x_dtype=2), dict(q_dtype=-1), dict(ld=508), dict(ld=514), dict(ldq=252), dict(ldq=258), dict(ld=1 << 41),
+    dict(x_dtype=1, ld=516), dict(q_heads=0), dict(q_heads=1025), dict(rope_rows=0), dict(rot_dim=0), dict(rot_dim=12),
+    dict(rot_dim=72), dict(q_norm=A), dict(k_norm=A), dict(q_norm=A, k_norm=At(8)), dict(q_norm=A, k_norm=A, eps=-1.0),
+    dict(q_norm=A, k_norm=A, eps=float("nan")), dict(table=At(4)), dict(qkv=At(20)), dict(q_out=At(40)),
+    dict(qkv=At(None)), dict(q_out=At(None)), dict(table=At(None)),
+    # q_out inside qkv's span, or qkv itself with another type or stride
+    dict(q_out=At((1 << 24) + 1024)), dict(q_out=At(1 << 24), q_dtype=1), dict(q_out=At(1 << 24))])
+def test_qk_norm_rope_refuses_arguments(kw):
+    refused(qk, **kw)
+
+
+def test_the_last_error_names_the_call():
+    with pytest.raises(rqmv.RqmvError, match="paged_plan: block_size must be"):
+        plan(c=cache(block=24))
+    with pytest.raises(rqmv.RqmvError, match="qk_norm_rope: batch is NULL"):
+        rqmv._check(rqmv.lib().lib.rqmv_qk_norm_rope(None, rqmv.byref(cache().struct), *([None, 0, 0, 0, None, None, 0.0,
+                                                     None, 0, 0, None, 0, 0, None])), "rqmv_qk_norm_rope")
+    assert np.int32(rqmv.PLAN_LENGTH | rqmv.PLAN_TOKENS | rqmv.PLAN_POOL) == 7
