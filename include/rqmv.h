@@ -347,6 +347,30 @@ int rqmv_qk_norm_rope(const rqmv_paged_batch* batch, const rqmv_paged_cache* cac
                       const float* rope_table, int rot_dim, int rope_rows, void* q_out, int q_dtype, int64_t ldq,
                       void* stream);
 
+/* Grouped-query attention of the batch's new tokens over their pages: for each
+ * query head of the row at position p (rows of q and out: q + row * ldq, out +
+ * row * ldo elements, q_heads heads of head_dim) softmax(scale q k) v over the
+ * positions max(0, p - window + 1)..p of its sequence (window 0: 0..p) whose
+ * pages are present, in kv head h / (q_heads / kv_heads); zeros where there is
+ * none. The new tokens' own keys and values are in the cache
+ * already (rqmv_qk_norm_rope). out has the dtype of q: fp32 rows are computed to fp32
+ * accuracy, fp16 rows with the softmax weights rounded to fp16; sums and
+ * statistics are fp32 in both. A position that is not attended to never touches
+ * the result, whatever its key and value hold. A NaN or an infinity in a query, or
+ * in a key or value attended to, makes its rows non-finite. Rows of no sequence are
+ * not written. q_heads is a multiple of kv_heads, both at most 1024; scale is positive; ldq
+ * and ldo are multiples of 16 bytes, q and out 16-byte aligned, and out may be q
+ * itself only with ldo = ldq. Reads q_start, kv_len, block_table of the batch. One
+ * launch, two where the keys are split over workgroups: then the workspace (16-byte
+ * aligned, rqmv_paged_attention_workspace_size bytes for this batch's counts, cache and
+ * q_heads on the current device; 0: may be NULL) holds partial results, and calls
+ * that share it must not overlap. */
+int rqmv_paged_attention_workspace_size(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, int q_heads,
+                                        size_t* bytes);
+int rqmv_paged_attention(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, const void* q, int dtype,
+                         int64_t ldq, int q_heads, float scale, int window, void* workspace, size_t workspace_bytes,
+                         void* out, int64_t ldo, void* stream);
+
 /* out[i] = silu(gate_up[i]) * gate_up[n + i]. */
 int rqmv_silu_mul(const float* gate_up, int n, float* out, void* stream);
 

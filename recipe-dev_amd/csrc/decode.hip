@@ -14,6 +14,7 @@
 #include <type_traits>
 
 #include "decode.h"
+#include "lanes.h"
 #include "stage.h"
 
 namespace rq {
@@ -136,50 +137,12 @@ __device__ __forceinline__ float sum_lanes(float v) {
     if constexpr (LPP >= 16)
         v += __builtin_bit_cast(float,
                                 __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xf, 0xf, false));
-    if constexpr (LPP >= 32) {  // lane ^ 16 through v_permlane16_swap (see swap16 below)
+    if constexpr (LPP >= 32) {  // lane ^ 16 through v_permlane16_swap (see swap16 in lanes.h)
         float a = v, b = v;
         asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
         v = a + b;
     }
     return v;
-}
-
-// v combined with the value of lane ^ 16 and of lane ^ 32 through gfx950's
-// VALU lane swaps (no LDS crossbar): v_permlane16_swap_b32 / 32 exchange odd
-// 16-lane rows (upper 32 lanes) of the first register with even rows (lower
-// 32 lanes) of the second; applied to two copies of v they leave, in every
-// lane, the lower lane's value in the first and the upper lane's in the
-// second. Written as inline assembly: this compiler's builtin loses the second
-// result. The s_nop gives the wait states a VALU write needs before the swap
-// reads it.
-struct LanePair {
-    float lo, hi;
-};
-__device__ __forceinline__ LanePair swap16(float v) {
-    float a = v, b = v;
-    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-    return LanePair{a, b};
-}
-__device__ __forceinline__ LanePair swap32(float v) {
-    float a = v, b = v;
-    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
-    return LanePair{a, b};
-}
-__device__ __forceinline__ float swap16_sum(float v) {
-    const LanePair p = swap16(v);
-    return p.lo + p.hi;
-}
-__device__ __forceinline__ float swap32_sum(float v) {
-    const LanePair p = swap32(v);
-    return p.lo + p.hi;
-}
-__device__ __forceinline__ float swap16_max(float v) {
-    const LanePair p = swap16(v);
-    return fmaxf(p.lo, p.hi);
-}
-__device__ __forceinline__ float swap32_max(float v) {
-    const LanePair p = swap32(v);
-    return fmaxf(p.lo, p.hi);
 }
 
 // Maximum and sum over the 64 lanes of a wave, every lane getting the result:

@@ -1,0 +1,46 @@
+// Exchanges between the lanes of a wave that need no LDS.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+namespace rq {
+
+// v combined with the value of lane ^ 16 and of lane ^ 32 through gfx950's
+// VALU lane swaps (no LDS crossbar): v_permlane16_swap_b32 / 32 exchange odd
+// 16-lane rows (upper 32 lanes) of the first register with even rows (lower
+// 32 lanes) of the second; applied to two copies of v they leave, in every
+// lane, the lower lane's value in the first and the upper lane's in the
+// second. Written as inline assembly: this compiler's builtin loses the second
+// result. The s_nop gives the wait states a VALU write needs before the swap
+// reads it.
+struct LanePair {
+    float lo, hi;
+};
+__device__ __forceinline__ LanePair swap16(float v) {
+    float a = v, b = v;
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+    return LanePair{a, b};
+}
+__device__ __forceinline__ LanePair swap32(float v) {
+    float a = v, b = v;
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(a), "+v"(b));
+    return LanePair{a, b};
+}
+__device__ __forceinline__ float swap16_sum(float v) {
+    const LanePair p = swap16(v);
+    return p.lo + p.hi;
+}
+__device__ __forceinline__ float swap32_sum(float v) {
+    const LanePair p = swap32(v);
+    return p.lo + p.hi;
+}
+__device__ __forceinline__ float swap16_max(float v) {
+    const LanePair p = swap16(v);
+    return fmaxf(p.lo, p.hi);
+}
+__device__ __forceinline__ float swap32_max(float v) {
+    const LanePair p = swap32(v);
+    return fmaxf(p.lo, p.hi);
+}
+
+}  // namespace rq

@@ -1,5 +1,5 @@
 // Paged serving: the step's tables, queries and keys into the paged cache
-// (paged.hip).
+// (paged.hip), attention over the pages (paged_attention.hip).
 #pragma once
 
 #include <hip/hip_fp16.h>
@@ -46,5 +46,12 @@ struct QkNormRope {
 };
 hipError_t launch_qk_norm_rope(const PagedBatch& b, const PagedCache& c, const QkNormRope& p, bool x_f16, bool q_f16,
                                hipStream_t stream);
+
+// Whether the launches' grids hold this batch.
+bool paged_attention_fits(const PagedBatch& b, const PagedCache& c, int q_heads);
+size_t paged_attention_workspace(const PagedBatch& b, const PagedCache& c, int q_heads, int cus);
+hipError_t launch_paged_attention(const PagedBatch& b, const PagedCache& c, const void* q, bool f32, int64_t ldq,
+                                  int q_heads, float scale, int window, void* workspace, void* out, int64_t ldo, int cus,
+                                  hipStream_t stream);
 
 }  // namespace rq

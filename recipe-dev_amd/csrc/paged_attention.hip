@@ -1,0 +1,781 @@
+// Attention of several sequences' new tokens over their pages
+// (rqmv_paged_attention).
+//
+// For query head h of a token at position p of its sequence:
+//     out = sum_k e^(s_k) v_k / sum_k e^(s_k),  s_k = scale q . k_k,
+// over the positions k of max(0, p - window + 1)..p whose pages are present, in
+// one pass over the keys with a running reference m (e^(s - m) throughout; a sum
+// is rescaled when its reference moves).
+//
+// Rows. A sequence with n new tokens has n * group rows per kv head (row r:
+// token r / group, head r % group of its group), cut into tiles of TM rows that
+// share the keys and values read. Tile i of sequence s is number floor(q_start[s]
+// * group / TM) + s + i: no two tiles share a number, the numbers grow with s, so
+// a workgroup finds its sequence by searching q_start, and tokens * group / TM +
+// seqs numbers always suffice (some stay empty).
+//
+// Matrix cores. S^T = K Q^T in 32 x 32 tiles: a lane then holds one query (its
+// column) and 16 of the tile's 32 keys, the other 16 in lane ^ 32, so a row's
+// maximum is taken over registers and one lane swap, and the weights already
+// lie where the second product takes them: O^T = V^T P^T needs, per 16 keys,
+// eight of them per lane, which may come in any order as long as V's operand has
+// the same; keys 4h..4h+3 and 8+4h..8+4h+3 (h = lane / 32) are the lane's own
+// scores. V's operand is read transposed from LDS (ds_read_b64_tr_b16).
+// Queries stay in registers. fp16 queries: the weights are rounded to fp16 (2^-12
+// of each weight on average, as fp16 outputs are rounded; references move
+// only when a maximum passes them by 2^8, and the weights are taken times 2^6,
+// so that they lie in fp16's normal range down to 2^-20 of the largest). fp32
+// queries: queries and weights are split into a high and a low fp16 part, two
+// products each (22 bits; queries scaled by a power of two per row, weights by
+// 2^15). Sums are fp32.
+//
+// Keys and values go from the pages straight into LDS (global_load_lds, 16
+// bytes a lane), 16 keys of one page at a time, at most 64 keys per step. A row's 16-byte
+// pieces are stored XORed with the row number, so that the operand reads hit
+// every bank once.
+//
+// Masked places: a masked score is -infinity by selection, and V must not meet
+// its zero weight as a NaN: in steps where some row may not see some key, dead
+// keys' values are zeroed in LDS, and non-finite values are added to the rows
+// that see them and then zeroed.
+#include "lanes.h"
+#include "paged.h"
+
+#include <limits.h>
+
+#include "halfcode.h"
+
+namespace rq {
+
+namespace {
+
+typedef float f16_t __attribute__((ext_vector_type(16)));
+typedef float f2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef short s4_t __attribute__((ext_vector_type(4)));
+
+struct AttnArgs {
+    const void* q;
+    void* out;
+    int64_t ldq, ldo;
+    PagedBatch b;
+    PagedCache c;
+    int group, cap;     // query heads per kv head; positions that the table reaches
+    int window;         // 0: none
+    float scale;        // times log2 e: scores are taken to the base 2
+    int tiles, splits, min_chunk;
+    float* o;           // [splits][tokens][q_heads][head_dim]
+    float2* ml;         // [splits][tokens][q_heads]: reference and weight sum
+};
+
+// One tile of rows and its keys.
+struct Tile {
+    int seq, token0, n, kv;  // the sequence, its first row of q, its new tokens, its positions
+    int row0, rows;          // the tile's first row in the sequence, the sequence's rows
+    int first, end;          // keys first..end-1 (first a multiple of 64)
+    int chunk, live;         // keys per split, splits that have any
+    int all_from, all_to;    // every row sees keys all_from..all_to-1
+};
+
+// Largest s with floor(q_start[s] * group / TM) + s <= number, 64 candidates at a time.
+template <int TM>
+__device__ __forceinline__ int find_seq(const PagedBatch& b, int group, int number) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = b.seqs;
+    while (n > 1) {
+        const int step = (n + 63) >> 6, i = lane * step;
+        bool le = false;
+        if (i < n) le = min(max(b.q_start[lo + i], 0), b.tokens) * group / TM + lo + i <= number;
+        const int c = max((int)__popcll(__ballot(le)), 1) - 1;
+        lo += c * step;
+        n = min(step, n - c * step);
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// Row starts and lengths are read as they are found and brought into range.
+template <int TM>
+__device__ __forceinline__ Tile make_tile(const AttnArgs& a, int seq, int row0) {
+    Tile t;
+    t.seq = seq;
+    t.token0 = min(max(a.b.q_start[seq], 0), a.b.tokens);
+    t.n = min(max(a.b.q_start[seq + 1], t.token0), a.b.tokens) - t.token0;
+    t.kv = max(a.b.kv_len[seq], 0);
+    t.row0 = row0;
+    t.rows = t.n * a.group;
+    const int last = min(row0 + TM, t.rows) - 1;
+    const int p0 = t.kv - t.n + row0 / a.group, p1 = t.kv - t.n + max(last, 0) / a.group;
+    t.end = max(min(p1 + 1, a.cap), 0);
+    t.first = a.window ? max(p0 - a.window + 1, 0) & ~63 : 0;
+    if (t.first > t.end) t.first = t.end & ~63;
+    const int len = t.end - t.first;
+    const int even = (len + a.splits - 1) / a.splits;
+    t.chunk = max((even + 63) & ~63, a.min_chunk);
+    t.live = (len + t.chunk - 1) / t.chunk;
+    t.all_from = a.window ? max(p1 - a.window + 1, 0) : 0;
+    t.all_to = min(p0 + 1, a.cap);
+    return t;
+}
+
+// 16 bytes per lane from `base` + `offset` (bytes) straight into LDS at `lds` +
+// 16 lane. Inline assembly, so that the compiler does not make every later LDS
+// read wait for it: the kernel waits for these loads itself. (M0 holds the LDS
+// address; a write of M0 needs one wait state before a load to LDS.)
+__device__ __forceinline__ void load_lds(const void* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(offset), "s"(base), "s"(lds)
+                 : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+template <int HD>
+struct Lay {
+    static constexpr int PCS = HD / 8;    // 16-byte pieces per row
+    static constexpr int RPI = 64 / PCS;  // rows per load instruction
+    static constexpr int NI = 16 / RPI;   // instructions per 16 keys
+    static constexpr int ROW = HD * 2;    // bytes per row
+    // the XOR of a row's piece numbers: K is read 16 rows at one piece, V four
+    // rows at four pieces in a row (a row of 64 dims is half the banks)
+    __device__ static constexpr int kx(int row) { return HD == 64 ? (row >> 1) & 7 : row & 15; }
+    __device__ static constexpr int vx(int row) { return HD == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
+};
+
+// The ids of a sequence's pages, 64 at a time in a wave's lanes.
+struct Pages {
+    const int* row;
+    int last, blocks, shift, from, held;
+    __device__ __forceinline__ void fetch(int page) {
+        from = page;
+        held = row[min(page + (int)(threadIdx.x & 63), last)];
+    }
+    __device__ __forceinline__ void need(int page0, int page1) {  // pages page0..page1 (at most 4)
+        if (page0 < from || page1 >= from + 64) fetch(page0);
+    }
+    __device__ __forceinline__ int at(int page) const { return __builtin_amdgcn_readlane(held, page - from); }
+    __device__ __forceinline__ bool absent(int id) const { return (unsigned)id >= (unsigned)blocks; }
+};
+
+// The 16 keys from `key` on of one page (id clamped into the cache) of `cache`, to LDS.
+template <int HD, bool VALUES>
+__device__ __forceinline__ void load_group(const __half* cache, const PagedCache& c, int kh, int id, int key,
+                                           uint32_t lds) {
+    typedef Lay<HD> L;
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (((int64_t)id * c.kv_heads + kh) << c.block_shift) + (key & ((1 << c.block_shift) - 1));
+    const __half* base = cache + row * HD;
+#pragma unroll
+    for (int i = 0; i < L::NI; ++i) {
+        const int r = i * L::RPI + lane / L::PCS;
+        const int piece = (lane % L::PCS) ^ (VALUES ? L::vx(r) : L::kx(r));
+        load_lds(base, (uint32_t)(r * L::ROW + piece * 16), lds + i * 1024);
+    }
+}
+
+// A wave's rows: queries as operands, output sums, references, weight sums.
+template <int HD, int QT, bool F32>
+struct Rows {
+    static constexpr int NK = HD / 16, ND = HD / 32, QP = F32 ? 2 : 1;
+    h8_t q[QT][NK][QP];
+    f16_t o[QT][ND];
+    float m[QT], l[QT], c[QT];  // reference (times c), weight sum of the lane's own keys, factor of the scores
+    int lo[QT], hi[QT];         // the row sees keys lo..hi
+};
+
+__device__ __forceinline__ h8_t cvt8(const float (&v)[8]) {
+    h8_t r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const h2_t p = __builtin_convertvector((f2_t{v[2 * e], v[2 * e + 1]}), h2_t);
+        r[2 * e] = p[0];
+        r[2 * e + 1] = p[1];
+    }
+    return r;
+}
+
+template <int HD, int QT, bool F32>
+__device__ __forceinline__ void load_rows(const AttnArgs& a, const Tile& t, int kh, int row, Rows<HD, QT, F32>& w) {
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        const int r = min(row + 32 * i + (lane & 31), t.rows - 1);  // (rows past the last repeat it)
+        const int tok = r / a.group, pos = t.kv - t.n + tok;
+        const int64_t at = (int64_t)(t.token0 + tok) * a.ldq + (kh * a.group + r % a.group) * HD + 8 * h;
+        w.hi[i] = min(pos, a.cap - 1);
+        w.lo[i] = a.window ? pos - a.window + 1 : 0;
+        w.m[i] = -INFINITY;
+        w.l[i] = 0.f;
+        w.c[i] = a.scale;
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w.o[i][d][e] = 0.f;
+        if constexpr (!F32) {
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k)
+                w.q[i][k][0] = *reinterpret_cast<const h8_t*>(static_cast<const _Float16*>(a.q) + at + 16 * k);
+        } else {
+            const float* src = static_cast<const float*>(a.q) + at;
+            float v[HD / 16][8], top = 0.f;
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+                const float4 x = *reinterpret_cast<const float4*>(src + 16 * k);
+                const float4 y = *reinterpret_cast<const float4*>(src + 16 * k + 4);
+                v[k][0] = x.x, v[k][1] = x.y, v[k][2] = x.z, v[k][3] = x.w;
+                v[k][4] = y.x, v[k][5] = y.y, v[k][6] = y.z, v[k][7] = y.w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[k][e]));
+            }
+            top = swap32_max(top);
+            // 2^up brings the row's largest magnitude into [2^13, 2^14); the low
+            // part's smallest step is then 2^-37 of it
+            int up = top > 0.f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+            up = min(max(up, -115), 100);
+            w.c[i] = ldexpf(a.scale, -up);
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+                float lo[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[k][e] = ldexpf(v[k][e], up);
+                w.q[i][k][0] = cvt8(v[k]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) lo[e] = v[k][e] - (float)w.q[i][k][0][e];
+                w.q[i][k][1] = cvt8(lo);
+            }
+        }
+    }
+}
+
+// S^T of 32 KT keys: s[i][t] holds, per lane, query lane % 32 of row tile i and
+// keys 32 t + 8 (e / 4) + 4 h + e % 4.
+template <int HD, int QT, int KT, bool F32>
+__device__ __forceinline__ void scores(const char* K, const Rows<HD, QT, F32>& w, f16_t (&s)[QT][KT]) {
+    typedef Lay<HD> L;
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < QT; ++i)
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[i][t][e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            const int r = 32 * t + (lane & 31);
+            const h8_t key = *reinterpret_cast<const h8_t*>(K + r * L::ROW + ((2 * k + h) ^ L::kx(r)) * 16);
+#pragma unroll
+            for (int i = 0; i < QT; ++i)
+#pragma unroll
+                for (int p = 0; p < Rows<HD, QT, F32>::QP; ++p)
+                    s[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, w.q[i][k][p], s[i][t], 0, 0, 0);
+        }
+}
+
+template <int HD, int QT, int KT, bool F32>
+__device__ __forceinline__ bool sees(const Rows<HD, QT, F32>& w, int i, int key0, int off, unsigned bad) {
+    return key0 + off <= w.hi[i] && key0 + off >= w.lo[i] && !((bad >> (off >> 4)) & 1);
+}
+
+// Scores to weights: masks, moves the references, adds up the weights and
+// rounds them to the second product's operands.
+template <int HD, int QT, int KT, bool F32>
+__device__ __forceinline__ void weights(Rows<HD, QT, F32>& w, f16_t (&s)[QT][KT], int key0, bool masked, unsigned bad,
+                                        h8_t (&p)[QT][2 * KT][F32 ? 2 : 1]) {
+    const int h = (threadIdx.x & 63) >> 5;
+    constexpr float SHIFT = F32 ? 15.f : 6.f, SLACK = F32 ? 0.f : 8.f;
+    if (masked) {
+#pragma unroll
+        for (int i = 0; i < QT; ++i)
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int off = 32 * t + 8 * (e / 4) + 4 * h + e % 4;
+                    if (!sees<HD, QT, KT, F32>(w, i, key0, off, bad)) s[i][t][e] = -INFINITY;
+                }
+    }
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        float top = s[i][0][0];
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, s[i][t][e]);
+        top = swap32_max(top) * w.c[i];
+        if (__any(top > w.m[i] + SLACK)) {
+            const float m = fmaxf(w.m[i], top);
+            const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(w.m[i] - m);
+            w.m[i] = m;
+            w.l[i] *= f;
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) w.o[i][d][e] *= f;
+        }
+        const float ref = w.m[i] == -INFINITY ? 0.f : w.m[i] - SHIFT;
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[e] = __builtin_amdgcn_exp2f(fmaf(s[i][t][8 * b + e], w.c[i], -ref));
+                    w.l[i] += v[e];
+                }
+                h8_t& hi = p[i][2 * t + b][0];
+                hi = cvt8(v);
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] -= (float)hi[e];
+                    p[i][2 * t + b][1] = cvt8(v);
+                }
+            }
+    }
+}
+
+// O^T += V^T P^T over 32 KT keys.
+template <int HD, int QT, int KT, bool F32>
+__device__ __forceinline__ void add_values(const char* V, Rows<HD, QT, F32>& w,
+                                           const h8_t (&p)[QT][2 * KT][F32 ? 2 : 1]) {
+    typedef Lay<HD> L;
+    const int lane = threadIdx.x & 63;
+    // 16 lanes read 16 dims of four keys; key bits 0-1 are (lane & 15) / 4
+    const int r = 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int low = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+    for (int b = 0; b < 2 * KT; ++b)
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d) {
+            const char* at = V + (16 * b + r) * L::ROW + ((4 * d + low) ^ L::vx(r)) * 16 + (lane & 1) * 8;
+            const char* at8 = V + (16 * b + 8 + r) * L::ROW + ((4 * d + low) ^ L::vx(8 + r)) * 16 + (lane & 1) * 8;
+            typedef __attribute__((address_space(3))) s4_t lds4;
+            const s4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)at);
+            const s4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)at8);
+            const h8_t v = __builtin_bit_cast(h8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+            for (int i = 0; i < QT; ++i)
+#pragma unroll
+                for (int part = 0; part < (F32 ? 2 : 1); ++part)
+                    w.o[i][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[i][b][part], w.o[i][d], 0, 0, 0);
+        }
+}
+
+// fp16 pairs with an exponent of all ones leave 0x8000 bits here.
+__device__ __forceinline__ uint32_t odd_bits(uint32_t x) { return ((x & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
+
+// A step in which some row may not see some key: zeroes the values of keys that
+// no row sees (key0 + row >= end, absent pages), and returns whether a value of
+// another is NaN or infinite. `thread` of `threads` walks the tile.
+template <int HD, int KEYS>
+__device__ __forceinline__ bool zero_dead(char* V, int key0, int end, unsigned bad, int thread, int threads) {
+    bool odd = false;
+    for (int u = thread; u < KEYS * (HD / 8); u += threads) {
+        const int row = u / (HD / 8);
+        uint4* at = reinterpret_cast<uint4*>(V + u * 16);
+        if (key0 + row >= end || ((bad >> (row >> 4)) & 1)) {
+            *at = make_uint4(0, 0, 0, 0);
+        } else {
+            const uint4 x = *at;
+            odd |= (odd_bits(x.x) | odd_bits(x.y) | odd_bits(x.z) | odd_bits(x.w)) != 0;
+        }
+    }
+    return odd;
+}
+
+// The rare step with such values: added to the rows that see them ...
+template <int HD, int QT, int KT, bool F32>
+__device__ __forceinline__ void add_odd(const char* V, Rows<HD, QT, F32>& w, int key0, unsigned bad) {
+    typedef Lay<HD> L;
+    const int h = (threadIdx.x & 63) >> 5;
+    for (int row = 0; row < 32 * KT; ++row)
+#pragma unroll
+        for (int i = 0; i < QT; ++i) {
+            const bool seen = sees<HD, QT, KT, F32>(w, i, key0, row, bad);
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int dim = 32 * d + 8 * (e / 4) + 4 * h + e % 4;
+                    const float v = (float)*reinterpret_cast<const _Float16*>(
+                        V + row * L::ROW + ((dim >> 3) ^ L::vx(row)) * 16 + (dim & 7) * 2);
+                    if (seen && !(fabsf(v) < INFINITY)) w.o[i][d][e] += v;
+                }
+        }
+}
+
+// ... and zeroed.
+template <int HD, int KEYS>
+__device__ __forceinline__ void zero_odd(char* V, int thread, int threads) {
+    for (int u = thread; u < KEYS * (HD / 2); u += threads) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(V + u * 4);
+        const uint32_t odd = odd_bits(*at);
+        if (odd) *at &= ~(((odd >> 15) & 0x00010001u) * 0xFFFFu);
+    }
+}
+
+// Four consecutive dims of a row to the output or, with several live splits, to the workspace.
+__device__ __forceinline__ void put4(const AttnArgs& a, bool f16_out, bool whole, int split, int token, int head, int hd,
+                                     int dim, const float (&v)[4]) {
+    if (whole) {
+        if (f16_out) {
+            uint2 u;
+            u.x = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t{v[0], v[1]}), h2_t));
+            u.y = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2_t{v[2], v[3]}), h2_t));
+            *reinterpret_cast<uint2*>(static_cast<_Float16*>(a.out) + (int64_t)token * a.ldo + head * hd + dim) = u;
+        } else {
+            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + (int64_t)token * a.ldo + head * hd + dim) =
+                make_float4(v[0], v[1], v[2], v[3]);
+        }
+    } else {
+        const int64_t row = ((int64_t)split * a.b.tokens + token) * (a.group * a.c.kv_heads) + head;
+        *reinterpret_cast<float4*>(a.o + row * hd + dim) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+__device__ __forceinline__ float reciprocal(float l) { return l == 0.f ? 0.f : 1.f / l; }  // (no key: zeros)
+
+// ------------------------------------------- few rows: keys over the waves ----
+
+// At most 32 rows a tile (a decode step, a few speculated tokens): bound by
+// reading the keys and values. Each of four waves takes every fourth step of 32
+// keys of the split into LDS of its own, without barriers; its K buffer is filled
+// again while it works on the values and the other way round, and a second workgroup
+// on the CU fills the rest. At the end the waves' sums are joined through LDS.
+template <int HD, bool F32>
+__global__ void __launch_bounds__(256) paged_few_kernel(AttnArgs a) {
+    typedef Lay<HD> L;
+    constexpr int TM = 32, KEYS = 32, HALF = KEYS * HD * 2;  // HALF: bytes of a wave's K (and V) buffer
+    extern __shared__ __align__(16) char lds[];
+    __shared__ float2 sums[4][32];
+    const int kh = blockIdx.x % a.c.kv_heads, number = blockIdx.x / a.c.kv_heads, split = blockIdx.y;
+    const int seq = find_seq<TM>(a.b, a.group, number);
+    const int first = min(max(a.b.q_start[seq], 0), a.b.tokens) * a.group / TM + seq;
+    const Tile t = make_tile<TM>(a, seq, (number - first) * TM);
+    if (t.row0 >= t.rows) return;
+    const int begin = t.first + split * t.chunk, end = min(begin + t.chunk, t.end);
+    if (split && begin >= end) return;  // (split 0 of a tile without keys writes its zeros)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    char* K = lds + wave * 2 * HALF;
+    char* V = K + HALF;
+    const uint32_t k_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)K, v_lds = k_lds + HALF;
+    Pages pages{a.b.table + seq * a.b.table_stride, a.b.max_blocks - 1, a.c.blocks, a.c.block_shift, INT_MIN / 2, 0};
+    Rows<HD, 1, F32> w;
+    load_rows<HD, 1, F32>(a, t, kh, t.row0, w);
+
+    int id[2], next[2];
+    auto look = [&](int key0, int (&ids)[2]) {  // the page ids of keys key0.. and key0 + 16..
+        const int p0 = key0 >> pages.shift, p1 = (key0 + 16) >> pages.shift;
+        pages.need(p0, p1);
+        ids[0] = pages.at(p0);
+        ids[1] = pages.at(p1);
+    };
+    auto load = [&](auto values, int key0, const int (&ids)[2]) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+            load_group<HD, decltype(values)::value>(decltype(values)::value ? a.c.v : a.c.k, a.c, kh,
+                                                    pages.absent(ids[g]) ? 0 : ids[g], key0 + 16 * g,
+                                                    (decltype(values)::value ? v_lds : k_lds) + g * 16 * L::ROW);
+    };
+    int key0 = begin + wave * KEYS;
+    if (key0 < end) {
+        look(key0, id);
+        load(std::false_type{}, key0, id);
+        load(std::true_type{}, key0, id);
+    }
+    while (key0 < end) {
+        const int after = key0 + 4 * KEYS;
+        const bool more = after < end;
+        wait_loads<2 * L::NI>();  // K (V's loads were issued after it)
+        f16_t s[1][1];
+        scores<HD, 1, 1, F32>(K, w, s);
+        if (more) {
+            look(after, next);
+            // the operand reads have returned (their products are the scores)
+            asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s[0][0]) : : "memory");
+            load(std::false_type{}, after, next);
+        }
+        const unsigned bad = (pages.absent(id[0]) ? 1 : 0) | (pages.absent(id[1]) ? 2 : 0);
+        const bool masked = key0 < t.all_from || key0 + KEYS > t.all_to || bad;
+        h8_t p[1][2][F32 ? 2 : 1];
+        weights<HD, 1, 1, F32>(w, s, key0, masked, bad, p);
+        if (more) wait_loads<2 * L::NI>();
+        else wait_loads<0>();
+        if (masked && __any(zero_dead<HD, KEYS>(V, key0, t.end, bad, lane, 64))) {
+            add_odd<HD, 1, 1, F32>(V, w, key0, bad);
+            zero_odd<HD, KEYS>(V, lane, 64);
+        }
+        add_values<HD, 1, 1, F32>(V, w, p);
+        if (more) {
+            asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(w.o[0][0]) : : "memory");
+            load(std::true_type{}, after, next);
+            id[0] = next[0], id[1] = next[1];
+        }
+        key0 = after;
+    }
+    wait_loads<0>();
+    // the waves' sums, each in its own LDS (32 rows of HD values, pieces XORed with the row)
+    const int q = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int piece = (32 * d + 8 * e + 4 * h) / 4;
+            *reinterpret_cast<float4*>(K + q * HD * 4 + (piece ^ (q & 15)) * 16) =
+                make_float4(w.o[0][d][4 * e], w.o[0][d][4 * e + 1], w.o[0][d][4 * e + 2], w.o[0][d][4 * e + 3]);
+        }
+    const float l = swap32_sum(w.l[0]);
+    if (h == 0) sums[wave][q] = make_float2(w.m[0], l);
+    __syncthreads();
+    const int rows = min(t.rows - t.row0, TM);
+    const bool whole = t.live <= 1;
+    for (int u = threadIdx.x; u < rows * (HD / 4); u += 256) {
+        const int row = u / (HD / 4), piece = u % (HD / 4);
+        float m = sums[0][row].x, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 1; i < 4; ++i) m = fmaxf(m, sums[i][row].x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 ml = sums[i][row];
+            const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml.x - m);
+            const float4 x = *reinterpret_cast<const float4*>(lds + i * 2 * HALF + row * HD * 4 + (piece ^ (row & 15)) * 16);
+            sum = fmaf(f, ml.y, sum);
+            v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
+        }
+        const int tok = (t.row0 + row) / a.group, head = kh * a.group + (t.row0 + row) % a.group;
+        if (whole) {
+            const float inv = reciprocal(sum);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] *= inv;
+        } else if (piece == 0) {
+            a.ml[((int64_t)split * a.b.tokens + t.token0 + tok) * (a.group * a.c.kv_heads) + head] = make_float2(m, sum);
+        }
+        put4(a, !F32, whole, split, t.token0 + tok, head, HD, 4 * piece, v);
+    }
+}
+
+// --------------------------------------------- many rows: rows over the waves ----
+
+// TM = 128 QT rows a tile (prompts, chunks of prompts): bound by the matrix
+// cores and the exponentials. Four waves of 32 QT rows share steps of 64 keys in two LDS
+// buffers, one barrier a step.
+template <int HD, int QT, bool F32>
+__global__ void __launch_bounds__(256) paged_many_kernel(AttnArgs a) {
+    typedef Lay<HD> L;
+    constexpr int TM = 128 * QT, KEYS = 64, HALF = KEYS * HD * 2;
+    extern __shared__ __align__(16) char lds[];
+    // the last tiles first: of one sequence's they have the most keys
+    const int kh = blockIdx.x % a.c.kv_heads, number = a.tiles - 1 - blockIdx.x / a.c.kv_heads, split = blockIdx.y;
+    const int seq = find_seq<TM>(a.b, a.group, number);
+    const int first = min(max(a.b.q_start[seq], 0), a.b.tokens) * a.group / TM + seq;
+    const Tile t = make_tile<TM>(a, seq, (number - first) * TM);
+    if (t.row0 >= t.rows) return;
+    const int begin = t.first + split * t.chunk, end = min(begin + t.chunk, t.end);
+    if (split && begin >= end) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = t.row0 + 32 * QT * wave;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+    Pages pages{a.b.table + seq * a.b.table_stride, a.b.max_blocks - 1, a.c.blocks, a.c.block_shift, INT_MIN / 2, 0};
+    Rows<HD, QT, F32> w;
+    load_rows<HD, QT, F32>(a, t, kh, row, w);
+
+    // step i is in buffer i % 2; the wave loads its 16 keys of K and V. Returns which groups are absent.
+    auto load = [&](int key0, int buffer) -> unsigned {
+        pages.need(key0 >> pages.shift, (key0 + 48) >> pages.shift);
+        unsigned bad = 0;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) bad |= pages.absent(pages.at((key0 + 16 * g) >> pages.shift)) ? 1u << g : 0u;
+        const int key = key0 + 16 * wave, id = pages.at(key >> pages.shift);
+        const uint32_t at = lds0 + buffer * 2 * HALF + wave * 16 * L::ROW;
+        load_group<HD, false>(a.c.k, a.c, kh, pages.absent(id) ? 0 : id, key, at);
+        load_group<HD, true>(a.c.v, a.c, kh, pages.absent(id) ? 0 : id, key, at + HALF);
+        return bad;
+    };
+    unsigned bad = 0, bad_next = 0;
+    int buffer = 0;
+    if (begin < end) bad = load(begin, 0);
+    for (int key0 = begin; key0 < end; key0 += KEYS) {
+        wait_loads<0>();
+        __syncthreads();  // the step is in LDS, and the other buffer is free
+        if (key0 + KEYS < end) bad_next = load(key0 + KEYS, buffer ^ 1);
+        char* K = lds + buffer * 2 * HALF;
+        char* V = K + HALF;
+        const bool masked = key0 < t.all_from || key0 + KEYS > t.all_to || bad;
+        f16_t s[QT][2];
+        scores<HD, QT, 2, F32>(K, w, s);
+        h8_t p[QT][4][F32 ? 2 : 1];
+        weights<HD, QT, 2, F32>(w, s, key0, masked, bad, p);
+        if (masked && __syncthreads_or(zero_dead<HD, KEYS>(V, key0, t.end, bad, threadIdx.x, 256))) {
+            add_odd<HD, QT, 2, F32>(V, w, key0, bad);
+            __syncthreads();
+            zero_odd<HD, KEYS>(V, threadIdx.x, 256);
+            __syncthreads();
+        }
+        add_values<HD, QT, 2, F32>(V, w, p);
+        bad = bad_next;
+        buffer ^= 1;
+    }
+    const bool whole = t.live <= 1;
+    const int h = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        const int r = row + 32 * i + (lane & 31);
+        const float l = swap32_sum(w.l[i]);
+        const float f = whole ? reciprocal(l) : 1.f;
+        if (r >= t.rows) continue;
+        const int tok = t.token0 + r / a.group, head = kh * a.group + r % a.group;
+        if (!whole && h == 0)
+            a.ml[((int64_t)split * a.b.tokens + tok) * (a.group * a.c.kv_heads) + head] = make_float2(w.m[i], l);
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float v[4] = {w.o[i][d][4 * e] * f, w.o[i][d][4 * e + 1] * f, w.o[i][d][4 * e + 2] * f,
+                                    w.o[i][d][4 * e + 3] * f};
+                put4(a, !F32, whole, split, tok, head, HD, 32 * d + 8 * e + 4 * h, v);
+            }
+    }
+}
+
+// ---------------------------------------------------------- the splits' join ----
+
+// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's live splits.
+template <int HD, int TM, bool F32>
+__global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a) {
+    constexpr int TPR = HD / 4;  // threads per row
+    const int heads = a.group * a.c.kv_heads;
+    const int64_t unit = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const int token = (int)min(unit / heads, (int64_t)a.b.tokens - 1), head = (int)(unit % heads);
+    // the token's sequence: the last one that starts at or before it
+    int lo = 0, n = a.b.seqs;
+    while (n > 1) {
+        const int half = n >> 1;
+        if (a.b.q_start[lo + half] <= token) lo += half, n -= half;
+        else n = half;
+    }
+    if (unit >= (int64_t)a.b.tokens * heads) return;
+    if (token < a.b.q_start[lo] || token >= a.b.q_start[lo + 1]) return;
+    const int row = (token - a.b.q_start[lo]) * a.group + head % a.group;
+    const Tile t = make_tile<TM>(a, lo, row / TM * TM);
+    if (t.live <= 1) return;
+    const int dim = 4 * (threadIdx.x % TPR);
+    float M = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    const int64_t at = (int64_t)token * heads + head, step = (int64_t)a.b.tokens * heads;
+    for (int c = 0; c < t.live; ++c) M = fmaxf(M, a.ml[at + c * step].x);
+    for (int c = 0; c < t.live; ++c) {
+        const float2 ml = a.ml[at + c * step];
+        const float4 x = *reinterpret_cast<const float4*>(a.o + (at + c * step) * HD + dim);
+        const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml.x - M);
+        sum = fmaf(f, ml.y, sum);
+        v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
+    }
+    const float inv = reciprocal(sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= inv;
+    put4(a, !F32, true, 0, token, head, HD, dim, v);
+}
+
+// ------------------------------------------------------------------ launches ----
+
+constexpr int few_lds(int hd) { return 4 * 2 * 32 * hd * 2; }
+constexpr int many_lds(int hd) { return 2 * 2 * 64 * hd * 2; }
+// 32-row tiles per wave of the many-rows form: the output sums and queries of two fit the
+// registers up to 128 dims of fp16 rows
+constexpr int many_qt(int hd, bool f32) { return hd == 256 || (hd == 128 && f32) ? 1 : 2; }
+
+struct AttnPlan {
+    bool few;
+    int tm, splits, min_chunk;
+    int64_t tiles;
+};
+
+AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus) {
+    AttnPlan p;
+    p.few = (int64_t)tokens * group <= (int64_t)32 * seqs;
+    p.tm = p.few ? 32 : 128 * many_qt(hd, f32);
+    p.tiles = (int64_t)tokens * group / p.tm + seqs;
+    p.min_chunk = p.few ? 128 : 512;
+    const int64_t wgs = p.tiles * kv_heads, want = p.few ? 2 * cus : cus;
+    int64_t s = wgs >= want ? 1 : (want + wgs - 1) / wgs;
+    const int64_t most = (cap + p.min_chunk - 1) / p.min_chunk;
+    if (s > most) s = most;
+    if (s > 64) s = 64;
+    p.splits = (int)(s < 1 ? 1 : s);
+    return p;
+}
+
+template <int HD, bool F32>
+hipError_t launch_attention_hd(const AttnPlan& p, const AttnArgs& a, hipStream_t stream) {
+    constexpr int QT = many_qt(HD, F32);
+    const dim3 grid((unsigned)(p.tiles * a.c.kv_heads), p.splits);
+    const void* f = p.few ? reinterpret_cast<const void*>(paged_few_kernel<HD, F32>)
+                          : reinterpret_cast<const void*>(paged_many_kernel<HD, QT, F32>);
+    const int lds = p.few ? few_lds(HD) : many_lds(HD);
+    if (lds > 48 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+    }
+    if (p.few) hipLaunchKernelGGL((paged_few_kernel<HD, F32>), grid, dim3(256), lds, stream, a);
+    else hipLaunchKernelGGL((paged_many_kernel<HD, QT, F32>), grid, dim3(256), lds, stream, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.splits == 1) return e;
+    const int64_t rows = (int64_t)a.b.tokens * a.group * a.c.kv_heads;
+    const dim3 join((unsigned)((rows + 256 / (HD / 4) - 1) / (256 / (HD / 4))));
+    if (p.few) hipLaunchKernelGGL((paged_join_kernel<HD, 32, F32>), join, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((paged_join_kernel<HD, 128 * QT, F32>), join, dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+bool paged_attention_fits(const PagedBatch& b, const PagedCache& c, int q_heads) {
+    return ((int64_t)b.tokens * (q_heads / c.kv_heads) / 32 + b.seqs) * c.kv_heads <= (1 << 23) &&
+           (int64_t)b.tokens * q_heads <= (1 << 26);
+}
+
+size_t paged_attention_workspace(const PagedBatch& b, const PagedCache& c, int q_heads, int cus) {
+    // (the larger of the two types', so that one workspace serves both)
+    size_t most = 0;
+    for (int f32 = 0; f32 < 2; ++f32) {
+        const AttnPlan p = plan_attention(b.tokens, b.seqs, (int64_t)b.max_blocks << c.block_shift, c.kv_heads,
+                                          q_heads / c.kv_heads, c.head_dim, f32, cus);
+        const size_t rows = p.splits > 1 ? (size_t)p.splits * b.tokens * q_heads : 0;
+        const size_t bytes = rows * (c.head_dim * sizeof(float) + sizeof(float2));
+        most = bytes > most ? bytes : most;
+    }
+    return most;
+}
+
+hipError_t launch_paged_attention(const PagedBatch& b, const PagedCache& c, const void* q, bool f32, int64_t ldq,
+                                  int q_heads, float scale, int window, void* workspace, void* out, int64_t ldo, int cus,
+                                  hipStream_t stream) {
+    const int group = q_heads / c.kv_heads;
+    const int64_t cap = (int64_t)b.max_blocks << c.block_shift;
+    const AttnPlan p = plan_attention(b.tokens, b.seqs, cap, c.kv_heads, group, c.head_dim, f32, cus);
+    AttnArgs a;
+    a.q = q;
+    a.out = out;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.b = b;
+    a.c = c;
+    a.group = group;
+    a.cap = (int)(cap < (1 << 30) ? cap : (1 << 30));
+    a.window = window;
+    a.scale = scale * 1.44269504088896340736f;
+    a.tiles = (int)p.tiles;
+    a.splits = p.splits;
+    a.min_chunk = p.min_chunk;
+    a.o = static_cast<float*>(workspace);
+    a.ml = reinterpret_cast<float2*>(a.o + (p.splits > 1 ? (size_t)p.splits * b.tokens * q_heads * c.head_dim : 0));
+    if (c.head_dim == 64) return f32 ? launch_attention_hd<64, true>(p, a, stream) : launch_attention_hd<64, false>(p, a, stream);
+    if (c.head_dim == 128)
+        return f32 ? launch_attention_hd<128, true>(p, a, stream) : launch_attention_hd<128, false>(p, a, stream);
+    return f32 ? launch_attention_hd<256, true>(p, a, stream) : launch_attention_hd<256, false>(p, a, stream);
+}
+
+}  // namespace rq

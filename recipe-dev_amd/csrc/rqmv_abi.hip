@@ -871,6 +871,56 @@ int rqmv_qk_norm_rope(const rqmv_paged_batch* batch, const rqmv_paged_cache* cac
     return e == hipSuccess ? RQMV_OK : hip_fail(e, "qk_norm_rope launch");
 }
 
+static int paged_attention_check(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, int q_heads,
+                                 rq::PagedCache* c, DeviceInfo* info) {
+    int rc = check_paged_cache(cache, "paged_attention", c);
+    if (rc == RQMV_OK) rc = check_paged_batch(batch, "paged_attention");
+    if (rc == RQMV_OK) rc = check_paged_table(batch, "paged_attention");
+    if (rc != RQMV_OK) return rc;
+    if (q_heads <= 0 || q_heads > kPagedMaxHeads || q_heads % c->kv_heads)
+        return fail(RQMV_EINVAL, "paged_attention: q_heads must be a multiple of kv_heads, at most 1024");
+    if (!rq::paged_attention_fits(paged_batch(batch), *c, q_heads))
+        return fail(RQMV_EINVAL, "paged_attention: tokens * q_heads must be at most 2^26, and (tokens * q_heads / kv_heads "
+                                 "/ 32 + seqs) * kv_heads at most 2^23");
+    const int dev = current_device(info);
+    return dev < 0 ? dev : RQMV_OK;
+}
+
+int rqmv_paged_attention_workspace_size(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, int q_heads,
+                                        size_t* bytes) {
+    if (!bytes) return fail(RQMV_EINVAL, "paged_attention: NULL size");
+    rq::PagedCache c;
+    DeviceInfo info;
+    const int rc = paged_attention_check(batch, cache, q_heads, &c, &info);
+    if (rc != RQMV_OK) return rc;
+    *bytes = rq::paged_attention_workspace(paged_batch(batch), c, q_heads, info.cus);
+    return RQMV_OK;
+}
+
+int rqmv_paged_attention(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, const void* q, int dtype,
+                         int64_t ldq, int q_heads, float scale, int window, void* workspace, size_t workspace_bytes,
+                         void* out, int64_t ldo, void* stream) {
+    if (!q || !out || (dtype != RQMV_DTYPE_F16 && dtype != RQMV_DTYPE_F32) || !(scale > 0.f) || scale > 1e30f || window < 0)
+        return fail(RQMV_EINVAL, "paged_attention: bad arguments");
+    rq::PagedCache c;
+    DeviceInfo info;
+    const int rc = paged_attention_check(batch, cache, q_heads, &c, &info);
+    if (rc != RQMV_OK) return rc;
+    if (!batch->q_start || !batch->kv_len || !batch->block_table)
+        return fail(RQMV_EINVAL, "paged_attention: q_start, kv_len and block_table are needed");
+    const int64_t size = dtype == RQMV_DTYPE_F16 ? 2 : 4, row = (int64_t)q_heads * c.head_dim;
+    if (batch->tokens > 1 && (ldq < row || ldo < row || ldq > kPagedMaxStride || ldo > kPagedMaxStride ||
+                              ldq * size % 16 || ldo * size % 16))
+        return fail(RQMV_EINVAL, "paged_attention: ldq or ldo is too small, too large or no multiple of 16 bytes");
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15)
+        return fail(RQMV_EINVAL, "paged_attention: q, out and the workspace must be 16-byte aligned");
+    const size_t need = rq::paged_attention_workspace(paged_batch(batch), c, q_heads, info.cus);
+    if (workspace_bytes < need || (need && !workspace)) return fail(RQMV_EINVAL, "paged_attention: workspace too small");
+    hipError_t e = rq::launch_paged_attention(paged_batch(batch), c, q, dtype == RQMV_DTYPE_F32, ldq, q_heads, scale,
+                                              window, workspace, out, ldo, info.cus, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? RQMV_OK : hip_fail(e, "paged_attention launch");
+}
+
 int rqmv_silu_mul(const float* gate_up, int n, float* out, void* stream) {
     if (!gate_up || !out || n <= 0) return fail(RQMV_EINVAL, "silu_mul: bad arguments");
     hipError_t e = rq::launch_silu_mul(gate_up, n, out, static_cast<hipStream_t>(stream));

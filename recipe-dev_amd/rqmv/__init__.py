@@ -99,6 +99,9 @@ class _Lib:
                                       c_void_p, c_void_p]
         L.rqmv_qk_norm_rope.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p,
                                         c_float, c_void_p, c_int, c_int, c_void_p, c_int, c_int64, c_void_p]
+        L.rqmv_paged_attention_workspace_size.argtypes = [c_void_p, c_void_p, c_int, POINTER(c_size_t)]
+        L.rqmv_paged_attention.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_float, c_int, c_void_p,
+                                           c_size_t, c_void_p, c_int64, c_void_p]
         L.rqmv_glu_weight_create.argtypes = [c_int, c_int64, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]
         L.rqmv_matvec_fused.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
         L.rqmv_layout_bytes.argtypes = [c_int, c_int64, c_int64, POINTER(c_size_t)]
@@ -734,6 +737,27 @@ def qk_norm_rope(batch: PagedBatch, cache: PagedCache, qkv, x_dtype: int, ld: in
                                        _p(q_norm), _p(k_norm), eps, table.ptr,
                                        cache.head_dim if rot_dim is None else rot_dim, rope_rows, q_out.ptr, q_dtype,
                                        ldq, _sh(stream)), "rqmv_qk_norm_rope")
+
+
+def paged_attention_workspace_size(batch: PagedBatch, cache: PagedCache, q_heads: int) -> int:
+    n = c_size_t()
+    _check(lib().lib.rqmv_paged_attention_workspace_size(byref(batch.struct), byref(cache.struct), q_heads, byref(n)),
+           "rqmv_paged_attention_workspace_size")
+    return n.value
+
+
+def paged_attention_workspace(batch: PagedBatch, cache: PagedCache, q_heads: int) -> DeviceBuffer:
+    return DeviceBuffer(paged_attention_workspace_size(batch, cache, q_heads))
+
+
+def paged_attention(batch: PagedBatch, cache: PagedCache, q, dtype: int, ldq: int, q_heads: int, out, ldo: int,
+                    workspace=None, scale: float | None = None, window: int = 0, stream: Stream | None = None):
+    """The new tokens' attention over their pages (rqmv_paged_attention); scale
+    defaults to 1 / sqrt(head_dim)."""
+    _check(lib().lib.rqmv_paged_attention(byref(batch.struct), byref(cache.struct), q.ptr, dtype, ldq, q_heads,
+                                          cache.head_dim ** -0.5 if scale is None else scale, window, _p(workspace),
+                                          workspace.nbytes if workspace is not None else 0, out.ptr, ldo, _sh(stream)),
+           "rqmv_paged_attention")
 
 
 # ------------------------------------------------------- fused products ----

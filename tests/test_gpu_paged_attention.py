@@ -1,0 +1,319 @@
+"""GPU parity of rqmv_paged_attention against the f64 reference of
+oracle/paged.py.
+
+Bars. Per row, with w the reference's weights (sum 1) and A = sum w |v|:
+ - a score s = scale q.k is off by at most E, counted here per element: fp32
+   rows carry q to 2^-21 of the row's largest magnitude (two fp16 parts) and every
+   product and sum of the dot rounds to 2^-24 of the magnitudes' sum (head_dim / 8 + 8
+   roundings in a row), fp16 rows only the latter; then the product with the scale
+   and the reference, 4 * 2^-24 |s|, and 2^-22 for the exponential. Weights
+   are then off by a factor e^(+-E), their quotient by e^(2 E).
+ - fp16 rows: each weight is rounded to fp16 (2^-11 relative, or 2^-25 of the
+   scale where the largest is 2^6 or more: 2^-31), and so is the output (2^-11).
+   fp32 rows: weights in two parts, 2^-21.
+ - sums of n products: (n / 16 + 40) * 2^-24 of A, and the joins of waves and splits
+   lie within the 40.
+So |out - ref| <= (e^(2 E) - 1 + weights + sums) A + output rounding.
+"""
+import numpy as np
+import pytest
+
+from oracle import paged as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(gpu, a):
+    return gpu.DeviceBuffer.from_array(np.asarray(a, np.int32))
+
+
+class Case:
+    """A batch of sequences (new, cached) over a shuffled pool, on the host."""
+
+    def __init__(self, seqs, nq, nkv, hd, block, f16, seed, spread=1.0, extra_rows=0, max_blocks=None):
+        rng = np.random.default_rng(seed)
+        self.nq, self.nkv, self.hd, self.block, self.f16 = nq, nkv, hd, block, f16
+        need = [ref.pages(c + n, block) for n, c in seqs]
+        self.width = max_blocks or max(max(need), 1)
+        self.blocks = sum(need) + 2
+        ids = rng.permutation(self.blocks)
+        self.table = np.full((len(seqs), self.width), -1, np.int32)
+        at = 0
+        for s, n in enumerate(need):
+            n = min(n, self.width)
+            self.table[s, :n] = ids[at:at + n]
+            at += n
+        self.q_start = np.concatenate(([0], np.cumsum([n for n, _ in seqs]))).astype(np.int32)
+        self.kv_len = np.array([n + c for n, c in seqs], np.int32)
+        self.rows = int(self.q_start[-1]) + extra_rows
+        dt = np.float16 if f16 else np.float32
+        self.q = (rng.standard_normal((max(self.rows, 1), nq, hd)) * spread).astype(dt)
+        self.k = rng.standard_normal((self.blocks, nkv, block, hd)).astype(np.float16)
+        self.v = rng.standard_normal((self.blocks, nkv, block, hd)).astype(np.float16)
+
+    def run(self, gpu, scale=None, window=0, pad=0, stride=None, stream=None):
+        dt = np.float16 if self.f16 else np.float32
+        rows, row = max(self.rows, 1), self.nq * self.hd
+        q = np.full((rows, row + pad), 3, dt)
+        q[:, :row] = self.q.reshape(rows, row)
+        bits = np.uint16 if self.f16 else np.uint32
+        Q = gpu.DeviceBuffer.from_array(q.view(bits))
+        self.sentinel = np.full((rows, row + pad), 7, dt)
+        O = gpu.DeviceBuffer.from_array(self.sentinel.view(bits))
+        stride = stride or self.width
+        table = np.full((len(self.kv_len), stride), -1, np.int32)
+        table[:, :self.width] = self.table
+        batch = gpu.PagedBatch(len(self.kv_len), rows, self.width, i32(gpu, self.q_start), i32(gpu, self.kv_len),
+                               i32(gpu, table), table_stride=stride)
+        cache = gpu.PagedCache(gpu.DeviceBuffer.from_array(self.k.view(np.uint16)),
+                               gpu.DeviceBuffer.from_array(self.v.view(np.uint16)), self.blocks, self.block, self.nkv,
+                               self.hd)
+        ws = gpu.paged_attention_workspace(batch, cache, self.nq)
+        gpu.paged_attention(batch, cache, Q, gpu.DTYPE_F16 if self.f16 else gpu.DTYPE_F32, row + pad, self.nq, O,
+                            row + pad, ws, scale, window, stream)
+        gpu.synchronize()
+        out = O.download(bits).view(dt).reshape(rows, row + pad)
+        assert np.all(out[:, row:] == 7)
+        return out[:, :row].reshape(rows, self.nq, self.hd)
+
+    def want(self, scale=None, window=0):
+        scale = self.hd ** -0.5 if scale is None else scale
+        out = ref.attention(self.q, self.k, self.v, self.q_start, self.kv_len, self.table, self.width, scale, window)
+        size = ref.attention(self.q, self.k, np.abs(self.v), self.q_start, self.kv_len, self.table, self.width, scale,
+                             window)
+        return out, size
+
+    def check(self, gpu, scale=None, window=0, **kw):
+        got = self.run(gpu, scale, window, **kw)
+        out, size = self.want(scale, window)
+        live = int(self.q_start[-1])
+        assert np.all(got[live:] == 7)  # rows of no sequence
+        got, out, size = got[:live].astype(np.float64), out[:live], size[:live]
+        assert np.all(np.isfinite(got))
+        sc = self.hd ** -0.5 if scale is None else scale
+        q = np.abs(self.q[:live].astype(np.float64))
+        kmax = float(np.abs(self.k).max())
+        s = sc * q.sum(-1, keepdims=True) * kmax  # at least every |s| and every sum of magnitudes
+        e = s * (self.hd / 8 + 8 + 4) * 2.0 ** -24 + 2.0 ** -22
+        if not self.f16:
+            e = e + sc * q.max(-1, keepdims=True) * 2.0 ** -21 * kmax * self.hd
+        sums = (max(self.kv_len, default=0) / 16 + 40) * 2.0 ** -24
+        w = 2.0 ** -11 + 2.0 ** -31 * max(self.kv_len, default=0) if self.f16 else 2.0 ** -21
+        bar = (np.expm1(2 * e) + w + sums) * size + (2.0 ** -11 * np.abs(out) * 1.01 + 2.0 ** -25 if self.f16 else 0)
+        off = np.abs(got - out)
+        assert np.all(off <= bar), float(np.nanmax(off / np.maximum(bar, 1e-300)))
+
+
+HEADS = [(4, 2, 64, 16), (32, 8, 128, 64), (6, 6, 128, 16), (14, 2, 64, 32), (4, 1, 256, 128), (10, 2, 256, 16),
+         (40, 1, 64, 256)]
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("nq,nkv,hd,block", HEADS)
+@pytest.mark.parametrize("ctx", [0, 1, 15, 16, 31, 63, 64, 127, 128, 300])
+def test_one_new_token(gpu, nq, nkv, hd, block, ctx, f16):
+    Case([(1, ctx)], nq, nkv, hd, block, f16, ctx).check(gpu)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("nq,nkv,hd,block", HEADS)
+@pytest.mark.parametrize("seqs", [[(1, 70), (0, 50), (1, 0), (1, 513), (0, 0), (2, 33)], [(5, 95), (3, 200), (7, 0)],
+                                  [(1, 5)] * 9 + [(1, 900)]])
+def test_decode_batches(gpu, nq, nkv, hd, block, seqs, f16):
+    Case(seqs, nq, nkv, hd, block, f16, len(seqs), extra_rows=3).check(gpu, pad=8, stride=70)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("nq,nkv,hd,block", HEADS)
+@pytest.mark.parametrize("seqs", [[(130, 0)], [(65, 3), (1, 80), (0, 9), (97, 131)], [(64, 64), (200, 100)]])
+def test_prompts(gpu, nq, nkv, hd, block, seqs, f16):
+    Case(seqs, nq, nkv, hd, block, f16, 1 + len(seqs), extra_rows=2).check(gpu, pad=16)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("seqs", [[(1, 400), (3, 77), (2, 0)], [(90, 0), (70, 150)]])
+@pytest.mark.parametrize("window", [1, 2, 17, 64, 100, 5000])
+def test_windows(gpu, seqs, window, f16):
+    Case(seqs, 4, 2, 128, 16, f16, window).check(gpu, window=window)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("seqs", [[(1, 4999), (1, 30)], [(40, 2500)]])
+def test_split_keys(gpu, seqs, f16):
+    """Keys over many workgroups and their join, peaked scores among them."""
+    Case(seqs, 8, 2, 128, 32, f16, 5).check(gpu)
+    Case(seqs, 8, 2, 64, 32, f16, 6, spread=4.0).check(gpu, scale=0.5)
+    Case(seqs, 2, 1, 256, 16, f16, 7).check(gpu, window=1500)
+
+
+def test_many_sequences(gpu):
+    """More sequences than one search step tells apart."""
+    seqs = [(i % 3, (7 * i) % 40) for i in range(700)]
+    Case(seqs, 2, 1, 64, 16, True, 8).check(gpu)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_scores_that_grow_along_the_keys(gpu, f16):
+    """The reference moves at every step: key i has i times the same direction."""
+    for new in (1, 150):
+        c = Case([(new, 700)], 4, 1, 64, 16, f16, 9)
+        order = c.table[0, np.arange(700 + new) // 16], np.arange(700 + new) % 16
+        c.k[order[0], 0, order[1]] = (np.arange(700 + new)[:, None] / 256.0 * np.ones(64)).astype(np.float16)
+        c.q[:] = 1.0
+        c.check(gpu, scale=1.0)
+        c.q[:] = -1.0
+        c.check(gpu, scale=1.0)
+
+
+@pytest.mark.parametrize("new,ctx", [(1, 37), (3, 200), (100, 50)])
+def test_extreme_rows_fp32(gpu, new, ctx):
+    """fp32 queries past fp16's range and far below it."""
+    c = Case([(new, ctx)], 4, 2, 128, 16, False, 10)
+    c.q[:, 0] *= 1e6
+    c.q[:, 1] *= 1e-6
+    c.q[:, 2] *= 1e-30
+    c.q[0, 3, 0] = 1e5
+    c.check(gpu, scale=1e-6)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("new,ctx", [(1, 37), (5, 219), (100, 77), (300, 0)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_masked_places_never_touch_the_result(gpu, new, ctx, bad, f16):
+    """NaN and infinities in every row of the cache that no position uses, and in the last token's key and value,
+    which only that token's rows may see."""
+    c = Case([(new, ctx), (new, ctx)], 4, 2, 64, 16, f16, 11)
+    clean = c.run(gpu)
+    used = np.zeros((c.blocks, c.block), bool)
+    for s in range(2):
+        p = np.arange(new + ctx)
+        used[c.table[s, p // 16], p % 16] = True
+    for cache in (c.k, c.v):
+        cache.transpose(0, 2, 1, 3)[~used] = bad
+    got = c.run(gpu)
+    assert np.array_equal(got, clean)
+    if new > 1:
+        last = new + ctx - 1
+        c.v[c.table[0, last // 16], 1, last % 16, 5] = bad
+        got = c.run(gpu)
+        hurt = np.zeros(got.shape, bool)
+        hurt[new - 1, 2:, 5] = True  # kv head 1's query heads of sequence 0's last row
+        assert np.array_equal(got[~hurt], clean[~hurt]) and not np.isfinite(got[hurt]).any()
+        c.k[c.table[0, last // 16], 0, last % 16, 3] = np.nan
+        got = c.run(gpu)
+        hurt[new - 1, :2] = True
+        assert np.array_equal(got[~hurt], clean[~hurt]) and not np.isfinite(got[hurt]).any()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_non_finite_values_that_all_rows_see(gpu, f16):
+    for new in (1, 80):
+        c = Case([(new, 300)], 2, 1, 64, 16, f16, 12)
+        c.v[c.table[0, 3], 0, 5, 9] = np.inf
+        got = c.run(gpu)
+        assert not np.isfinite(got[:, :, 9]).any()
+        got[:, :, 9] = 0
+        assert np.isfinite(got).all()
+        c = Case([(new, 300)], 2, 1, 64, 16, f16, 12)
+        c.q[new - 1, 1, 0] = np.nan
+        got = c.run(gpu)
+        assert np.isnan(got[new - 1, 1]).all()
+        got[new - 1, 1] = 0
+        assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("block", [16, 64])
+def test_absent_pages_are_not_attended_to(gpu, block, f16):
+    for new, ctx in ((1, 200), (3, 150), (90, 210)):
+        c = Case([(new, ctx), (new, ctx)], 4, 2, 64, block, f16, 13)
+        c.table[0, 0] = -1
+        c.table[0, 2] = c.blocks
+        c.table[1, :] = 2 ** 31 - 1  # nothing left: zeros
+        c.check(gpu)
+        assert not c.run(gpu)[new:2 * new].any()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_lengths_the_table_does_not_reach(gpu, f16):
+    """Positions past max_blocks pages are not attended to; kv_len below the new tokens leaves rows without keys."""
+    c = Case([(1, 100), (2, 90)], 2, 1, 64, 16, f16, 14, max_blocks=4)
+    c.check(gpu)
+    c = Case([(6, 0), (70, 10)], 2, 1, 64, 16, f16, 15)
+    c.kv_len[:] = (3, 40)
+    c.check(gpu)
+    c.kv_len[:] = (0, -5)
+    assert not c.run(gpu)[:76].any()
+
+
+def test_starts_out_of_range_stay_inside_the_rows(gpu):
+    """q_start past the batch's rows or decreasing: whatever the rows hold, nothing outside them is written."""
+    c = Case([(2, 20), (3, 20)], 2, 1, 64, 16, True, 16)
+    for start in ([0, 2, 400], [-9, 2, 5], [0, 5, 2], [7, 7, 7]):
+        c.q_start = np.array(start, np.int32)
+        c.run(gpu, pad=8)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_in_place(gpu, f16):
+    """out = q."""
+    for seqs in ([(1, 300), (2, 5)], [(140, 33)]):
+        c = Case(seqs, 4, 2, 128, 16, f16, 17)
+        want = c.run(gpu)
+        bits = np.uint16 if f16 else np.uint32
+        Q = gpu.DeviceBuffer.from_array(c.q.view(bits))
+        batch = gpu.PagedBatch(len(seqs), c.rows, c.width, i32(gpu, c.q_start), i32(gpu, c.kv_len), i32(gpu, c.table))
+        cache = gpu.PagedCache(gpu.DeviceBuffer.from_array(c.k.view(np.uint16)),
+                               gpu.DeviceBuffer.from_array(c.v.view(np.uint16)), c.blocks, 16, 2, 128)
+        gpu.paged_attention(batch, cache, Q, 1 if f16 else 0, 512, 4, Q, 512,
+                            gpu.paged_attention_workspace(batch, cache, 4))
+        gpu.synchronize()
+        assert np.array_equal(Q.download(bits).reshape(-1), want.view(bits).reshape(-1))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_same_result_every_time_and_from_a_graph(gpu, f16):
+    """Captured once, replayed as the lengths grow; each replay has the bits of an eager call."""
+    c = Case([(1, 40), (1, 700)], 8, 2, 128, 16, f16, 18, max_blocks=60)
+    free = [b for b in range(c.blocks) if b not in c.table]
+    c.table[0, 3], c.table[1, 44] = free[0], free[1]  # pages for the positions to come
+    bits, size = (np.uint16, 2) if f16 else (np.uint32, 4)
+    KV = i32(gpu, c.kv_len)
+    batch = gpu.PagedBatch(2, 2, c.width, i32(gpu, c.q_start), KV, i32(gpu, c.table))
+    cache = gpu.PagedCache(gpu.DeviceBuffer.from_array(c.k.view(np.uint16)),
+                           gpu.DeviceBuffer.from_array(c.v.view(np.uint16)), c.blocks, 16, 2, 128)
+    Q = gpu.DeviceBuffer.from_array(c.q.view(bits))
+    O, E = gpu.DeviceBuffer(2 * 1024 * size), gpu.DeviceBuffer(2 * 1024 * size)
+    ws = gpu.paged_attention_workspace(batch, cache, 8)
+    stream = gpu.Stream()
+    call = lambda out, s: gpu.paged_attention(batch, cache, Q, 1 if f16 else 0, 1024, 8, out, 1024, ws, stream=s)  # noqa: E731
+    graph = gpu.Graph(stream, lambda: call(O, stream))
+    for step in range(12):
+        KV.upload(c.kv_len + step)
+        graph.launch(stream)
+        stream.synchronize()
+        call(E, stream)
+        stream.synchronize()
+        assert np.array_equal(O.download(bits), E.download(bits))
+    graph.close()
+
+
+def test_offsets_past_4_gib(gpu):
+    """A cache of more than 2^32 bytes per tensor: pages at its end give what the same pages at its start give."""
+    nkv, hd, block, blocks = 8, 128, 128, 17000
+    c = Case([(2, 300), (70, 100)], 16, nkv, hd, block, True, 19)
+    want = c.run(gpu)
+    K, V = gpu.DeviceBuffer(2 * blocks * nkv * block * hd), gpu.DeviceBuffer(2 * blocks * nkv * block * hd)
+    assert K.nbytes > 1 << 32
+    page = 2 * nkv * block * hd
+    for buf, src in ((K, c.k), (V, c.v)):
+        small = gpu.DeviceBuffer.from_array(src.view(np.uint16))
+        at = (blocks - c.blocks) * page
+        gpu._hip(gpu.lib().hip.hipMemcpy(buf.ptr + at, small.ptr, small.nbytes, 3), "hipMemcpy")
+    batch = gpu.PagedBatch(2, 72, c.width, i32(gpu, c.q_start), i32(gpu, c.kv_len),
+                           i32(gpu, np.where(c.table < 0, -1, c.table + blocks - c.blocks)))
+    cache = gpu.PagedCache(K, V, blocks, block, nkv, hd)
+    Q, O = gpu.DeviceBuffer.from_array(c.q.view(np.uint16)), gpu.DeviceBuffer(c.q.nbytes)
+    gpu.paged_attention(batch, cache, Q, 1, 16 * hd, 16, O, 16 * hd, gpu.paged_attention_workspace(batch, cache, 16))
+    gpu.synchronize()
+    assert np.array_equal(O.download(np.uint16).reshape(-1), want.view(np.uint16).reshape(-1))

@@ -101,3 +101,47 @@ def test_the_last_error_names_the_call():
         rqmv._check(rqmv.lib().lib.rqmv_qk_norm_rope(None, rqmv.byref(cache().struct), *([None, 0, 0, 0, None, None, 0.0,
                                                      None, 0, 0, None, 0, 0, None])), "rqmv_qk_norm_rope")
     assert np.int32(rqmv.PLAN_LENGTH | rqmv.PLAN_TOKENS | rqmv.PLAN_POOL) == 7
+
+
+def attend(b=None, c=None, **kw):
+    a = dict(q=A, dtype=0, ldq=256, q_heads=4, out=A, ldo=256, workspace=A)
+    a.update(kw)
+    rqmv.paged_attention(b or batch(), c or cache(), **a)
+
+
+@pytest.mark.parametrize("kw", BAD_CACHES + [dict(kv=0), dict(hd=32), dict(hd=96), dict(k=None), dict(v=At(24))])
+def test_paged_attention_refuses_caches(kw):
+    refused(attend, c=cache(**kw))
+    refused(rqmv.paged_attention_workspace_size, batch(), cache(**kw), 4)
+
+
+@pytest.mark.parametrize("kw", BAD_BATCHES + BAD_TABLES)
+def test_paged_attention_refuses_batches(kw):
+    refused(attend, b=batch(**kw))
+    refused(rqmv.paged_attention_workspace_size, batch(**kw), cache(), 4)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q=At(None)), dict(out=At(None)), dict(dtype=2), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
+    dict(scale=float("inf")), dict(window=-1), dict(q_heads=3), dict(q_heads=0), dict(q_heads=1026)])
+def test_paged_attention_refuses_arguments(kw):
+    refused(attend, **kw)
+
+
+def test_paged_attention_refuses_grids_it_cannot_launch():
+    refused(attend, b=batch(tokens=1 << 20), q_heads=512, ldq=512 * 64, ldo=512 * 64)
+    refused(rqmv.paged_attention_workspace_size, batch(tokens=1 << 20, seqs=8192), cache(kv=1024), 1024)
+
+
+def test_a_call_without_a_device_is_an_error():
+    """Past the checks of its arguments the call needs a device that rqmv_init has prepared."""
+    import subprocess
+    import sys
+
+    code = ("import sys; sys.path[:0] = %r\n"
+            "import rqmv, tests.test_paged_refusals as t\n"
+            "try:\n    rqmv.paged_attention_workspace_size(t.batch(), t.cache(), 4)\n"
+            "except rqmv.RqmvError as e:\n    print('raised', e)\n" % sys.path)
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120,
+                         env={**__import__("os").environ, "HIP_VISIBLE_DEVICES": ""})
+    assert "raised" in out.stdout and "(-1)" not in out.stdout, out.stdout + out.stderr
