@@ -380,6 +380,30 @@ int rqmv_silu_mul(const float* gate_up, int n, float* out, void* stream);
 int rqmv_argmax_workspace_size(size_t* bytes);
 int rqmv_argmax(const float* values, int n, int* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The next tokens of `rows` rows of n logits (row r at logits + r * ld): for each
+ * row, with its own temperature, top_k, top_p and min_p (device arrays of `rows`
+ * values; NULL: 1, off, off, off) and a given random number u in [0, 1),
+ *   the candidates (logits above -infinity, no NaNs) in descending order, the
+ *   lowest index first among equals, have e = exp((logit - largest) / temperature);
+ *   the first top_k are kept (top_k <= 0 or >= n: all); of these the shortest
+ *   prefix whose sum of e is at least top_p times theirs, one candidate at least
+ *   (top_p outside [0, 1): all); of these those with e >= min_p (min_p <= 0: all,
+ *   above 1 as 1);
+ *   tokens[r] is the candidate at which the running sum of e in that order first
+ *   exceeds u times the kept sum (u < 0 or NaN as 0, u >= 1 the last one), and
+ *   probs[r] (probs may be NULL) its e over the kept sum.
+ * temperature <= 0 (or NaN): the first candidate, with probability 1 (rqmv_argmax's
+ * choice). A row without candidates gives -1, with probability 0. Sums are exact sums
+ * of e in units of 2^-42, so a row's token does not depend on the other rows or on
+ * scheduling. n is at most 2^20, rows at most 2^20. The workspace is 16-byte aligned
+ * (rqmv_sample_workspace_size bytes on the current device; 0: may be NULL); calls
+ * sharing it must not overlap. No counterpart in the reference's kernels (its driver
+ * samples on the host, recipe.rs:20286-20296). */
+int rqmv_sample_workspace_size(int rows, int n, size_t* bytes);
+int rqmv_sample(const float* logits, int rows, int n, int64_t ld, const float* u, const float* temperature,
+                const int* top_k, const float* top_p, const float* min_p, int* tokens, float* probs, void* workspace,
+                size_t workspace_bytes, void* stream);
+
 /* out = table[token mod rows] (rows x n fp32): the next token's embedding. */
 int rqmv_embed_row(const float* table, int rows, int n, const int* token, float* out, void* stream);
 

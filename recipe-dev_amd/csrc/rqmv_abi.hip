@@ -17,6 +17,7 @@
 #include "paged.h"
 #include "repack.h"
 #include "requant.h"
+#include "sample.h"
 
 struct rqmv_weight {
     int fmt;
@@ -972,6 +973,38 @@ int rqmv_argmax(const float* values, int n, int* out, void* workspace, size_t wo
     if (workspace_bytes < rq::argmax_workspace_bytes()) return fail(RQMV_EINVAL, "argmax: workspace too small");
     hipError_t e = rq::launch_argmax(values, n, out, workspace, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? RQMV_OK : hip_fail(e, "argmax launch");
+}
+
+static int sample_check(int rows, int n, DeviceInfo* info) {
+    if (rows <= 0 || rows > (1 << 20) || n <= 0 || n > rq::kSampleMaxN)
+        return fail(RQMV_EINVAL, "sample: rows and n must be 1..2^20");
+    const int dev = current_device(info);
+    return dev < 0 ? dev : RQMV_OK;
+}
+
+int rqmv_sample_workspace_size(int rows, int n, size_t* bytes) {
+    if (!bytes) return fail(RQMV_EINVAL, "sample: NULL size");
+    DeviceInfo info;
+    const int rc = sample_check(rows, n, &info);
+    if (rc != RQMV_OK) return rc;
+    *bytes = rq::sample_workspace(rows, n, info.cus);
+    return RQMV_OK;
+}
+
+int rqmv_sample(const float* logits, int rows, int n, int64_t ld, const float* u, const float* temperature,
+                const int* top_k, const float* top_p, const float* min_p, int* tokens, float* probs, void* workspace,
+                size_t workspace_bytes, void* stream) {
+    if (!logits || !u || !tokens) return fail(RQMV_EINVAL, "sample: bad arguments");
+    if (rows > 1 && (ld < n || ld > kPagedMaxStride)) return fail(RQMV_EINVAL, "sample: ld must be at least n");
+    DeviceInfo info;
+    const int rc = sample_check(rows, n, &info);
+    if (rc != RQMV_OK) return rc;
+    if ((uintptr_t)workspace & 15) return fail(RQMV_EINVAL, "sample: the workspace must be 16-byte aligned");
+    const size_t need = rq::sample_workspace(rows, n, info.cus);
+    if (workspace_bytes < need || (need && !workspace)) return fail(RQMV_EINVAL, "sample: workspace too small");
+    const rq::SampleArgs a{logits, ld, rows, n, u, temperature, top_k, top_p, min_p, tokens, probs};
+    hipError_t e = rq::launch_sample(a, workspace, info.cus, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? RQMV_OK : hip_fail(e, "sample launch");
 }
 
 int rqmv_embed_row(const float* table, int rows, int n, const int* token, float* out, void* stream) {

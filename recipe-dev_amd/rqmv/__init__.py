@@ -102,6 +102,9 @@ class _Lib:
         L.rqmv_paged_attention_workspace_size.argtypes = [c_void_p, c_void_p, c_int, POINTER(c_size_t)]
         L.rqmv_paged_attention.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_float, c_int, c_void_p,
                                            c_size_t, c_void_p, c_int64, c_void_p]
+        L.rqmv_sample_workspace_size.argtypes = [c_int, c_int, POINTER(c_size_t)]
+        L.rqmv_sample.argtypes = [c_void_p, c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
         L.rqmv_glu_weight_create.argtypes = [c_int, c_int64, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]
         L.rqmv_matvec_fused.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
         L.rqmv_layout_bytes.argtypes = [c_int, c_int64, c_int64, POINTER(c_size_t)]
@@ -758,6 +761,25 @@ def paged_attention(batch: PagedBatch, cache: PagedCache, q, dtype: int, ldq: in
                                           cache.head_dim ** -0.5 if scale is None else scale, window, _p(workspace),
                                           workspace.nbytes if workspace is not None else 0, out.ptr, ldo, _sh(stream)),
            "rqmv_paged_attention")
+
+
+def sample_workspace_size(rows: int, n: int) -> int:
+    size = c_size_t()
+    _check(lib().lib.rqmv_sample_workspace_size(rows, n, byref(size)), "rqmv_sample_workspace_size")
+    return size.value
+
+
+def sample_workspace(rows: int, n: int) -> DeviceBuffer:
+    return DeviceBuffer(sample_workspace_size(rows, n))
+
+
+def sample(logits, rows: int, n: int, ld: int, u, tokens, workspace=None, temperature=None, top_k=None, top_p=None,
+           min_p=None, prob=None, stream: Stream | None = None):
+    """The next token of each row of logits from given random numbers u, with the
+    rows' own settings (rqmv_sample)."""
+    _check(lib().lib.rqmv_sample(logits.ptr, rows, n, ld, u.ptr, _p(temperature), _p(top_k), _p(top_p), _p(min_p),
+                                 tokens.ptr, _p(prob), _p(workspace), workspace.nbytes if workspace is not None else 0,
+                                 _sh(stream)), "rqmv_sample")
 
 
 # ------------------------------------------------------- fused products ----

@@ -1,0 +1,172 @@
+"""GPU parity of rqmv_sample against the definition in oracle/paged.py.
+
+Tokens are whole numbers and equal: the reference sums f64 exponentials
+exactly, the library their roundings to 2^-42, and the draws here lie further
+than n * 2^-42 of the largest from every border (checked on the host; rows
+whose border is exact, equal logits, agree by construction). The probability is one
+f64 quotient of such sums rounded to fp32: 2^-24 of it, and 2^-42 n of the sums.
+"""
+import numpy as np
+import pytest
+
+from oracle import paged as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def buf(gpu, a, dt):
+    return None if a is None else gpu.DeviceBuffer.from_array(np.ascontiguousarray(a, dtype=dt))
+
+
+def run(gpu, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, ld=None, offset=0, ws=None):
+    m, n = logits.shape
+    ld = ld or n
+    wide = np.full(m * ld + offset, 1e30, np.float32)  # (larger than any logit: reading past a row would show)
+    for r in range(m):
+        wide[offset + r * ld:offset + r * ld + n] = logits[r]
+    L = gpu.DeviceBuffer.from_array(wide)
+    T, P = buf(gpu, np.full(m, -9), np.int32), buf(gpu, np.full(m, -9), np.float32)
+    gpu.sample(L.view(4 * offset, 4 * m * ld), m, n, ld, buf(gpu, u, np.float32), T, ws or gpu.sample_workspace(m, n),
+               buf(gpu, temperature, np.float32), buf(gpu, top_k, np.int32), buf(gpu, top_p, np.float32),
+               buf(gpu, min_p, np.float32), P)
+    gpu.synchronize()
+    return T.download(np.int32), P.download(np.float32)
+
+
+def check(gpu, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, **kw):
+    m, n = logits.shape
+    tok, prob = run(gpu, logits, u, temperature, top_k, top_p, min_p, **kw)
+    at = lambda a, r, d: d if a is None else a[r]  # noqa: E731
+    for r in range(m):
+        t, p = ref.sample(logits[r], np.float32(u[r]), np.float32(at(temperature, r, 1.0)), int(at(top_k, r, 0)),
+                          np.float32(at(top_p, r, 1.0)), np.float32(at(min_p, r, 0.0)))
+        assert tok[r] == t, (r, tok[r], t)
+        assert abs(prob[r] - p) <= 2.0 ** -24 * p + 2.0 ** -42 * n, r
+
+
+def settings(rng, m):
+    return {"temperature": rng.choice([0.0, 0.3, 0.7, 1.0, 1.5, 5.0], m), "top_k": rng.choice([0, 1, 2, 7, 50, 400], m),
+            "top_p": rng.choice([0.0, 0.1, 0.5, 0.9, 0.99, 1.0, 2.0], m), "min_p": rng.choice([0.0, 0.0, 0.02, 0.3, 1.0], m)}
+
+
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 1000, 4099, 32000])
+@pytest.mark.parametrize("m,spread", [(1, 3.0), (24, 3.0), (24, 0.3), (5, 30.0)])
+def test_sample(gpu, n, m, spread):
+    rng = np.random.default_rng(n + m)
+    logits = (rng.standard_normal((m, n)) * spread).astype(np.float32)
+    check(gpu, logits, rng.random(m), **settings(rng, m))
+    check(gpu, logits, rng.random(m), ld=n + 3, offset=1)  # all settings off, rows at odd places
+
+
+@pytest.mark.parametrize("spread", [0.01, 2.0, 8.0])
+def test_large_vocabulary(gpu, spread):
+    rng = np.random.default_rng(5)
+    logits = (rng.standard_normal((9, 128256)) * spread).astype(np.float32)
+    check(gpu, logits, rng.random(9), temperature=[0, 1, 1, 1, 0.5, 2, 1, 1, 1], top_k=[0, 0, 50, 0, 5000, 0, 0, 100000, 1],
+          top_p=[1, 1, 1, 0.9, 0.5, 0.999, 1, 0.7, 1], min_p=[0, 0, 0, 0, 0, 0, 0.001, 0, 0])
+
+
+def test_largest_rows(gpu):
+    """2^20 logits of one value: every candidate the same, the sums at their largest; and one more row count."""
+    n = 1 << 20
+    logits = np.full((2, n), 3.25, np.float32)
+    tok, prob = run(gpu, logits, [0.75, 0.5 ** 20], top_p=[0.5, 1.0])
+    assert list(tok) == [int(0.75 * (n // 2)), 1]
+    assert prob[0] == 2.0 / n and prob[1] == 1.0 / n
+
+
+@pytest.mark.parametrize("step", [0.25, 4.0])
+def test_ties(gpu, step):
+    """Few distinct values, so that every border falls among equals."""
+    rng = np.random.default_rng(7)
+    logits = (np.round(rng.standard_normal((40, 999)) / step) * step).astype(np.float32)
+    check(gpu, logits, rng.random(40), **settings(rng, 40))
+
+
+def test_exact_borders(gpu):
+    """Equal logits: u and top_p at whole fractions, where the running sum meets the target exactly."""
+    logits = np.zeros((8, 8), np.float32)
+    logits[:, ::2] = -0.0  # the same value as +0
+    tok, prob = run(gpu, logits, [0.0, 0.125, 0.5, 0.875, 0.0, 0.5, 0.75, 0.5], top_p=[1, 1, 1, 1, 0.5, 0.5, 0.5, 0.25],
+                    top_k=[0, 0, 0, 0, 0, 0, 0, 4])
+    assert list(tok) == [0, 1, 4, 7, 0, 2, 3, 0]
+    assert list(prob) == [0.125] * 4 + [0.25] * 3 + [1.0]
+
+
+def test_masked_logits(gpu):
+    """-infinity, the type's lowest value, NaN and +infinity among the logits; rows with nothing left."""
+    rng = np.random.default_rng(8)
+    low = np.finfo(np.float32).min
+    logits = rng.standard_normal((9, 300)).astype(np.float32)
+    logits[0, ::2] = -np.inf
+    logits[1, 1::2] = low
+    logits[2, 5:] = np.nan
+    logits[3, 7] = logits[3, 200] = np.inf
+    logits[4, :] = low
+    logits[5, :] = -np.inf
+    logits[6, :] = np.nan
+    logits[7, :] = -np.inf
+    logits[7, 299] = low
+    logits[8, :200] = low
+    u = [0.3, 0.9, 0.99, 0.6, 0.5, 0.5, 0.5, 0.5, 0.5]
+    for t in (1.0, 0.0, 1e-30, 1e30):
+        for kw in ({}, {"top_k": [3] * 9}, {"top_p": [0.5] * 9}, {"min_p": [0.5] * 9}):
+            check(gpu, logits, u, temperature=[t] * 9, **kw)
+    tok, prob = run(gpu, logits, u)
+    assert tok[5] == tok[6] == -1 and prob[5] == prob[6] == 0 and tok[7] == 299 and tok[3] == 200
+
+
+def test_settings_out_of_range(gpu):
+    """Settings that switch a step off, or that are brought into range."""
+    rng = np.random.default_rng(9)
+    logits = (rng.standard_normal((12, 500)) * 2).astype(np.float32)
+    nan = np.nan
+    check(gpu, logits, [0.1, 0.2, 0.3, 0.4, 0.5, 0.6, 0.7, 0.8, 0.9, -1.0, 1.0, nan],
+          temperature=[nan, -1, 1, 1, 1, 1, 1, 1, np.inf, 1, 1, 1], top_k=[5, 5, -3, 10 ** 9, 500, 0, 0, 0, 0, 0, 0, 0],
+          top_p=[1, 1, 1, 1, 1, -0.5, nan, 1.5, 1, 1, 0.5, 1], min_p=[0, 0, 0, 0, nan, -1, 0, 2, 0, 0, 0, 0])
+
+
+def test_temperature_zero_is_argmax(gpu):
+    rng = np.random.default_rng(10)
+    logits = rng.standard_normal((3, 70001)).astype(np.float32)
+    logits[1, 69000] = logits[1, 123] = 9.0
+    tok, prob = run(gpu, logits, [0.9] * 3, temperature=[0] * 3)
+    assert list(tok) == [int(np.argmax(r)) for r in logits] and list(prob) == [1.0] * 3
+
+
+def test_draws_follow_the_probabilities(gpu):
+    """u over an even grid: each token comes as often as its probability says, within one grid step at each end."""
+    rng = np.random.default_rng(11)
+    row = (rng.standard_normal(40) * 1.5).astype(np.float32)
+    m = 4096
+    tok, prob = run(gpu, np.tile(row, (m, 1)), (np.arange(m) + 0.5) / m, temperature=[0.8] * m)
+    p = np.exp(row.astype(np.float64) / np.float64(np.float32(0.8)))
+    p /= p.sum()
+    assert np.all(np.abs(np.bincount(tok, minlength=40) / m - p) <= 1.0 / m + 1e-9)
+    assert np.allclose(prob, p[tok], rtol=2.0 ** -23, atol=0)
+
+
+def test_replayed_from_a_graph(gpu):
+    """Captured once; each replay has the logits and numbers that it finds, on the workspace that eager calls use too."""
+    rng = np.random.default_rng(12)
+    m, n = 6, 40000
+    L, U = gpu.DeviceBuffer(4 * m * n), gpu.DeviceBuffer(4 * m)
+    T, K, P = buf(gpu, np.zeros(m), np.int32), buf(gpu, [0, 0, 50, 50, 0, 0], np.int32), gpu.DeviceBuffer(4 * m)
+    top_p = buf(gpu, [1, 0.9, 1, 0.9, 0.5, 1], np.float32)
+    ws = gpu.sample_workspace(m, n)
+    stream = gpu.Stream()
+    graph = gpu.Graph(stream, lambda: gpu.sample(L, m, n, n, U, T, ws, None, K, top_p, None, P, stream))
+    for i in range(4):
+        logits = (rng.standard_normal((m, n)) * (0.2 + 2 * i)).astype(np.float32)
+        u = rng.random(m).astype(np.float32)
+        L.upload(logits)
+        U.upload(u)
+        graph.launch(stream)
+        stream.synchronize()
+        got = T.download(np.int32), P.download(np.float32)
+        eager = run(gpu, logits, u, None, [0, 0, 50, 50, 0, 0], [1, 0.9, 1, 0.9, 0.5, 1], None, ws=ws)
+        assert np.array_equal(got[0], eager[0]) and np.array_equal(got[1], eager[1])
+        for r in range(m):
+            assert got[0][r] == ref.sample(logits[r], u[r], 1.0, [0, 0, 50, 50, 0, 0][r],
+                                           np.float32([1, 0.9, 1, 0.9, 0.5, 1][r]))[0]
+    graph.close()

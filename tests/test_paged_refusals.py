@@ -145,3 +145,14 @@ def test_a_call_without_a_device_is_an_error():
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120,
                          env={**__import__("os").environ, "HIP_VISIBLE_DEVICES": ""})
     assert "raised" in out.stdout and "(-1)" not in out.stdout, out.stdout + out.stderr
+
+
+@pytest.mark.parametrize("kw", [dict(logits=At(None)), dict(u=At(None)), dict(tokens=At(None)), dict(rows=0),
+                                dict(rows=(1 << 20) + 1), dict(n=0), dict(n=(1 << 20) + 1), dict(ld=99), dict(rows=-1),
+                                dict(ld=1 << 41)])
+def test_sample_refuses_arguments(kw):
+    a = dict(logits=A, rows=2, n=100, ld=100, u=A, tokens=A, workspace=A)
+    a.update(kw)
+    refused(rqmv.sample, **a)
+    if set(kw) & {"rows", "n"}:
+        refused(rqmv.sample_workspace_size, a["rows"], a["n"])
