@@ -77,20 +77,27 @@ struct Tile {
     int all_from, all_to;    // every row sees keys all_from..all_to-1
 };
 
-// Largest s with floor(q_start[s] * group / TM) + s <= number, 64 candidates at a time.
-template <int TM>
-__device__ __forceinline__ int find_seq(const PagedBatch& b, int group, int number) {
+// The last sequence s for which at_most(s) holds (it holds up to some s >= 0), 64 candidates at a time.
+template <typename F>
+__device__ __forceinline__ int last_seq(int seqs, F at_most) {
     const int lane = threadIdx.x & 63;
-    int lo = 0, n = b.seqs;
+    int lo = 0, n = seqs;
     while (n > 1) {
         const int step = (n + 63) >> 6, i = lane * step;
-        bool le = false;
-        if (i < n) le = min(max(b.q_start[lo + i], 0), b.tokens) * group / TM + lo + i <= number;
-        const int c = max((int)__popcll(__ballot(le)), 1) - 1;
+        const int c = max((int)__popcll(__ballot(i < n && at_most(lo + min(i, n - 1)))), 1) - 1;
         lo += c * step;
         n = min(step, n - c * step);
     }
     return __builtin_amdgcn_readfirstlane(lo);
+}
+__device__ __forceinline__ int start_of(const PagedBatch& b, int s) { return min(max(b.q_start[s], 0), b.tokens); }
+// Of tile `number`: floor(q_start[s] * group / TM) + s <= number.
+template <int TM>
+__device__ __forceinline__ int find_seq(const PagedBatch& b, int group, int number) {
+    return last_seq(b.seqs, [&](int s) { return start_of(b, s) * group / TM + s <= number; });
+}
+__device__ __forceinline__ int find_seq_of_token(const PagedBatch& b, int token) {
+    return last_seq(b.seqs, [&](int s) { return b.q_start[s] <= token; });
 }
 
 // Row starts and lengths are read as they are found and brought into range.
@@ -98,7 +105,7 @@ template <int TM>
 __device__ __forceinline__ Tile make_tile(const AttnArgs& a, int seq, int row0) {
     Tile t;
     t.seq = seq;
-    t.token0 = min(max(a.b.q_start[seq], 0), a.b.tokens);
+    t.token0 = start_of(a.b, seq);
     t.n = min(max(a.b.q_start[seq + 1], t.token0), a.b.tokens) - t.token0;
     t.kv = max(a.b.kv_len[seq], 0);
     t.row0 = row0;
@@ -249,6 +256,19 @@ __device__ __forceinline__ void load_rows(const AttnArgs& a, const Tile& t, int 
     }
 }
 
+// The queries are in their registers from here on: without this the compiler waits
+// for their loads at their first use in the loop, in every step, and so for the
+// step's own loads behind them.
+template <int HD, int QT, bool F32>
+__device__ __forceinline__ void arrived(Rows<HD, QT, F32>& w) {
+#pragma unroll
+    for (int i = 0; i < QT; ++i)
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+            for (int p = 0; p < Rows<HD, QT, F32>::QP; ++p) asm volatile("" : "+v"(w.q[i][k][p]));
+}
+
 // S^T of 32 KT keys: s[i][t] holds, per lane, query lane % 32 of row tile i and
 // keys 32 t + 8 (e / 4) + 4 h + e % 4.
 template <int HD, int QT, int KT, bool F32>
@@ -275,37 +295,55 @@ __device__ __forceinline__ void scores(const char* K, const Rows<HD, QT, F32>& w
         }
 }
 
+// -infinity for the keys that a row does not see.
 template <int HD, int QT, int KT, bool F32>
-__device__ __forceinline__ bool sees(const Rows<HD, QT, F32>& w, int i, int key0, int off, unsigned bad) {
-    return key0 + off <= w.hi[i] && key0 + off >= w.lo[i] && !((bad >> (off >> 4)) & 1);
-}
-
-// Scores to weights: masks, moves the references, adds up the weights and
-// rounds them to the second product's operands.
-template <int HD, int QT, int KT, bool F32>
-__device__ __forceinline__ void weights(Rows<HD, QT, F32>& w, f16_t (&s)[QT][KT], int key0, bool masked, unsigned bad,
-                                        h8_t (&p)[QT][2 * KT][F32 ? 2 : 1]) {
+__device__ __forceinline__ void mask_scores(const Rows<HD, QT, F32>& w, f16_t (&s)[QT][KT], int key0, unsigned bad) {
     const int h = (threadIdx.x & 63) >> 5;
-    constexpr float SHIFT = F32 ? 15.f : 6.f, SLACK = F32 ? 0.f : 8.f;
-    if (masked) {
-#pragma unroll
-        for (int i = 0; i < QT; ++i)
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int off = 32 * t + 8 * (e / 4) + 4 * h + e % 4;
-                    if (!sees<HD, QT, KT, F32>(w, i, key0, off, bad)) s[i][t][e] = -INFINITY;
-                }
-    }
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-        float top = s[i][0][0];
+        // keys key0 + 4 h + off with off - from <= width, unsigned (a row without keys: none)
+        const bool some = w.hi[i] >= w.lo[i];
+        const int from = some ? w.lo[i] - key0 - 4 * h : 1 << 30;
+        const unsigned width = some ? (unsigned)(w.hi[i] - w.lo[i]) : 0u;
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) top = fmaxf(top, s[i][t][e]);
-        top = swap32_max(top) * w.c[i];
+            for (int e = 0; e < 16; ++e)
+                if ((unsigned)(32 * t + 8 * (e / 4) + e % 4 - from) > width) s[i][t][e] = -INFINITY;
+    }
+    if (bad) {
+#pragma unroll
+        for (int g = 0; g < 2 * KT; ++g)
+            if ((bad >> g) & 1) {
+#pragma unroll
+                for (int i = 0; i < QT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s[i][g / 2][8 * (g % 2) + e] = -INFINITY;
+            }
+    }
+}
+
+// The rows' largest scores (NaNs apart).
+template <int QT, int KT>
+__device__ __forceinline__ void largest(const f16_t (&s)[QT][KT], float (&top)[QT]) {
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        float m = s[i][0][0];
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) m = fmaxf(m, s[i][t][e]);
+        top[i] = swap32_max(m);
+    }
+}
+
+// Moves the references to the rows' maxima where one lies more than the slack above.
+template <int HD, int QT, bool F32>
+__device__ __forceinline__ void move_references(Rows<HD, QT, F32>& w, const float (&largest)[QT]) {
+    constexpr float SLACK = F32 ? 0.f : 8.f;
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
+        const float top = largest[i] * w.c[i];
         if (__any(top > w.m[i] + SLACK)) {
             const float m = fmaxf(w.m[i], top);
             const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(w.m[i] - m);
@@ -316,6 +354,16 @@ __device__ __forceinline__ void weights(Rows<HD, QT, F32>& w, f16_t (&s)[QT][KT]
 #pragma unroll
                 for (int e = 0; e < 16; ++e) w.o[i][d][e] *= f;
         }
+    }
+}
+
+// Scores to weights, added up and rounded to the second product's operands.
+template <int HD, int QT, int KT, bool F32>
+__device__ __forceinline__ void weights(Rows<HD, QT, F32>& w, const f16_t (&s)[QT][KT],
+                                        h8_t (&p)[QT][2 * KT][F32 ? 2 : 1]) {
+    constexpr float SHIFT = F32 ? 15.f : 6.f;
+#pragma unroll
+    for (int i = 0; i < QT; ++i) {
         const float ref = w.m[i] == -INFINITY ? 0.f : w.m[i] - SHIFT;
 #pragma unroll
         for (int t = 0; t < KT; ++t)
@@ -367,13 +415,15 @@ __device__ __forceinline__ void add_values(const char* V, Rows<HD, QT, F32>& w,
 
 // fp16 pairs with an exponent of all ones leave 0x8000 bits here.
 __device__ __forceinline__ uint32_t odd_bits(uint32_t x) { return ((x & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
+__device__ __forceinline__ uint32_t even_part(uint32_t x) { return x & ~((odd_bits(x) >> 15) * 0xFFFFu); }
 
 // A step in which some row may not see some key: zeroes the values of keys that
-// no row sees (key0 + row >= end, absent pages), and returns whether a value of
-// another is NaN or infinite. `thread` of `threads` walks the tile.
+// no row sees (key0 + row >= end, absent pages) and the others' that are NaN or infinite.
+// Returns whether there are such (they come into the sums at the end, add_odd). `thread`
+// of `threads` walks the tile.
 template <int HD, int KEYS>
 __device__ __forceinline__ bool zero_dead(char* V, int key0, int end, unsigned bad, int thread, int threads) {
-    bool odd = false;
+    bool any = false;
     for (int u = thread; u < KEYS * (HD / 8); u += threads) {
         const int row = u / (HD / 8);
         uint4* at = reinterpret_cast<uint4*>(V + u * 16);
@@ -381,40 +431,43 @@ __device__ __forceinline__ bool zero_dead(char* V, int key0, int end, unsigned b
             *at = make_uint4(0, 0, 0, 0);
         } else {
             const uint4 x = *at;
-            odd |= (odd_bits(x.x) | odd_bits(x.y) | odd_bits(x.z) | odd_bits(x.w)) != 0;
+            if (odd_bits(x.x) | odd_bits(x.y) | odd_bits(x.z) | odd_bits(x.w)) {
+                any = true;
+                *at = make_uint4(even_part(x.x), even_part(x.y), even_part(x.z), even_part(x.w));
+            }
         }
     }
-    return odd;
+    return any;
 }
 
-// The rare step with such values: added to the rows that see them ...
-template <int HD, int QT, int KT, bool F32>
-__device__ __forceinline__ void add_odd(const char* V, Rows<HD, QT, F32>& w, int key0, unsigned bad) {
-    typedef Lay<HD> L;
-    const int h = (threadIdx.x & 63) >> 5;
-    for (int row = 0; row < 32 * KT; ++row)
+// The NaN and infinite values of keys from..to-1 in present pages, read from the cache, added to the
+// rows that see them: rare, after the last step (the sums are final but for the division).
+template <int HD, int QT, bool F32>
+__device__ __forceinline__ void add_odd(const AttnArgs& a, const Tile& t, int kh, int from, int to,
+                                        Rows<HD, QT, F32>& w) {
+    typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+    const int h = (threadIdx.x & 63) >> 5, shift = a.c.block_shift;
+    const int* table = a.b.table + t.seq * a.b.table_stride;
+#pragma unroll 1
+    for (int key = from; key < to; ++key) {
+        const int id = table[key >> shift];
+        if ((unsigned)id >= (unsigned)a.c.blocks) continue;
+        const _Float16* row = reinterpret_cast<const _Float16*>(a.c.v) +
+                              ((((int64_t)id * a.c.kv_heads + kh) << shift) + (key & ((1 << shift) - 1))) * HD + 4 * h;
 #pragma unroll
-        for (int i = 0; i < QT; ++i) {
-            const bool seen = sees<HD, QT, KT, F32>(w, i, key0, row, bad);
+        for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
-            for (int d = 0; d < HD / 32; ++d)
+            for (int e = 0; e < 4; ++e) {  // dims 32 d + 8 e + 4 h ..
+                const h4_t v = *reinterpret_cast<const h4_t*>(row + 32 * d + 8 * e);
+                asm volatile("" ::: "memory");  // (a read at a time: few registers)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int dim = 32 * d + 8 * (e / 4) + 4 * h + e % 4;
-                    const float v = (float)*reinterpret_cast<const _Float16*>(
-                        V + row * L::ROW + ((dim >> 3) ^ L::vx(row)) * 16 + (dim & 7) * 2);
-                    if (seen && !(fabsf(v) < INFINITY)) w.o[i][d][e] += v;
-                }
-        }
-}
-
-// ... and zeroed.
-template <int HD, int KEYS>
-__device__ __forceinline__ void zero_odd(char* V, int thread, int threads) {
-    for (int u = thread; u < KEYS * (HD / 2); u += threads) {
-        uint32_t* at = reinterpret_cast<uint32_t*>(V + u * 4);
-        const uint32_t odd = odd_bits(*at);
-        if (odd) *at &= ~(((odd >> 15) & 0x00010001u) * 0xFFFFu);
+                for (int i = 0; i < QT; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float x = (float)v[j];
+                        w.o[i][d][4 * e + j] += key >= w.lo[i] && key <= w.hi[i] && !(fabsf(x) < INFINITY) ? x : 0.f;
+                    }
+            }
     }
 }
 
@@ -447,14 +500,14 @@ __device__ __forceinline__ float reciprocal(float l) { return l == 0.f ? 0.f : 1
 // again while it works on the values and the other way round, and a second workgroup
 // on the CU fills the rest. At the end the waves' sums are joined through LDS.
 template <int HD, bool F32>
-__global__ void __launch_bounds__(256) paged_few_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnArgs a) {
     typedef Lay<HD> L;
     constexpr int TM = 32, KEYS = 32, HALF = KEYS * HD * 2;  // HALF: bytes of a wave's K (and V) buffer
     extern __shared__ __align__(16) char lds[];
     __shared__ float2 sums[4][32];
     const int kh = blockIdx.x % a.c.kv_heads, number = blockIdx.x / a.c.kv_heads, split = blockIdx.y;
     const int seq = find_seq<TM>(a.b, a.group, number);
-    const int first = min(max(a.b.q_start[seq], 0), a.b.tokens) * a.group / TM + seq;
+    const int first = start_of(a.b, seq) * a.group / TM + seq;
     const Tile t = make_tile<TM>(a, seq, (number - first) * TM);
     if (t.row0 >= t.rows) return;
     const int begin = t.first + split * t.chunk, end = min(begin + t.chunk, t.end);
@@ -465,7 +518,6 @@ __global__ void __launch_bounds__(256) paged_few_kernel(AttnArgs a) {
     const uint32_t k_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)K, v_lds = k_lds + HALF;
     Pages pages{a.b.table + seq * a.b.table_stride, a.b.max_blocks - 1, a.c.blocks, a.c.block_shift, INT_MIN / 2, 0};
     Rows<HD, 1, F32> w;
-    load_rows<HD, 1, F32>(a, t, kh, t.row0, w);
 
     int id[2], next[2];
     auto look = [&](int key0, int (&ids)[2]) {  // the page ids of keys key0.. and key0 + 16..
@@ -482,11 +534,14 @@ __global__ void __launch_bounds__(256) paged_few_kernel(AttnArgs a) {
                                                     (decltype(values)::value ? v_lds : k_lds) + g * 16 * L::ROW);
     };
     int key0 = begin + wave * KEYS;
+    bool odd = false;
     if (key0 < end) {
         look(key0, id);
         load(std::false_type{}, key0, id);
         load(std::true_type{}, key0, id);
     }
+    load_rows<HD, 1, F32>(a, t, kh, t.row0, w);
+    arrived(w);
     while (key0 < end) {
         const int after = key0 + 4 * KEYS;
         const bool more = after < end;
@@ -501,14 +556,15 @@ __global__ void __launch_bounds__(256) paged_few_kernel(AttnArgs a) {
         }
         const unsigned bad = (pages.absent(id[0]) ? 1 : 0) | (pages.absent(id[1]) ? 2 : 0);
         const bool masked = key0 < t.all_from || key0 + KEYS > t.all_to || bad;
+        if (masked) mask_scores<HD, 1, 1, F32>(w, s, key0, bad);
+        float top[1];
+        largest<1, 1>(s, top);
+        move_references<HD, 1, F32>(w, top);
         h8_t p[1][2][F32 ? 2 : 1];
-        weights<HD, 1, 1, F32>(w, s, key0, masked, bad, p);
+        weights<HD, 1, 1, F32>(w, s, p);
         if (more) wait_loads<2 * L::NI>();
         else wait_loads<0>();
-        if (masked && __any(zero_dead<HD, KEYS>(V, key0, t.end, bad, lane, 64))) {
-            add_odd<HD, 1, 1, F32>(V, w, key0, bad);
-            zero_odd<HD, KEYS>(V, lane, 64);
-        }
+        if (masked && __any(zero_dead<HD, KEYS>(V, key0, t.end, bad, lane, 64))) odd = true;
         add_values<HD, 1, 1, F32>(V, w, p);
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(w.o[0][0]) : : "memory");
@@ -518,6 +574,10 @@ __global__ void __launch_bounds__(256) paged_few_kernel(AttnArgs a) {
         key0 = after;
     }
     wait_loads<0>();
+    if (odd) {  // (the wave's own steps; unmasked ones went through whole)
+        for (int k = begin + wave * KEYS; k < end; k += 4 * KEYS)
+            if (k < t.all_from || k + KEYS > t.all_to) add_odd<HD, 1, F32>(a, t, kh, k, min(k + KEYS, t.end), w);
+    }
     // the waves' sums, each in its own LDS (32 rows of HD values, pieces XORed with the row)
     const int q = lane & 31, h = lane >> 5;
 #pragma unroll
@@ -560,44 +620,52 @@ __global__ void __launch_bounds__(256) paged_few_kernel(AttnArgs a) {
 
 // --------------------------------------------- many rows: rows over the waves ----
 
-// TM = 128 QT rows a tile (prompts, chunks of prompts): bound by the matrix
-// cores and the exponentials. Four waves of 32 QT rows share steps of 64 keys in two LDS
-// buffers, one barrier a step.
-template <int HD, int QT, bool F32>
-__global__ void __launch_bounds__(256) paged_many_kernel(AttnArgs a) {
+// TM = 32 WAVES rows a tile (prompts, chunks of prompts): bound by the matrix
+// cores and the exponentials. Each wave has 32 rows; the waves share steps of 64 keys in
+// two LDS buffers, one barrier a step. Eight waves (two per SIMD, 256 registers each), so
+// that one multiplies while the other takes exponentials; four where the sums and
+// queries need more registers.
+constexpr int many_waves(int hd) { return hd == 256 ? 4 : 8; }
+
+template <int HD, bool F32>
+__global__ void __launch_bounds__(64 * many_waves(HD), many_waves(HD) / 4) paged_many_kernel(AttnArgs a) {
     typedef Lay<HD> L;
-    constexpr int TM = 128 * QT, KEYS = 64, HALF = KEYS * HD * 2;
+    constexpr int WAVES = many_waves(HD), TM = 32 * WAVES, KEYS = 64, HALF = KEYS * HD * 2;
     extern __shared__ __align__(16) char lds[];
     // the last tiles first: of one sequence's they have the most keys
     const int kh = blockIdx.x % a.c.kv_heads, number = a.tiles - 1 - blockIdx.x / a.c.kv_heads, split = blockIdx.y;
     const int seq = find_seq<TM>(a.b, a.group, number);
-    const int first = min(max(a.b.q_start[seq], 0), a.b.tokens) * a.group / TM + seq;
+    const int first = start_of(a.b, seq) * a.group / TM + seq;
     const Tile t = make_tile<TM>(a, seq, (number - first) * TM);
     if (t.row0 >= t.rows) return;
     const int begin = t.first + split * t.chunk, end = min(begin + t.chunk, t.end);
     if (split && begin >= end) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row = t.row0 + 32 * QT * wave;
+    const int row = t.row0 + 32 * wave;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
     Pages pages{a.b.table + seq * a.b.table_stride, a.b.max_blocks - 1, a.c.blocks, a.c.block_shift, INT_MIN / 2, 0};
-    Rows<HD, QT, F32> w;
-    load_rows<HD, QT, F32>(a, t, kh, row, w);
+    Rows<HD, 1, F32> w;
 
-    // step i is in buffer i % 2; the wave loads its 16 keys of K and V. Returns which groups are absent.
+    // Step i is in buffer i % 2, keys before values. Of eight waves, four load 16 rows of
+    // keys each and four of values; of four, each loads both. Returns which groups are absent.
     auto load = [&](int key0, int buffer) -> unsigned {
         pages.need(key0 >> pages.shift, (key0 + 48) >> pages.shift);
         unsigned bad = 0;
 #pragma unroll
         for (int g = 0; g < 4; ++g) bad |= pages.absent(pages.at((key0 + 16 * g) >> pages.shift)) ? 1u << g : 0u;
-        const int key = key0 + 16 * wave, id = pages.at(key >> pages.shift);
-        const uint32_t at = lds0 + buffer * 2 * HALF + wave * 16 * L::ROW;
-        load_group<HD, false>(a.c.k, a.c, kh, pages.absent(id) ? 0 : id, key, at);
-        load_group<HD, true>(a.c.v, a.c, kh, pages.absent(id) ? 0 : id, key, at + HALF);
+        const int g = wave % 4, key = key0 + 16 * g, id = pages.at(key >> pages.shift);
+        const int page = pages.absent(id) ? 0 : id;
+        const uint32_t at = lds0 + buffer * 2 * HALF + g * 16 * L::ROW;
+        if (WAVES == 4 || wave < 4) load_group<HD, false>(a.c.k, a.c, kh, page, key, at);
+        if (WAVES == 4 || wave >= 4) load_group<HD, true>(a.c.v, a.c, kh, page, key, at + HALF);
         return bad;
     };
     unsigned bad = 0, bad_next = 0;
     int buffer = 0;
+    bool odd = false;
     if (begin < end) bad = load(begin, 0);
+    load_rows<HD, 1, F32>(a, t, kh, row, w);
+    arrived(w);
     for (int key0 = begin; key0 < end; key0 += KEYS) {
         wait_loads<0>();
         __syncthreads();  // the step is in LDS, and the other buffer is free
@@ -605,87 +673,110 @@ __global__ void __launch_bounds__(256) paged_many_kernel(AttnArgs a) {
         char* K = lds + buffer * 2 * HALF;
         char* V = K + HALF;
         const bool masked = key0 < t.all_from || key0 + KEYS > t.all_to || bad;
-        f16_t s[QT][2];
-        scores<HD, QT, 2, F32>(K, w, s);
-        h8_t p[QT][4][F32 ? 2 : 1];
-        weights<HD, QT, 2, F32>(w, s, key0, masked, bad, p);
-        if (masked && __syncthreads_or(zero_dead<HD, KEYS>(V, key0, t.end, bad, threadIdx.x, 256))) {
-            add_odd<HD, QT, 2, F32>(V, w, key0, bad);
-            __syncthreads();
-            zero_odd<HD, KEYS>(V, threadIdx.x, 256);
-            __syncthreads();
-        }
-        add_values<HD, QT, 2, F32>(V, w, p);
+        if (masked && __syncthreads_or(zero_dead<HD, KEYS>(V, key0, t.end, bad, threadIdx.x, 64 * WAVES))) odd = true;
+        f16_t s[1][2];
+        scores<HD, 1, 2, F32>(K, w, s);
+        if (masked) mask_scores<HD, 1, 2, F32>(w, s, key0, bad);
+        float top[1];
+        largest<1, 2>(s, top);
+        move_references<HD, 1, F32>(w, top);
+        h8_t p[1][4][F32 ? 2 : 1];
+        weights<HD, 1, 2, F32>(w, s, p);
+        add_values<HD, 1, 2, F32>(V, w, p);
         bad = bad_next;
         buffer ^= 1;
     }
-    const bool whole = t.live <= 1;
-    const int h = lane >> 5;
-#pragma unroll
-    for (int i = 0; i < QT; ++i) {
-        const int r = row + 32 * i + (lane & 31);
-        const float l = swap32_sum(w.l[i]);
-        const float f = whole ? reciprocal(l) : 1.f;
-        if (r >= t.rows) continue;
-        const int tok = t.token0 + r / a.group, head = kh * a.group + r % a.group;
-        if (!whole && h == 0)
-            a.ml[((int64_t)split * a.b.tokens + tok) * (a.group * a.c.kv_heads) + head] = make_float2(w.m[i], l);
-#pragma unroll
-        for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float v[4] = {w.o[i][d][4 * e] * f, w.o[i][d][4 * e + 1] * f, w.o[i][d][4 * e + 2] * f,
-                                    w.o[i][d][4 * e + 3] * f};
-                put4(a, !F32, whole, split, tok, head, HD, 32 * d + 8 * e + 4 * h, v);
-            }
+    if (odd) {
+        for (int k = begin; k < end; k += KEYS)
+            if (k < t.all_from || k + KEYS > t.all_to) add_odd<HD, 1, F32>(a, t, kh, k, min(k + KEYS, t.end), w);
     }
+    const bool whole = t.live <= 1;
+    const int h = lane >> 5, r = row + (lane & 31);
+    const float l = swap32_sum(w.l[0]);
+    const float f = whole ? reciprocal(l) : 1.f;
+    if (r >= t.rows) return;
+    const int tok = t.token0 + r / a.group, head = kh * a.group + r % a.group;
+    if (!whole && h == 0)
+        a.ml[((int64_t)split * a.b.tokens + tok) * (a.group * a.c.kv_heads) + head] = make_float2(w.m[0], l);
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float v[4] = {w.o[0][d][4 * e] * f, w.o[0][d][4 * e + 1] * f, w.o[0][d][4 * e + 2] * f,
+                                w.o[0][d][4 * e + 3] * f};
+            put4(a, !F32, whole, split, tok, head, HD, 32 * d + 8 * e + 4 * h, v);
+        }
 }
 
 // ---------------------------------------------------------- the splits' join ----
 
-// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's live splits.
+// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's live splits. A
+// workgroup per row (token, query head): HD / 4 threads take a split's 16-byte
+// columns, the other threads further splits, whose partial results are all
+// requested before it is known how many are live.
+constexpr int kMaxSplits = 64;
 template <int HD, int TM, bool F32>
 __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a) {
-    constexpr int TPR = HD / 4;  // threads per row
+    constexpr int TPR = HD / 4, SIDE = 256 / TPR, PER = kMaxSplits / SIDE;
+    __shared__ float4 part[256];
+    __shared__ float2 sums[SIDE];
     const int heads = a.group * a.c.kv_heads;
-    const int64_t unit = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-    const int token = (int)min(unit / heads, (int64_t)a.b.tokens - 1), head = (int)(unit % heads);
-    // the token's sequence: the last one that starts at or before it
-    int lo = 0, n = a.b.seqs;
-    while (n > 1) {
-        const int half = n >> 1;
-        if (a.b.q_start[lo + half] <= token) lo += half, n -= half;
-        else n = half;
-    }
-    if (unit >= (int64_t)a.b.tokens * heads) return;
-    if (token < a.b.q_start[lo] || token >= a.b.q_start[lo + 1]) return;
-    const int row = (token - a.b.q_start[lo]) * a.group + head % a.group;
-    const Tile t = make_tile<TM>(a, lo, row / TM * TM);
+    const int token = blockIdx.x / heads, head = blockIdx.x % heads;
+    const int col = threadIdx.x % TPR, side = threadIdx.x / TPR;
+    const int64_t at = (int64_t)token * heads + head, next = (int64_t)a.b.tokens * heads;
+    float4 x[PER];
+    float2 ml[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+        if (k * SIDE < a.splits) {
+            const int64_t row = at + min(side + k * SIDE, a.splits - 1) * next;
+            x[k] = *reinterpret_cast<const float4*>(a.o + row * HD + 4 * col);
+            ml[k] = a.ml[row];
+        }
+    // the token's sequence, the last one that starts at or before it
+    const int seq = find_seq_of_token(a.b, token);
+    if (token < a.b.q_start[seq] || token >= a.b.q_start[seq + 1]) return;
+    const int row = (token - a.b.q_start[seq]) * a.group + head % a.group;
+    const Tile t = make_tile<TM>(a, seq, row / TM * TM);
     if (t.live <= 1) return;
-    const int dim = 4 * (threadIdx.x % TPR);
-    float M = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-    const int64_t at = (int64_t)token * heads + head, step = (int64_t)a.b.tokens * heads;
-    for (int c = 0; c < t.live; ++c) M = fmaxf(M, a.ml[at + c * step].x);
-    for (int c = 0; c < t.live; ++c) {
-        const float2 ml = a.ml[at + c * step];
-        const float4 x = *reinterpret_cast<const float4*>(a.o + (at + c * step) * HD + dim);
-        const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml.x - M);
-        sum = fmaf(f, ml.y, sum);
-        v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
+    float m = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+        if (side + k * SIDE < t.live) m = fmaxf(m, ml[k].x);
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+        if (side + k * SIDE < t.live) {
+            const float f = ml[k].x == -INFINITY ? (ml[k].y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml[k].x - m);
+            sum = fmaf(f, ml[k].y, sum);
+            v[0] = fmaf(f, x[k].x, v[0]), v[1] = fmaf(f, x[k].y, v[1]);
+            v[2] = fmaf(f, x[k].z, v[2]), v[3] = fmaf(f, x[k].w, v[3]);
+        }
+    part[threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
+    if (col == 0) sums[side] = make_float2(m, sum);
+    __syncthreads();
+    if (side) return;
+    m = -INFINITY, sum = 0.f;
+    v[0] = v[1] = v[2] = v[3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < SIDE; ++k) m = fmaxf(m, sums[k].x);
+#pragma unroll
+    for (int k = 0; k < SIDE; ++k) {
+        const float2 s = sums[k];
+        const float4 y = part[k * TPR + col];
+        const float f = s.x == -INFINITY ? (s.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(s.x - m);
+        sum = fmaf(f, s.y, sum);
+        v[0] = fmaf(f, y.x, v[0]), v[1] = fmaf(f, y.y, v[1]), v[2] = fmaf(f, y.z, v[2]), v[3] = fmaf(f, y.w, v[3]);
     }
     const float inv = reciprocal(sum);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] *= inv;
-    put4(a, !F32, true, 0, token, head, HD, dim, v);
+    put4(a, !F32, true, 0, token, head, HD, 4 * col, v);
 }
 
 // ------------------------------------------------------------------ launches ----
 
 constexpr int few_lds(int hd) { return 4 * 2 * 32 * hd * 2; }
 constexpr int many_lds(int hd) { return 2 * 2 * 64 * hd * 2; }
-// 32-row tiles per wave of the many-rows form: the output sums and queries of two fit the
-// registers up to 128 dims of fp16 rows
-constexpr int many_qt(int hd, bool f32) { return hd == 256 || (hd == 128 && f32) ? 1 : 2; }
 
 struct AttnPlan {
     bool few;
@@ -696,37 +787,35 @@ struct AttnPlan {
 AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus) {
     AttnPlan p;
     p.few = (int64_t)tokens * group <= (int64_t)32 * seqs;
-    p.tm = p.few ? 32 : 128 * many_qt(hd, f32);
+    p.tm = p.few ? 32 : 32 * many_waves(hd);
     p.tiles = (int64_t)tokens * group / p.tm + seqs;
     p.min_chunk = p.few ? 128 : 512;
     const int64_t wgs = p.tiles * kv_heads, want = p.few ? 2 * cus : cus;
     int64_t s = wgs >= want ? 1 : (want + wgs - 1) / wgs;
     const int64_t most = (cap + p.min_chunk - 1) / p.min_chunk;
     if (s > most) s = most;
-    if (s > 64) s = 64;
+    if (s > kMaxSplits) s = kMaxSplits;
     p.splits = (int)(s < 1 ? 1 : s);
     return p;
 }
 
 template <int HD, bool F32>
 hipError_t launch_attention_hd(const AttnPlan& p, const AttnArgs& a, hipStream_t stream) {
-    constexpr int QT = many_qt(HD, F32);
     const dim3 grid((unsigned)(p.tiles * a.c.kv_heads), p.splits);
     const void* f = p.few ? reinterpret_cast<const void*>(paged_few_kernel<HD, F32>)
-                          : reinterpret_cast<const void*>(paged_many_kernel<HD, QT, F32>);
+                          : reinterpret_cast<const void*>(paged_many_kernel<HD, F32>);
     const int lds = p.few ? few_lds(HD) : many_lds(HD);
     if (lds > 48 * 1024) {
         const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
     }
     if (p.few) hipLaunchKernelGGL((paged_few_kernel<HD, F32>), grid, dim3(256), lds, stream, a);
-    else hipLaunchKernelGGL((paged_many_kernel<HD, QT, F32>), grid, dim3(256), lds, stream, a);
+    else hipLaunchKernelGGL((paged_many_kernel<HD, F32>), grid, dim3(64 * many_waves(HD)), lds, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    const int64_t rows = (int64_t)a.b.tokens * a.group * a.c.kv_heads;
-    const dim3 join((unsigned)((rows + 256 / (HD / 4) - 1) / (256 / (HD / 4))));
+    const dim3 join((unsigned)(a.b.tokens * a.group * a.c.kv_heads));
     if (p.few) hipLaunchKernelGGL((paged_join_kernel<HD, 32, F32>), join, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((paged_join_kernel<HD, 128 * QT, F32>), join, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((paged_join_kernel<HD, 32 * many_waves(HD), F32>), join, dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
