@@ -11,8 +11,24 @@
 // rounded once), and all sums are sums of whole numbers: they do not depend on
 // their order, no partial sum is rounded, and the tokens are those of the
 // definition in 64 bits but for draws within 2^-42 n of a border. The thresholds
-// u and top_p are multiplied out in 128 bits. No sort: a prefix is found by
-// its count or its mass in a radix select over the logits' bits.
+// u and top_p are multiplied out in 128 bits.
+//
+// A row is never sorted. Its logits are binned by their distance from the largest
+// (kBins bins over the logits' range, or over the 30 temperatures below which a
+// mass rounds to zero), and the bins' counts and masses tell in which bins the
+// three prefixes and the draw can end; only their candidates are collected, sorted
+// and summed one by one. Four launches over slices of the rows:
+//   bounds   largest logit with its lowest index, smallest logit, per slice
+//   bins     counts (rows with a top_k) or masses (without; both for a top_k above
+//            kFewKept) per slice
+//   collect  every slice adds up its row's bins, finds the wanted ones and appends its
+//            candidates in them to the row's list; with a top_k up to kFewKept
+//            these are all bins that hold any of the first top_k
+//   finish   one workgroup per row
+// Rows of at most kList logits need the last one only, on all of their candidates. A
+// row whose wanted bins hold more than kList candidates (many equal logits, or an
+// outlier far above a narrow rest) takes radix selects over its logits' bits instead,
+// up to sixteen passes by one workgroup.
 #include "sample.h"
 
 #include <math.h>
@@ -95,6 +111,18 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int row) {
     const float u = a.u[row];
     s.u = u > 0.f ? fminf(u, 1.f) : 0.f;
     return s;
+}
+
+// What the steps compare running sums with: top_p's prefix ends at the first candidate
+// that reaches this, the draw is the first that passes this, min_p keeps masses of at least this.
+__device__ __forceinline__ uint64_t p_target(const Settings& s, uint64_t mass) {
+    return max(part_of(s.p, mass, true), (uint64_t)1);
+}
+__device__ __forceinline__ uint64_t u_target(const Settings& s, uint64_t kept) {
+    return min(part_of(s.u, kept, false), kept - 1);
+}
+__device__ __forceinline__ uint64_t least_mass(const Settings& s) {
+    return (uint64_t)ceil((double)s.m * (double)(1ull << kMassBits));
 }
 
 // ------------------------------------------------- a row by one workgroup ----
@@ -203,57 +231,469 @@ __device__ int index_of(RowShared& sh, const float* row, int n, uint32_t key, ui
     return found;
 }
 
-__global__ void __launch_bounds__(kRowThreads) sample_row_kernel(SampleArgs a) {
-    __shared__ RowShared sh;
-    const int r = blockIdx.x;
-    const float* row = a.logits + (int64_t)r * a.ld;
-    const Settings s = settings_of(a, r);
-    uint32_t best = 0;
-    for (int i = threadIdx.x; i < a.n; i += kRowThreads) best = max(best, key_of(row[i]));
+// The whole row: (token, probability).
+__device__ void sample_row(RowShared& sh, const float* row, int n, const Settings& s, uint32_t best, int* token,
+                           float* prob) {
+    const float top = logit_of(best);
+    uint64_t total = 0, large = 0;
+    unsigned candidates = 0;
+    const uint64_t least = least_mass(s);
+    for (int i = threadIdx.x; i < n; i += kRowThreads) {
+        const uint32_t k = key_of(row[i]);
+        if (!k) continue;
+        const uint64_t m = mass_of(logit_of(k), top, s.inv_t);
+        total += m;
+        ++candidates;
+        if (m >= least) large += m;
+    }
+    total = block_sum(sh, total);
+    large = block_sum(sh, large);
+    candidates = (unsigned)block_sum(sh, candidates);
+    uint64_t kept = total;
+    if (s.k && (unsigned)s.k < candidates) {
+        const Cut c = select(sh, row, n, top, s.inv_t, false, s.k);
+        kept = c.above + (s.k - c.count) * mass_of(logit_of(c.key), top, s.inv_t);
+    }
+    if (s.p < 1.f) {
+        const uint64_t target = p_target(s, kept);
+        const Cut c = select(sh, row, n, top, s.inv_t, true, target);
+        const uint64_t m = mass_of(logit_of(c.key), top, s.inv_t);
+        kept = c.above + (target - c.above + m - 1) / m * m;
+    }
+    kept = min(kept, large);
+    const uint64_t at = u_target(s, kept);
+    const Cut c = select(sh, row, n, top, s.inv_t, true, at + 1);
+    const uint64_t m = mass_of(logit_of(c.key), top, s.inv_t);
+    *token = index_of(sh, row, n, c.key, (at - c.above) / m);
+    *prob = (float)((double)m / (double)kept);
+}
+
+// ------------------------------------------------------ rows by their bins ----
+
+constexpr int kBins = 1024;      // one per thread of a workgroup
+constexpr int kThreads = kRowThreads;
+constexpr int kList = 4096;      // candidates that finish sorts in LDS
+constexpr int kFewKept = 1024;   // top_k up to which the whole kept set is collected
+constexpr int kMaxSlices = 16;
+constexpr int kRowsAtOnce = 1024;  // rows that one workspace holds
+
+struct Bound {
+    uint64_t best;  // key of the largest logit, then ~index (the lowest index among equals is the largest)
+    uint32_t least, unused;
+};
+
+// A row's part of the workspace.
+struct RowWork {
+    Bound* bound;               // [slices]
+    unsigned long long* mass;   // [slices][kBins]
+    unsigned* count;            // [slices][kBins]
+    unsigned long long* above;  // [kBins]: mass of the bins before
+    unsigned long long* list;   // [kList]: key, ~index
+    unsigned long long* total;  // [2]: mass of all bins, of the bins that min_p keeps for certain
+    unsigned* listed;           // [1]
+    unsigned* before;           // [kBins]: candidates in the bins before
+};
+__host__ __device__ constexpr size_t row_work_bytes(int slices) {
+    return (size_t)slices * (sizeof(Bound) + kBins * 12) + kBins * 8 + kList * 8 + 16 + 16 + kBins * 4;
+}
+__device__ __forceinline__ RowWork row_work(void* ws, int row, int slices) {
+    char* p = static_cast<char*>(ws) + row * row_work_bytes(slices);
+    RowWork w;
+    w.bound = reinterpret_cast<Bound*>(p);
+    p += slices * sizeof(Bound);
+    w.mass = reinterpret_cast<unsigned long long*>(p);
+    p += (size_t)slices * kBins * 8;
+    w.above = reinterpret_cast<unsigned long long*>(p);
+    p += kBins * 8;
+    w.list = reinterpret_cast<unsigned long long*>(p);
+    p += kList * 8;
+    w.total = reinterpret_cast<unsigned long long*>(p);
+    p += 16;
+    w.listed = reinterpret_cast<unsigned*>(p);
+    p += 16;
+    w.before = reinterpret_cast<unsigned*>(p);
+    p += kBins * 4;
+    w.count = reinterpret_cast<unsigned*>(p);
+    return w;
+}
+
+// f(index, logit) over a workgroup's part lo..hi-1 of a row, eight loads in flight per thread.
+template <typename F>
+__device__ __forceinline__ void walk(const float* row, int lo, int hi, F f) {
+    for (int base = lo + threadIdx.x; base < hi; base += 8 * kThreads) {
+        float v[8];
 #pragma unroll
-    for (int d = 32; d; d >>= 1) best = max(best, (uint32_t)__shfl_xor((int)best, d));
-    if ((threadIdx.x & 63) == 0) sh.redi[threadIdx.x >> 6] = best;
+        for (int j = 0; j < 8; ++j) v[j] = row[min(base + j * kThreads, hi - 1)];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (base + j * kThreads < hi) f(base + j * kThreads, v[j]);
+    }
+}
+__device__ __forceinline__ int slice_at(int n, int slices, int i) { return (int)((int64_t)n * i / slices); }
+
+// All slices' bounds, the same in every thread.
+__device__ __forceinline__ Bound row_bound(const RowWork& w, int slices) {
+    Bound b = w.bound[0];
+    for (int i = 1; i < slices; ++i) {
+        b.best = max(b.best, w.bound[i].best);
+        b.least = min(b.least, w.bound[i].least);
+    }
+    return b;
+}
+
+// Logits to bins, in the order of the logits: every step rounds monotonically.
+struct Bins {
+    float top, per;
+    bool clipped;  // the last bin holds what lies 30 temperatures and more below: masses of zero
+    __device__ __forceinline__ int at(float l) const { return (int)fminf((top - l) * per, (float)(kBins - 1)); }
+};
+__device__ __forceinline__ Bins bins_of(const Bound& b, const Settings& s) {
+    Bins r;
+    r.top = logit_of((uint32_t)(b.best >> 32));
+    const float all = r.top - logit_of(b.least);
+    const double most = 30.0 / s.inv_t;  // (e^-30 (1 - 1/kBins) 2^42 = 0.43)
+    r.clipped = (double)all > most;
+    const float range = r.clipped ? (float)most : all;
+    r.per = range > 1e-30f ? (float)kBins / range : 0.f;
+    return r;
+}
+__device__ __forceinline__ bool by_bins(const Bound& b, const Settings& s) {
+    // (an infinite range, from an infinite largest logit or the type's two ends, has no bins)
+    return b.best && !s.greedy && logit_of((uint32_t)(b.best >> 32)) - logit_of(b.least) < INFINITY;
+}
+
+__global__ void __launch_bounds__(kThreads) sample_bounds_kernel(SampleArgs a, void* ws, int slices) {
+    __shared__ uint64_t best_of[kThreads / 64];
+    __shared__ uint32_t least_of[kThreads / 64];
+    const int r = blockIdx.y, slice = blockIdx.x;
+    const RowWork w = row_work(ws, r, slices);
+    uint64_t best = 0;
+    uint32_t least = ~0u;
+    walk(a.logits + r * a.ld, slice_at(a.n, slices, slice), slice_at(a.n, slices, slice + 1), [&](int i, float l) {
+        const uint32_t k = key_of(l);
+        if (!k) return;
+        best = max(best, (uint64_t)k << 32 | (uint32_t)~i);
+        least = min(least, k);
+    });
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        best = max(best, (uint64_t)__shfl_xor((unsigned long long)best, d));
+        least = min(least, (uint32_t)__shfl_xor((int)least, d));
+    }
+    if ((threadIdx.x & 63) == 0) best_of[threadIdx.x >> 6] = best, least_of[threadIdx.x >> 6] = least;
     __syncthreads();
-    for (int w = 0; w < kRowThreads / 64; ++w) best = max(best, sh.redi[w]);
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < kThreads / 64; ++i) best = max(best, best_of[i]), least = min(least, least_of[i]);
+        w.bound[slice] = Bound{best, least, 0};
+        if (slice == 0) *w.listed = 0;
+    }
+}
+
+__global__ void __launch_bounds__(kThreads) sample_bins_kernel(SampleArgs a, void* ws, int slices) {
+    __shared__ unsigned long long mass[kBins];
+    __shared__ unsigned count[kBins];
+    const int r = blockIdx.y, slice = blockIdx.x;
+    const RowWork w = row_work(ws, r, slices);
+    const Settings s = settings_of(a, r);
+    const Bound b = row_bound(w, slices);
+    if (!by_bins(b, s)) return;
+    const Bins bins = bins_of(b, s);
+    const bool counts = s.k, masses = !s.k || s.k > kFewKept;
+    mass[threadIdx.x] = 0;
+    count[threadIdx.x] = 0;
     __syncthreads();
+    walk(a.logits + r * a.ld, slice_at(a.n, slices, slice), slice_at(a.n, slices, slice + 1), [&](int, float l) {
+        if (!(l > -INFINITY)) return;
+        const int bin = bins.at(l);
+        if (counts) atomicAdd(&count[bin], 1u);
+        if (masses) {
+            const uint64_t m = mass_of(l, bins.top, s.inv_t);
+            if (m) atomicAdd(&mass[bin], (unsigned long long)m);
+        }
+    });
+    __syncthreads();
+    if (counts) w.count[slice * kBins + threadIdx.x] = count[threadIdx.x];
+    if (masses) w.mass[slice * kBins + threadIdx.x] = mass[threadIdx.x];
+}
+
+// Inclusive prefix sums over the workgroup.
+template <typename T>
+__device__ __forceinline__ T scan(T v, T* part) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const T u = __shfl_up(v, d);
+        if (lane >= d) v += u;
+    }
+    __syncthreads();
+    if (lane == 63) part[wave] = v;
+    __syncthreads();
+    for (int i = 0; i < wave; ++i) v += part[i];
+    return v;
+}
+
+// Which of the row's bins are wanted (thread b: bin b). Every border lies between a
+// lowest and a highest value that follow from the bins alone; a bin is wanted where it
+// meets one of these ranges.
+struct Wanted {
+    bool mine;
+    uint64_t above, total, sure;
+    unsigned before;
+};
+__device__ Wanted wanted_bins(const RowWork& w, int slices, const Settings& s, const Bins& bins,
+                              unsigned long long* part, unsigned long long* box) {
+    const int b = threadIdx.x;
+    uint64_t m = 0;
+    unsigned c = 0;
+    const bool counts = s.k, masses = !s.k || s.k > kFewKept;
+    for (int i = 0; i < slices; ++i) {
+        if (counts) c += w.count[i * kBins + b];
+        if (masses) m += w.mass[i * kBins + b];
+    }
+    Wanted r{};
+    unsigned long long candidates = 0;
+    if (counts) {
+        const unsigned long long upto = scan((unsigned long long)c, part);
+        r.before = (unsigned)upto - c;
+        if (b == kBins - 1) box[0] = upto;
+        __syncthreads();
+        candidates = box[0];
+        __syncthreads();
+    }
+    const bool dead = bins.clipped && b == kBins - 1;  // masses of zero
+    if (!masses) {
+        r.mine = c && r.before < (unsigned)s.k && !dead;
+        return r;
+    }
+    const unsigned long long upto = scan((unsigned long long)m, part);
+    r.above = upto - m;
+    // box: total; the first top_k's mass, lowest and highest; top_p's; min_p's
+    if (b == kBins - 1) {
+        box[0] = upto;
+        box[1] = box[2] = box[4] = box[5] = upto;
+    }
+    if (b == 0) box[3] = 0;
+    __syncthreads();
+    r.total = box[0];
+    if (s.k && (unsigned)s.k < candidates && r.before < (unsigned)s.k && (unsigned)s.k <= r.before + c && !dead) {
+        r.mine = true;
+        box[1] = max(r.above, (uint64_t)1);
+        box[2] = upto;
+    }
+    __syncthreads();
+    uint64_t lo = box[1], hi = box[2];
+    if (s.p < 1.f) {
+        const uint64_t t_lo = p_target(s, lo), t_hi = p_target(s, hi);
+        if (m && r.above < t_hi && upto >= t_lo) {
+            r.mine = true;
+            atomicMax(&box[3], upto);
+        }
+        __syncthreads();
+        lo = min(lo, t_lo);
+        hi = min(hi, (uint64_t)box[3]);
+    }
+    r.sure = r.total;
+    if (s.m > 0.f) {
+        // the bin of the logit whose e is min_p, and its neighbours
+        const float cut = (float)(-log((double)s.m) / s.inv_t) * bins.per;
+        if (cut < (float)kBins) {
+            const int first = max((int)cut - 1, 0), last = min((int)cut + 1, kBins - 1);
+            if (m && b >= first && b <= last) r.mine = true;
+            if (b == first) box[4] = r.above;
+            if (b == last) box[5] = upto;
+            __syncthreads();
+            r.sure = box[4];
+            lo = min(lo, max((uint64_t)box[4], (uint64_t)1));
+            hi = min(hi, (uint64_t)box[5]);
+        }
+    }
+    if (m && r.above <= u_target(s, hi) && upto > u_target(s, lo)) r.mine = true;
+    return r;
+}
+
+__global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs a, void* ws, int slices) {
+    __shared__ unsigned long long part[kThreads / 64], box[6], list[kList];
+    __shared__ unsigned long long want[kBins / 64];
+    __shared__ unsigned count, base;
+    const int r = blockIdx.y, slice = blockIdx.x;
+    const RowWork w = row_work(ws, r, slices);
+    const Settings s = settings_of(a, r);
+    const Bound b = row_bound(w, slices);
+    if (!by_bins(b, s)) return;
+    const Bins bins = bins_of(b, s);
+    const Wanted mine = wanted_bins(w, slices, s, bins, part, box);
+    const unsigned long long bits = __ballot(mine.mine);
+    if ((threadIdx.x & 63) == 0) want[threadIdx.x >> 6] = bits;
+    if (threadIdx.x == 0) count = 0;
+    if (slice == 0) {
+        w.above[threadIdx.x] = mine.above;
+        w.before[threadIdx.x] = mine.before;
+        if (threadIdx.x == 0) w.total[0] = mine.total, w.total[1] = mine.sure;
+    }
+    __syncthreads();
+    walk(a.logits + r * a.ld, slice_at(a.n, slices, slice), slice_at(a.n, slices, slice + 1), [&](int i, float l) {
+        if (!(l > -INFINITY)) return;
+        const int bin = bins.at(l);
+        if (!((want[bin >> 6] >> (bin & 63)) & 1)) return;
+        const unsigned at = atomicAdd(&count, 1u);
+        if (at < kList) list[at] = (unsigned long long)key_of(l) << 32 | (uint32_t)~i;
+    });
+    __syncthreads();
+    if (threadIdx.x == 0) base = count ? atomicAdd(w.listed, count) : 0;
+    __syncthreads();
+    for (unsigned i = threadIdx.x; i < min(count, (unsigned)kList); i += kThreads)
+        if (base + i < kList) w.list[base + i] = list[i];
+}
+
+// `n` values in descending order, by bitonic merges over the next power of two (zeros behind them).
+__device__ void sort_list(unsigned long long* v, int n) {
+    int size = 64;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += kThreads) v[i] = 0;
+    __syncthreads();
+    for (int k = 2; k <= size; k <<= 1)
+        for (int j = k >> 1; j; j >>= 1) {
+            for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+                const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+                const unsigned long long x = v[lo], y = v[hi];
+                if ((x < y) == !(lo & k)) v[lo] = y, v[hi] = x;
+            }
+            __syncthreads();
+        }
+}
+
+__global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a, void* ws, int slices) {
+    __shared__ unsigned long long list[kList];
+    __shared__ union {
+        RowShared row;
+        struct {
+            unsigned long long first_sum[kBins];
+            unsigned first_at[kBins];
+            unsigned long long part[kThreads / 64], box[3];
+        } l;
+    } sh;
+    __shared__ unsigned listed;
+    const int r = blockIdx.x;
+    const float* row = a.logits + r * a.ld;
+    const Settings s = settings_of(a, r);
     int token = -1;
     float prob = 0.f;
-    if (best && s.greedy) {
-        token = index_of(sh, row, a.n, best, 0);
-        prob = 1.f;
-    } else if (best) {
-        const float top = logit_of(best);
-        uint64_t total = 0, large = 0;
-        unsigned candidates = 0;
-        const uint64_t least = (uint64_t)ceil((double)s.m * (double)(1ull << kMassBits));
-        for (int i = threadIdx.x; i < a.n; i += kRowThreads) {
+    Bound b{};
+    Bins bins{};
+    unsigned n = 0;
+    const bool whole = !slices;  // all of the row's candidates
+    if (whole) {
+        if (threadIdx.x == 0) listed = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.n; i += kThreads) {
             const uint32_t k = key_of(row[i]);
-            if (!k) continue;
-            const uint64_t m = mass_of(logit_of(k), top, s.inv_t);
-            total += m;
-            ++candidates;
-            if (m >= least) large += m;
+            if (k) list[atomicAdd(&listed, 1u)] = (unsigned long long)k << 32 | (uint32_t)~i;
         }
-        total = block_sum(sh, total);
-        large = block_sum(sh, large);
-        candidates = (unsigned)block_sum(sh, candidates);
-        uint64_t kept = total;
-        if (s.k && (unsigned)s.k < candidates) {
-            const Cut c = select(sh, row, a.n, top, s.inv_t, false, s.k);
-            kept = c.above + (s.k - c.count) * mass_of(logit_of(c.key), top, s.inv_t);
+        __syncthreads();
+        n = listed;
+        if (n) {
+            sort_list(list, n);
+            b.best = list[0];
         }
+    } else {
+        const RowWork w = row_work(ws, r, slices);
+        b = row_bound(w, slices);
+        if (b.best && !s.greedy) {
+            bins = bins_of(b, s);
+            n = by_bins(b, s) ? *w.listed : kList + 1;
+            if (n > kList) {
+                sample_row(sh.row, row, a.n, s, (uint32_t)(b.best >> 32), &token, &prob);
+                if (threadIdx.x == 0) {
+                    a.tokens[r] = token;
+                    if (a.probs) a.probs[r] = prob;
+                }
+                return;
+            }
+            for (unsigned i = threadIdx.x; i < n; i += kThreads) list[i] = w.list[i];
+            __syncthreads();
+            sort_list(list, n);
+        }
+    }
+    if (b.best && s.greedy) {
+        token = (int)~(uint32_t)b.best;
+        prob = 1.f;
+    } else if (b.best) {
+        // Four candidates per thread: mass, running sum and rank of each. A list that starts
+        // with the row's first candidate needs no more; otherwise each bin's own run
+        // continues from what lies above the bin.
+        const bool prefix = whole || (s.k && s.k <= kFewKept);
+        const float top = logit_of((uint32_t)(b.best >> 32));
+        constexpr int PER = kList / kThreads;
+        uint64_t m[PER], end[PER], sum = 0;
+        unsigned rank[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const unsigned i = threadIdx.x * PER + j;
+            m[j] = i < n ? mass_of(logit_of((uint32_t)(list[i] >> 32)), top, s.inv_t) : 0;
+            sum += m[j];
+        }
+        uint64_t run = scan((unsigned long long)sum, sh.l.part) - sum;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const unsigned i = threadIdx.x * PER + j;
+            run += m[j];
+            end[j] = run;
+            rank[j] = i;
+            if (!prefix && i < n) {
+                const int bin = bins.at(logit_of((uint32_t)(list[i] >> 32)));
+                if (i == 0 || bins.at(logit_of((uint32_t)(list[i - 1] >> 32))) != bin) {
+                    sh.l.first_sum[bin] = run - m[j];
+                    sh.l.first_at[bin] = i;
+                }
+            }
+        }
+        const RowWork w = row_work(ws, r, max(slices, 1));
+        // box: the mass of the first top_k, of top_p's prefix, of min_p's
+        if (threadIdx.x == kThreads - 1) {
+            const uint64_t all = prefix ? run : w.total[0];
+            sh.l.box[0] = sh.l.box[1] = all;
+            sh.l.box[2] = prefix ? 0 : w.total[1];
+        }
+        __syncthreads();
+        if (!prefix) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const unsigned i = threadIdx.x * PER + j;
+                if (i >= n) continue;
+                const int bin = bins.at(logit_of((uint32_t)(list[i] >> 32)));
+                end[j] += w.above[bin] - sh.l.first_sum[bin];
+                rank[j] += w.before[bin] - sh.l.first_at[bin];
+            }
+        }
+        const uint64_t least = least_mass(s);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const unsigned i = threadIdx.x * PER + j;
+            if (i >= n) continue;
+            if (s.k && rank[j] == (unsigned)s.k - 1) sh.l.box[0] = end[j];
+            if (m[j] >= least) atomicMax(&sh.l.box[2], (unsigned long long)end[j]);
+        }
+        __syncthreads();
+        uint64_t kept = sh.l.box[0];
         if (s.p < 1.f) {
-            const uint64_t target = max(part_of(s.p, kept, true), (uint64_t)1);
-            const Cut c = select(sh, row, a.n, top, s.inv_t, true, target);
-            const uint64_t m = mass_of(logit_of(c.key), top, s.inv_t);
-            kept = c.above + (target - c.above + m - 1) / m * m;
+            const uint64_t target = p_target(s, kept);
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (threadIdx.x * PER + j < n && end[j] >= target && end[j] - m[j] < target) sh.l.box[1] = end[j];
+            __syncthreads();
+            kept = min(kept, (uint64_t)sh.l.box[1]);
         }
-        kept = min(kept, large);
-        const uint64_t at = min(part_of(s.u, kept, false), kept - 1);
-        const Cut c = select(sh, row, a.n, top, s.inv_t, true, at + 1);
-        const uint64_t m = mass_of(logit_of(c.key), top, s.inv_t);
-        token = index_of(sh, row, a.n, c.key, (at - c.above) / m);
-        prob = (float)((double)m / (double)kept);
+        kept = min(kept, (uint64_t)sh.l.box[2]);
+        const uint64_t at = u_target(s, kept);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const unsigned i = threadIdx.x * PER + j;
+            if (i < n && end[j] - m[j] <= at && at < end[j]) {  // (one candidate: the runs do not overlap)
+                a.tokens[r] = (int)~(uint32_t)list[i];
+                if (a.probs) a.probs[r] = (float)((double)m[j] / (double)kept);
+            }
+        }
+        return;
     }
     if (threadIdx.x == 0) {
         a.tokens[r] = token;
@@ -261,12 +701,44 @@ __global__ void __launch_bounds__(kRowThreads) sample_row_kernel(SampleArgs a) {
     }
 }
 
+// Slices per row: two workgroups per CU, of 4096 logits at least.
+int slices_of(int rows, int n, int cus) {
+    int s = (2 * cus + rows - 1) / rows;
+    if (s > kMaxSlices) s = kMaxSlices;
+    const int most = (n + kList - 1) / kList;
+    return s < most ? s : most;
+}
+
 }  // namespace
 
-size_t sample_workspace(int, int, int) { return 0; }
+size_t sample_workspace(int rows, int n, int cus) {
+    if (n <= kList) return 0;
+    const int at_once = rows < kRowsAtOnce ? rows : kRowsAtOnce;
+    return at_once * row_work_bytes(slices_of(at_once, n, cus));
+}
 
-hipError_t launch_sample(const SampleArgs& a, void*, int, hipStream_t stream) {
-    hipLaunchKernelGGL(sample_row_kernel, dim3(a.rows), dim3(kRowThreads), 0, stream, a);
+hipError_t launch_sample(const SampleArgs& all, void* workspace, int cus, hipStream_t stream) {
+    const int at_once = all.n <= kList ? all.rows : all.rows < kRowsAtOnce ? all.rows : kRowsAtOnce;
+    const int slices = all.n <= kList ? 0 : slices_of(at_once, all.n, cus);
+    for (int row = 0; row < all.rows; row += at_once) {
+        SampleArgs a = all;
+        a.rows = all.rows - row < at_once ? all.rows - row : at_once;
+        a.logits += row * all.ld;
+        a.u += row;
+        a.temperature += a.temperature ? row : 0;
+        a.top_k += a.top_k ? row : 0;
+        a.top_p += a.top_p ? row : 0;
+        a.min_p += a.min_p ? row : 0;
+        a.tokens += row;
+        a.probs += a.probs ? row : 0;
+        const dim3 grid(slices, a.rows);
+        if (slices) {
+            hipLaunchKernelGGL(sample_bounds_kernel, grid, dim3(kThreads), 0, stream, a, workspace, slices);
+            hipLaunchKernelGGL(sample_bins_kernel, grid, dim3(kThreads), 0, stream, a, workspace, slices);
+            hipLaunchKernelGGL(sample_collect_kernel, grid, dim3(kThreads), 0, stream, a, workspace, slices);
+        }
+        hipLaunchKernelGGL(sample_finish_kernel, dim3(a.rows), dim3(kThreads), 0, stream, a, workspace, slices);
+    }
     return hipGetLastError();
 }
 
