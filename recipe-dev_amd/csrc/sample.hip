@@ -286,57 +286,70 @@ struct Bound {
 struct RowWork {
     Bound* bound;               // [slices]
     unsigned long long* mass;   // [slices][kBins]
-    unsigned* count;            // [slices][kBins]
+    unsigned long long* list;   // [slices][kList]: key, ~index
     unsigned long long* above;  // [kBins]: mass of the bins before
-    unsigned long long* list;   // [kList]: key, ~index
     unsigned long long* total;  // [2]: mass of all bins, of the bins that min_p keeps for certain
-    unsigned* listed;           // [1]
+    unsigned* listed;           // [kMaxSlices]
     unsigned* before;           // [kBins]: candidates in the bins before
+    unsigned* count;            // [slices][kBins]
 };
 __host__ __device__ constexpr size_t row_work_bytes(int slices) {
-    return (size_t)slices * (sizeof(Bound) + kBins * 12) + kBins * 8 + kList * 8 + 16 + 16 + kBins * 4;
+    return (size_t)slices * (sizeof(Bound) + kBins * 12 + kList * 8) + kBins * 12 + 16 + kMaxSlices * 4;
 }
 __device__ __forceinline__ RowWork row_work(void* ws, int row, int slices) {
     char* p = static_cast<char*>(ws) + row * row_work_bytes(slices);
+    auto take = [&](size_t bytes) {
+        char* at = p;
+        p += bytes;
+        return at;
+    };
     RowWork w;
-    w.bound = reinterpret_cast<Bound*>(p);
-    p += slices * sizeof(Bound);
-    w.mass = reinterpret_cast<unsigned long long*>(p);
-    p += (size_t)slices * kBins * 8;
-    w.above = reinterpret_cast<unsigned long long*>(p);
-    p += kBins * 8;
-    w.list = reinterpret_cast<unsigned long long*>(p);
-    p += kList * 8;
-    w.total = reinterpret_cast<unsigned long long*>(p);
-    p += 16;
-    w.listed = reinterpret_cast<unsigned*>(p);
-    p += 16;
-    w.before = reinterpret_cast<unsigned*>(p);
-    p += kBins * 4;
-    w.count = reinterpret_cast<unsigned*>(p);
+    w.bound = reinterpret_cast<Bound*>(take(slices * sizeof(Bound)));
+    w.mass = reinterpret_cast<unsigned long long*>(take((size_t)slices * kBins * 8));
+    w.list = reinterpret_cast<unsigned long long*>(take((size_t)slices * kList * 8));
+    w.above = reinterpret_cast<unsigned long long*>(take(kBins * 8));
+    w.total = reinterpret_cast<unsigned long long*>(take(16));
+    w.listed = reinterpret_cast<unsigned*>(take(kMaxSlices * 4));
+    w.before = reinterpret_cast<unsigned*>(take(kBins * 4));
+    w.count = reinterpret_cast<unsigned*>(take((size_t)slices * kBins * 4));
     return w;
 }
 
-// f(index, logit) over a workgroup's part lo..hi-1 of a row, eight loads in flight per thread.
-template <typename F>
-__device__ __forceinline__ void walk(const float* row, int lo, int hi, F f) {
-    for (int base = lo + threadIdx.x; base < hi; base += 8 * kThreads) {
-        float v[8];
+// A workgroup's part of a row, eight logits per thread at a time. The first eight are
+// requested when the kernel starts, before it has read what it needs to use them.
+struct Slice {
+    const float* row;
+    int lo, hi;
+    float v[8];
+    __device__ __forceinline__ void load(int base) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = row[min(base + j * kThreads, hi - 1)];
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (base + j * kThreads < hi) f(base + j * kThreads, v[j]);
     }
-}
-__device__ __forceinline__ int slice_at(int n, int slices, int i) { return (int)((int64_t)n * i / slices); }
+    __device__ __forceinline__ Slice(const SampleArgs& a, int r, int slice, int slices)
+        : row(a.logits + r * a.ld), lo((int)((int64_t)a.n * slice / slices)),
+          hi((int)((int64_t)a.n * (slice + 1) / slices)) {
+        load(lo + threadIdx.x);
+    }
+    template <typename F>
+    __device__ __forceinline__ void walk(F f) {  // f(index, logit)
+        for (int base = lo + threadIdx.x;;) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (base + j * kThreads < hi) f(base + j * kThreads, v[j]);
+            base += 8 * kThreads;
+            if (base >= hi) break;
+            load(base);
+        }
+    }
+};
 
-// All slices' bounds, the same in every thread.
+// All slices' bounds, the same in every thread (a slice per lane).
 __device__ __forceinline__ Bound row_bound(const RowWork& w, int slices) {
-    Bound b = w.bound[0];
-    for (int i = 1; i < slices; ++i) {
-        b.best = max(b.best, w.bound[i].best);
-        b.least = min(b.least, w.bound[i].least);
+    Bound b = w.bound[min((int)(threadIdx.x & (kMaxSlices - 1)), slices - 1)];
+#pragma unroll
+    for (int d = kMaxSlices / 2; d; d >>= 1) {
+        b.best = max(b.best, (uint64_t)__shfl_xor((unsigned long long)b.best, d));
+        b.least = min(b.least, (uint32_t)__shfl_xor((int)b.least, d));
     }
     return b;
 }
@@ -367,9 +380,10 @@ __global__ void __launch_bounds__(kThreads) sample_bounds_kernel(SampleArgs a, v
     __shared__ uint32_t least_of[kThreads / 64];
     const int r = blockIdx.y, slice = blockIdx.x;
     const RowWork w = row_work(ws, r, slices);
+    Slice logits(a, r, slice, slices);
     uint64_t best = 0;
     uint32_t least = ~0u;
-    walk(a.logits + r * a.ld, slice_at(a.n, slices, slice), slice_at(a.n, slices, slice + 1), [&](int i, float l) {
+    logits.walk([&](int i, float l) {
         const uint32_t k = key_of(l);
         if (!k) return;
         best = max(best, (uint64_t)k << 32 | (uint32_t)~i);
@@ -385,7 +399,6 @@ __global__ void __launch_bounds__(kThreads) sample_bounds_kernel(SampleArgs a, v
     if (threadIdx.x == 0) {
         for (int i = 1; i < kThreads / 64; ++i) best = max(best, best_of[i]), least = min(least, least_of[i]);
         w.bound[slice] = Bound{best, least, 0};
-        if (slice == 0) *w.listed = 0;
     }
 }
 
@@ -394,6 +407,7 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SampleArgs a, voi
     __shared__ unsigned count[kBins];
     const int r = blockIdx.y, slice = blockIdx.x;
     const RowWork w = row_work(ws, r, slices);
+    Slice logits(a, r, slice, slices);
     const Settings s = settings_of(a, r);
     const Bound b = row_bound(w, slices);
     if (!by_bins(b, s)) return;
@@ -402,7 +416,7 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SampleArgs a, voi
     mass[threadIdx.x] = 0;
     count[threadIdx.x] = 0;
     __syncthreads();
-    walk(a.logits + r * a.ld, slice_at(a.n, slices, slice), slice_at(a.n, slices, slice + 1), [&](int, float l) {
+    logits.walk([&](int, float l) {
         if (!(l > -INFINITY)) return;
         const int bin = bins.at(l);
         if (counts) atomicAdd(&count[bin], 1u);
@@ -428,8 +442,10 @@ __device__ __forceinline__ T scan(T v, T* part) {
     __syncthreads();
     if (lane == 63) part[wave] = v;
     __syncthreads();
-    for (int i = 0; i < wave; ++i) v += part[i];
-    return v;
+    T before = 0;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) before += i < wave ? part[i] : 0;
+    return v + before;
 }
 
 // Which of the row's bins are wanted (thread b: bin b). Every border lies between a
@@ -446,9 +462,20 @@ __device__ Wanted wanted_bins(const RowWork& w, int slices, const Settings& s, c
     uint64_t m = 0;
     unsigned c = 0;
     const bool counts = s.k, masses = !s.k || s.k > kFewKept;
-    for (int i = 0; i < slices; ++i) {
-        if (counts) c += w.count[i * kBins + b];
-        if (masses) m += w.mass[i * kBins + b];
+    // (every slice's value requested before the first is added)
+    if (counts) {
+        unsigned v[kMaxSlices];
+#pragma unroll
+        for (int i = 0; i < kMaxSlices; ++i) v[i] = w.count[min(i, slices - 1) * kBins + b];
+#pragma unroll
+        for (int i = 0; i < kMaxSlices; ++i) c += i < slices ? v[i] : 0;
+    }
+    if (masses) {
+        unsigned long long v[kMaxSlices];
+#pragma unroll
+        for (int i = 0; i < kMaxSlices; ++i) v[i] = w.mass[min(i, slices - 1) * kBins + b];
+#pragma unroll
+        for (int i = 0; i < kMaxSlices; ++i) m += i < slices ? v[i] : 0;
     }
     Wanted r{};
     unsigned long long candidates = 0;
@@ -514,9 +541,10 @@ __device__ Wanted wanted_bins(const RowWork& w, int slices, const Settings& s, c
 __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs a, void* ws, int slices) {
     __shared__ unsigned long long part[kThreads / 64], box[6], list[kList];
     __shared__ unsigned long long want[kBins / 64];
-    __shared__ unsigned count, base;
+    __shared__ unsigned count;
     const int r = blockIdx.y, slice = blockIdx.x;
     const RowWork w = row_work(ws, r, slices);
+    Slice logits(a, r, slice, slices);
     const Settings s = settings_of(a, r);
     const Bound b = row_bound(w, slices);
     if (!by_bins(b, s)) return;
@@ -531,7 +559,7 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs a, 
         if (threadIdx.x == 0) w.total[0] = mine.total, w.total[1] = mine.sure;
     }
     __syncthreads();
-    walk(a.logits + r * a.ld, slice_at(a.n, slices, slice), slice_at(a.n, slices, slice + 1), [&](int i, float l) {
+    logits.walk([&](int i, float l) {
         if (!(l > -INFINITY)) return;
         const int bin = bins.at(l);
         if (!((want[bin >> 6] >> (bin & 63)) & 1)) return;
@@ -539,26 +567,167 @@ __global__ void __launch_bounds__(kThreads) sample_collect_kernel(SampleArgs a, 
         if (at < kList) list[at] = (unsigned long long)key_of(l) << 32 | (uint32_t)~i;
     });
     __syncthreads();
-    if (threadIdx.x == 0) base = count ? atomicAdd(w.listed, count) : 0;
-    __syncthreads();
-    for (unsigned i = threadIdx.x; i < min(count, (unsigned)kList); i += kThreads)
-        if (base + i < kList) w.list[base + i] = list[i];
+    if (threadIdx.x == 0) w.listed[slice] = count;
+    for (unsigned i = threadIdx.x; i < min(count, (unsigned)kList); i += kThreads) w.list[slice * kList + i] = list[i];
 }
 
-// `n` values in descending order, by bitonic merges over the next power of two (zeros behind them).
-__device__ void sort_list(unsigned long long* v, int n) {
-    int size = 64;
-    while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += kThreads) v[i] = 0;
-    __syncthreads();
+// `n` values in descending order, by bitonic merges over the next power of two (zeros
+// behind them). A thread holds values t and, PER > 1, t + 1024, ..: exchanges over fewer than 64
+// places are lane exchanges, over 1024 and more register ones; only those between go
+// through LDS and its barriers.
+template <int PER>
+__device__ void sort_list(unsigned long long* v, int n, int size) {
+    const int t = threadIdx.x;
+    unsigned long long x[PER];
+#pragma unroll
+    for (int r = 0; r < PER; ++r) x[r] = r * kThreads + t < n ? v[r * kThreads + t] : 0;
     for (int k = 2; k <= size; k <<= 1)
         for (int j = k >> 1; j; j >>= 1) {
-            for (int i = threadIdx.x; i < size / 2; i += kThreads) {
-                const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
-                const unsigned long long x = v[lo], y = v[hi];
-                if ((x < y) == !(lo & k)) v[lo] = y, v[hi] = x;
+            if (j >= kThreads) {
+                if constexpr (PER == 4) {
+                    // places r and r ^ (j / 1024)
+#pragma unroll
+                    for (int r = 0; r < PER; ++r) {
+                        const int o = r ^ 1, o2 = r ^ 2;
+                        const bool down = !((r * kThreads) & k);
+                        if (j == kThreads && r < o && (x[r] < x[o]) == down) {
+                            const unsigned long long y = x[r];
+                            x[r] = x[o], x[o] = y;
+                        }
+                        if (j == 2 * kThreads && r < o2 && (x[r] < x[o2]) == down) {
+                            const unsigned long long y = x[r];
+                            x[r] = x[o2], x[o2] = y;
+                        }
+                    }
+                }
+                continue;
             }
-            __syncthreads();
+            unsigned long long y[PER];
+            if (j >= 64) {
+                __syncthreads();
+#pragma unroll
+                for (int r = 0; r < PER; ++r) v[r * kThreads + t] = x[r];
+                __syncthreads();
+#pragma unroll
+                for (int r = 0; r < PER; ++r) y[r] = v[r * kThreads + (t ^ j)];
+            } else {
+#pragma unroll
+                for (int r = 0; r < PER; ++r) y[r] = __shfl_xor(x[r], j);
+            }
+#pragma unroll
+            for (int r = 0; r < PER; ++r) {
+                const bool larger = !((r * kThreads + t) & k) == !(t & j);  // this place keeps the larger one
+                x[r] = (x[r] < y[r]) == larger ? y[r] : x[r];
+            }
+        }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < PER; ++r) v[r * kThreads + t] = x[r];
+    __syncthreads();
+}
+// Short lists: a value's place is the number of larger ones (no two are equal), counted
+// by 1024 / 256 threads each. 60 values: 0.6 us, by merges 3.4.
+constexpr int kShort = 256;
+__device__ void rank_list(unsigned long long* v, unsigned* rank, int n) {
+    const int e = threadIdx.x % kShort, part = threadIdx.x / kShort;
+    if (threadIdx.x < kShort) rank[threadIdx.x] = 0;
+    const unsigned long long mine = e < n ? v[e] : 0;
+    __syncthreads();
+    constexpr int PARTS = kThreads / kShort;
+    unsigned larger = 0;
+    for (int i = part; i < n; i += PARTS) larger += v[i] > mine;
+    if (e < n) atomicAdd(&rank[e], larger);
+    __syncthreads();
+    if (threadIdx.x < n) v[rank[threadIdx.x]] = mine;
+    __syncthreads();
+}
+__device__ __forceinline__ void sort_list(unsigned long long* v, unsigned* rank, int n) {
+    if (n <= kShort) return rank_list(v, rank, n);
+    int size = 2;
+    while (size < n) size <<= 1;
+    if (size <= kThreads) sort_list<1>(v, n, size);
+    else sort_list<kList / kThreads>(v, n, size);
+}
+
+struct DrawShared {
+    unsigned long long first_sum[kBins];
+    unsigned first_at[kBins];
+    unsigned long long part[kThreads / 64], box[3];
+};
+
+// The draw from the sorted list, PER candidates per thread: mass, running sum and rank of
+// each. A list that starts with the row's first candidate needs no more; otherwise
+// each bin's own run continues from what lies above the bin.
+template <int PER>
+__device__ void draw(const SampleArgs& a, void* ws, int slices, int r, const Settings& s, const Bound& b,
+                     const Bins& bins, const unsigned long long* list, unsigned n, DrawShared& sh) {
+    const bool prefix = !slices || (s.k && s.k <= kFewKept);
+    const float top = logit_of((uint32_t)(b.best >> 32));
+    const unsigned i0 = threadIdx.x * PER;
+    uint64_t m[PER], end[PER], sum = 0;
+    unsigned rank[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        m[j] = i0 + j < n ? mass_of(logit_of((uint32_t)(list[i0 + j] >> 32)), top, s.inv_t) : 0;
+        sum += m[j];
+    }
+    uint64_t run = scan((unsigned long long)sum, sh.part) - sum;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const unsigned i = i0 + j;
+        run += m[j];
+        end[j] = run;
+        rank[j] = i;
+        if (!prefix && i < n) {
+            const int bin = bins.at(logit_of((uint32_t)(list[i] >> 32)));
+            if (i == 0 || bins.at(logit_of((uint32_t)(list[i - 1] >> 32))) != bin) {
+                sh.first_sum[bin] = run - m[j];
+                sh.first_at[bin] = i;
+            }
+        }
+    }
+    const RowWork w = row_work(ws, r, max(slices, 1));
+    // box: the mass of the first top_k, of top_p's prefix, of min_p's
+    if (threadIdx.x == kThreads - 1) {
+        const uint64_t all = prefix ? run : w.total[0];
+        sh.box[0] = sh.box[1] = all;
+        sh.box[2] = prefix ? 0 : w.total[1];
+    }
+    __syncthreads();
+    const uint64_t least = least_mass(s);
+    uint64_t large = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const unsigned i = i0 + j;
+        if (i >= n) continue;
+        if (!prefix) {
+            const int bin = bins.at(logit_of((uint32_t)(list[i] >> 32)));
+            end[j] += w.above[bin] - sh.first_sum[bin];
+            rank[j] += w.before[bin] - sh.first_at[bin];
+        }
+        if (s.k && rank[j] == (unsigned)s.k - 1) sh.box[0] = end[j];
+        if (m[j] >= least) large = end[j];
+    }
+    // (the last candidate that min_p keeps: of a wave, in the last lane that has one)
+    const unsigned long long keeps = __ballot(large != 0);
+    if (keeps && (int)(threadIdx.x & 63) == 63 - __clzll(keeps)) atomicMax(&sh.box[2], (unsigned long long)large);
+    __syncthreads();
+    uint64_t kept = sh.box[0];
+    if (s.p < 1.f) {
+        const uint64_t target = p_target(s, kept);
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            if (i0 + j < n && end[j] >= target && end[j] - m[j] < target) sh.box[1] = end[j];
+        __syncthreads();
+        kept = min(kept, (uint64_t)sh.box[1]);
+    }
+    kept = min(kept, (uint64_t)sh.box[2]);
+    const uint64_t at = u_target(s, kept);
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+        if (i0 + j < n && end[j] - m[j] <= at && at < end[j]) {  // (one candidate: the runs do not overlap)
+            a.tokens[r] = (int)~(uint32_t)list[i0 + j];
+            if (a.probs) a.probs[r] = (float)((double)m[j] / (double)kept);
         }
 }
 
@@ -566,11 +735,8 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a, v
     __shared__ unsigned long long list[kList];
     __shared__ union {
         RowShared row;
-        struct {
-            unsigned long long first_sum[kBins];
-            unsigned first_at[kBins];
-            unsigned long long part[kThreads / 64], box[3];
-        } l;
+        unsigned rank[kShort];
+        DrawShared l;
     } sh;
     __shared__ unsigned listed;
     const int r = blockIdx.x;
@@ -592,15 +758,31 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a, v
         __syncthreads();
         n = listed;
         if (n) {
-            sort_list(list, n);
+            sort_list(list, sh.rank, n);
             b.best = list[0];
         }
     } else {
+        // the slices' lists, 64 threads to a slice: the first 64 of each are requested before the counts are known
         const RowWork w = row_work(ws, r, slices);
+        const int slice = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        const unsigned long long* mine = w.list + min(slice, slices - 1) * kList;
+        const unsigned long long early = mine[lane];
+        const unsigned count = lane < slices ? w.listed[lane] : 0;
         b = row_bound(w, slices);
         if (b.best && !s.greedy) {
             bins = bins_of(b, s);
-            n = by_bins(b, s) ? *w.listed : kList + 1;
+            unsigned from = 0, own = 0;
+            if (by_bins(b, s)) {
+#pragma unroll
+                for (int i = 0; i < kMaxSlices; ++i) {
+                    const unsigned c = __shfl(count, i);
+                    from += i < slice ? c : 0;
+                    own = i == slice ? c : own;
+                    n += c;
+                }
+            } else {
+                n = kList + 1;
+            }
             if (n > kList) {
                 sample_row(sh.row, row, a.n, s, (uint32_t)(b.best >> 32), &token, &prob);
                 if (threadIdx.x == 0) {
@@ -609,90 +791,18 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a, v
                 }
                 return;
             }
-            for (unsigned i = threadIdx.x; i < n; i += kThreads) list[i] = w.list[i];
+            if (lane < own) list[from + lane] = early;
+            for (unsigned i = 64 + lane; i < own; i += 64) list[from + i] = mine[i];
             __syncthreads();
-            sort_list(list, n);
+            sort_list(list, sh.rank, n);
         }
     }
     if (b.best && s.greedy) {
         token = (int)~(uint32_t)b.best;
         prob = 1.f;
     } else if (b.best) {
-        // Four candidates per thread: mass, running sum and rank of each. A list that starts
-        // with the row's first candidate needs no more; otherwise each bin's own run
-        // continues from what lies above the bin.
-        const bool prefix = whole || (s.k && s.k <= kFewKept);
-        const float top = logit_of((uint32_t)(b.best >> 32));
-        constexpr int PER = kList / kThreads;
-        uint64_t m[PER], end[PER], sum = 0;
-        unsigned rank[PER];
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const unsigned i = threadIdx.x * PER + j;
-            m[j] = i < n ? mass_of(logit_of((uint32_t)(list[i] >> 32)), top, s.inv_t) : 0;
-            sum += m[j];
-        }
-        uint64_t run = scan((unsigned long long)sum, sh.l.part) - sum;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const unsigned i = threadIdx.x * PER + j;
-            run += m[j];
-            end[j] = run;
-            rank[j] = i;
-            if (!prefix && i < n) {
-                const int bin = bins.at(logit_of((uint32_t)(list[i] >> 32)));
-                if (i == 0 || bins.at(logit_of((uint32_t)(list[i - 1] >> 32))) != bin) {
-                    sh.l.first_sum[bin] = run - m[j];
-                    sh.l.first_at[bin] = i;
-                }
-            }
-        }
-        const RowWork w = row_work(ws, r, max(slices, 1));
-        // box: the mass of the first top_k, of top_p's prefix, of min_p's
-        if (threadIdx.x == kThreads - 1) {
-            const uint64_t all = prefix ? run : w.total[0];
-            sh.l.box[0] = sh.l.box[1] = all;
-            sh.l.box[2] = prefix ? 0 : w.total[1];
-        }
-        __syncthreads();
-        if (!prefix) {
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-                const unsigned i = threadIdx.x * PER + j;
-                if (i >= n) continue;
-                const int bin = bins.at(logit_of((uint32_t)(list[i] >> 32)));
-                end[j] += w.above[bin] - sh.l.first_sum[bin];
-                rank[j] += w.before[bin] - sh.l.first_at[bin];
-            }
-        }
-        const uint64_t least = least_mass(s);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const unsigned i = threadIdx.x * PER + j;
-            if (i >= n) continue;
-            if (s.k && rank[j] == (unsigned)s.k - 1) sh.l.box[0] = end[j];
-            if (m[j] >= least) atomicMax(&sh.l.box[2], (unsigned long long)end[j]);
-        }
-        __syncthreads();
-        uint64_t kept = sh.l.box[0];
-        if (s.p < 1.f) {
-            const uint64_t target = p_target(s, kept);
-#pragma unroll
-            for (int j = 0; j < PER; ++j)
-                if (threadIdx.x * PER + j < n && end[j] >= target && end[j] - m[j] < target) sh.l.box[1] = end[j];
-            __syncthreads();
-            kept = min(kept, (uint64_t)sh.l.box[1]);
-        }
-        kept = min(kept, (uint64_t)sh.l.box[2]);
-        const uint64_t at = u_target(s, kept);
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const unsigned i = threadIdx.x * PER + j;
-            if (i < n && end[j] - m[j] <= at && at < end[j]) {  // (one candidate: the runs do not overlap)
-                a.tokens[r] = (int)~(uint32_t)list[i];
-                if (a.probs) a.probs[r] = (float)((double)m[j] / (double)kept);
-            }
-        }
+        if (n <= kThreads) draw<1>(a, ws, slices, r, s, b, bins, list, n, sh.l);
+        else draw<kList / kThreads>(a, ws, slices, r, s, b, bins, list, n, sh.l);
         return;
     }
     if (threadIdx.x == 0) {
