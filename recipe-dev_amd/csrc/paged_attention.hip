@@ -54,6 +54,8 @@ typedef float f2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef short s4_t __attribute__((ext_vector_type(4)));
 
+constexpr int kMaxSplits = 64;  // of one tile's keys
+
 struct AttnArgs {
     const void* q;
     void* out;
@@ -64,8 +66,12 @@ struct AttnArgs {
     int window;         // 0: none
     float scale;        // times log2 e: scores are taken to the base 2
     int tiles, splits, min_chunk;
-    float* o;           // [splits][tokens][q_heads][head_dim]
-    float2* ml;         // [splits][tokens][q_heads]: reference and weight sum
+    // partial results, where a tile's keys are split (a part is one row's: head_dim sums, and
+    // reference and weight sum), and for each token and head of a group where its are
+    float* o;           // [parts][head_dim]
+    float2* ml;         // [parts]
+    int2* info;         // [tokens][group]: live splits, first item (paged_few_kernel); null: nothing is split
+    int64_t parts;
 };
 
 // One tile of rows and its keys.
@@ -95,9 +101,6 @@ __device__ __forceinline__ int start_of(const PagedBatch& b, int s) { return min
 template <int TM>
 __device__ __forceinline__ int find_seq(const PagedBatch& b, int group, int number) {
     return last_seq(b.seqs, [&](int s) { return start_of(b, s) * group / TM + s <= number; });
-}
-__device__ __forceinline__ int find_seq_of_token(const PagedBatch& b, int token) {
-    return last_seq(b.seqs, [&](int s) { return b.q_start[s] <= token; });
 }
 
 // Row starts and lengths are read as they are found and brought into range.
@@ -472,8 +475,8 @@ __device__ __forceinline__ void add_odd(const AttnArgs& a, const Tile& t, int kh
 }
 
 // Four consecutive dims of a row to the output or, with several live splits, to the workspace.
-__device__ __forceinline__ void put4(const AttnArgs& a, bool f16_out, bool whole, int split, int token, int head, int hd,
-                                     int dim, const float (&v)[4]) {
+__device__ __forceinline__ void put4(const AttnArgs& a, bool f16_out, bool whole, int64_t part, int token, int head,
+                                     int hd, int dim, const float (&v)[4]) {
     if (whole) {
         if (f16_out) {
             uint2 u;
@@ -485,8 +488,7 @@ __device__ __forceinline__ void put4(const AttnArgs& a, bool f16_out, bool whole
                 make_float4(v[0], v[1], v[2], v[3]);
         }
     } else {
-        const int64_t row = ((int64_t)split * a.b.tokens + token) * (a.group * a.c.kv_heads) + head;
-        *reinterpret_cast<float4*>(a.o + row * hd + dim) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(a.o + part * hd + dim) = make_float4(v[0], v[1], v[2], v[3]);
     }
 }
 
@@ -495,23 +497,112 @@ __device__ __forceinline__ float reciprocal(float l) { return l == 0.f ? 0.f : 1
 // ------------------------------------------- few rows: keys over the waves ----
 
 // At most 32 rows a tile (a decode step, a few speculated tokens): bound by
-// reading the keys and values. Each of four waves takes every fourth step of 32
+// reading the keys and values.
+//
+// Items. The lengths are known on the device alone, and may differ by orders of magnitude: every
+// workgroup adds up the batch's keys and cuts each tile's into chunks of one length, about
+// total / `splits`, so that tiles + splits items per kv head suffice whatever the
+// lengths are, and finds its own among them.
+//
+// Each of four waves takes every fourth step of 32
 // keys of the split into LDS of its own, without barriers; its K buffer is filled
 // again while it works on the values and the other way round, and a second workgroup
 // on the CU fills the rest. At the end the waves' sums are joined through LDS.
+struct Item {
+    int seq, tile, split, first, chunk, live, id;
+};
+
+// A sequence's tiles, and the first and the number of its keys.
+template <int TM>
+__device__ __forceinline__ void seq_size(const AttnArgs& a, int s, int* tiles, int* first, int* keys) {
+    const int from = start_of(a.b, s), n = min(max(a.b.q_start[s + 1], from), a.b.tokens) - from;
+    const int kv = max(a.b.kv_len[s], 0);
+    *tiles = (n * a.group + TM - 1) / TM;
+    *first = a.window ? max(min(kv - n, a.cap) - a.window + 1, 0) & ~63 : 0;
+    *keys = max(min(kv, a.cap) - *first, 0);
+}
+// 64-key units per item, for a batch of `total` units.
+__device__ __forceinline__ int chunk_units(const AttnArgs& a, int64_t total, int units) {
+    const int even = (int)min((total + a.splits - 1) / a.splits, (int64_t)(1 << 24));
+    return max(max(even, a.min_chunk / 64), (units + kMaxSplits - 1) / kMaxSplits);
+}
+__device__ __forceinline__ int64_t sum_wave(int64_t v) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor((long long)v, d);
+    return v;
+}
+
+// Item `number` of the batch (of 256 threads); false: there is none.
+template <int TM>
+__device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* item) {
+    __shared__ int part[4], found[6];
+    __shared__ int64_t totals[4];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    int tiles = 0, first = 0, keys = 0;
+    int64_t total = 0;
+    for (int s = t; s < a.b.seqs; s += 256) {
+        seq_size<TM>(a, s, &tiles, &first, &keys);
+        total += (int64_t)tiles * ((keys + 63) >> 6);
+    }
+    if (t == 0) found[0] = -1;
+    total = sum_wave(total);
+    if (lane == 0) totals[wave] = total;
+    __syncthreads();
+    total = totals[0] + totals[1] + totals[2] + totals[3];
+    int before = 0;
+    for (int s0 = 0; s0 < a.b.seqs; s0 += 256) {
+        const int s = s0 + t;
+        int items = 0, live = 1, chunk = 1;
+        if (s < a.b.seqs) {
+            if (a.b.seqs > 256) seq_size<TM>(a, s, &tiles, &first, &keys);
+            const int units = (keys + 63) >> 6;
+            chunk = chunk_units(a, total, units);
+            live = max((units + chunk - 1) / chunk, 1);
+            items = tiles * live;
+        }
+        int upto = items;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int v = __shfl_up(upto, d);
+            if (lane >= d) upto += v;
+        }
+        __syncthreads();
+        if (lane == 63) part[wave] = upto;
+        __syncthreads();
+        int from = before + upto - items;
+        for (int w = 0; w < 4; ++w) {
+            from += w < wave ? part[w] : 0;
+            before += part[w];
+        }
+        if (number >= from && number < from + items) {
+            found[0] = s, found[1] = (number - from) / live, found[2] = (number - from) % live, found[3] = first;
+            found[4] = chunk * 64, found[5] = live;
+        }
+    }
+    __syncthreads();
+    if (found[0] < 0) return false;
+    item->seq = __builtin_amdgcn_readfirstlane(found[0]);
+    item->tile = __builtin_amdgcn_readfirstlane(found[1]);
+    item->split = __builtin_amdgcn_readfirstlane(found[2]);
+    item->first = __builtin_amdgcn_readfirstlane(found[3]);
+    item->chunk = __builtin_amdgcn_readfirstlane(found[4]);
+    item->live = __builtin_amdgcn_readfirstlane(found[5]);
+    item->id = number;
+    return true;
+}
+
 template <int HD, bool F32>
 __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnArgs a) {
     typedef Lay<HD> L;
     constexpr int TM = 32, KEYS = 32, HALF = KEYS * HD * 2;  // HALF: bytes of a wave's K (and V) buffer
     extern __shared__ __align__(16) char lds[];
     __shared__ float2 sums[4][32];
-    const int kh = blockIdx.x % a.c.kv_heads, number = blockIdx.x / a.c.kv_heads, split = blockIdx.y;
-    const int seq = find_seq<TM>(a.b, a.group, number);
-    const int first = start_of(a.b, seq) * a.group / TM + seq;
-    const Tile t = make_tile<TM>(a, seq, (number - first) * TM);
-    if (t.row0 >= t.rows) return;
-    const int begin = t.first + split * t.chunk, end = min(begin + t.chunk, t.end);
-    if (split && begin >= end) return;  // (split 0 of a tile without keys writes its zeros)
+    const int kh = blockIdx.x % a.c.kv_heads;
+    Item item;
+    if (!find_item<TM>(a, blockIdx.x / a.c.kv_heads, &item)) return;
+    const int seq = item.seq;
+    const Tile t = make_tile<TM>(a, seq, item.tile * TM);
+    const int begin = item.first + item.split * item.chunk, end = min(begin + item.chunk, t.end);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     char* K = lds + wave * 2 * HALF;
     char* V = K + HALF;
@@ -592,7 +683,11 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
     if (h == 0) sums[wave][q] = make_float2(w.m[0], l);
     __syncthreads();
     const int rows = min(t.rows - t.row0, TM);
-    const bool whole = t.live <= 1;
+    const bool whole = item.live <= 1;
+    const int64_t part0 = ((int64_t)item.id * a.c.kv_heads + kh) * TM;
+    if (a.info && kh == 0 && item.split == 0)
+        for (int u = threadIdx.x; u < rows; u += 256)
+            a.info[(int64_t)t.token0 * a.group + t.row0 + u] = make_int2(item.live, item.id);
     for (int u = threadIdx.x; u < rows * (HD / 4); u += 256) {
         const int row = u / (HD / 4), piece = u % (HD / 4);
         float m = sums[0][row].x, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -612,9 +707,9 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] *= inv;
         } else if (piece == 0) {
-            a.ml[((int64_t)split * a.b.tokens + t.token0 + tok) * (a.group * a.c.kv_heads) + head] = make_float2(m, sum);
+            a.ml[part0 + row] = make_float2(m, sum);
         }
-        put4(a, !F32, whole, split, t.token0 + tok, head, HD, 4 * piece, v);
+        put4(a, !F32, whole, part0 + row, t.token0 + tok, head, HD, 4 * piece, v);
     }
 }
 
@@ -696,15 +791,16 @@ __global__ void __launch_bounds__(64 * many_waves(HD), many_waves(HD) / 4) paged
     const float f = whole ? reciprocal(l) : 1.f;
     if (r >= t.rows) return;
     const int tok = t.token0 + r / a.group, head = kh * a.group + r % a.group;
-    if (!whole && h == 0)
-        a.ml[((int64_t)split * a.b.tokens + tok) * (a.group * a.c.kv_heads) + head] = make_float2(w.m[0], l);
+    const int64_t part = ((int64_t)split * a.b.tokens + tok) * (a.group * a.c.kv_heads) + head;
+    if (!whole && h == 0) a.ml[part] = make_float2(w.m[0], l);
+    if (a.info && kh == 0 && split == 0 && h == 0) a.info[(int64_t)t.token0 * a.group + r] = make_int2(t.live, 0);
 #pragma unroll
     for (int d = 0; d < HD / 32; ++d)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const float v[4] = {w.o[0][d][4 * e] * f, w.o[0][d][4 * e + 1] * f, w.o[0][d][4 * e + 2] * f,
                                 w.o[0][d][4 * e + 3] * f};
-            put4(a, !F32, whole, split, tok, head, HD, 32 * d + 8 * e + 4 * h, v);
+            put4(a, !F32, whole, part, tok, head, HD, 32 * d + 8 * e + 4 * h, v);
         }
 }
 
@@ -712,40 +808,45 @@ __global__ void __launch_bounds__(64 * many_waves(HD), many_waves(HD) / 4) paged
 
 // out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's live splits. A
 // workgroup per row (token, query head): HD / 4 threads take a split's 16-byte
-// columns, the other threads further splits, whose partial results are all
-// requested before it is known how many are live.
-constexpr int kMaxSplits = 64;
-template <int HD, int TM, bool F32>
-__global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a) {
+// columns, the other threads further splits, all requested at once.
+template <int HD, bool F32>
+__global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a, bool few) {
     constexpr int TPR = HD / 4, SIDE = 256 / TPR, PER = kMaxSplits / SIDE;
     __shared__ float4 part[256];
     __shared__ float2 sums[SIDE];
     const int heads = a.group * a.c.kv_heads;
-    const int token = blockIdx.x / heads, head = blockIdx.x % heads;
+    const int token = blockIdx.x / heads, head = blockIdx.x % heads, kh = head / a.group;
     const int col = threadIdx.x % TPR, side = threadIdx.x / TPR;
-    const int64_t at = (int64_t)token * heads + head, next = (int64_t)a.b.tokens * heads;
+    const int2 info = a.info[(int64_t)token * a.group + head % a.group];
+    const int from = a.b.q_start[0], to = a.b.q_start[a.b.seqs];
+    // (rows of no sequence have no info; that of rows of starts out of order may be an older call's)
+    const int live = info.x;
+    if (token < from || token >= to || live <= 1 || live > kMaxSplits) return;
+    int64_t at = (int64_t)token * heads + head, next = (int64_t)a.b.tokens * heads;
+    if (few) {
+        // the row's number in its tile: rows of a sequence's tiles start at the sequence's first
+        const int seq = last_seq(a.b.seqs, [&](int s) { return a.b.q_start[s] <= token; });
+        const int row = (token - start_of(a.b, seq)) * a.group + head % a.group;
+        at = ((int64_t)info.y * a.c.kv_heads + kh) * 32 + (row & 31);
+        next = (int64_t)a.c.kv_heads * 32;
+    }
+    if (at < 0 || at + (live - 1) * next >= a.parts) return;
     float4 x[PER];
     float2 ml[PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k)
-        if (k * SIDE < a.splits) {
-            const int64_t row = at + min(side + k * SIDE, a.splits - 1) * next;
+        if (k * SIDE < live) {
+            const int64_t row = at + min(side + k * SIDE, live - 1) * next;
             x[k] = *reinterpret_cast<const float4*>(a.o + row * HD + 4 * col);
             ml[k] = a.ml[row];
         }
-    // the token's sequence, the last one that starts at or before it
-    const int seq = find_seq_of_token(a.b, token);
-    if (token < a.b.q_start[seq] || token >= a.b.q_start[seq + 1]) return;
-    const int row = (token - a.b.q_start[seq]) * a.group + head % a.group;
-    const Tile t = make_tile<TM>(a, seq, row / TM * TM);
-    if (t.live <= 1) return;
     float m = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < PER; ++k)
-        if (side + k * SIDE < t.live) m = fmaxf(m, ml[k].x);
+        if (side + k * SIDE < live) m = fmaxf(m, ml[k].x);
 #pragma unroll
     for (int k = 0; k < PER; ++k)
-        if (side + k * SIDE < t.live) {
+        if (side + k * SIDE < live) {
             const float f = ml[k].x == -INFINITY ? (ml[k].y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml[k].x - m);
             sum = fmaf(f, ml[k].y, sum);
             v[0] = fmaf(f, x[k].x, v[0]), v[1] = fmaf(f, x[k].y, v[1]);
@@ -775,33 +876,51 @@ __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a) {
 
 // ------------------------------------------------------------------ launches ----
 
+#ifndef FEW_ITEMS
+#define FEW_ITEMS 2
+#endif
+constexpr int kFewItems = FEW_ITEMS;
 constexpr int few_lds(int hd) { return 4 * 2 * 32 * hd * 2; }
 constexpr int many_lds(int hd) { return 2 * 2 * 64 * hd * 2; }
 
 struct AttnPlan {
-    bool few;
-    int tm, splits, min_chunk;
-    int64_t tiles;
+    bool few, join;
+    int splits, min_chunk;
+    int64_t tiles, parts;
 };
 
-AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus) {
+AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, int cus) {
     AttnPlan p;
+    const int heads = kv_heads * group;
     p.few = (int64_t)tokens * group <= (int64_t)32 * seqs;
-    p.tm = p.few ? 32 : 32 * many_waves(hd);
-    p.tiles = (int64_t)tokens * group / p.tm + seqs;
-    p.min_chunk = p.few ? 128 : 512;
-    const int64_t wgs = p.tiles * kv_heads, want = p.few ? 2 * cus : cus;
-    int64_t s = wgs >= want ? 1 : (want + wgs - 1) / wgs;
-    const int64_t most = (cap + p.min_chunk - 1) / p.min_chunk;
-    if (s > most) s = most;
-    if (s > kMaxSplits) s = kMaxSplits;
-    p.splits = (int)(s < 1 ? 1 : s);
+    if (p.few) {
+        p.tiles = (int64_t)tokens * group / 32 + seqs;
+        p.min_chunk = 128;  // a step for each wave
+        const int64_t want = kFewItems * cus / kv_heads;
+        p.splits = (int)(want < 1 ? 1 : want);
+        p.join = cap > p.min_chunk;
+        p.parts = p.join ? (p.tiles + p.splits) * kv_heads * 32 : 0;
+    } else {
+        p.tiles = (int64_t)tokens * group / (32 * many_waves(hd)) + seqs;
+        p.min_chunk = 512;
+        const int64_t wgs = p.tiles * kv_heads;
+        int64_t s = wgs >= cus ? 1 : (cus + wgs - 1) / wgs;
+        const int64_t most = (cap + p.min_chunk - 1) / p.min_chunk;
+        if (s > most) s = most;
+        p.splits = (int)(s > kMaxSplits ? kMaxSplits : s < 1 ? 1 : s);
+        p.join = p.splits > 1;
+        p.parts = p.join ? (int64_t)p.splits * tokens * heads : 0;
+    }
     return p;
+}
+
+size_t workspace_bytes(const AttnPlan& p, int tokens, int group, int hd) {
+    return p.join ? p.parts * (hd * sizeof(float) + sizeof(float2)) + (size_t)tokens * group * sizeof(int2) : 0;
 }
 
 template <int HD, bool F32>
 hipError_t launch_attention_hd(const AttnPlan& p, const AttnArgs& a, hipStream_t stream) {
-    const dim3 grid((unsigned)(p.tiles * a.c.kv_heads), p.splits);
+    const dim3 grid((unsigned)((p.tiles + (p.few ? p.splits : 0)) * a.c.kv_heads), p.few ? 1 : p.splits);
     const void* f = p.few ? reinterpret_cast<const void*>(paged_few_kernel<HD, F32>)
                           : reinterpret_cast<const void*>(paged_many_kernel<HD, F32>);
     const int lds = p.few ? few_lds(HD) : many_lds(HD);
@@ -812,10 +931,9 @@ hipError_t launch_attention_hd(const AttnPlan& p, const AttnArgs& a, hipStream_t
     if (p.few) hipLaunchKernelGGL((paged_few_kernel<HD, F32>), grid, dim3(256), lds, stream, a);
     else hipLaunchKernelGGL((paged_many_kernel<HD, F32>), grid, dim3(64 * many_waves(HD)), lds, stream, a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.splits == 1) return e;
-    const dim3 join((unsigned)(a.b.tokens * a.group * a.c.kv_heads));
-    if (p.few) hipLaunchKernelGGL((paged_join_kernel<HD, 32, F32>), join, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((paged_join_kernel<HD, 32 * many_waves(HD), F32>), join, dim3(256), 0, stream, a);
+    if (e != hipSuccess || !p.join) return e;
+    hipLaunchKernelGGL((paged_join_kernel<HD, F32>), dim3((unsigned)(a.b.tokens * a.group * a.c.kv_heads)), dim3(256), 0,
+                       stream, a, p.few);
     return hipGetLastError();
 }
 
@@ -827,16 +945,9 @@ bool paged_attention_fits(const PagedBatch& b, const PagedCache& c, int q_heads)
 }
 
 size_t paged_attention_workspace(const PagedBatch& b, const PagedCache& c, int q_heads, int cus) {
-    // (the larger of the two types', so that one workspace serves both)
-    size_t most = 0;
-    for (int f32 = 0; f32 < 2; ++f32) {
-        const AttnPlan p = plan_attention(b.tokens, b.seqs, (int64_t)b.max_blocks << c.block_shift, c.kv_heads,
-                                          q_heads / c.kv_heads, c.head_dim, f32, cus);
-        const size_t rows = p.splits > 1 ? (size_t)p.splits * b.tokens * q_heads : 0;
-        const size_t bytes = rows * (c.head_dim * sizeof(float) + sizeof(float2));
-        most = bytes > most ? bytes : most;
-    }
-    return most;
+    const int group = q_heads / c.kv_heads;
+    return workspace_bytes(plan_attention(b.tokens, b.seqs, (int64_t)b.max_blocks << c.block_shift, c.kv_heads, group,
+                                          c.head_dim, cus), b.tokens, group, c.head_dim);
 }
 
 hipError_t launch_paged_attention(const PagedBatch& b, const PagedCache& c, const void* q, bool f32, int64_t ldq,
@@ -844,7 +955,7 @@ hipError_t launch_paged_attention(const PagedBatch& b, const PagedCache& c, cons
                                   hipStream_t stream) {
     const int group = q_heads / c.kv_heads;
     const int64_t cap = (int64_t)b.max_blocks << c.block_shift;
-    const AttnPlan p = plan_attention(b.tokens, b.seqs, cap, c.kv_heads, group, c.head_dim, f32, cus);
+    const AttnPlan p = plan_attention(b.tokens, b.seqs, cap, c.kv_heads, group, c.head_dim, cus);
     AttnArgs a;
     a.q = q;
     a.out = out;
@@ -860,7 +971,9 @@ hipError_t launch_paged_attention(const PagedBatch& b, const PagedCache& c, cons
     a.splits = p.splits;
     a.min_chunk = p.min_chunk;
     a.o = static_cast<float*>(workspace);
-    a.ml = reinterpret_cast<float2*>(a.o + (p.splits > 1 ? (size_t)p.splits * b.tokens * q_heads * c.head_dim : 0));
+    a.ml = reinterpret_cast<float2*>(a.o + p.parts * c.head_dim);
+    a.info = p.join ? reinterpret_cast<int2*>(a.ml + p.parts) : nullptr;
+    a.parts = p.parts;
     if (c.head_dim == 64) return f32 ? launch_attention_hd<64, true>(p, a, stream) : launch_attention_hd<64, false>(p, a, stream);
     if (c.head_dim == 128)
         return f32 ? launch_attention_hd<128, true>(p, a, stream) : launch_attention_hd<128, false>(p, a, stream);
