@@ -755,6 +755,9 @@ __global__ void __launch_bounds__(64 * many_waves(HD), many_waves(HD) / 4) paged
         if (WAVES == 4 || wave >= 4) load_group<HD, true>(a.c.v, a.c, kh, page, key, at + HALF);
         return bad;
     };
+    // the keys that any of the wave's rows sees
+    const int p0 = t.kv - t.n + row / a.group, p1 = t.kv - t.n + (min(row + 32, t.rows) - 1) / a.group;
+    const int wave_to = row < t.rows ? p1 + 1 : 0, wave_from = a.window ? p0 - a.window + 1 : 0;
     unsigned bad = 0, bad_next = 0;
     int buffer = 0;
     bool odd = false;
@@ -769,15 +772,17 @@ __global__ void __launch_bounds__(64 * many_waves(HD), many_waves(HD) / 4) paged
         char* V = K + HALF;
         const bool masked = key0 < t.all_from || key0 + KEYS > t.all_to || bad;
         if (masked && __syncthreads_or(zero_dead<HD, KEYS>(V, key0, t.end, bad, threadIdx.x, 64 * WAVES))) odd = true;
-        f16_t s[1][2];
-        scores<HD, 1, 2, F32>(K, w, s);
-        if (masked) mask_scores<HD, 1, 2, F32>(w, s, key0, bad);
-        float top[1];
-        largest<1, 2>(s, top);
-        move_references<HD, 1, F32>(w, top);
-        h8_t p[1][4][F32 ? 2 : 1];
-        weights<HD, 1, 2, F32>(w, s, p);
-        add_values<HD, 1, 2, F32>(V, w, p);
+        if (key0 < wave_to && key0 + KEYS > wave_from) {  // (a wave whose rows see none of the step only loads)
+            f16_t s[1][2];
+            scores<HD, 1, 2, F32>(K, w, s);
+            if (masked) mask_scores<HD, 1, 2, F32>(w, s, key0, bad);
+            float top[1];
+            largest<1, 2>(s, top);
+            move_references<HD, 1, F32>(w, top);
+            h8_t p[1][4][F32 ? 2 : 1];
+            weights<HD, 1, 2, F32>(w, s, p);
+            add_values<HD, 1, 2, F32>(V, w, p);
+        }
         bad = bad_next;
         buffer ^= 1;
     }
@@ -876,10 +881,6 @@ __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a, bool few) {
 
 // ------------------------------------------------------------------ launches ----
 
-#ifndef FEW_ITEMS
-#define FEW_ITEMS 2
-#endif
-constexpr int kFewItems = FEW_ITEMS;
 constexpr int few_lds(int hd) { return 4 * 2 * 32 * hd * 2; }
 constexpr int many_lds(int hd) { return 2 * 2 * 64 * hd * 2; }
 
@@ -892,12 +893,21 @@ struct AttnPlan {
 AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, int cus) {
     AttnPlan p;
     const int heads = kv_heads * group;
-    p.few = (int64_t)tokens * group <= (int64_t)32 * seqs;
+    // The few-rows form where the sequences' rows fill at most half of a many-rows tile, or where there
+    // are so few that its tiles leave CUs idle. 32/8 heads of 128, fp16, few against many, us: 32
+    // sequences of 128 rows per kv head over 6,000 positions 238 / 341, of 256 398 / 350; one sequence of
+    // 1024 rows over 1,000 29 / 35, of 4096 without context 51 / 50; four of 2048 over 6,000 357 / 221.
+    // Heads of 256 (four waves a tile): one of 512 rows over 1,000 34 / 40, of 2048 65 / 57.
+    p.tiles = (int64_t)tokens * group / 32 + seqs;
+    p.few = (int64_t)tokens * group <= (int64_t)16 * many_waves(hd) * seqs ||
+            (int64_t)tokens * heads / 32 <= (hd == 256 ? cus / 2 : 2 * cus);
     if (p.few) {
-        p.tiles = (int64_t)tokens * group / 32 + seqs;
-        p.min_chunk = 128;  // a step for each wave
-        const int64_t want = kFewItems * cus / kv_heads;
-        p.splits = (int)(want < 1 ? 1 : want);
+        // Two items per CU over the whole batch (32 requests of 60 to 8,192 positions: 35.1 us; one
+        // per CU 37.6, four 37.6), of two steps for each wave at least (one request at 4,097: 10.5 us; of
+        // one step 12.4, of four 12.3).
+        p.min_chunk = 256;
+        const int64_t want = 2 * cus / kv_heads, most = p.tiles * ((cap + p.min_chunk - 1) / p.min_chunk);
+        p.splits = (int)(most < want ? most : want < 1 ? 1 : want);
         p.join = cap > p.min_chunk;
         p.parts = p.join ? (p.tiles + p.splits) * kv_heads * 32 : 0;
     } else {
