@@ -43,4 +43,26 @@ __device__ __forceinline__ float swap32_max(float v) {
     return fmaxf(p.lo, p.hi);
 }
 
+// v of the lane that a DPP control selects, 0 where it selects none (rows outside `ROWS` too).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned dpp(unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long dpp(unsigned long long v) {
+    return (unsigned long long)dpp<CTRL, ROWS>((unsigned)(v >> 32)) << 32 | dpp<CTRL, ROWS>((unsigned)v);
+}
+// Inclusive prefix sums over the wave: within rows of 16 by shifts, then each row's last
+// sum to the row behind it and the lower half's to the upper (no LDS crossbar).
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+    v += dpp<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+    v += dpp<0x112, 0xf>(v);
+    v += dpp<0x114, 0xf>(v);
+    v += dpp<0x118, 0xf>(v);
+    v += dpp<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+    v += dpp<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
 }  // namespace rq

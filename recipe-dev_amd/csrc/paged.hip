@@ -4,6 +4,8 @@
 
 #include <limits.h>
 
+#include "lanes.h"
+
 namespace rq {
 
 // --------------------------------------------------------------- tables ----
@@ -26,11 +28,8 @@ constexpr int kPlanRows = 2048;
 // Inclusive prefix sums of two values over the workgroup; `total` gets the sums.
 __device__ __forceinline__ void scan2(int& a, int& b, int (&total)[2], int (*part)[2]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int ua = __shfl_up(a, d), ub = __shfl_up(b, d);
-        if (lane >= d) a += ua, b += ub;
-    }
+    a = (int)wave_scan((unsigned)a);
+    b = (int)wave_scan((unsigned)b);
     if (lane == 63) part[wave][0] = a, part[wave][1] = b;
     __syncthreads();
     total[0] = total[1] = 0;

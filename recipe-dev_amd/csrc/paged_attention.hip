@@ -560,12 +560,7 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* i
             live = max((units + chunk - 1) / chunk, 1);
             items = tiles * live;
         }
-        int upto = items;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int v = __shfl_up(upto, d);
-            if (lane >= d) upto += v;
-        }
+        const int upto = (int)wave_scan((unsigned)items);
         __syncthreads();
         if (lane == 63) part[wave] = upto;
         __syncthreads();

@@ -33,6 +33,8 @@
 
 #include <math.h>
 
+#include "lanes.h"
+
 namespace rq {
 
 namespace {
@@ -49,32 +51,38 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
-// exp((l - top) / temperature) in units of 2^-42, to the nearest: 2^t = 2^n e^x with
-// t = n + f, x = f ln 2, |x| <= 0.3466, e^x by its series up to x^12 (the next term
-// is below 2^-52).
-__device__ __forceinline__ uint64_t mass_of(float l, float top, double inv_t) {
-    const double d = (double)l - (double)top;
-    if (l == top) return 1ull << kMassBits;
-    const double t = d * inv_t * 1.4426950408889634;
-    if (!(t > -64.0)) return 0;  // (an infinite top leaves only its equals)
-    const double n = rint(t);
-    const double x = (t - n) * 0.69314718055994531;
-    double p = 1.0 / 479001600.0;
-    p = fma(p, x, 1.0 / 39916800.0);
-    p = fma(p, x, 1.0 / 3628800.0);
-    p = fma(p, x, 1.0 / 362880.0);
-    p = fma(p, x, 1.0 / 40320.0);
-    p = fma(p, x, 1.0 / 5040.0);
-    p = fma(p, x, 1.0 / 720.0);
-    p = fma(p, x, 1.0 / 120.0);
-    p = fma(p, x, 1.0 / 24.0);
-    p = fma(p, x, 1.0 / 6.0);
-    p = fma(p, x, 0.5);
-    p = fma(p, x, 1.0);
-    p = fma(p, x, 1.0);
-    const double scale = __longlong_as_double((long long)(1023 + kMassBits + (int)n) << 52);
-    // adding 2^52 leaves the rounded whole number in the low mantissa bits (p scale <= 2^42)
-    return (uint64_t)__double_as_longlong(fma(p, scale, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+// exp((l - top) / temperature) in units of 2^-42, to the nearest: e^z = 2^(m / 32) e^x with
+// m = rint(32 z / ln 2) and x = z - m ln 2 / 32, |x| <= 0.0109, e^x by its series up to
+// x^5 (the next term is below 2^-48). m needs no care, so it is taken in fp32; z and x are
+// f64. `pow2` holds 2^(j / 32) in LDS. (The bins of 64 rows of 128,256 take 14.6 us, with a series
+// to x^12 and no table 17.0.)
+struct Masses {
+    float top, c;
+    double dtop, inv_t;
+    const double* pow2;
+    __device__ __forceinline__ Masses(float top_, double inv_t_, const double* pow2_)
+        : top(top_), c((float)(inv_t_ * 46.166241308446828)), dtop(top_), inv_t(inv_t_), pow2(pow2_) {}
+    __device__ __forceinline__ uint64_t operator()(float l) const {
+        if (l == top) return 1ull << kMassBits;
+        const float m = rintf((l - top) * c);
+        if (!(m > -2000.f)) return 0;  // (an infinite top leaves only its equals)
+        const double x = fma((double)m, -0.021660849392498290, ((double)l - dtop) * inv_t);
+        double p = 1.0 / 120.0;
+        p = fma(p, x, 1.0 / 24.0);
+        p = fma(p, x, 1.0 / 6.0);
+        p = fma(p, x, 0.5);
+        p = fma(p, x, 1.0);
+        p = fma(p, x, 1.0);
+        const int i = (int)m;
+        const double scale = __longlong_as_double(__double_as_longlong(pow2[i & 31]) +
+                                                  ((long long)(kMassBits + (i >> 5)) << 52));
+        // adding 2^52 leaves the rounded whole number in the low mantissa bits (p scale <= 2^42)
+        return (uint64_t)__double_as_longlong(fma(p, scale, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+    }
+};
+// (the workgroup's barrier before the first use is the caller's)
+__device__ __forceinline__ void fill_pow2(double* pow2) {
+    if (threadIdx.x < 32) pow2[threadIdx.x] = exp2((double)threadIdx.x / 32.0);
 }
 
 // floor(v * mass) and ceil(v * mass) for 0 <= v <= 1.
@@ -160,7 +168,7 @@ __device__ __forceinline__ uint64_t block_sum(RowShared& sh, uint64_t v) {
 }
 
 // The key at which the count (by_mass: the mass) of the candidates in order first reaches `target` (>= 1, reachable).
-__device__ Cut select(RowShared& sh, const float* row, int n, float top, double inv_t, bool by_mass, uint64_t target) {
+__device__ Cut select(RowShared& sh, const float* row, int n, const Masses& mass_of, bool by_mass, uint64_t target) {
     uint32_t prefix = 0;
     uint64_t above = 0;
     unsigned count = 0;
@@ -173,7 +181,7 @@ __device__ Cut select(RowShared& sh, const float* row, int n, float top, double 
             if (!k || (k & mask) != prefix) continue;
             const uint32_t digit = (k >> shift) & 255;
             atomicAdd(&sh.count[digit], 1u);
-            const uint64_t m = mass_of(logit_of(k), top, inv_t);
+            const uint64_t m = mass_of(logit_of(k));
             if (m) atomicAdd(&sh.mass[digit], (unsigned long long)m);
         }
         __syncthreads();
@@ -232,16 +240,15 @@ __device__ int index_of(RowShared& sh, const float* row, int n, uint32_t key, ui
 }
 
 // The whole row: (token, probability).
-__device__ void sample_row(RowShared& sh, const float* row, int n, const Settings& s, uint32_t best, int* token,
+__device__ void sample_row(RowShared& sh, const float* row, int n, const Settings& s, const Masses& mass_of, int* token,
                            float* prob) {
-    const float top = logit_of(best);
     uint64_t total = 0, large = 0;
     unsigned candidates = 0;
     const uint64_t least = least_mass(s);
     for (int i = threadIdx.x; i < n; i += kRowThreads) {
         const uint32_t k = key_of(row[i]);
         if (!k) continue;
-        const uint64_t m = mass_of(logit_of(k), top, s.inv_t);
+        const uint64_t m = mass_of(logit_of(k));
         total += m;
         ++candidates;
         if (m >= least) large += m;
@@ -251,19 +258,19 @@ __device__ void sample_row(RowShared& sh, const float* row, int n, const Setting
     candidates = (unsigned)block_sum(sh, candidates);
     uint64_t kept = total;
     if (s.k && (unsigned)s.k < candidates) {
-        const Cut c = select(sh, row, n, top, s.inv_t, false, s.k);
-        kept = c.above + (s.k - c.count) * mass_of(logit_of(c.key), top, s.inv_t);
+        const Cut c = select(sh, row, n, mass_of, false, s.k);
+        kept = c.above + (s.k - c.count) * mass_of(logit_of(c.key));
     }
     if (s.p < 1.f) {
         const uint64_t target = p_target(s, kept);
-        const Cut c = select(sh, row, n, top, s.inv_t, true, target);
-        const uint64_t m = mass_of(logit_of(c.key), top, s.inv_t);
+        const Cut c = select(sh, row, n, mass_of, true, target);
+        const uint64_t m = mass_of(logit_of(c.key));
         kept = c.above + (target - c.above + m - 1) / m * m;
     }
     kept = min(kept, large);
     const uint64_t at = u_target(s, kept);
-    const Cut c = select(sh, row, n, top, s.inv_t, true, at + 1);
-    const uint64_t m = mass_of(logit_of(c.key), top, s.inv_t);
+    const Cut c = select(sh, row, n, mass_of, true, at + 1);
+    const uint64_t m = mass_of(logit_of(c.key));
     *token = index_of(sh, row, n, c.key, (at - c.above) / m);
     *prob = (float)((double)m / (double)kept);
 }
@@ -405,6 +412,7 @@ __global__ void __launch_bounds__(kThreads) sample_bounds_kernel(SampleArgs a, v
 __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SampleArgs a, void* ws, int slices) {
     __shared__ unsigned long long mass[kBins];
     __shared__ unsigned count[kBins];
+    __shared__ double pow2[32];
     const int r = blockIdx.y, slice = blockIdx.x;
     const RowWork w = row_work(ws, r, slices);
     Slice logits(a, r, slice, slices);
@@ -415,13 +423,15 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SampleArgs a, voi
     const bool counts = s.k, masses = !s.k || s.k > kFewKept;
     mass[threadIdx.x] = 0;
     count[threadIdx.x] = 0;
+    fill_pow2(pow2);
+    const Masses mass_of(bins.top, s.inv_t, pow2);
     __syncthreads();
     logits.walk([&](int, float l) {
         if (!(l > -INFINITY)) return;
         const int bin = bins.at(l);
         if (counts) atomicAdd(&count[bin], 1u);
         if (masses) {
-            const uint64_t m = mass_of(l, bins.top, s.inv_t);
+            const uint64_t m = mass_of(l);
             if (m) atomicAdd(&mass[bin], (unsigned long long)m);
         }
     });
@@ -434,11 +444,7 @@ __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SampleArgs a, voi
 template <typename T>
 __device__ __forceinline__ T scan(T v, T* part) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const T u = __shfl_up(v, d);
-        if (lane >= d) v += u;
-    }
+    v = wave_scan(v);
     __syncthreads();
     if (lane == 63) part[wave] = v;
     __syncthreads();
@@ -648,7 +654,7 @@ __device__ void rank_list(unsigned long long* v, unsigned* rank, int n) {
 }
 // Longer lists of a row with bins: by bins (the largest logits have the lowest), then by
 // counting within each. False, and nothing changed, where a bin has more than kPerBin values.
-constexpr unsigned kPerBin = 64;
+constexpr unsigned kPerBin = 512;
 struct BinSort {
     unsigned count[kBins], start[kBins], part[kThreads / 64], most;
 };
@@ -709,16 +715,16 @@ struct DrawShared {
 // each. A list that starts with the row's first candidate needs no more; otherwise
 // each bin's own run continues from what lies above the bin.
 template <int PER>
-__device__ void draw(const SampleArgs& a, void* ws, int slices, int r, const Settings& s, const Bound& b,
-                     const Bins& bins, const unsigned long long* list, unsigned n, DrawShared& sh) {
+__device__ void draw(const SampleArgs& a, void* ws, int slices, int r, const Settings& s, const Bins& bins,
+                     const Masses& mass_of, const unsigned long long* list, unsigned n,
+                     DrawShared& sh) {
     const bool prefix = !slices || (s.k && s.k <= kFewKept);
-    const float top = logit_of((uint32_t)(b.best >> 32));
     const unsigned i0 = threadIdx.x * PER;
     uint64_t m[PER], end[PER], sum = 0;
     unsigned rank[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        m[j] = i0 + j < n ? mass_of(logit_of((uint32_t)(list[i0 + j] >> 32)), top, s.inv_t) : 0;
+        m[j] = i0 + j < n ? mass_of(logit_of((uint32_t)(list[i0 + j] >> 32))) : 0;
         sum += m[j];
     }
     uint64_t run = scan((unsigned long long)sum, sh.part) - sum;
@@ -790,7 +796,9 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a, v
         DrawShared l;
     } sh;
     __shared__ unsigned listed;
+    __shared__ double pow2[32];
     const int r = blockIdx.x;
+    fill_pow2(pow2);  // (barriers follow before it is read)
     const float* row = a.logits + r * a.ld;
     const Settings s = settings_of(a, r);
     int token = -1;
@@ -836,7 +844,8 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a, v
                 n = kList + 1;
             }
             if (n > kList) {
-                sample_row(sh.row, row, a.n, s, (uint32_t)(b.best >> 32), &token, &prob);
+                __syncthreads();
+                sample_row(sh.row, row, a.n, s, Masses(logit_of((uint32_t)(b.best >> 32)), s.inv_t, pow2), &token, &prob);
                 if (threadIdx.x == 0) {
                     a.tokens[r] = token;
                     if (a.probs) a.probs[r] = prob;
@@ -854,8 +863,9 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a, v
         token = (int)~(uint32_t)b.best;
         prob = 1.f;
     } else if (b.best) {
-        if (n <= kThreads) draw<1>(a, ws, slices, r, s, b, bins, list, n, sh.l);
-        else draw<kList / kThreads>(a, ws, slices, r, s, b, bins, list, n, sh.l);
+        const Masses mass_of(logit_of((uint32_t)(b.best >> 32)), s.inv_t, pow2);
+        if (n <= kThreads) draw<1>(a, ws, slices, r, s, bins, mass_of, list, n, sh.l);
+        else draw<kList / kThreads>(a, ws, slices, r, s, bins, mass_of, list, n, sh.l);
         return;
     }
     if (threadIdx.x == 0) {
