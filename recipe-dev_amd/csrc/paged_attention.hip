@@ -70,7 +70,7 @@ struct AttnArgs {
     // reference and weight sum), and for each token and head of a group where its are
     float* o;           // [parts][head_dim]
     float2* ml;         // [parts]
-    int2* info;         // [tokens][group]: live splits, first item (paged_few_kernel); null: nothing is split
+    int2* info;         // [tokens][group]: live splits, 32 first item + row (paged_few_kernel); null: nothing is split
     int64_t parts;
 };
 
@@ -492,6 +492,11 @@ __device__ __forceinline__ void put4(const AttnArgs& a, bool f16_out, bool whole
     }
 }
 
+// The factor of sums with reference m when they join others with reference `to` >= m (sums
+// without a reference are 0, or NaN, which stays).
+__device__ __forceinline__ float part_weight(float m, float l, float to) {
+    return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - to);
+}
 __device__ __forceinline__ float reciprocal(float l) { return l == 0.f ? 0.f : 1.f / l; }  // (no key: zeros)
 
 // ------------------------------------------- few rows: keys over the waves ----
@@ -682,7 +687,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
     const int64_t part0 = ((int64_t)item.id * a.c.kv_heads + kh) * TM;
     if (a.info && kh == 0 && item.split == 0)
         for (int u = threadIdx.x; u < rows; u += 256)
-            a.info[(int64_t)t.token0 * a.group + t.row0 + u] = make_int2(item.live, item.id);
+            a.info[(int64_t)t.token0 * a.group + t.row0 + u] = make_int2(item.live, item.id << 5 | u);
     for (int u = threadIdx.x; u < rows * (HD / 4); u += 256) {
         const int row = u / (HD / 4), piece = u % (HD / 4);
         float m = sums[0][row].x, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -691,7 +696,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 ml = sums[i][row];
-            const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml.x - m);
+            const float f = part_weight(ml.x, ml.y, m);
             const float4 x = *reinterpret_cast<const float4*>(lds + i * 2 * HALF + row * HD * 4 + (piece ^ (row & 15)) * 16);
             sum = fmaf(f, ml.y, sum);
             v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
@@ -806,67 +811,58 @@ __global__ void __launch_bounds__(64 * many_waves(HD), many_waves(HD) / 4) paged
 
 // ---------------------------------------------------------- the splits' join ----
 
-// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's live splits. A
-// workgroup per row (token, query head): HD / 4 threads take a split's 16-byte
-// columns, the other threads further splits, all requested at once.
-template <int HD, bool F32>
+// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's live splits. HD / 4
+// threads take a split's 16-byte columns, SIDE of them in a row (token, query head) take every
+// SIDE-th split, four at a time.
+template <int HD, int SIDE, bool F32>
 __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a, bool few) {
-    constexpr int TPR = HD / 4, SIDE = 256 / TPR, PER = kMaxSplits / SIDE;
-    __shared__ float4 part[256];
-    __shared__ float2 sums[SIDE];
+    constexpr int TPR = HD / 4, ROWS = 256 / (TPR * SIDE);
+    __shared__ float4 part[SIDE > 1 ? 256 : 1];
+    __shared__ float2 sums[SIDE > 1 ? SIDE : 1];
     const int heads = a.group * a.c.kv_heads;
-    const int token = blockIdx.x / heads, head = blockIdx.x % heads, kh = head / a.group;
-    const int col = threadIdx.x % TPR, side = threadIdx.x / TPR;
+    const int64_t unit = (int64_t)blockIdx.x * ROWS + threadIdx.x / (TPR * SIDE);
+    if (unit >= (int64_t)a.b.tokens * heads) return;  // (SIDE > 1: a row per workgroup, all of it leaves)
+    const int token = (int)(unit / heads), head = (int)(unit % heads), kh = head / a.group;
+    const int col = threadIdx.x % TPR, side = threadIdx.x / TPR % SIDE;
     const int2 info = a.info[(int64_t)token * a.group + head % a.group];
     const int from = a.b.q_start[0], to = a.b.q_start[a.b.seqs];
     // (rows of no sequence have no info; that of rows of starts out of order may be an older call's)
     const int live = info.x;
     if (token < from || token >= to || live <= 1 || live > kMaxSplits) return;
-    int64_t at = (int64_t)token * heads + head, next = (int64_t)a.b.tokens * heads;
+    int64_t at = unit, next = (int64_t)a.b.tokens * heads;
     if (few) {
-        // the row's number in its tile: rows of a sequence's tiles start at the sequence's first
-        const int seq = last_seq(a.b.seqs, [&](int s) { return a.b.q_start[s] <= token; });
-        const int row = (token - start_of(a.b, seq)) * a.group + head % a.group;
-        at = ((int64_t)info.y * a.c.kv_heads + kh) * 32 + (row & 31);
+        at = ((int64_t)(info.y >> 5) * a.c.kv_heads + kh) * 32 + (info.y & 31);
         next = (int64_t)a.c.kv_heads * 32;
     }
     if (at < 0 || at + (live - 1) * next >= a.parts) return;
-    float4 x[PER];
-    float2 ml[PER];
+    float m = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](float2 ml, float4 x) {
+        const float to = fmaxf(m, ml.x);
+        const float f = part_weight(m, sum, to), g = part_weight(ml.x, ml.y, to);
+        m = to;
+        sum = f * sum + g * ml.y;
+        v[0] = f * v[0] + g * x.x, v[1] = f * v[1] + g * x.y, v[2] = f * v[2] + g * x.z, v[3] = f * v[3] + g * x.w;
+    };
+    for (int c = side; c < live; c += 4 * SIDE) {
+        float4 x[4];
+        float2 ml[4];
 #pragma unroll
-    for (int k = 0; k < PER; ++k)
-        if (k * SIDE < live) {
-            const int64_t row = at + min(side + k * SIDE, live - 1) * next;
+        for (int k = 0; k < 4; ++k) {
+            const int64_t row = at + min(c + k * SIDE, live - 1) * next;
             x[k] = *reinterpret_cast<const float4*>(a.o + row * HD + 4 * col);
             ml[k] = a.ml[row];
         }
-    float m = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < PER; ++k)
-        if (side + k * SIDE < live) m = fmaxf(m, ml[k].x);
+        for (int k = 0; k < 4; ++k)
+            if (c + k * SIDE < live) add(ml[k], x[k]);
+    }
+    if constexpr (SIDE > 1) {
+        part[threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
+        if (col == 0) sums[side] = make_float2(m, sum);
+        __syncthreads();
+        if (side) return;
 #pragma unroll
-    for (int k = 0; k < PER; ++k)
-        if (side + k * SIDE < live) {
-            const float f = ml[k].x == -INFINITY ? (ml[k].y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(ml[k].x - m);
-            sum = fmaf(f, ml[k].y, sum);
-            v[0] = fmaf(f, x[k].x, v[0]), v[1] = fmaf(f, x[k].y, v[1]);
-            v[2] = fmaf(f, x[k].z, v[2]), v[3] = fmaf(f, x[k].w, v[3]);
-        }
-    part[threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
-    if (col == 0) sums[side] = make_float2(m, sum);
-    __syncthreads();
-    if (side) return;
-    m = -INFINITY, sum = 0.f;
-    v[0] = v[1] = v[2] = v[3] = 0.f;
-#pragma unroll
-    for (int k = 0; k < SIDE; ++k) m = fmaxf(m, sums[k].x);
-#pragma unroll
-    for (int k = 0; k < SIDE; ++k) {
-        const float2 s = sums[k];
-        const float4 y = part[k * TPR + col];
-        const float f = s.x == -INFINITY ? (s.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(s.x - m);
-        sum = fmaf(f, s.y, sum);
-        v[0] = fmaf(f, y.x, v[0]), v[1] = fmaf(f, y.y, v[1]), v[2] = fmaf(f, y.z, v[2]), v[3] = fmaf(f, y.w, v[3]);
+        for (int k = 1; k < SIDE; ++k) add(sums[k], part[k * TPR + col]);
     }
     const float inv = reciprocal(sum);
 #pragma unroll
@@ -889,13 +885,14 @@ AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int gro
     AttnPlan p;
     const int heads = kv_heads * group;
     // The few-rows form where the sequences' rows fill at most half of a many-rows tile, or where there
-    // are so few that its tiles leave CUs idle. 32/8 heads of 128, fp16, few against many, us: 32
-    // sequences of 128 rows per kv head over 6,000 positions 238 / 341, of 256 398 / 350; one sequence of
-    // 1024 rows over 1,000 29 / 35, of 4096 without context 51 / 50; four of 2048 over 6,000 357 / 221.
-    // Heads of 256 (four waves a tile): one of 512 rows over 1,000 34 / 40, of 2048 65 / 57.
+    // are so few that its tiles leave CUs idle: up to 768, 512 or 128 tiles of 32 rows over all heads (64,
+    // 128, 256 dims; 256 CUs). Over 222 batches of 1 to 16 sequences, 64 to 1024 new tokens and 0 to 6,000
+    // cached ones the choice takes 1 %, 2 % and 5 % more than the better form. Few against many, 32/8
+    // heads of 128, fp16, us: 32 sequences of 128 rows over 6,000 positions 238 / 341, of 256 398 / 350; one
+    // of 1024 rows over 1,000 23 / 27; four of 2048 over 6,000 350 / 221.
     p.tiles = (int64_t)tokens * group / 32 + seqs;
     p.few = (int64_t)tokens * group <= (int64_t)16 * many_waves(hd) * seqs ||
-            (int64_t)tokens * heads / 32 <= (hd == 256 ? cus / 2 : 2 * cus);
+            (int64_t)tokens * heads / 32 <= (hd == 64 ? 3 * cus : hd == 128 ? 2 * cus : cus / 2);
     if (p.few) {
         // Two items per CU over the whole batch (32 requests of 60 to 8,192 positions: 35.1 us; one
         // per CU 37.6, four 37.6), of two steps for each wave at least (one request at 4,097: 10.5 us; of
@@ -907,9 +904,11 @@ AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int gro
         p.parts = p.join ? (p.tiles + p.splits) * kv_heads * 32 : 0;
     } else {
         p.tiles = (int64_t)tokens * group / (32 * many_waves(hd)) + seqs;
-        p.min_chunk = 512;
+        // Keys are split where the tiles take at most half of the CUs (at less, a split's uneven second part
+        // costs more than it gives: eight sequences of 300 tokens, 8/4 heads of 256, 41 us split, 25 whole).
+        p.min_chunk = 128;
         const int64_t wgs = p.tiles * kv_heads;
-        int64_t s = wgs >= cus ? 1 : (cus + wgs - 1) / wgs;
+        int64_t s = cus / wgs;
         const int64_t most = (cap + p.min_chunk - 1) / p.min_chunk;
         if (s > most) s = most;
         p.splits = (int)(s > kMaxSplits ? kMaxSplits : s < 1 ? 1 : s);
@@ -937,8 +936,15 @@ hipError_t launch_attention_hd(const AttnPlan& p, const AttnArgs& a, hipStream_t
     else hipLaunchKernelGGL((paged_many_kernel<HD, F32>), grid, dim3(64 * many_waves(HD)), lds, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.join) return e;
-    hipLaunchKernelGGL((paged_join_kernel<HD, F32>), dim3((unsigned)(a.b.tokens * a.group * a.c.kv_heads)), dim3(256), 0,
-                       stream, a, p.few);
+    // A workgroup per row for few of them, for 1024 / HD rows of many (eight sequences of 300 tokens, 16 heads of
+    // 64: 24 us less). One row of 33 splits: 3.8 us by a workgroup, 6.3 by HD / 4 threads.
+    const int64_t rows = (int64_t)a.b.tokens * a.group * a.c.kv_heads;
+    constexpr int SIDE = 1024 / HD;
+    if (rows <= 2048)
+        hipLaunchKernelGGL((paged_join_kernel<HD, SIDE, F32>), dim3((unsigned)rows), dim3(256), 0, stream, a, p.few);
+    else
+        hipLaunchKernelGGL((paged_join_kernel<HD, 1, F32>), dim3((unsigned)((rows + SIDE - 1) / SIDE)), dim3(256), 0,
+                           stream, a, p.few);
     return hipGetLastError();
 }
 

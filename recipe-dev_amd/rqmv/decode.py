@@ -22,6 +22,11 @@ next product's prologue, which also takes the sum of squares for its norm and
 writes the updated stream (two buffers, alternating); the rotary and the cache
 append are folded into attention (rqmv_attention_rope). Six launches per
 layer: QKV, attention (two), output, gate/up, down. The residual stream and every activation are fp32; the KV cache is fp16.
+
+A step with a Sampling (DecodeModel.sampling) draws its token instead:
+rqmv_sample at the settings and the random number that the Sampling's device
+buffers hold when the step runs, so a captured step draws a new token at every
+replay.
 """
 from __future__ import annotations
 
@@ -30,7 +35,8 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import (EPI_GLU, EPI_PLAIN, DeviceBuffer, Graph, Stream, Weight, advance, argmax, argmax_workspace,
-               attention_rope, attention_workspace, embed_row, glu_weight, matvec_fused, rope_table)
+               attention_rope, attention_workspace, embed_row, glu_weight, matvec_fused, rope_table, sample,
+               sample_workspace)
 
 
 @dataclass(frozen=True)
@@ -99,6 +105,25 @@ class LayerTensors:
         if sum(r for _, r, _ in runs) != q_rows + 2 * kv_rows:
             raise ValueError("qkv_parts must hold the Q, K and V rows")
         return runs
+
+
+class Sampling:
+    """How a step draws its token (rqmv_sample): temperature, top_k, top_p and
+    min_p, and the random number u in [0, 1) of the next step (set_random before
+    each). prob holds the drawn token's probability afterwards."""
+
+    def __init__(self, vocab: int, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0):
+        f32 = lambda v: DeviceBuffer.from_array(np.array([v], dtype=np.float32))  # noqa: E731
+        self.u, self.prob = f32(0.0), f32(0.0)
+        self.temperature, self.top_p, self.min_p = f32(temperature), f32(top_p), f32(min_p)
+        self.top_k = DeviceBuffer.from_array(np.array([top_k], dtype=np.int32))
+        self.workspace = sample_workspace(1, vocab)
+
+    def set_random(self, u: float):
+        self.u.upload(np.array([u], dtype=np.float32))
+
+    def read_prob(self) -> float:
+        return float(self.prob.download(np.float32, 1)[0])
 
 
 class DecodeModel:
@@ -195,10 +220,14 @@ class DecodeModel:
             raise ValueError(f"{steps} step(s) from position {self._pos} run past the cache's {self.max_ctx} "
                              "positions: the token window is outside the placement capacity")
 
-    def step(self, stream: Stream | None = None):
+    def sampling(self, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0) -> Sampling:
+        """Settings for steps that draw their token (step, enqueue_step, capture)."""
+        return Sampling(self.shape.vocab, temperature, top_k, top_p, min_p)
+
+    def step(self, stream: Stream | None = None, sampling: Sampling | None = None):
         """One eager step at the current position; raises before a step past the cache."""
         self._room(1)
-        self.enqueue_step(stream)
+        self.enqueue_step(stream, sampling=sampling)
         self._pos += 1
 
     def replay(self, graph: Graph, stream: Stream, times: int = 1):
@@ -218,9 +247,10 @@ class DecodeModel:
                                "token window is outside the placement capacity")
 
     # ----------------------------------------------------------------- step
-    def enqueue_step(self, stream: Stream | None = None, layers: int | None = None):
+    def enqueue_step(self, stream: Stream | None = None, layers: int | None = None, sampling: Sampling | None = None):
         """Enqueue one decode step on `stream` (capturable: no allocation, no
-        host synchronisation). `layers` < the decoder's depth runs only the
+        host synchronisation). The next token is the argmax, or drawn as
+        `sampling` says. `layers` < the decoder's depth runs only the
         first `layers` layers before the head (an early exit); read_hidden()
         then returns the stream that layer `layers` would take as input."""
         s = self.shape
@@ -252,12 +282,16 @@ class DecodeModel:
         matvec_fused(self.head, xs[cur], self.logits, EPI_PLAIN, self.out_norm, s.eps, pending, xs[1 - cur],
                      stream=stream)
         self._hidden = xs[1 - cur]
-        argmax(self.logits, s.vocab, self.token, self.argmax_ws, stream)
+        if sampling is None:
+            argmax(self.logits, s.vocab, self.token, self.argmax_ws, stream)
+        else:
+            sample(self.logits, 1, s.vocab, s.vocab, sampling.u, self.token, sampling.workspace, sampling.temperature,
+                   sampling.top_k, sampling.top_p, sampling.min_p, sampling.prob, stream)
         advance(self.pos, stream)
 
-    def capture(self, stream: Stream) -> Graph:
+    def capture(self, stream: Stream, sampling: Sampling | None = None) -> Graph:
         """A HIP graph of one step; each launch decodes the next token."""
-        return Graph(stream, lambda: self.enqueue_step(stream))
+        return Graph(stream, lambda: self.enqueue_step(stream, sampling=sampling))
 
     def read_logits(self) -> np.ndarray:
         self._check_inside()
