@@ -280,7 +280,7 @@ int rqmv_attention_rope(const float* qkv, const float* rope_table, void* k_cache
  * 0; rows from q_start[seqs] on belong to no sequence and are padding), the
  * last of its kv_len[s] positions. Its position p lies in block
  * block_table[s * table_stride + p / block_size] at row p % block_size, for p
- * < max_blocks * block_size; a table entry outside 0..blocks-1 is an absent
+ * < max_blocks * block_size (at most 2^30); a table entry outside 0..blocks-1 is an absent
  * page, whose positions are never attended to. positions and slots hold each
  * row's position and slot (-1: none). Each call names the fields it reads;
  * the others may be NULL. */
@@ -350,7 +350,8 @@ int rqmv_qk_norm_rope(const rqmv_paged_batch* batch, const rqmv_paged_cache* cac
 /* Grouped-query attention of the batch's new tokens over their pages: for each
  * query head of the row at position p (rows of q and out: q + row * ldq, out +
  * row * ldo elements, q_heads heads of head_dim) softmax(scale q k) v over the
- * positions max(0, p - window + 1)..p of its sequence (window 0: 0..p) whose
+ * positions max(0, p - window + 1)..p of its sequence (window 0 or above 2^30:
+ * 0..p) whose
  * pages are present, in kv head h / (q_heads / kv_heads); zeros where there is
  * none. The new tokens' own keys and values are in the cache
  * already (rqmv_qk_norm_rope). out has the dtype of q: fp32 rows are computed to fp32
@@ -359,8 +360,8 @@ int rqmv_qk_norm_rope(const rqmv_paged_batch* batch, const rqmv_paged_cache* cac
  * the result, whatever its key and value hold. A NaN or an infinity in a query, or
  * in a key or value attended to, makes its rows non-finite. Rows of no sequence are
  * not written. q_heads is a multiple of kv_heads, both at most 1024; scale is positive; ldq
- * and ldo are multiples of 16 bytes, q and out 16-byte aligned, and out may be q
- * itself only with ldo = ldq. Reads q_start, kv_len, block_table of the batch. One
+ * and ldo are multiples of 16 bytes, q and out 16-byte aligned; out is q itself (ldo
+ * = ldq) or spans none of its memory. Reads q_start, kv_len, block_table of the batch. One
  * launch, two where the keys are split over workgroups: then the workspace (16-byte
  * aligned, rqmv_paged_attention_workspace_size bytes for this batch's counts, cache and
  * q_heads on the current device; 0: may be NULL) holds partial results, and calls

@@ -70,7 +70,7 @@ struct AttnArgs {
     // reference and weight sum), and for each token and head of a group where its are
     float* o;           // [parts][head_dim]
     float2* ml;         // [parts]
-    int2* info;         // [tokens][group]: live splits, 32 first item + row (paged_few_kernel); null: nothing is split
+    int2* info;         // [tokens][group]: live splits, 32 first part + row (paged_few_kernel); null: nothing is split
     int64_t parts;
 };
 
@@ -514,7 +514,8 @@ __device__ __forceinline__ float reciprocal(float l) { return l == 0.f ? 0.f : 1
 // again while it works on the values and the other way round, and a second workgroup
 // on the CU fills the rest. At the end the waves' sums are joined through LDS.
 struct Item {
-    int seq, tile, split, first, chunk, live, id;
+    int seq, tile, split, first, chunk, live;
+    int part;  // its number among the items of split tiles
 };
 
 // A sequence's tiles, and the first and the number of its keys.
@@ -537,11 +538,14 @@ __device__ __forceinline__ int64_t sum_wave(int64_t v) {
     return v;
 }
 
-// Item `number` of the batch (of 256 threads); false: there is none.
+// Item `number` of the batch (of 256 threads); false: there is none. Of the items only those of
+// split tiles have partial results, and these are at most 2 `splits`: a tile of u units in chunks of c < u
+// has at most 2 u / c.
 template <int TM>
 __device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* item) {
-    __shared__ int part[4], found[6];
+    __shared__ unsigned long long upto_of[4];
     __shared__ int64_t totals[4];
+    __shared__ Item found;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     int tiles = 0, first = 0, keys = 0;
     int64_t total = 0;
@@ -549,12 +553,12 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* i
         seq_size<TM>(a, s, &tiles, &first, &keys);
         total += (int64_t)tiles * ((keys + 63) >> 6);
     }
-    if (t == 0) found[0] = -1;
+    if (t == 0) found.seq = -1;
     total = sum_wave(total);
     if (lane == 0) totals[wave] = total;
     __syncthreads();
     total = totals[0] + totals[1] + totals[2] + totals[3];
-    int before = 0;
+    unsigned long long before = 0;  // items, and those of split tiles in the upper half
     for (int s0 = 0; s0 < a.b.seqs; s0 += 256) {
         const int s = s0 + t;
         int items = 0, live = 1, chunk = 1;
@@ -565,29 +569,29 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* i
             live = max((units + chunk - 1) / chunk, 1);
             items = tiles * live;
         }
-        const int upto = (int)wave_scan((unsigned)items);
+        const unsigned long long own = (unsigned long long)(live > 1 ? items : 0) << 32 | (unsigned)items;
+        const unsigned long long upto = wave_scan(own);
         __syncthreads();
-        if (lane == 63) part[wave] = upto;
+        if (lane == 63) upto_of[wave] = upto;
         __syncthreads();
-        int from = before + upto - items;
+        unsigned long long from = before + upto - own;
         for (int w = 0; w < 4; ++w) {
-            from += w < wave ? part[w] : 0;
-            before += part[w];
+            from += w < wave ? upto_of[w] : 0;
+            before += upto_of[w];
         }
-        if (number >= from && number < from + items) {
-            found[0] = s, found[1] = (number - from) / live, found[2] = (number - from) % live, found[3] = first;
-            found[4] = chunk * 64, found[5] = live;
-        }
+        const int at = number - (int)(unsigned)from;
+        if (at >= 0 && at < items)
+            found = Item{s, at / live, at % live, first, chunk * 64, live, (int)(from >> 32) + at};
     }
     __syncthreads();
-    if (found[0] < 0) return false;
-    item->seq = __builtin_amdgcn_readfirstlane(found[0]);
-    item->tile = __builtin_amdgcn_readfirstlane(found[1]);
-    item->split = __builtin_amdgcn_readfirstlane(found[2]);
-    item->first = __builtin_amdgcn_readfirstlane(found[3]);
-    item->chunk = __builtin_amdgcn_readfirstlane(found[4]);
-    item->live = __builtin_amdgcn_readfirstlane(found[5]);
-    item->id = number;
+    if (found.seq < 0) return false;
+    item->seq = __builtin_amdgcn_readfirstlane(found.seq);
+    item->tile = __builtin_amdgcn_readfirstlane(found.tile);
+    item->split = __builtin_amdgcn_readfirstlane(found.split);
+    item->first = __builtin_amdgcn_readfirstlane(found.first);
+    item->chunk = __builtin_amdgcn_readfirstlane(found.chunk);
+    item->live = __builtin_amdgcn_readfirstlane(found.live);
+    item->part = __builtin_amdgcn_readfirstlane(found.part);
     return true;
 }
 
@@ -684,10 +688,10 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
     __syncthreads();
     const int rows = min(t.rows - t.row0, TM);
     const bool whole = item.live <= 1;
-    const int64_t part0 = ((int64_t)item.id * a.c.kv_heads + kh) * TM;
+    const int64_t part0 = ((int64_t)item.part * a.c.kv_heads + kh) * TM;
     if (a.info && kh == 0 && item.split == 0)
         for (int u = threadIdx.x; u < rows; u += 256)
-            a.info[(int64_t)t.token0 * a.group + t.row0 + u] = make_int2(item.live, item.id << 5 | u);
+            a.info[(int64_t)t.token0 * a.group + t.row0 + u] = make_int2(item.live, item.part << 5 | u);
     for (int u = threadIdx.x; u < rows * (HD / 4); u += 256) {
         const int row = u / (HD / 4), piece = u % (HD / 4);
         float m = sums[0][row].x, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
@@ -901,7 +905,7 @@ AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int gro
         const int64_t want = 2 * cus / kv_heads, most = p.tiles * ((cap + p.min_chunk - 1) / p.min_chunk);
         p.splits = (int)(most < want ? most : want < 1 ? 1 : want);
         p.join = cap > p.min_chunk;
-        p.parts = p.join ? (p.tiles + p.splits) * kv_heads * 32 : 0;
+        p.parts = p.join ? (int64_t)2 * p.splits * kv_heads * 32 : 0;
     } else {
         p.tiles = (int64_t)tokens * group / (32 * many_waves(hd)) + seqs;
         // Keys are split where the tiles take at most half of the CUs (at less, a split's uneven second part
@@ -975,8 +979,8 @@ hipError_t launch_paged_attention(const PagedBatch& b, const PagedCache& c, cons
     a.b = b;
     a.c = c;
     a.group = group;
-    a.cap = (int)(cap < (1 << 30) ? cap : (1 << 30));
-    a.window = window;
+    a.cap = (int)cap;
+    a.window = window > (1 << 30) ? 0 : window;  // (the table reaches 2^30 positions at most)
     a.scale = scale * 1.44269504088896340736f;
     a.tiles = (int)p.tiles;
     a.splits = p.splits;

@@ -295,7 +295,9 @@ int check_paged_batch(const rqmv_paged_batch* b, const char* what) {
     return RQMV_OK;
 }
 
-int check_paged_table(const rqmv_paged_batch* b, const char* what) {
+int check_paged_table(const rqmv_paged_batch* b, int shift, const char* what) {
+    if (b->max_blocks > (1 << (30 - shift)))
+        return fail(RQMV_EINVAL, std::string(what) + ": max_blocks * block_size must be at most 2^30");
     if (b->max_blocks < 1 || (b->seqs > 1 && (b->table_stride < b->max_blocks || b->table_stride > kPagedMaxStride)))
         return fail(RQMV_EINVAL, std::string(what) + ": max_blocks must be positive and at most table_stride");
     return RQMV_OK;
@@ -819,7 +821,7 @@ int rqmv_paged_plan(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache
     if (!batch->q_start || !batch->kv_len || !batch->block_table || !batch->positions || !batch->slots || !cached_len ||
         !new_len || !free_head || !free_head_out || !status || free_count < 0 || (!free_list && free_count > 0))
         return fail(RQMV_EINVAL, "paged_plan: bad arguments");
-    rc = check_paged_table(batch, "paged_plan");
+    rc = check_paged_table(batch, shift, "paged_plan");
     if (rc != RQMV_OK) return rc;
     hipError_t e = rq::launch_paged_plan(paged_batch(batch), (int)cache->blocks, shift, cached_len, new_len, free_list,
                                          free_count, free_head, free_head_out, status, static_cast<hipStream_t>(stream));
@@ -873,18 +875,17 @@ int rqmv_qk_norm_rope(const rqmv_paged_batch* batch, const rqmv_paged_cache* cac
 }
 
 static int paged_attention_check(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, int q_heads,
-                                 rq::PagedCache* c, DeviceInfo* info) {
+                                 rq::PagedCache* c) {
     int rc = check_paged_cache(cache, "paged_attention", c);
     if (rc == RQMV_OK) rc = check_paged_batch(batch, "paged_attention");
-    if (rc == RQMV_OK) rc = check_paged_table(batch, "paged_attention");
+    if (rc == RQMV_OK) rc = check_paged_table(batch, c->block_shift, "paged_attention");
     if (rc != RQMV_OK) return rc;
     if (q_heads <= 0 || q_heads > kPagedMaxHeads || q_heads % c->kv_heads)
         return fail(RQMV_EINVAL, "paged_attention: q_heads must be a multiple of kv_heads, at most 1024");
     if (!rq::paged_attention_fits(paged_batch(batch), *c, q_heads))
         return fail(RQMV_EINVAL, "paged_attention: tokens * q_heads must be at most 2^26, and (tokens * q_heads / kv_heads "
                                  "/ 32 + seqs) * kv_heads at most 2^23");
-    const int dev = current_device(info);
-    return dev < 0 ? dev : RQMV_OK;
+    return RQMV_OK;
 }
 
 int rqmv_paged_attention_workspace_size(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, int q_heads,
@@ -892,8 +893,10 @@ int rqmv_paged_attention_workspace_size(const rqmv_paged_batch* batch, const rqm
     if (!bytes) return fail(RQMV_EINVAL, "paged_attention: NULL size");
     rq::PagedCache c;
     DeviceInfo info;
-    const int rc = paged_attention_check(batch, cache, q_heads, &c, &info);
+    const int rc = paged_attention_check(batch, cache, q_heads, &c);
     if (rc != RQMV_OK) return rc;
+    const int dev = current_device(&info);
+    if (dev < 0) return dev;
     *bytes = rq::paged_attention_workspace(paged_batch(batch), c, q_heads, info.cus);
     return RQMV_OK;
 }
@@ -905,7 +908,7 @@ int rqmv_paged_attention(const rqmv_paged_batch* batch, const rqmv_paged_cache* 
         return fail(RQMV_EINVAL, "paged_attention: bad arguments");
     rq::PagedCache c;
     DeviceInfo info;
-    const int rc = paged_attention_check(batch, cache, q_heads, &c, &info);
+    const int rc = paged_attention_check(batch, cache, q_heads, &c);
     if (rc != RQMV_OK) return rc;
     if (!batch->q_start || !batch->kv_len || !batch->block_table)
         return fail(RQMV_EINVAL, "paged_attention: q_start, kv_len and block_table are needed");
@@ -915,6 +918,13 @@ int rqmv_paged_attention(const rqmv_paged_batch* batch, const rqmv_paged_cache* 
         return fail(RQMV_EINVAL, "paged_attention: ldq or ldo is too small, too large or no multiple of 16 bytes");
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15)
         return fail(RQMV_EINVAL, "paged_attention: q, out and the workspace must be 16-byte aligned");
+    const uintptr_t span = (uintptr_t)((batch->tokens > 1 ? (batch->tokens - 1) * ldq : 0) + row) * size;
+    const uintptr_t out_span = (uintptr_t)((batch->tokens > 1 ? (batch->tokens - 1) * ldo : 0) + row) * size;
+    const bool same = q == out && (batch->tokens == 1 || ldq == ldo);
+    if (!same && (uintptr_t)q < (uintptr_t)out + out_span && (uintptr_t)out < (uintptr_t)q + span)
+        return fail(RQMV_EINVAL, "paged_attention: out must be q itself or lie outside it");
+    const int dev = current_device(&info);
+    if (dev < 0) return dev;
     const size_t need = rq::paged_attention_workspace(paged_batch(batch), c, q_heads, info.cus);
     if (workspace_bytes < need || (need && !workspace)) return fail(RQMV_EINVAL, "paged_attention: workspace too small");
     hipError_t e = rq::launch_paged_attention(paged_batch(batch), c, q, dtype == RQMV_DTYPE_F32, ldq, q_heads, scale,

@@ -29,7 +29,7 @@ def cache(blocks=10, block=16, kv=2, hd=64, k=A, v=A):
 BAD_CACHES = [dict(block=8), dict(block=48), dict(block=512), dict(block=0), dict(blocks=0), dict(blocks=-1),
               dict(blocks=1 << 27)]
 BAD_BATCHES = [dict(seqs=0), dict(seqs=8193), dict(tokens=0), dict(tokens=(1 << 20) + 1)]
-BAD_TABLES = [dict(max_blocks=0), dict(max_blocks=5, stride=4), dict(stride=1 << 41)]
+BAD_TABLES = [dict(max_blocks=0), dict(max_blocks=5, stride=4), dict(stride=1 << 41), dict(max_blocks=(1 << 26) + 1)]
 
 
 def refused(call, *args, **kw):
@@ -125,6 +125,11 @@ def test_paged_attention_refuses_batches(kw):
     dict(q=At(None)), dict(out=At(None)), dict(dtype=2), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
     dict(scale=float("inf")), dict(window=-1), dict(q_heads=3), dict(q_heads=0), dict(q_heads=1026)])
 def test_paged_attention_refuses_arguments(kw):
+    refused(attend, **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(out=At(A.ptr + 512)), dict(q=At(A.ptr + 16)), dict(ldo=512), dict(dtype=1, ldq=512)])
+def test_paged_attention_refuses_overlapping_outputs(kw):
     refused(attend, **kw)
 
 
