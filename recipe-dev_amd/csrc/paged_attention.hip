@@ -170,7 +170,8 @@ struct Pages {
 };
 
 // The 16 keys from `key` on of one page (id clamped into the cache) of `cache`, to LDS.
-template <int HD, bool VALUES>
+// (FROM..TO-1: which of its instructions)
+template <int HD, bool VALUES, int FROM = 0, int TO = Lay<HD>::NI>
 __device__ __forceinline__ void load_group(const __half* cache, const PagedCache& c, int kh, int id, int key,
                                            uint32_t lds) {
     typedef Lay<HD> L;
@@ -178,7 +179,7 @@ __device__ __forceinline__ void load_group(const __half* cache, const PagedCache
     const int64_t row = (((int64_t)id * c.kv_heads + kh) << c.block_shift) + (key & ((1 << c.block_shift) - 1));
     const __half* base = cache + row * HD;
 #pragma unroll
-    for (int i = 0; i < L::NI; ++i) {
+    for (int i = FROM; i < TO; ++i) {
         const int r = i * L::RPI + lane / L::PCS;
         const int piece = (lane % L::PCS) ^ (VALUES ? L::vx(r) : L::kx(r));
         load_lds(base, (uint32_t)(r * L::ROW + piece * 16), lds + i * 1024);
@@ -296,6 +297,18 @@ __device__ __forceinline__ void scores(const char* K, const Rows<HD, QT, F32>& w
                 for (int p = 0; p < Rows<HD, QT, F32>::QP; ++p)
                     s[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, w.q[i][k][p], s[i][t], 0, 0, 0);
         }
+    if constexpr (HD == 128 && KT == 2) {
+        // four key operands ahead of their products (2048 tokens over 14,336, fp16: 537 -> 529 us; heads of 64
+        // and 256 lose 3 % and 1 % so)
+        constexpr int READS = HD / 16 * KT, EACH = QT * Rows<HD, QT, F32>::QP;
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int i = 0; i < READS - 4; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 4 * EACH, 0);
+    }
 }
 
 // -infinity for the keys that a row does not see.
@@ -722,14 +735,19 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
 // TM = 32 WAVES rows a tile (prompts, chunks of prompts): bound by the matrix
 // cores and the exponentials. Each wave has 32 rows; the waves share steps of 64 keys in
 // two LDS buffers, one barrier a step. Eight waves (two per SIMD, 256 registers each), so
-// that one multiplies while the other takes exponentials; four where the sums and
-// queries need more registers.
-constexpr int many_waves(int hd) { return hd == 256 ? 4 : 8; }
+// that one multiplies while the other takes exponentials; steps of 32 keys at 256 dims of
+// fp16 (fewer registers: 310 us against 368 with four waves of 64-key steps, 2048 tokens over 6,000, 8/4
+// heads), four waves at 256 dims of fp32. 2048 tokens over 14,336, 32/8 heads of 128,
+// fp16: 528 us, 976 TFLOP/s (a library product of 8192^3: 1162). Four waves of 64 rows took 1224:
+// their sums lay in accumulator registers and were moved at every step.
+constexpr int many_waves(int hd, bool f32) { return hd == 256 && f32 ? 4 : 8; }
+constexpr int many_keys(int hd, bool f32) { return hd == 256 && !f32 ? 32 : 64; }
 
 template <int HD, bool F32>
-__global__ void __launch_bounds__(64 * many_waves(HD), many_waves(HD) / 4) paged_many_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(64 * many_waves(HD, F32), many_waves(HD, F32) / 4) paged_many_kernel(AttnArgs a) {
     typedef Lay<HD> L;
-    constexpr int WAVES = many_waves(HD), TM = 32 * WAVES, KEYS = 64, HALF = KEYS * HD * 2;
+    constexpr int WAVES = many_waves(HD, F32), TM = 32 * WAVES, KEYS = many_keys(HD, F32), KT = KEYS / 32;
+    constexpr int HALF = KEYS * HD * 2;
     extern __shared__ __align__(16) char lds[];
     // the last tiles first: of one sequence's they have the most keys
     const int kh = blockIdx.x % a.c.kv_heads, number = a.tiles - 1 - blockIdx.x / a.c.kv_heads, split = blockIdx.y;
@@ -748,15 +766,24 @@ __global__ void __launch_bounds__(64 * many_waves(HD), many_waves(HD) / 4) paged
     // Step i is in buffer i % 2, keys before values. Of eight waves, four load 16 rows of
     // keys each and four of values; of four, each loads both. Returns which groups are absent.
     auto load = [&](int key0, int buffer) -> unsigned {
-        pages.need(key0 >> pages.shift, (key0 + 48) >> pages.shift);
+        pages.need(key0 >> pages.shift, (key0 + KEYS - 16) >> pages.shift);
         unsigned bad = 0;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) bad |= pages.absent(pages.at((key0 + 16 * g) >> pages.shift)) ? 1u << g : 0u;
-        const int g = wave % 4, key = key0 + 16 * g, id = pages.at(key >> pages.shift);
+        for (int g = 0; g < KEYS / 16; ++g) bad |= pages.absent(pages.at((key0 + 16 * g) >> pages.shift)) ? 1u << g : 0u;
+        const int g = wave % (KEYS / 16), key = key0 + 16 * g, id = pages.at(key >> pages.shift);
         const int page = pages.absent(id) ? 0 : id;
         const uint32_t at = lds0 + buffer * 2 * HALF + g * 16 * L::ROW;
-        if (WAVES == 4 || wave < 4) load_group<HD, false>(a.c.k, a.c, kh, page, key, at);
-        if (WAVES == 4 || wave >= 4) load_group<HD, true>(a.c.v, a.c, kh, page, key, at + HALF);
+        if constexpr (KEYS == 64) {
+            if (WAVES == 4 || wave < 4) load_group<HD, false>(a.c.k, a.c, kh, page, key, at);
+            if (WAVES == 4 || wave >= 4) load_group<HD, true>(a.c.v, a.c, kh, page, key, at + HALF);
+        } else {
+            constexpr int NI = L::NI;
+            const int part = wave >> 1;  // halves of keys' and of values' groups
+            if (part == 0) load_group<HD, false, 0, NI / 2>(a.c.k, a.c, kh, page, key, at);
+            else if (part == 1) load_group<HD, false, NI / 2, NI>(a.c.k, a.c, kh, page, key, at);
+            else if (part == 2) load_group<HD, true, 0, NI / 2>(a.c.v, a.c, kh, page, key, at + HALF);
+            else load_group<HD, true, NI / 2, NI>(a.c.v, a.c, kh, page, key, at + HALF);
+        }
         return bad;
     };
     // the keys that any of the wave's rows sees
@@ -777,15 +804,15 @@ __global__ void __launch_bounds__(64 * many_waves(HD), many_waves(HD) / 4) paged
         const bool masked = key0 < t.all_from || key0 + KEYS > t.all_to || bad;
         if (masked && __syncthreads_or(zero_dead<HD, KEYS>(V, key0, t.end, bad, threadIdx.x, 64 * WAVES))) odd = true;
         if (key0 < wave_to && key0 + KEYS > wave_from) {  // (a wave whose rows see none of the step only loads)
-            f16_t s[1][2];
-            scores<HD, 1, 2, F32>(K, w, s);
-            if (masked) mask_scores<HD, 1, 2, F32>(w, s, key0, bad);
+            f16_t s[1][KT];
+            scores<HD, 1, KT, F32>(K, w, s);
+            if (masked) mask_scores<HD, 1, KT, F32>(w, s, key0, bad);
             float top[1];
-            largest<1, 2>(s, top);
+            largest<1, KT>(s, top);
             move_references<HD, 1, F32>(w, top);
-            h8_t p[1][4][F32 ? 2 : 1];
-            weights<HD, 1, 2, F32>(w, s, p);
-            add_values<HD, 1, 2, F32>(V, w, p);
+            h8_t p[1][2 * KT][F32 ? 2 : 1];
+            weights<HD, 1, KT, F32>(w, s, p);
+            add_values<HD, 1, KT, F32>(V, w, p);
         }
         bad = bad_next;
         buffer ^= 1;
@@ -877,7 +904,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a, bool few) {
 // ------------------------------------------------------------------ launches ----
 
 constexpr int few_lds(int hd) { return 4 * 2 * 32 * hd * 2; }
-constexpr int many_lds(int hd) { return 2 * 2 * 64 * hd * 2; }
+constexpr int many_lds(int hd, bool f32) { return 2 * 2 * many_keys(hd, f32) * hd * 2; }
 
 struct AttnPlan {
     bool few, join;
@@ -885,18 +912,19 @@ struct AttnPlan {
     int64_t tiles, parts;
 };
 
-AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, int cus) {
+AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus) {
     AttnPlan p;
     const int heads = kv_heads * group;
-    // The few-rows form where the sequences' rows fill at most half of a many-rows tile, or where there
-    // are so few that its tiles leave CUs idle: up to 768, 512 or 128 tiles of 32 rows over all heads (64,
-    // 128, 256 dims; 256 CUs). Over 222 batches of 1 to 16 sequences, 64 to 1024 new tokens and 0 to 6,000
-    // cached ones the choice takes 1 %, 2 % and 5 % more than the better form. Few against many, 32/8
-    // heads of 128, fp16, us: 32 sequences of 128 rows over 6,000 positions 238 / 341, of 256 398 / 350; one
-    // of 1024 rows over 1,000 23 / 27; four of 2048 over 6,000 350 / 221.
+    // The few-rows form up to 128 rows a sequence and kv head on average, or where there are so few that
+    // the large tiles leave CUs idle: tiles of 32 rows over all heads up to 4 a CU (64 and 256 dims, fp16),
+    // 2 (128 dims; 64, fp32) or a half (256, fp32, whose large tiles have 128 rows). Over 222
+    // batches of 1 to 16 sequences, 64 to 1024 new tokens and 0 to 6,000 cached ones the choice takes 0.5 to
+    // 4.5 % more than the better form. Few against many, 32/8 heads of 128, fp16, us: 32 sequences of 128
+    // rows over 6,000 positions 238 / 341, of 256 398 / 350; one of 1024 rows over 1,000 23 / 27; four of 2048
+    // over 6,000 350 / 221.
     p.tiles = (int64_t)tokens * group / 32 + seqs;
-    p.few = (int64_t)tokens * group <= (int64_t)16 * many_waves(hd) * seqs ||
-            (int64_t)tokens * heads / 32 <= (hd == 64 ? 3 * cus : hd == 128 ? 2 * cus : cus / 2);
+    const int64_t few_tiles = hd == 128 ? 2 * cus : hd == 64 ? (f32 ? 2 : 4) * cus : f32 ? cus / 2 : 4 * cus;
+    p.few = (int64_t)tokens * group <= (int64_t)128 * seqs || (int64_t)tokens * heads / 32 <= few_tiles;
     if (p.few) {
         // Two items per CU over the whole batch (32 requests of 60 to 8,192 positions: 35.1 us; one
         // per CU 37.6, four 37.6), of two steps for each wave at least (one request at 4,097: 10.5 us; of
@@ -907,7 +935,7 @@ AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int gro
         p.join = cap > p.min_chunk;
         p.parts = p.join ? (int64_t)2 * p.splits * kv_heads * 32 : 0;
     } else {
-        p.tiles = (int64_t)tokens * group / (32 * many_waves(hd)) + seqs;
+        p.tiles = (int64_t)tokens * group / (32 * many_waves(hd, f32)) + seqs;
         // Keys are split where the tiles take at most half of the CUs (at less, a split's uneven second part
         // costs more than it gives: eight sequences of 300 tokens, 8/4 heads of 256, 41 us split, 25 whole).
         p.min_chunk = 128;
@@ -931,13 +959,13 @@ hipError_t launch_attention_hd(const AttnPlan& p, const AttnArgs& a, hipStream_t
     const dim3 grid((unsigned)((p.tiles + (p.few ? p.splits : 0)) * a.c.kv_heads), p.few ? 1 : p.splits);
     const void* f = p.few ? reinterpret_cast<const void*>(paged_few_kernel<HD, F32>)
                           : reinterpret_cast<const void*>(paged_many_kernel<HD, F32>);
-    const int lds = p.few ? few_lds(HD) : many_lds(HD);
+    const int lds = p.few ? few_lds(HD) : many_lds(HD, F32);
     if (lds > 48 * 1024) {
         const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
     }
     if (p.few) hipLaunchKernelGGL((paged_few_kernel<HD, F32>), grid, dim3(256), lds, stream, a);
-    else hipLaunchKernelGGL((paged_many_kernel<HD, F32>), grid, dim3(64 * many_waves(HD)), lds, stream, a);
+    else hipLaunchKernelGGL((paged_many_kernel<HD, F32>), grid, dim3(64 * many_waves(HD, F32)), lds, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.join) return e;
     // A workgroup per row for few of them, for 1024 / HD rows of many (eight sequences of 300 tokens, 16 heads of
@@ -961,8 +989,14 @@ bool paged_attention_fits(const PagedBatch& b, const PagedCache& c, int q_heads)
 
 size_t paged_attention_workspace(const PagedBatch& b, const PagedCache& c, int q_heads, int cus) {
     const int group = q_heads / c.kv_heads;
-    return workspace_bytes(plan_attention(b.tokens, b.seqs, (int64_t)b.max_blocks << c.block_shift, c.kv_heads, group,
-                                          c.head_dim, cus), b.tokens, group, c.head_dim);
+    const int64_t cap = (int64_t)b.max_blocks << c.block_shift;
+    size_t most = 0;
+    for (const bool f32 : {false, true}) {  // (one workspace serves both types)
+        const AttnPlan p = plan_attention(b.tokens, b.seqs, cap, c.kv_heads, group, c.head_dim, f32, cus);
+        const size_t bytes = workspace_bytes(p, b.tokens, group, c.head_dim);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
 }
 
 hipError_t launch_paged_attention(const PagedBatch& b, const PagedCache& c, const void* q, bool f32, int64_t ldq,
@@ -970,7 +1004,7 @@ hipError_t launch_paged_attention(const PagedBatch& b, const PagedCache& c, cons
                                   hipStream_t stream) {
     const int group = q_heads / c.kv_heads;
     const int64_t cap = (int64_t)b.max_blocks << c.block_shift;
-    const AttnPlan p = plan_attention(b.tokens, b.seqs, cap, c.kv_heads, group, c.head_dim, cus);
+    const AttnPlan p = plan_attention(b.tokens, b.seqs, cap, c.kv_heads, group, c.head_dim, f32, cus);
     AttnArgs a;
     a.q = q;
     a.out = out;
