@@ -383,9 +383,27 @@ __device__ __forceinline__ bool by_bins(const Bound& b, const Settings& s) {
     return b.best && !s.greedy && logit_of((uint32_t)(b.best >> 32)) - logit_of(b.least) < INFINITY;
 }
 
+struct BoundShared {
+    uint64_t best[kThreads / 64];
+    uint32_t least[kThreads / 64];
+};
+// The workgroup's, the same in every thread.
+__device__ __forceinline__ Bound block_bound(uint64_t best, uint32_t least, BoundShared& sh) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        best = max(best, (uint64_t)__shfl_xor((unsigned long long)best, d));
+        least = min(least, (uint32_t)__shfl_xor((int)least, d));
+    }
+    if ((threadIdx.x & 63) == 0) sh.best[threadIdx.x >> 6] = best, sh.least[threadIdx.x >> 6] = least;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) best = max(best, sh.best[i]), least = min(least, sh.least[i]);
+    __syncthreads();
+    return Bound{best, least, 0};
+}
+
 __global__ void __launch_bounds__(kThreads) sample_bounds_kernel(SampleArgs a, void* ws, int slices) {
-    __shared__ uint64_t best_of[kThreads / 64];
-    __shared__ uint32_t least_of[kThreads / 64];
+    __shared__ BoundShared sh;
     const int r = blockIdx.y, slice = blockIdx.x;
     const RowWork w = row_work(ws, r, slices);
     Slice logits(a, r, slice, slices);
@@ -397,17 +415,8 @@ __global__ void __launch_bounds__(kThreads) sample_bounds_kernel(SampleArgs a, v
         best = max(best, (uint64_t)k << 32 | (uint32_t)~i);
         least = min(least, k);
     });
-#pragma unroll
-    for (int d = 32; d; d >>= 1) {
-        best = max(best, (uint64_t)__shfl_xor((unsigned long long)best, d));
-        least = min(least, (uint32_t)__shfl_xor((int)least, d));
-    }
-    if ((threadIdx.x & 63) == 0) best_of[threadIdx.x >> 6] = best, least_of[threadIdx.x >> 6] = least;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < kThreads / 64; ++i) best = max(best, best_of[i]), least = min(least, least_of[i]);
-        w.bound[slice] = Bound{best, least, 0};
-    }
+    const Bound b = block_bound(best, least, sh);
+    if (threadIdx.x == 0) w.bound[slice] = b;
 }
 
 __global__ void __launch_bounds__(kThreads) sample_bins_kernel(SampleArgs a, void* ws, int slices) {
@@ -816,6 +825,7 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a, v
     __shared__ unsigned long long list[kList];
     __shared__ union {
         RowShared row;
+        BoundShared bounds;
         unsigned rank[kShort];
         BinSort bins;
         DrawShared l;
@@ -833,18 +843,44 @@ __global__ void __launch_bounds__(kThreads) sample_finish_kernel(SampleArgs a, v
     unsigned n = 0;
     const bool whole = !slices;  // all of the row's candidates
     if (whole) {
-        if (threadIdx.x == 0) listed = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < a.n; i += kThreads) {
-            const uint32_t k = key_of(row[i]);
-            if (k) list[atomicAdd(&listed, 1u)] = (unsigned long long)k << 32 | (uint32_t)~i;
+        constexpr int PER = kList / kThreads;
+        float l[PER];
+        uint64_t best = 0;
+        uint32_t least = ~0u;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) l[j] = row[min(j * kThreads + (int)threadIdx.x, a.n - 1)];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = j * kThreads + threadIdx.x;
+            const uint32_t k = key_of(l[j]);
+            if (!k || i >= a.n) continue;
+            best = max(best, (uint64_t)k << 32 | (uint32_t)~i);
+            least = min(least, k);
         }
-        __syncthreads();
-        n = listed;
-        if (n) {
+        b = block_bound(best, least, sh.bounds);
+        if (b.best && !s.greedy) {
+            // the candidates whose mass is not zero for certain
+            bins = bins_of(b, s);
+            const bool binned = by_bins(b, s), some = binned && bins.clipped;
+            bool mine[PER];
+            unsigned count = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                mine[j] = j * kThreads + (int)threadIdx.x < a.n && l[j] > -INFINITY &&
+                          !(some && bins.at(l[j]) == kBins - 1);
+                count += mine[j];
+            }
+            const unsigned upto = scan(count, sh.bins.part);
+            if (threadIdx.x == kThreads - 1) listed = upto;
+            unsigned at = upto - count;
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                if (mine[j])
+                    list[at++] = (unsigned long long)key_of(l[j]) << 32 | (uint32_t)~(j * kThreads + threadIdx.x);
+            __syncthreads();
+            n = listed;
             if (n <= kShort) rank_list(list, sh.rank, n);
-            else sort_list(list, n);
-            b.best = list[0];
+            else if (!binned || !bin_list(list, sh.bins, bins, n)) sort_list(list, n);
         }
     } else {
         // the slices' lists, 64 threads to a slice: the first 64 of each are requested before the counts are known
