@@ -86,12 +86,12 @@ def attention(q, k, v, q_start, kv_len, table, max_blocks, scale, window=0):
             if not live.any():
                 out[row] = 0.0
                 continue
-            for h in range(nq):
-                g = h // (nq // nkv)
-                sc = keys[live, g] @ q[row, h].astype(np.float64) * scale
+            for g in range(nkv):
+                h = slice(g * (nq // nkv), (g + 1) * (nq // nkv))
+                sc = q[row, h].astype(np.float64) @ keys[live, g].T * scale  # [the group's heads, keys]
                 with np.errstate(invalid="ignore"):
-                    e = np.exp(sc - sc.max())
-                    out[row, h] = (e / e.sum()) @ values[live, g]
+                    e = np.exp(sc - sc.max(-1, keepdims=True))
+                    out[row, h] = (e / e.sum(-1, keepdims=True)) @ values[live, g]
     return out
 
 

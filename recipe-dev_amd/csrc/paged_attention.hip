@@ -30,14 +30,15 @@
 // 2^15). Sums are fp32.
 //
 // Keys and values go from the pages straight into LDS (global_load_lds, 16
-// bytes a lane), 16 keys of one page at a time, at most 64 keys per step. A row's 16-byte
-// pieces are stored XORed with the row number, so that the operand reads hit
-// every bank once.
+// bytes a lane), 16 keys of one page at a time, 32 or 64 keys per step. A row's
+// 16-byte pieces are stored XORed with the row number, so that the operand reads
+// hit every bank once.
 //
 // Masked places: a masked score is -infinity by selection, and V must not meet
-// its zero weight as a NaN: in steps where some row may not see some key, dead
-// keys' values are zeroed in LDS, and non-finite values are added to the rows
-// that see them and then zeroed.
+// its zero weight as a NaN: in steps where some row may not see some key, the
+// values of keys that no row sees are zeroed in LDS, and so are NaN and infinite
+// ones of the others; where there are such, they are read again from the cache
+// after the last step and added to the rows that see them.
 #include "lanes.h"
 #include "paged.h"
 
@@ -682,9 +683,9 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
         key0 = after;
     }
     wait_loads<0>();
-    if (odd) {  // (the wave's own steps; unmasked ones went through whole)
+    if (odd) {  // (the wave's own steps; what unmasked ones let through is there already, and stays)
         for (int k = begin + wave * KEYS; k < end; k += 4 * KEYS)
-            if (k < t.all_from || k + KEYS > t.all_to) add_odd<HD, 1, F32>(a, t, kh, k, min(k + KEYS, t.end), w);
+            add_odd<HD, 1, F32>(a, t, kh, k, min(k + KEYS, t.end), w);
     }
     // the waves' sums, each in its own LDS (32 rows of HD values, pieces XORed with the row)
     const int q = lane & 31, h = lane >> 5;
@@ -763,8 +764,9 @@ __global__ void __launch_bounds__(64 * many_waves(HD, F32), many_waves(HD, F32) 
     Pages pages{a.b.table + seq * a.b.table_stride, a.b.max_blocks - 1, a.c.blocks, a.c.block_shift, INT_MIN / 2, 0};
     Rows<HD, 1, F32> w;
 
-    // Step i is in buffer i % 2, keys before values. Of eight waves, four load 16 rows of
-    // keys each and four of values; of four, each loads both. Returns which groups are absent.
+    // Step i is in buffer i % 2, keys before values. Of eight waves, four load 16 rows of keys each and
+    // four of values (in steps of 32 keys half of 16 rows each); of four, each loads both. Returns which
+    // groups are absent.
     auto load = [&](int key0, int buffer) -> unsigned {
         pages.need(key0 >> pages.shift, (key0 + KEYS - 16) >> pages.shift);
         unsigned bad = 0;
@@ -817,10 +819,7 @@ __global__ void __launch_bounds__(64 * many_waves(HD, F32), many_waves(HD, F32) 
         bad = bad_next;
         buffer ^= 1;
     }
-    if (odd) {
-        for (int k = begin; k < end; k += KEYS)
-            if (k < t.all_from || k + KEYS > t.all_to) add_odd<HD, 1, F32>(a, t, kh, k, min(k + KEYS, t.end), w);
-    }
+    if (odd) add_odd<HD, 1, F32>(a, t, kh, begin, end, w);
     const bool whole = t.live <= 1;
     const int h = lane >> 5, r = row + (lane & 31);
     const float l = swap32_sum(w.l[0]);

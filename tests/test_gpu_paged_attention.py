@@ -317,3 +317,145 @@ def test_offsets_past_4_gib(gpu):
     gpu.paged_attention(batch, cache, Q, 1, 16 * hd, 16, O, 16 * hd, gpu.paged_attention_workspace(batch, cache, 16))
     gpu.synchronize()
     assert np.array_equal(O.download(np.uint16).reshape(-1), want.view(np.uint16).reshape(-1))
+
+
+# Batches of so many rows that the large tiles take them (more than 1024 tiles of 32 rows over all heads), and
+# of heads over one kv head, where those tiles' keys are split as well.
+LARGE = [(128, 2, 64, 16), (126, 18, 64, 64), (128, 1, 128, 16), (132, 44, 128, 32), (128, 2, 256, 16),
+         (130, 26, 256, 128)]
+SPLIT = [(64, 1, 64, 16, False), (64, 1, 128, 16, False), (64, 1, 128, 32, True), (32, 1, 256, 16, False)]
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("nq,nkv,hd,block", LARGE)
+@pytest.mark.parametrize("seqs,window", [([(270, 0)], 0), ([(150, 3), (1, 80), (0, 9), (119, 331)], 0),
+                                         ([(270, 200)], 33), ([(200, 1), (75, 500)], 128)])
+def test_many_rows(gpu, nq, nkv, hd, block, seqs, window, f16):
+    Case(seqs, nq, nkv, hd, block, f16, 20 + len(seqs), extra_rows=2).check(gpu, window=window, pad=8)
+
+
+@pytest.mark.parametrize("nq,nkv,hd,block,f16", SPLIT)
+@pytest.mark.parametrize("seqs,window", [([(261, 700)], 0), ([(100, 900), (161, 30)], 0), ([(262, 800)], 333),
+                                         ([(270, 3)], 0)])
+def test_many_rows_split_keys(gpu, nq, nkv, hd, block, seqs, window, f16):
+    Case(seqs, nq, nkv, hd, block, f16, 25 + len(seqs), extra_rows=1).check(gpu, window=window)
+    Case(seqs, nq, nkv, hd, block, f16, 27, spread=3.0).check(gpu, window=window, scale=0.3)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("nq,nkv,hd", [(128, 2, 64), (128, 2, 128), (128, 2, 256), (64, 1, 128)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_many_rows_masked_places(gpu, nq, nkv, hd, bad, f16):
+    """As test_masked_places_never_touch_the_result, at many rows."""
+    new, ctx = 270, 45
+    c = Case([(new, ctx)], nq, nkv, hd, 16, f16, 30)
+    clean = c.run(gpu)
+    used = np.zeros((c.blocks, c.block), bool)
+    p = np.arange(new + ctx)
+    used[c.table[0, p // 16], p % 16] = True
+    for cache in (c.k, c.v):
+        cache.transpose(0, 2, 1, 3)[~used] = bad
+    assert np.array_equal(c.run(gpu), clean)
+    hurt = np.zeros(clean.shape, bool)
+    for at, dim in ((new + ctx - 1, 5), (200, 40)):  # a value is for the rows from its position on
+        c.v[c.table[0, at // 16], nkv - 1, at % 16, dim] = bad
+        hurt[at - ctx:, nq - nq // nkv:, dim] = True
+        got = c.run(gpu)
+        assert np.array_equal(got[~hurt], clean[~hurt]) and not np.isfinite(got[hurt]).any()
+    c.k[c.table[0, 250 // 16], 0, 250 % 16, 3] = np.nan
+    hurt[250 - ctx:, :nq // nkv] = True
+    got = c.run(gpu)
+    assert np.array_equal(got[~hurt], clean[~hurt]) and not np.isfinite(got[hurt]).any()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("nq,nkv,hd", [(128, 2, 64), (128, 2, 128), (128, 2, 256), (64, 1, 128)])
+def test_many_rows_absent_pages(gpu, nq, nkv, hd, f16):
+    c = Case([(200, 100), (75, 10)], nq, nkv, hd, 16, f16, 31)
+    c.table[0, 0] = -1
+    c.table[0, 2] = c.blocks
+    c.table[1, :] = -2 ** 31  # nothing left: zeros
+    c.check(gpu)
+    assert not c.run(gpu)[200:275].any()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("nq,nkv,new", [(4, 2, 1), (4, 2, 60), (128, 2, 270)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_non_finite_values_beside_an_absent_page(gpu, nq, nkv, new, bad, f16):
+    """Every row sees key 35; the pages around its own are absent."""
+    c = Case([(new, 200)], nq, nkv, 128, 16, f16, 32)
+    c.table[0, [1, 3]] = -1
+    clean = c.run(gpu)
+    c.v[c.table[0, 2], 1, 3, 7] = bad
+    got = c.run(gpu)
+    hurt = np.zeros(got.shape, bool)
+    hurt[:, nq // 2:, 7] = True
+    assert np.array_equal(got[~hurt], clean[~hurt]) and not np.isfinite(got[hurt]).any()
+
+
+def test_many_extreme_rows_fp32(gpu):
+    for hd in (64, 128, 256):
+        c = Case([(270, 30)], 128, 2, hd, 16, False, 33)
+        c.q[:, 0] *= 1e6
+        c.q[:, 1] *= 1e-6
+        c.q[:, 2] *= 1e-30
+        c.q[0, 3, 0] = 1e5
+        c.check(gpu, scale=1e-6)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_many_rows_lengths(gpu, f16):
+    """Positions past the table, and kv_len below the new tokens."""
+    Case([(270, 100)], 128, 2, 64, 16, f16, 34, max_blocks=9).check(gpu)
+    c = Case([(200, 0), (75, 10)], 128, 1, 128, 16, f16, 35)
+    c.kv_len[:] = (3, 40)
+    c.check(gpu)
+    c.kv_len[:] = (0, -5)
+    assert not c.run(gpu)[:275].any()
+
+
+@pytest.mark.parametrize("nq,nkv,hd,block,f16", SPLIT + [(128, 2, 64, 16, True), (128, 2, 256, 16, True)])
+def test_many_rows_in_place_from_a_graph(gpu, nq, nkv, hd, block, f16):
+    """out = q; each replay has the bits of an eager call on the same rows."""
+    c = Case([(200, 0), (62, 400)], nq, nkv, hd, block, f16, 36)
+    bits, row = (np.uint16 if f16 else np.uint32), nq * hd
+    KV = i32(gpu, c.kv_len)
+    batch = gpu.PagedBatch(2, c.rows, c.width, i32(gpu, c.q_start), KV, i32(gpu, c.table))
+    cache = gpu.PagedCache(gpu.DeviceBuffer.from_array(c.k.view(np.uint16)),
+                           gpu.DeviceBuffer.from_array(c.v.view(np.uint16)), c.blocks, block, nkv, hd)
+    Q = gpu.DeviceBuffer.from_array(c.q.view(bits))
+    O = gpu.DeviceBuffer(c.q.nbytes)
+    ws = gpu.paged_attention_workspace(batch, cache, nq)
+    stream = gpu.Stream()
+    call = lambda q, out: gpu.paged_attention(batch, cache, q, 1 if f16 else 0, row, nq, out, row, ws,  # noqa: E731
+                                              stream=stream)
+    graph = gpu.Graph(stream, lambda: call(Q, Q))
+    for step in range(4):
+        KV.upload(c.kv_len - 9 * step)
+        Q.upload(c.q.view(bits))
+        call(Q, O)
+        stream.synchronize()
+        graph.launch(stream)
+        stream.synchronize()
+        assert np.array_equal(Q.download(bits), O.download(bits))
+    graph.close()
+
+
+def test_two_streams_with_a_workspace_each(gpu):
+    """Two batches at once on two streams, again and again, give what each gives alone."""
+    cases = [Case([(1, 3000), (3, 50)], 32, 8, 128, 16, True, 37), Case([(261, 700)], 64, 1, 128, 16, True, 38)]
+    want = [c.run(gpu) for c in cases]
+    runs = []
+    for c in cases:
+        batch = gpu.PagedBatch(len(c.kv_len), c.rows, c.width, i32(gpu, c.q_start), i32(gpu, c.kv_len), i32(gpu, c.table))
+        cache = gpu.PagedCache(gpu.DeviceBuffer.from_array(c.k.view(np.uint16)),
+                               gpu.DeviceBuffer.from_array(c.v.view(np.uint16)), c.blocks, 16, c.nkv, 128)
+        runs.append((batch, cache, gpu.DeviceBuffer.from_array(c.q.view(np.uint16)), gpu.DeviceBuffer(c.q.nbytes),
+                     gpu.paged_attention_workspace(batch, cache, c.nq), gpu.Stream()))
+    for _ in range(8):
+        for c, (batch, cache, q, out, ws, stream) in zip(cases, runs):
+            gpu.paged_attention(batch, cache, q, 1, c.nq * 128, c.nq, out, c.nq * 128, ws, stream=stream)
+    for c, run, w in zip(cases, runs, want):
+        run[5].synchronize()
+        assert np.array_equal(run[3].download(np.uint16).reshape(-1), w.view(np.uint16).reshape(-1))
