@@ -362,10 +362,10 @@ int rqmv_qk_norm_rope(const rqmv_paged_batch* batch, const rqmv_paged_cache* cac
  * not written. q_heads is a multiple of kv_heads, both at most 1024; scale is positive; ldq
  * and ldo are multiples of 16 bytes, q and out 16-byte aligned; out is q itself (ldo
  * = ldq) or spans none of its memory. Reads q_start, kv_len, block_table of the batch. One
- * launch, two where the keys are split over workgroups: then the workspace (16-byte
- * aligned, rqmv_paged_attention_workspace_size bytes for this batch's counts, cache and
- * q_heads on the current device; 0: may be NULL) holds partial results, and calls
- * that share it must not overlap. */
+ * launch, one more where the keys are split over workgroups and one above 256 sequences:
+ * then the workspace (16-byte aligned, rqmv_paged_attention_workspace_size bytes for this
+ * batch's counts, cache and q_heads on the current device; 0: may be NULL) holds partial
+ * results, and calls that share it must not overlap. */
 int rqmv_paged_attention_workspace_size(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, int q_heads,
                                         size_t* bytes);
 int rqmv_paged_attention(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, const void* q, int dtype,

@@ -72,6 +72,7 @@ struct AttnArgs {
     float* o;           // [parts][head_dim]
     float2* ml;         // [parts]
     int2* info;         // [tokens][group]: live splits, 32 first part + row (paged_few_kernel); null: nothing is split
+    const int2* items;  // paged_items_kernel's; null: at most kItemSeqs sequences, or paged_many_kernel
     int64_t parts;
 };
 
@@ -552,60 +553,107 @@ __device__ __forceinline__ int64_t sum_wave(int64_t v) {
     return v;
 }
 
+// A sequence's items: chunk (in units), live splits of each tile, items.
+template <int TM>
+__device__ __forceinline__ int seq_items(const AttnArgs& a, int64_t total, int tiles, int keys, int* chunk, int* live) {
+    const int units = (keys + 63) >> 6;
+    *chunk = chunk_units(a, total, units);
+    *live = max((units + *chunk - 1) / *chunk, 1);
+    return tiles * *live;
+}
+// Items, and those of split tiles in the upper half.
+__device__ __forceinline__ unsigned long long both_counts(int items, int live) {
+    return (unsigned long long)(live > 1 ? items : 0) << 32 | (unsigned)items;
+}
+
 // Item `number` of the batch (of 256 threads); false: there is none. Of the items only those of
 // split tiles have partial results, and these are at most 2 `splits`: a tile of u units in chunks of c < u
-// has at most 2 u / c.
+// has at most 2 u / c. Up to kItemSeqs sequences every workgroup adds them up by itself, a sequence a
+// thread; more are added up by a launch before (32/8 heads of 128, 100 to 300 positions each: 8192 sequences
+// 1370 us, by every workgroup 4840; 512 sequences 95, 107).
+constexpr int kItemSeqs = 256;
+
+// The first item of each sequence and the first of its partial results; behind them the total.
 template <int TM>
-__device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* item) {
-    __shared__ unsigned long long upto_of[4];
-    __shared__ int64_t totals[4];
-    __shared__ Item found;
+__global__ void __launch_bounds__(1024) paged_items_kernel(AttnArgs a, int2* out) {
+    __shared__ unsigned long long upto_of[16];
+    __shared__ int64_t totals[16];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    int tiles = 0, first = 0, keys = 0;
+    int tiles, first, keys, chunk, live;
     int64_t total = 0;
-    for (int s = t; s < a.b.seqs; s += 256) {
+    for (int s = t; s < a.b.seqs; s += 1024) {
         seq_size<TM>(a, s, &tiles, &first, &keys);
         total += (int64_t)tiles * ((keys + 63) >> 6);
     }
-    if (t == 0) found.seq = -1;
     total = sum_wave(total);
     if (lane == 0) totals[wave] = total;
     __syncthreads();
-    total = totals[0] + totals[1] + totals[2] + totals[3];
-    unsigned long long before = 0;  // items, and those of split tiles in the upper half
-    for (int s0 = 0; s0 < a.b.seqs; s0 += 256) {
+    total = 0;
+    for (int w = 0; w < 16; ++w) total += totals[w];
+    unsigned long long before = 0;
+    for (int s0 = 0; s0 < a.b.seqs; s0 += 1024) {
         const int s = s0 + t;
-        int items = 0, live = 1, chunk = 1;
+        unsigned long long own = 0;
         if (s < a.b.seqs) {
-            if (a.b.seqs > 256) seq_size<TM>(a, s, &tiles, &first, &keys);
-            const int units = (keys + 63) >> 6;
-            chunk = chunk_units(a, total, units);
-            live = max((units + chunk - 1) / chunk, 1);
-            items = tiles * live;
+            seq_size<TM>(a, s, &tiles, &first, &keys);
+            const int items = seq_items<TM>(a, total, tiles, keys, &chunk, &live);
+            own = both_counts(items, live);
         }
-        const unsigned long long own = (unsigned long long)(live > 1 ? items : 0) << 32 | (unsigned)items;
         const unsigned long long upto = wave_scan(own);
         __syncthreads();
         if (lane == 63) upto_of[wave] = upto;
         __syncthreads();
         unsigned long long from = before + upto - own;
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < 16; ++w) {
             from += w < wave ? upto_of[w] : 0;
             before += upto_of[w];
         }
+        if (s < a.b.seqs) out[s] = make_int2((int)(unsigned)from, (int)(from >> 32));
+    }
+    if (t == 0) out[a.b.seqs] = make_int2((int)(unsigned)total, (int)(total >> 32));
+}
+
+template <int TM>
+__device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* item) {
+    int tiles = 0, first = 0, keys = 0, chunk, live;
+    if (a.items) {
+        const int s = last_seq(a.b.seqs, [&](int i) { return a.items[i].x <= number; });
+        const int2 from = a.items[s], sum = a.items[a.b.seqs];
+        seq_size<TM>(a, s, &tiles, &first, &keys);
+        const int items = seq_items<TM>(a, (int64_t)sum.y << 32 | (unsigned)sum.x, tiles, keys, &chunk, &live);
+        const int at = number - from.x;
+        if (at < 0 || at >= items) return false;
+        *item = Item{s, at / live, at % live, first, chunk * 64, live, from.y + at};
+    } else {
+        __shared__ unsigned long long upto_of[4];
+        __shared__ int64_t totals[4];
+        __shared__ Item found;
+        const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+        if (t < a.b.seqs) seq_size<TM>(a, t, &tiles, &first, &keys);
+        if (t == 0) found.seq = -1;
+        const int64_t own_total = sum_wave((int64_t)tiles * ((keys + 63) >> 6));
+        if (lane == 0) totals[wave] = own_total;
+        __syncthreads();
+        const int items = seq_items<TM>(a, totals[0] + totals[1] + totals[2] + totals[3], tiles, keys, &chunk, &live);
+        const unsigned long long own = both_counts(items, live), upto = wave_scan(own);
+        if (lane == 63) upto_of[wave] = upto;
+        __syncthreads();
+        unsigned long long from = upto - own;
+        for (int w = 0; w < 3; ++w) from += w < wave ? upto_of[w] : 0;
         const int at = number - (int)(unsigned)from;
         if (at >= 0 && at < items)
-            found = Item{s, at / live, at % live, first, chunk * 64, live, (int)(from >> 32) + at};
+            found = Item{t, at / live, at % live, first, chunk * 64, live, (int)(from >> 32) + at};
+        __syncthreads();
+        if (found.seq < 0) return false;
+        *item = found;
     }
-    __syncthreads();
-    if (found.seq < 0) return false;
-    item->seq = __builtin_amdgcn_readfirstlane(found.seq);
-    item->tile = __builtin_amdgcn_readfirstlane(found.tile);
-    item->split = __builtin_amdgcn_readfirstlane(found.split);
-    item->first = __builtin_amdgcn_readfirstlane(found.first);
-    item->chunk = __builtin_amdgcn_readfirstlane(found.chunk);
-    item->live = __builtin_amdgcn_readfirstlane(found.live);
-    item->part = __builtin_amdgcn_readfirstlane(found.part);
+    item->seq = __builtin_amdgcn_readfirstlane(item->seq);
+    item->tile = __builtin_amdgcn_readfirstlane(item->tile);
+    item->split = __builtin_amdgcn_readfirstlane(item->split);
+    item->first = __builtin_amdgcn_readfirstlane(item->first);
+    item->chunk = __builtin_amdgcn_readfirstlane(item->chunk);
+    item->live = __builtin_amdgcn_readfirstlane(item->live);
+    item->part = __builtin_amdgcn_readfirstlane(item->part);
     return true;
 }
 
@@ -618,6 +666,10 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
     const int kh = blockIdx.x % a.c.kv_heads;
     Item item;
     if (!find_item<TM>(a, blockIdx.x / a.c.kv_heads, &item)) return;
+    // (starts out of order may count past what the workspace holds)
+    const bool whole = item.live <= 1;
+    const int64_t part0 = ((int64_t)item.part * a.c.kv_heads + kh) * TM;
+    if (!whole && (part0 < 0 || part0 + TM > a.parts)) return;
     const int seq = item.seq;
     const Tile t = make_tile<TM>(a, seq, item.tile * TM);
     const int begin = item.first + item.split * item.chunk, end = min(begin + item.chunk, t.end);
@@ -701,8 +753,6 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
     if (h == 0) sums[wave][q] = make_float2(w.m[0], l);
     __syncthreads();
     const int rows = min(t.rows - t.row0, TM);
-    const bool whole = item.live <= 1;
-    const int64_t part0 = ((int64_t)item.part * a.c.kv_heads + kh) * TM;
     if (a.info && kh == 0 && item.split == 0)
         for (int u = threadIdx.x; u < rows; u += 256)
             a.info[(int64_t)t.token0 * a.group + t.row0 + u] = make_int2(item.live, item.part << 5 | u);
@@ -906,7 +956,7 @@ constexpr int few_lds(int hd) { return 4 * 2 * 32 * hd * 2; }
 constexpr int many_lds(int hd, bool f32) { return 2 * 2 * many_keys(hd, f32) * hd * 2; }
 
 struct AttnPlan {
-    bool few, join;
+    bool few, join, items;
     int splits, min_chunk;
     int64_t tiles, parts;
 };
@@ -924,6 +974,7 @@ AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int gro
     p.tiles = (int64_t)tokens * group / 32 + seqs;
     const int64_t few_tiles = hd == 128 ? 2 * cus : hd == 64 ? (f32 ? 2 : 4) * cus : f32 ? cus / 2 : 4 * cus;
     p.few = (int64_t)tokens * group <= (int64_t)128 * seqs || (int64_t)tokens * heads / 32 <= few_tiles;
+    p.items = p.few && seqs > kItemSeqs;
     if (p.few) {
         // Two items per CU over the whole batch (32 requests of 60 to 8,192 positions: 35.1 us; one
         // per CU 37.6, four 37.6), of two steps for each wave at least (one request at 4,097: 10.5 us; of
@@ -949,8 +1000,9 @@ AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int gro
     return p;
 }
 
-size_t workspace_bytes(const AttnPlan& p, int tokens, int group, int hd) {
-    return p.join ? p.parts * (hd * sizeof(float) + sizeof(float2)) + (size_t)tokens * group * sizeof(int2) : 0;
+size_t workspace_bytes(const AttnPlan& p, int tokens, int seqs, int group, int hd) {
+    return (p.join ? p.parts * (hd * sizeof(float) + sizeof(float2)) + (size_t)tokens * group * sizeof(int2) : 0) +
+           (p.items ? ((size_t)seqs + 1) * sizeof(int2) : 0);
 }
 
 template <int HD, bool F32>
@@ -992,7 +1044,7 @@ size_t paged_attention_workspace(const PagedBatch& b, const PagedCache& c, int q
     size_t most = 0;
     for (const bool f32 : {false, true}) {  // (one workspace serves both types)
         const AttnPlan p = plan_attention(b.tokens, b.seqs, cap, c.kv_heads, group, c.head_dim, f32, cus);
-        const size_t bytes = workspace_bytes(p, b.tokens, group, c.head_dim);
+        const size_t bytes = workspace_bytes(p, b.tokens, b.seqs, group, c.head_dim);
         most = bytes > most ? bytes : most;
     }
     return most;
@@ -1020,8 +1072,16 @@ hipError_t launch_paged_attention(const PagedBatch& b, const PagedCache& c, cons
     a.min_chunk = p.min_chunk;
     a.o = static_cast<float*>(workspace);
     a.ml = reinterpret_cast<float2*>(a.o + p.parts * c.head_dim);
-    a.info = p.join ? reinterpret_cast<int2*>(a.ml + p.parts) : nullptr;
+    int2* behind = reinterpret_cast<int2*>(a.ml + p.parts);
+    a.info = p.join ? behind : nullptr;
+    int2* items = p.items ? behind + (p.join ? (int64_t)b.tokens * group : 0) : nullptr;
+    a.items = items;
     a.parts = p.parts;
+    if (items) {
+        hipLaunchKernelGGL(paged_items_kernel<32>, dim3(1), dim3(1024), 0, stream, a, items);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
     if (c.head_dim == 64) return f32 ? launch_attention_hd<64, true>(p, a, stream) : launch_attention_hd<64, false>(p, a, stream);
     if (c.head_dim == 128)
         return f32 ? launch_attention_hd<128, true>(p, a, stream) : launch_attention_hd<128, false>(p, a, stream);

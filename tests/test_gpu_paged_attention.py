@@ -459,3 +459,22 @@ def test_two_streams_with_a_workspace_each(gpu):
     for c, run, w in zip(cases, runs, want):
         run[5].synchronize()
         assert np.array_equal(run[3].download(np.uint16).reshape(-1), w.view(np.uint16).reshape(-1))
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("seqs,window", [([(i % 3, (7 * i) % 40) for i in range(257)] + [(2, 5000), (40, 900)], 0),
+                                         ([(1, 2300)] + [(1, 3)] * 511 + [(1, 700)], 0),
+                                         ([(0, 9)] * 300 + [(1, 1500), (0, 0), (3, 2000)] + [(0, 4)] * 1000, 1100)])
+def test_more_sequences_than_threads(gpu, seqs, window, f16):
+    """Items found by the launch before, long sequences among short ones and empty ones."""
+    Case(seqs, 4, 2, 64, 16, f16, 40, extra_rows=2).check(gpu, window=window)
+    c = Case(seqs, 2, 1, 128, 32, f16, 41)
+    c.table[5, :] = -1
+    c.check(gpu, window=window)
+
+
+def test_many_starts_out_of_order_stay_inside_the_rows(gpu):
+    c = Case([(2, 600)] * 300, 2, 1, 64, 16, True, 42)
+    for start in (np.arange(301)[::-1] * 2, np.where(np.arange(301) % 2, 600, 0), np.full(301, -3), np.arange(301) * 9):
+        c.q_start = start.astype(np.int32)
+        c.run(gpu, pad=8)
