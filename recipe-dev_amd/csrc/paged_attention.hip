@@ -380,6 +380,11 @@ template <int HD, int QT, int KT, bool F32>
 __device__ __forceinline__ void weights(Rows<HD, QT, F32>& w, const f16_t (&s)[QT][KT],
                                         h8_t (&p)[QT][2 * KT][F32 ? 2 : 1]) {
     constexpr float SHIFT = F32 ? 15.f : 6.f;
+    // fp16, up to 128 dims: the sum of the rounded weights, two at a time. What a large weight's rounding adds
+    // to the row it adds to the divisor too, so a row of one large weight is off by its output's rounding alone
+    // (2048 tokens over 14,336: 507 -> 504 us; 6,000, 8/4 heads of 256: 204 -> 213 us, so there the weights
+    // are added before they are rounded).
+    constexpr bool PAIRS = !F32 && HD <= 128;
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
         const float ref = w.m[i] == -INFINITY ? 0.f : w.m[i] - SHIFT;
@@ -391,10 +396,16 @@ __device__ __forceinline__ void weights(Rows<HD, QT, F32>& w, const f16_t (&s)[Q
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     v[e] = __builtin_amdgcn_exp2f(fmaf(s[i][t][8 * b + e], w.c[i], -ref));
-                    w.l[i] += v[e];
+                    if constexpr (!PAIRS) w.l[i] += v[e];
                 }
                 h8_t& hi = p[i][2 * t + b][0];
                 hi = cvt8(v);
+                if constexpr (PAIRS) {
+                    const h2_t one = {(_Float16)1.f, (_Float16)1.f};
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2)
+                        w.l[i] = __builtin_amdgcn_fdot2(h2_t{hi[e], hi[e + 1]}, one, w.l[i], false);
+                }
                 if constexpr (F32) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[e] -= (float)hi[e];
