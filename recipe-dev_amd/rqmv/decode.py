@@ -290,8 +290,11 @@ class DecodeModel:
         advance(self.pos, stream)
 
     def capture(self, stream: Stream, sampling: Sampling | None = None) -> Graph:
-        """A HIP graph of one step; each launch decodes the next token."""
-        return Graph(stream, lambda: self.enqueue_step(stream, sampling=sampling))
+        """A HIP graph of one step; each launch decodes the next token. The graph
+        keeps the Sampling, whose buffers its launches read."""
+        graph = Graph(stream, lambda: self.enqueue_step(stream, sampling=sampling))
+        graph.sampling = sampling
+        return graph
 
     def read_logits(self) -> np.ndarray:
         self._check_inside()

@@ -7,6 +7,8 @@ Bars: logits within rel-L2 1e-3 of the restatement, the quantized products' own
 bar; tables equal; tokens those that oracle/paged.py draws from the device's
 logits.
 """
+import gc
+
 import numpy as np
 import pytest
 
@@ -179,3 +181,15 @@ def test_decoder_draws_its_tokens(gpu, captured):
             got.append(model.read_token())
         greedy.append(got)
     assert greedy[0] == greedy[1]
+    # a graph outlives the name of its Sampling
+    graph = model.capture(stream, model.sampling(temperature=0.0))
+    gc.collect()
+    junk = [gpu.DeviceBuffer.from_array(np.full(1 << 18, 0x7FC00000, np.uint32)) for _ in range(4)]
+    model.set_position(7, 8)
+    got = []
+    for _ in range(4):
+        model.replay(graph, stream)
+        stream.synchronize()
+        got.append(model.read_token())
+    assert got == greedy[0] and len(junk) == 4
+    graph.close()
