@@ -105,14 +105,22 @@ __device__ __forceinline__ int find_seq(const PagedBatch& b, int group, int numb
     return last_seq(b.seqs, [&](int s) { return start_of(b, s) * group / TM + s <= number; });
 }
 
-// Row starts and lengths are read as they are found and brought into range.
+// A sequence's first row of q, new tokens and positions, read as they are found and brought into range.
+struct Seq {
+    int token0, n, kv;
+};
+__device__ __forceinline__ Seq load_seq(const AttnArgs& a, int s) {
+    const int from = start_of(a.b, s);
+    return Seq{from, min(max(a.b.q_start[s + 1], from), a.b.tokens) - from, max(a.b.kv_len[s], 0)};
+}
+
 template <int TM>
-__device__ __forceinline__ Tile make_tile(const AttnArgs& a, int seq, int row0) {
+__device__ __forceinline__ Tile make_tile(const AttnArgs& a, int seq, const Seq& of, int row0) {
     Tile t;
     t.seq = seq;
-    t.token0 = start_of(a.b, seq);
-    t.n = min(max(a.b.q_start[seq + 1], t.token0), a.b.tokens) - t.token0;
-    t.kv = max(a.b.kv_len[seq], 0);
+    t.token0 = of.token0;
+    t.n = of.n;
+    t.kv = of.kv;
     t.row0 = row0;
     t.rows = t.n * a.group;
     const int last = min(row0 + TM, t.rows) - 1;
@@ -209,70 +217,89 @@ __device__ __forceinline__ h8_t cvt8(const float (&v)[8]) {
     return r;
 }
 
-template <int HD, int QT, bool F32>
-__device__ __forceinline__ void load_rows(const AttnArgs& a, const Tile& t, int kh, int row, Rows<HD, QT, F32>& w) {
+// A row's values as they are in memory, while they are on their way. (fp16: the operands)
+template <int HD, bool F32>
+struct RawRows {
+    float4 v[F32 ? HD / 16 : 1][2];
+};
+
+// Requests the wave's rows, with the first page ids on their way. `arrived` waits for them: the compiler
+// would wait for them at their first use in the loop, in every step, and for the step's own loads, which it does not
+// count, with them. fp32 rows are asked for before the first step's loads to LDS and become operands while these
+// are on their way (one token over 4,096: 13.9 -> 13.3 us; fp16 rows, which are operands already, come
+// behind those loads: 32 sequences 39.9 -> 39.6).
+template <int HD, bool F32>
+__device__ __forceinline__ void load_rows(const AttnArgs& a, const Tile& t, int kh, int row, Rows<HD, 1, F32>& w,
+                                          RawRows<HD, F32>& raw) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int r = min(row + (lane & 31), t.rows - 1);  // (rows past the last repeat it)
+    const int tok = r / a.group, pos = t.kv - t.n + tok;
+    const int64_t at = (int64_t)(t.token0 + tok) * a.ldq + (kh * a.group + r % a.group) * HD + 8 * h;
+    w.hi[0] = min(pos, a.cap - 1);
+    w.lo[0] = a.window ? pos - a.window + 1 : 0;
 #pragma unroll
-    for (int i = 0; i < QT; ++i) {
-        const int r = min(row + 32 * i + (lane & 31), t.rows - 1);  // (rows past the last repeat it)
-        const int tok = r / a.group, pos = t.kv - t.n + tok;
-        const int64_t at = (int64_t)(t.token0 + tok) * a.ldq + (kh * a.group + r % a.group) * HD + 8 * h;
-        w.hi[i] = min(pos, a.cap - 1);
-        w.lo[i] = a.window ? pos - a.window + 1 : 0;
-        w.m[i] = -INFINITY;
-        w.l[i] = 0.f;
-        w.c[i] = a.scale;
-#pragma unroll
-        for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) w.o[i][d][e] = 0.f;
-        if constexpr (!F32) {
-#pragma unroll
-            for (int k = 0; k < HD / 16; ++k)
-                w.q[i][k][0] = *reinterpret_cast<const h8_t*>(static_cast<const _Float16*>(a.q) + at + 16 * k);
+    for (int k = 0; k < HD / 16; ++k) {
+        if constexpr (F32) {
+            const float* src = static_cast<const float*>(a.q) + at + 16 * k;
+            raw.v[k][0] = *reinterpret_cast<const float4*>(src);
+            raw.v[k][1] = *reinterpret_cast<const float4*>(src + 4);
         } else {
-            const float* src = static_cast<const float*>(a.q) + at;
-            float v[HD / 16][8], top = 0.f;
-#pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-                const float4 x = *reinterpret_cast<const float4*>(src + 16 * k);
-                const float4 y = *reinterpret_cast<const float4*>(src + 16 * k + 4);
-                v[k][0] = x.x, v[k][1] = x.y, v[k][2] = x.z, v[k][3] = x.w;
-                v[k][4] = y.x, v[k][5] = y.y, v[k][6] = y.z, v[k][7] = y.w;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[k][e]));
-            }
-            top = swap32_max(top);
-            // 2^up brings the row's largest magnitude into [2^13, 2^14); the low
-            // part's smallest step is then 2^-37 of it
-            int up = top > 0.f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
-            up = min(max(up, -115), 100);
-            w.c[i] = ldexpf(a.scale, -up);
-#pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-                float lo[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[k][e] = ldexpf(v[k][e], up);
-                w.q[i][k][0] = cvt8(v[k]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) lo[e] = v[k][e] - (float)w.q[i][k][0][e];
-                w.q[i][k][1] = cvt8(lo);
-            }
+            w.q[0][k][0] = *reinterpret_cast<const h8_t*>(static_cast<const _Float16*>(a.q) + at + 16 * k);
         }
     }
 }
-
-// The queries are in their registers from here on: without this the compiler waits
-// for their loads at their first use in the loop, in every step, and so for the
-// step's own loads behind them.
-template <int HD, int QT, bool F32>
-__device__ __forceinline__ void arrived(Rows<HD, QT, F32>& w) {
+template <int HD, bool F32>
+__device__ __forceinline__ void arrived(Rows<HD, 1, F32>& w, RawRows<HD, F32>& raw) {
 #pragma unroll
-    for (int i = 0; i < QT; ++i)
+    for (int k = 0; k < HD / 16; ++k) {
+        if constexpr (F32) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float4& v = raw.v[k][j];
+                asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
+            }
+        } else {
+            asm volatile("" : "+v"(w.q[0][k][0]));
+        }
+    }
+}
+// Rows to operands (fp32: two fp16 parts), and nothing added up yet.
+template <int HD, bool F32>
+__device__ __forceinline__ void start_rows(const AttnArgs& a, Rows<HD, 1, F32>& w, const RawRows<HD, F32>& raw) {
+    w.m[0] = -INFINITY;
+    w.l[0] = 0.f;
+    w.c[0] = a.scale;
+    if constexpr (F32) {
+        float top = 0.f;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
 #pragma unroll
-            for (int p = 0; p < Rows<HD, QT, F32>::QP; ++p) asm volatile("" : "+v"(w.q[i][k][p]));
+            for (int j = 0; j < 2; ++j) {
+                const float4 x = raw.v[k][j];
+                top = fmaxf(fmaxf(top, fabsf(x.x)), fmaxf(fabsf(x.y), fmaxf(fabsf(x.z), fabsf(x.w))));
+            }
+        top = swap32_max(top);
+        // 2^up brings the row's largest magnitude into [2^13, 2^14); the low
+        // part's smallest step is then 2^-37 of it
+        int up = top > 0.f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+        up = min(max(up, -115), 100);
+        w.c[0] = ldexpf(a.scale, -up);
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+            const float4 x = raw.v[k][0], y = raw.v[k][1];
+            float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], up);
+            w.q[0][k][0] = cvt8(v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] -= (float)w.q[0][k][0][e];
+            w.q[0][k][1] = cvt8(v);
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < HD / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w.o[0][d][e] = 0.f;
 }
 
 // S^T of 32 KT keys: s[i][t] holds, per lane, query lane % 32 of row tile i and
@@ -542,16 +569,15 @@ __device__ __forceinline__ float reciprocal(float l) { return l == 0.f ? 0.f : 1
 struct Item {
     int seq, tile, split, first, chunk, live;
     int part;  // its number among the items of split tiles
+    Seq of;
 };
 
 // A sequence's tiles, and the first and the number of its keys.
 template <int TM>
-__device__ __forceinline__ void seq_size(const AttnArgs& a, int s, int* tiles, int* first, int* keys) {
-    const int from = start_of(a.b, s), n = min(max(a.b.q_start[s + 1], from), a.b.tokens) - from;
-    const int kv = max(a.b.kv_len[s], 0);
-    *tiles = (n * a.group + TM - 1) / TM;
-    *first = a.window ? max(min(kv - n, a.cap) - a.window + 1, 0) & ~63 : 0;
-    *keys = max(min(kv, a.cap) - *first, 0);
+__device__ __forceinline__ void seq_size(const AttnArgs& a, const Seq& of, int* tiles, int* first, int* keys) {
+    *tiles = (of.n * a.group + TM - 1) / TM;
+    *first = a.window ? max(min(of.kv - of.n, a.cap) - a.window + 1, 0) & ~63 : 0;
+    *keys = max(min(of.kv, a.cap) - *first, 0);
 }
 // 64-key units per item, for a batch of `total` units.
 __device__ __forceinline__ int chunk_units(const AttnArgs& a, int64_t total, int units) {
@@ -593,7 +619,7 @@ __global__ void __launch_bounds__(1024) paged_items_kernel(AttnArgs a, int2* out
     int tiles, first, keys, chunk, live;
     int64_t total = 0;
     for (int s = t; s < a.b.seqs; s += 1024) {
-        seq_size<TM>(a, s, &tiles, &first, &keys);
+        seq_size<TM>(a, load_seq(a, s), &tiles, &first, &keys);
         total += (int64_t)tiles * ((keys + 63) >> 6);
     }
     total = sum_wave(total);
@@ -606,7 +632,7 @@ __global__ void __launch_bounds__(1024) paged_items_kernel(AttnArgs a, int2* out
         const int s = s0 + t;
         unsigned long long own = 0;
         if (s < a.b.seqs) {
-            seq_size<TM>(a, s, &tiles, &first, &keys);
+            seq_size<TM>(a, load_seq(a, s), &tiles, &first, &keys);
             const int items = seq_items<TM>(a, total, tiles, keys, &chunk, &live);
             own = both_counts(items, live);
         }
@@ -630,17 +656,22 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* i
     if (a.items) {
         const int s = last_seq(a.b.seqs, [&](int i) { return a.items[i].x <= number; });
         const int2 from = a.items[s], sum = a.items[a.b.seqs];
-        seq_size<TM>(a, s, &tiles, &first, &keys);
+        const Seq of = load_seq(a, s);
+        seq_size<TM>(a, of, &tiles, &first, &keys);
         const int items = seq_items<TM>(a, (int64_t)sum.y << 32 | (unsigned)sum.x, tiles, keys, &chunk, &live);
         const int at = number - from.x;
         if (at < 0 || at >= items) return false;
-        *item = Item{s, at / live, at % live, first, chunk * 64, live, from.y + at};
+        *item = Item{s, at / live, at % live, first, chunk * 64, live, from.y + at, of};
     } else {
         __shared__ unsigned long long upto_of[4];
         __shared__ int64_t totals[4];
         __shared__ Item found;
         const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-        if (t < a.b.seqs) seq_size<TM>(a, t, &tiles, &first, &keys);
+        Seq of{};
+        if (t < a.b.seqs) {
+            of = load_seq(a, t);
+            seq_size<TM>(a, of, &tiles, &first, &keys);
+        }
         if (t == 0) found.seq = -1;
         const int64_t own_total = sum_wave((int64_t)tiles * ((keys + 63) >> 6));
         if (lane == 0) totals[wave] = own_total;
@@ -653,7 +684,7 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* i
         for (int w = 0; w < 3; ++w) from += w < wave ? upto_of[w] : 0;
         const int at = number - (int)(unsigned)from;
         if (at >= 0 && at < items)
-            found = Item{t, at / live, at % live, first, chunk * 64, live, (int)(from >> 32) + at};
+            found = Item{t, at / live, at % live, first, chunk * 64, live, (int)(from >> 32) + at, of};
         __syncthreads();
         if (found.seq < 0) return false;
         *item = found;
@@ -665,6 +696,9 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* i
     item->chunk = __builtin_amdgcn_readfirstlane(item->chunk);
     item->live = __builtin_amdgcn_readfirstlane(item->live);
     item->part = __builtin_amdgcn_readfirstlane(item->part);
+    item->of.token0 = __builtin_amdgcn_readfirstlane(item->of.token0);
+    item->of.n = __builtin_amdgcn_readfirstlane(item->of.n);
+    item->of.kv = __builtin_amdgcn_readfirstlane(item->of.kv);
     return true;
 }
 
@@ -682,7 +716,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
     const int64_t part0 = ((int64_t)item.part * a.c.kv_heads + kh) * TM;
     if (!whole && (part0 < 0 || part0 + TM > a.parts)) return;
     const int seq = item.seq;
-    const Tile t = make_tile<TM>(a, seq, item.tile * TM);
+    const Tile t = make_tile<TM>(a, seq, item.of, item.tile * TM);
     const int begin = item.first + item.split * item.chunk, end = min(begin + item.chunk, t.end);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     char* K = lds + wave * 2 * HALF;
@@ -707,13 +741,22 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
     };
     int key0 = begin + wave * KEYS;
     bool odd = false;
+    if (key0 < end) pages.fetch(key0 >> pages.shift);
+    RawRows<HD, F32> raw;
+    if constexpr (F32) {  // (they are converted while the first step is on its way)
+        load_rows<HD, F32>(a, t, kh, t.row0, w, raw);
+        arrived(w, raw);
+    }
     if (key0 < end) {
         look(key0, id);
         load(std::false_type{}, key0, id);
         load(std::true_type{}, key0, id);
     }
-    load_rows<HD, 1, F32>(a, t, kh, t.row0, w);
-    arrived(w);
+    if constexpr (!F32) {
+        load_rows<HD, F32>(a, t, kh, t.row0, w, raw);
+        arrived(w, raw);
+    }
+    start_rows(a, w, raw);
     while (key0 < end) {
         const int after = key0 + 4 * KEYS;
         const bool more = after < end;
@@ -815,7 +858,7 @@ __global__ void __launch_bounds__(64 * many_waves(HD, F32), many_waves(HD, F32) 
     const int kh = blockIdx.x % a.c.kv_heads, number = a.tiles - 1 - blockIdx.x / a.c.kv_heads, split = blockIdx.y;
     const int seq = find_seq<TM>(a.b, a.group, number);
     const int first = start_of(a.b, seq) * a.group / TM + seq;
-    const Tile t = make_tile<TM>(a, seq, (number - first) * TM);
+    const Tile t = make_tile<TM>(a, seq, load_seq(a, seq), (number - first) * TM);
     if (t.row0 >= t.rows) return;
     const int begin = t.first + split * t.chunk, end = min(begin + t.chunk, t.end);
     if (split && begin >= end) return;
@@ -855,9 +898,12 @@ __global__ void __launch_bounds__(64 * many_waves(HD, F32), many_waves(HD, F32) 
     unsigned bad = 0, bad_next = 0;
     int buffer = 0;
     bool odd = false;
+    if (begin < end) pages.fetch(begin >> pages.shift);
+    RawRows<HD, F32> raw;
+    load_rows<HD, F32>(a, t, kh, row, w, raw);
+    arrived(w, raw);
     if (begin < end) bad = load(begin, 0);
-    load_rows<HD, 1, F32>(a, t, kh, row, w);
-    arrived(w);
+    start_rows(a, w, raw);
     for (int key0 = begin; key0 < end; key0 += KEYS) {
         wait_loads<0>();
         __syncthreads();  // the step is in LDS, and the other buffer is free
