@@ -56,6 +56,7 @@ typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
 typedef short s4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxSplits = 64;  // of one tile's keys
+constexpr int64_t kEarlyBytes = int64_t(1) << 20;  // of parts that a join may ask for unseen
 
 struct AttnArgs {
     const void* q;
@@ -71,7 +72,8 @@ struct AttnArgs {
     // reference and weight sum), and for each token and head of a group where its are
     float* o;           // [parts][head_dim]
     float2* ml;         // [parts]
-    int2* info;         // [tokens][group]: live splits, 32 first part + row (paged_few_kernel); null: nothing is split
+    int most;           // splits of a tile at most, where parts are [split][token][query head]; 0: by item (paged_few_kernel)
+    int2* info;         // [tokens][group]: live splits, and where parts are by item 32 first part + row; null: nothing is split
     const int2* items;  // paged_items_kernel's; null: at most kItemSeqs sequences, or paged_many_kernel
     int64_t parts;
 };
@@ -714,7 +716,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
     // (starts out of order may count past what the workspace holds)
     const bool whole = item.live <= 1;
     const int64_t part0 = ((int64_t)item.part * a.c.kv_heads + kh) * TM;
-    if (!whole && (part0 < 0 || part0 + TM > a.parts)) return;
+    if (!whole && (a.most ? item.split >= a.most : part0 < 0 || part0 + TM > a.parts)) return;
     const int seq = item.seq;
     const Tile t = make_tile<TM>(a, seq, item.of, item.tile * TM);
     const int begin = item.first + item.split * item.chunk, end = min(begin + item.chunk, t.end);
@@ -824,14 +826,16 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
             v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
         }
         const int tok = (t.row0 + row) / a.group, head = kh * a.group + (t.row0 + row) % a.group;
+        const int64_t part = a.most ? ((int64_t)item.split * a.b.tokens + t.token0 + tok) * (a.group * a.c.kv_heads) + head
+                                    : part0 + row;
         if (whole) {
             const float inv = reciprocal(sum);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] *= inv;
         } else if (piece == 0) {
-            a.ml[part0 + row] = make_float2(m, sum);
+            a.ml[part] = make_float2(m, sum);
         }
-        put4(a, !F32, whole, part0 + row, t.token0 + tok, head, HD, 4 * piece, v);
+        put4(a, !F32, whole, part, t.token0 + tok, head, HD, 4 * piece, v);
     }
 }
 
@@ -948,11 +952,12 @@ __global__ void __launch_bounds__(64 * many_waves(HD, F32), many_waves(HD, F32) 
 
 // ---------------------------------------------------------- the splits' join ----
 
-// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's live splits. HD / 4
+// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's live splits (EARLY: of all places that
+// there are, before it is known which hold one). HD / 4
 // threads take a split's 16-byte columns, SIDE of them in a row (token, query head) take every
 // SIDE-th split, four at a time.
-template <int HD, int SIDE, bool F32>
-__global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a, bool few) {
+template <int HD, int SIDE, bool F32, bool EARLY>
+__global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a) {
     constexpr int TPR = HD / 4, ROWS = 256 / (TPR * SIDE);
     __shared__ float4 part[SIDE > 1 ? 256 : 1];
     __shared__ float2 sums[SIDE > 1 ? SIDE : 1];
@@ -964,14 +969,17 @@ __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a, bool few) {
     const int2 info = a.info[(int64_t)token * a.group + head % a.group];
     const int from = a.b.q_start[0], to = a.b.q_start[a.b.seqs];
     // (rows of no sequence have no info; that of rows of starts out of order may be an older call's)
-    const int live = info.x;
-    if (token < from || token >= to || live <= 1 || live > kMaxSplits) return;
+    int live = info.x, most = a.most;
     int64_t at = unit, next = (int64_t)a.b.tokens * heads;
-    if (few) {
-        at = ((int64_t)(info.y >> 5) * a.c.kv_heads + kh) * 32 + (info.y & 31);
-        next = (int64_t)a.c.kv_heads * 32;
+    if (!EARLY) {
+        if (token < from || token >= to || live <= 1 || live > kMaxSplits) return;
+        most = live;
+        if (!a.most) {
+            at = ((int64_t)(info.y >> 5) * a.c.kv_heads + kh) * 32 + (info.y & 31);
+            next = (int64_t)a.c.kv_heads * 32;
+        }
+        if (at < 0 || at + (live - 1) * next >= a.parts) return;
     }
-    if (at < 0 || at + (live - 1) * next >= a.parts) return;
     float m = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
     auto add = [&](float2 ml, float4 x) {
         const float to = fmaxf(m, ml.x);
@@ -980,12 +988,12 @@ __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a, bool few) {
         sum = f * sum + g * ml.y;
         v[0] = f * v[0] + g * x.x, v[1] = f * v[1] + g * x.y, v[2] = f * v[2] + g * x.z, v[3] = f * v[3] + g * x.w;
     };
-    for (int c = side; c < live; c += 4 * SIDE) {
+    for (int c = side; c < most; c += 4 * SIDE) {
         float4 x[4];
         float2 ml[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int64_t row = at + min(c + k * SIDE, live - 1) * next;
+            const int64_t row = at + min(c + k * SIDE, most - 1) * next;
             x[k] = *reinterpret_cast<const float4*>(a.o + row * HD + 4 * col);
             ml[k] = a.ml[row];
         }
@@ -993,6 +1001,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a, bool few) {
         for (int k = 0; k < 4; ++k)
             if (c + k * SIDE < live) add(ml[k], x[k]);
     }
+    if (EARLY && (token < from || token >= to || live <= 1 || live > most)) return;
     if constexpr (SIDE > 1) {
         part[threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
         if (col == 0) sums[side] = make_float2(m, sum);
@@ -1014,7 +1023,7 @@ constexpr int many_lds(int hd, bool f32) { return 2 * 2 * many_keys(hd, f32) * h
 
 struct AttnPlan {
     bool few, join, items;
-    int splits, min_chunk;
+    int splits, min_chunk, most;
     int64_t tiles, parts;
 };
 
@@ -1041,6 +1050,13 @@ AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int gro
         p.splits = (int)(most < want ? most : want < 1 ? 1 : want);
         p.join = cap > p.min_chunk;
         p.parts = p.join ? (int64_t)2 * p.splits * kv_heads * 32 : 0;
+        // Parts have fixed places where all that there could be take up to 1 MiB: the join then asks for them before
+        // it knows which there are (one token over 4,096, 0.3 MB: 13.4 -> 12.9 us; 40 over up to 3,000, 2 MB:
+        // 13.1 -> 13.4).
+        const int64_t all = (cap + p.min_chunk - 1) / p.min_chunk;
+        p.most = (int)(all < kMaxSplits ? all : kMaxSplits);
+        if (!p.join || (int64_t)tokens * heads * p.most * hd * 4 > kEarlyBytes) p.most = 0;
+        else p.parts = (int64_t)tokens * heads * p.most;
     } else {
         p.tiles = (int64_t)tokens * group / (32 * many_waves(hd, f32)) + seqs;
         // Keys are split where the tiles take at most half of the CUs (at less, a split's uneven second part
@@ -1053,6 +1069,7 @@ AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int gro
         p.splits = (int)(s > kMaxSplits ? kMaxSplits : s < 1 ? 1 : s);
         p.join = p.splits > 1;
         p.parts = p.join ? (int64_t)p.splits * tokens * heads : 0;
+        p.most = p.splits;
     }
     return p;
 }
@@ -1080,11 +1097,10 @@ hipError_t launch_attention_hd(const AttnPlan& p, const AttnArgs& a, hipStream_t
     // 64: 24 us less). One row of 33 splits: 3.8 us by a workgroup, 6.3 by HD / 4 threads.
     const int64_t rows = (int64_t)a.b.tokens * a.group * a.c.kv_heads;
     constexpr int SIDE = 1024 / HD;
-    if (rows <= 2048)
-        hipLaunchKernelGGL((paged_join_kernel<HD, SIDE, F32>), dim3((unsigned)rows), dim3(256), 0, stream, a, p.few);
-    else
-        hipLaunchKernelGGL((paged_join_kernel<HD, 1, F32>), dim3((unsigned)((rows + SIDE - 1) / SIDE)), dim3(256), 0,
-                           stream, a, p.few);
+    const dim3 wide((unsigned)rows), narrow((unsigned)((rows + SIDE - 1) / SIDE)), threads(256);
+    if (p.few && p.most) hipLaunchKernelGGL((paged_join_kernel<HD, SIDE, F32, true>), wide, threads, 0, stream, a);
+    else if (rows <= 2048) hipLaunchKernelGGL((paged_join_kernel<HD, SIDE, F32, false>), wide, threads, 0, stream, a);
+    else hipLaunchKernelGGL((paged_join_kernel<HD, 1, F32, false>), narrow, threads, 0, stream, a);
     return hipGetLastError();
 }
 
@@ -1127,6 +1143,7 @@ hipError_t launch_paged_attention(const PagedBatch& b, const PagedCache& c, cons
     a.tiles = (int)p.tiles;
     a.splits = p.splits;
     a.min_chunk = p.min_chunk;
+    a.most = p.most;
     a.o = static_cast<float*>(workspace);
     a.ml = reinterpret_cast<float2*>(a.o + p.parts * c.head_dim);
     int2* behind = reinterpret_cast<int2*>(a.ml + p.parts);
