@@ -694,6 +694,7 @@ class PagedCache:
         self.k, self.v = k, v
         self.blocks, self.block_size, self.kv_heads, self.head_dim = blocks, block_size, kv_heads, head_dim
         self.struct = _CacheStruct(_p(k), _p(v), blocks, block_size, kv_heads, head_dim)
+        self.ref = byref(self.struct)  # (what calls pass; making one takes 0.1 us a call)
 
     @classmethod
     def allocate(cls, blocks: int, block_size: int, kv_heads: int, head_dim: int) -> "PagedCache":
@@ -713,6 +714,7 @@ class PagedBatch:
         self.positions, self.slots = positions, slots
         self.struct = _BatchStruct(_p(q_start), _p(kv_len), _p(block_table), table_stride or max_blocks, max_blocks,
                                    seqs, tokens, _p(positions), _p(slots))
+        self.ref = byref(self.struct)
 
     @classmethod
     def allocate(cls, seqs: int, tokens: int, max_blocks: int) -> "PagedBatch":
@@ -726,7 +728,7 @@ def paged_plan(batch: PagedBatch, cache: PagedCache, cached_len, new_len, free_l
                free_head_out, status, stream: Stream | None = None):
     """Block tables, starts, positions and slots from the requests' lengths
     (rqmv_paged_plan); `status` (int32 on the device) says whether the step fits."""
-    _check(lib().lib.rqmv_paged_plan(byref(batch.struct), byref(cache.struct), cached_len.ptr, new_len.ptr,
+    _check(lib().lib.rqmv_paged_plan(batch.ref, cache.ref, cached_len.ptr, new_len.ptr,
                                      _p(free_list), free_count, free_head.ptr, free_head_out.ptr, status.ptr,
                                      _sh(stream)), "rqmv_paged_plan")
 
@@ -736,7 +738,7 @@ def qk_norm_rope(batch: PagedBatch, cache: PagedCache, qkv, x_dtype: int, ld: in
                  rot_dim: int | None = None, stream: Stream | None = None):
     """Per-head norms and rotation of queries and keys, the append to the paged
     cache (rqmv_qk_norm_rope); rot_dim defaults to the whole head."""
-    _check(lib().lib.rqmv_qk_norm_rope(byref(batch.struct), byref(cache.struct), qkv.ptr, x_dtype, ld, q_heads,
+    _check(lib().lib.rqmv_qk_norm_rope(batch.ref, cache.ref, qkv.ptr, x_dtype, ld, q_heads,
                                        _p(q_norm), _p(k_norm), eps, table.ptr,
                                        cache.head_dim if rot_dim is None else rot_dim, rope_rows, q_out.ptr, q_dtype,
                                        ldq, _sh(stream)), "rqmv_qk_norm_rope")
@@ -744,7 +746,7 @@ def qk_norm_rope(batch: PagedBatch, cache: PagedCache, qkv, x_dtype: int, ld: in
 
 def paged_attention_workspace_size(batch: PagedBatch, cache: PagedCache, q_heads: int) -> int:
     n = c_size_t()
-    _check(lib().lib.rqmv_paged_attention_workspace_size(byref(batch.struct), byref(cache.struct), q_heads, byref(n)),
+    _check(lib().lib.rqmv_paged_attention_workspace_size(batch.ref, cache.ref, q_heads, byref(n)),
            "rqmv_paged_attention_workspace_size")
     return n.value
 
@@ -757,7 +759,7 @@ def paged_attention(batch: PagedBatch, cache: PagedCache, q, dtype: int, ldq: in
                     workspace=None, scale: float | None = None, window: int = 0, stream: Stream | None = None):
     """The new tokens' attention over their pages (rqmv_paged_attention); scale
     defaults to 1 / sqrt(head_dim)."""
-    _check(lib().lib.rqmv_paged_attention(byref(batch.struct), byref(cache.struct), q.ptr, dtype, ldq, q_heads,
+    _check(lib().lib.rqmv_paged_attention(batch.ref, cache.ref, q.ptr, dtype, ldq, q_heads,
                                           cache.head_dim ** -0.5 if scale is None else scale, window, _p(workspace),
                                           workspace.nbytes if workspace is not None else 0, out.ptr, ldo, _sh(stream)),
            "rqmv_paged_attention")
