@@ -279,8 +279,8 @@ int rqmv_attention_rope(const float* qkv, const float* rope_table, void* k_cache
  * q_start[s + 1] - 1 (q_start holds seqs + 1 entries, never decreasing, from
  * 0; rows from q_start[seqs] on belong to no sequence and are padding), the
  * last of its kv_len[s] positions. Its position p lies in block
- * block_table[s * table_stride + p / block_size] at row p % block_size, for p
- * < max_blocks * block_size (at most 2^30); a table entry outside 0..blocks-1 is an absent
+ * block_table[s * table_stride + p / block_size] at row p % block_size, for
+ * p < max_blocks * block_size (at most 2^30); a table entry outside 0..blocks-1 is an absent
  * page, whose positions are never attended to. positions and slots hold each
  * row's position and slot (-1: none). Each call names the fields it reads;
  * the others may be NULL. */
@@ -350,22 +350,21 @@ int rqmv_qk_norm_rope(const rqmv_paged_batch* batch, const rqmv_paged_cache* cac
 /* Grouped-query attention of the batch's new tokens over their pages: for each
  * query head of the row at position p (rows of q and out: q + row * ldq, out +
  * row * ldo elements, q_heads heads of head_dim) softmax(scale q k) v over the
- * positions max(0, p - window + 1)..p of its sequence (window 0 or above 2^30:
- * 0..p) whose
- * pages are present, in kv head h / (q_heads / kv_heads); zeros where there is
- * none. The new tokens' own keys and values are in the cache
- * already (rqmv_qk_norm_rope). out has the dtype of q: fp32 rows are computed to fp32
- * accuracy, fp16 rows with the softmax weights rounded to fp16; sums and
- * statistics are fp32 in both. A position that is not attended to never touches
- * the result, whatever its key and value hold. A NaN or an infinity in a query, or
- * in a key or value attended to, makes its rows non-finite. Rows of no sequence are
- * not written. q_heads is a multiple of kv_heads, both at most 1024; scale is positive; ldq
- * and ldo are multiples of 16 bytes, q and out 16-byte aligned; out is q itself (ldo
- * = ldq) or spans none of its memory. Reads q_start, kv_len, block_table of the batch. One
- * launch, one more where the keys are split over workgroups and one above 256 sequences:
- * then the workspace (16-byte aligned, rqmv_paged_attention_workspace_size bytes for this
- * batch's counts, cache and q_heads on the current device; 0: may be NULL) holds partial
- * results, and calls that share it must not overlap. */
+ * positions max(0, p - window + 1)..p of its sequence (window 0 or above 2^30: 0..p)
+ * whose pages are present, in kv head h / (q_heads / kv_heads); zeros where there is
+ * none. The new tokens' own keys and values are in the cache already
+ * (rqmv_qk_norm_rope). out has the dtype of q: fp32 rows are computed to fp32 accuracy,
+ * fp16 rows with the softmax weights rounded to fp16; sums and statistics are fp32 in
+ * both. A position that is not attended to never touches the result, whatever its key
+ * and value hold. A NaN or an infinity in a query, or in a key or value attended to,
+ * makes its rows non-finite. Rows of no sequence are not written. q_heads is a multiple
+ * of kv_heads, both at most 1024; scale is positive; ldq and ldo are multiples of 16
+ * bytes, q and out 16-byte aligned; out is q itself (ldo = ldq) or spans none of its
+ * memory. Reads q_start, kv_len, block_table of the batch. One launch, one more where
+ * the keys are split over workgroups and one above 256 sequences: then the workspace
+ * (16-byte aligned, rqmv_paged_attention_workspace_size bytes for this batch's counts,
+ * cache and q_heads on the current device; 0: may be NULL) holds partial results, and
+ * calls that share it must not overlap. */
 int rqmv_paged_attention_workspace_size(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, int q_heads,
                                         size_t* bytes);
 int rqmv_paged_attention(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, const void* q, int dtype,
@@ -391,12 +390,13 @@ int rqmv_argmax(const float* values, int n, int* out, void* workspace, size_t wo
  *   (top_p outside [0, 1): all); of these those with e >= min_p (min_p <= 0: all,
  *   above 1 as 1);
  *   tokens[r] is the candidate at which the running sum of e in that order first
- *   exceeds u times the kept sum (u < 0 or NaN as 0, u >= 1 the last one), and
- *   probs[r] (probs may be NULL) its e over the kept sum.
+ *   exceeds u times the kept sum (u < 0 or NaN as 0, u >= 1 the last one that
+ *   counts, below), and probs[r] (probs may be NULL) its e over the kept sum.
  * temperature <= 0 (or NaN): the first candidate, with probability 1 (rqmv_argmax's
  * choice). A row without candidates gives -1, with probability 0. Sums are exact sums
- * of e in units of 2^-42, so a row's token does not depend on the other rows or on
- * scheduling. n is at most 2^20, rows at most 2^20. The workspace is 16-byte aligned
+ * of e in whole units of 2^-42, so a row's token does not depend on the other rows or
+ * on scheduling, and a candidate whose e rounds to 0 units (below 2^-43) is never
+ * drawn. n is at most 2^20, rows at most 2^20. The workspace is 16-byte aligned
  * (rqmv_sample_workspace_size bytes on the current device; 0: may be NULL); calls
  * sharing it must not overlap. No counterpart in the reference's kernels (its driver
  * samples on the host, recipe.rs:20286-20296). */
