@@ -408,7 +408,9 @@ __device__ __forceinline__ void move_references(Rows<HD, QT, F32>& w, const floa
 template <int HD, int QT, int KT, bool F32>
 __device__ __forceinline__ void weights(Rows<HD, QT, F32>& w, const f16_t (&s)[QT][KT],
                                         h8_t (&p)[QT][2 * KT][F32 ? 2 : 1]) {
-    constexpr float SHIFT = F32 ? 15.f : 6.f;
+    // fp32 rows: 2^15 comes after the exponential. With 15 added to the argument its last bit is 2^-20, and rows of
+    // six keys were off by 1.8e-7 instead of 1.2e-7 (as fast). fp16 rows: 2^6 in the argument is one
+    // instruction less and below the weights' own rounding.
     // fp16, up to 128 dims: the sum of the rounded weights, two at a time. What a large weight's rounding adds
     // to the row it adds to the divisor too, so a row of one large weight is off by its output's rounding alone
     // (2048 tokens over 14,336: 507 -> 504 us; 6,000, 8/4 heads of 256: 204 -> 213 us, so there the weights
@@ -416,7 +418,7 @@ __device__ __forceinline__ void weights(Rows<HD, QT, F32>& w, const f16_t (&s)[Q
     constexpr bool PAIRS = !F32 && HD <= 128;
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
-        const float ref = w.m[i] == -INFINITY ? 0.f : w.m[i] - SHIFT;
+        const float ref = w.m[i] == -INFINITY ? 0.f : w.m[i] - (F32 ? 0.f : 6.f);
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
@@ -425,6 +427,7 @@ __device__ __forceinline__ void weights(Rows<HD, QT, F32>& w, const f16_t (&s)[Q
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     v[e] = __builtin_amdgcn_exp2f(fmaf(s[i][t][8 * b + e], w.c[i], -ref));
+                    if constexpr (F32) v[e] *= 0x1p15f;
                     if constexpr (!PAIRS) w.l[i] += v[e];
                 }
                 h8_t& hi = p[i][2 * t + b][0];
