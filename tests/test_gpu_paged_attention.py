@@ -478,3 +478,31 @@ def test_many_starts_out_of_order_stay_inside_the_rows(gpu):
     for start in (np.arange(301)[::-1] * 2, np.where(np.arange(301) % 2, 600, 0), np.full(301, -3), np.arange(301) * 9):
         c.q_start = start.astype(np.int32)
         c.run(gpu, pad=8)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("nq,nkv,hd,new,ctx", [(4, 2, 128, 1, 700), (4, 1, 64, 3, 40), (8, 4, 256, 2, 300),
+                                               (128, 2, 64, 270, 30), (128, 2, 128, 270, 30), (128, 2, 256, 270, 30)])
+@pytest.mark.parametrize("scale", [1e3, 1e6, 1e20])
+def test_scores_whose_last_bit_passes_one(gpu, nq, nkv, hd, new, ctx, scale, f16):
+    """Scores of 10^5 and more: where the largest leads by 10^-4 of itself (a dot's rounding takes up to
+    (hd / 8 + 8) 2^-24 < 3e-6 of the magnitudes' sum, here up to ten times the score) its value is the row's."""
+    c = Case([(new, ctx)], nq, nkv, hd, 16, f16, 43)
+    c.q *= 100 if f16 else 1e5
+    got = c.run(gpu, scale=scale).astype(np.float64)
+    assert np.isfinite(got).all()
+    at = np.arange(new + ctx)
+    k, v = (x[c.table[0, at // 16], :, at % 16].astype(np.float64) for x in (c.k, c.v))
+    some = 0
+    for h in range(nq):
+        g = h // (nq // nkv)
+        s = c.q[:, h].astype(np.float64) @ k[:, g].T
+        s[at[None, :] > ctx + np.arange(new)[:, None]] = -np.inf
+        first = s.argmax(1)
+        best = np.take_along_axis(s, first[:, None], 1)[:, 0]
+        np.put_along_axis(s, first[:, None], -np.inf, 1)
+        size = np.abs(c.q[:, h].astype(np.float64)) @ np.abs(k[:, g]).T
+        sure = best - s.max(1) > 1e-4 * size.max(1) if s.shape[1] > 1 else np.ones(new, bool)
+        some += sure.sum()
+        assert np.all(np.abs(got[sure, h] - v[first[sure], g]) <= 2.0 ** -10 * np.abs(v[first[sure], g]))
+    assert some > new * nq // 2
