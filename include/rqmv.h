@@ -356,8 +356,11 @@ int rqmv_qk_norm_rope(const rqmv_paged_batch* batch, const rqmv_paged_cache* cac
  * (rqmv_qk_norm_rope). out has the dtype of q: fp32 rows are computed to fp32 accuracy,
  * fp16 rows with the softmax weights rounded to fp16; sums and statistics are fp32 in
  * both. A position that is not attended to never touches the result, whatever its key
- * and value hold. A NaN or an infinity in a query, or in a key or value attended to,
- * makes its rows non-finite. Rows of no sequence are not written. q_heads is a multiple
+ * and value hold. A NaN or an infinity in a query or in a value attended to, and a NaN in
+ * a key attended to, make their rows non-finite. So does an infinity in a key where the
+ * score is +infinity or NaN; where it is -infinity the key weighs nothing beside finite scores
+ * (fp32 rows may be NaN instead), and a row all of whose scores are -infinity is NaN.
+ * Rows of no sequence are not written. q_heads is a multiple
  * of kv_heads, both at most 1024; scale is positive; ldq and ldo are multiples of 16
  * bytes, q and out 16-byte aligned; out is q itself (ldo = ldq) or spans none of its
  * memory. Reads q_start, kv_len, block_table of the batch. One launch, one more where

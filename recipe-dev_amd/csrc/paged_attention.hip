@@ -572,6 +572,18 @@ __device__ __forceinline__ float part_weight(float m, float l, float to) {
     return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - to);
 }
 __device__ __forceinline__ float reciprocal(float l) { return l == 0.f ? 0.f : 1.f / l; }  // (no key: zeros)
+// The weight sum of a row that has seen keys, all of whose scores are -infinity: beside another part's sum it adds nothing,
+// and alone its reciprocal is infinite, which makes the row's sums of 0 NaN.
+constexpr float kNoWeight = 0x1p-140f;
+// Whether any of keys from..to of the sequence is in a present page.
+__device__ __forceinline__ bool sees_key(const AttnArgs& a, int seq, int from, int to) {
+    if (from > to) return false;
+    const int* table = a.b.table + seq * a.b.table_stride;
+#pragma unroll 1
+    for (int page = from >> a.c.block_shift; page <= to >> a.c.block_shift; ++page)
+        if ((unsigned)table[page] < (unsigned)a.c.blocks) return true;
+    return false;
+}
 
 // ------------------------------------------- few rows: keys over the waves ----
 
@@ -845,6 +857,10 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
             v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
         }
         const int tok = (t.row0 + row) / a.group, head = kh * a.group + (t.row0 + row) % a.group;
+        if (sum == 0.f) {
+            const int pos = t.kv - t.n + tok;
+            if (sees_key(a, seq, max(a.window ? pos - a.window + 1 : 0, begin), min(pos, end - 1))) sum = kNoWeight;
+        }
         const int64_t part = a.most ? ((int64_t)item.split * a.b.tokens + t.token0 + tok) * (a.group * a.c.kv_heads) + head
                                     : part0 + row;
         if (whole) {
@@ -952,7 +968,8 @@ __global__ void __launch_bounds__(64 * many_waves(HD, F32), many_waves(HD, F32) 
     if (odd) add_odd<HD, 1, F32>(a, t, kh, begin, end, w);
     const bool whole = t.live <= 1;
     const int h = lane >> 5, r = row + (lane & 31);
-    const float l = swap32_sum(w.l[0]);
+    float l = swap32_sum(w.l[0]);
+    if (l == 0.f && sees_key(a, t.seq, max(w.lo[0], begin), min(w.hi[0], end - 1))) l = kNoWeight;
     const float f = whole ? reciprocal(l) : 1.f;
     if (r >= t.rows) return;
     const int tok = t.token0 + r / a.group, head = kh * a.group + r % a.group;

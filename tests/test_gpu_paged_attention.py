@@ -506,3 +506,57 @@ def test_scores_whose_last_bit_passes_one(gpu, nq, nkv, hd, new, ctx, scale, f16
         some += sure.sum()
         assert np.all(np.abs(got[sure, h] - v[first[sure], g]) <= 2.0 ** -10 * np.abs(v[first[sure], g]))
     assert some > new * nq // 2
+
+
+ROWS_FORMS = [(4, 2, 64, 1), (4, 1, 256, 3), (8, 2, 128, 40), (128, 2, 64, 270), (128, 2, 128, 270), (128, 2, 256, 270),
+              (64, 1, 128, 262)]
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("nq,nkv,hd,new", ROWS_FORMS)
+@pytest.mark.parametrize("ctx", [0, 5, 900])
+def test_rows_whose_scores_are_all_minus_infinity(gpu, nq, nkv, hd, new, ctx, f16):
+    """An infinite query opposite to every key that it sees: e^(-inf - -inf) is undefined, and the row is NaN, not the zeros
+    of a row without keys."""
+    c = Case([(new, ctx)], nq, nkv, hd, 16, f16, 50)
+    c.k[..., 0] = -np.abs(c.k[..., 0]) - np.float16(0.25)
+    if ctx + new >= 32:
+        c.table[0, (ctx + new) // 32] = -1  # (an absent page among them, not the first)
+    clean = c.run(gpu)
+    assert np.isfinite(clean).all()
+    hurt = np.zeros(clean.shape, bool)
+    for row, head in ((0, 0), (new - 1, nq - 1), (new // 2, nq // 2)):
+        c.q[row, head, 0] = np.inf
+        hurt[row, head] = True
+    got = c.run(gpu)
+    assert np.isnan(got[hurt]).all() and np.array_equal(got[~hurt], clean[~hurt])
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("nq,nkv,hd,new", ROWS_FORMS)
+def test_infinite_keys(gpu, nq, nkv, hd, new, f16):
+    """A key whose score is -infinity weighs nothing beside finite ones (fp32 rows, whose queries are two parts, may
+    be NaN instead), and a row that sees only such keys is NaN; a score of +infinity makes the row NaN."""
+    ctx = 1500
+    c = Case([(new, ctx)], nq, nkv, hd, 16, f16, 51)
+    c.q[..., 0] = 8.0
+    at = lambda p: (c.table[0, p // 16], slice(None), p % 16, 0)  # noqa: E731
+    far = np.r_[0:1100, 1300, ctx - 1]  # (whole parts of split keys among them)
+    for p in far:
+        c.k[at(p)] = -60000.0  # a score of -480000 / sqrt(head_dim): a weight of zero
+    clean = c.run(gpu)
+    assert np.isfinite(clean).all()
+    for p in far:
+        c.k[at(p)] = -np.inf
+    got = c.run(gpu)
+    if f16:
+        assert np.array_equal(got, clean)
+    else:
+        whole = np.isfinite(got).all(-1)
+        assert np.array_equal(got[whole], clean[whole])
+    c.k[at(1200)] = np.inf
+    assert not np.isfinite(c.run(gpu)).any()
+    c.k[..., 0] = -np.inf
+    assert not np.isfinite(c.run(gpu)).any()
+    c.table[:] = -1  # no key at all
+    assert not c.run(gpu).any()
