@@ -42,6 +42,7 @@
 #include "lanes.h"
 #include "paged.h"
 
+#include <float.h>
 #include <limits.h>
 
 #include "halfcode.h"
@@ -285,7 +286,10 @@ __device__ __forceinline__ void start_rows(const AttnArgs& a, Rows<HD, 1, F32>& 
         // part's smallest step is then 2^-37 of it
         int up = top > 0.f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
         up = min(max(up, -115), 100);
-        w.c[0] = ldexpf(a.scale, -up);
+        // The scores' factor stays a normal number: 0 or infinite it would make NaN of masked scores or of zeros. (A lower
+        // `up` is for rows whose scores are below 2^-80, a lowered factor for scores far past fp32's range or 0.)
+        up = min(up, __builtin_amdgcn_frexp_expf(a.scale) + 125);
+        w.c[0] = fminf(ldexpf(a.scale, -up), FLT_MAX);
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
             const float4 x = raw.v[k][0], y = raw.v[k][1];

@@ -560,3 +560,32 @@ def test_infinite_keys(gpu, nq, nkv, hd, new, f16):
     assert not np.isfinite(c.run(gpu)).any()
     c.table[:] = -1  # no key at all
     assert not c.run(gpu).any()
+
+
+@pytest.mark.parametrize("hd,nq,nkv,new", [(64, 4, 2, 3), (128, 4, 2, 40), (256, 4, 1, 2), (64, 128, 2, 270),
+                                           (128, 128, 2, 270), (256, 128, 2, 270)])
+def test_factors_of_scores_at_the_ends_of_fp32(gpu, hd, nq, nkv, new):
+    """fp32 rows: tiny queries at a small scale, and queries near the type's end at a large one whose keys are zero there:
+    all scores are 0 or within 2^-60 of it, so each row is the mean of the values that it sees."""
+    ctx = 37
+    c = Case([(new, ctx)], nq, nkv, hd, 16, False, 52)
+    at = np.arange(new + ctx)
+    values = c.v[c.table[0, at // 16], :, at % 16].astype(np.float64)  # [keys, nkv, hd]
+
+    def check(scale):
+        got = c.run(gpu, scale=scale).astype(np.float64)
+        for i in range(new):
+            seen = values[:ctx + i + 1]
+            want = np.repeat(seen.mean(0), nq // nkv, 0)
+            size = np.repeat(np.abs(seen).mean(0), nq // nkv, 0)
+            # weights of 1 are exact; sums of up to 307 values, the division
+            assert np.all(np.abs(got[i] - want) <= (307 / 16 + 40) * 2.0 ** -24 * size), scale
+
+    c.q[:] *= np.float32(1e-30)
+    for scale in (1e-20, 1e-30, 1e-38, 1e-42):
+        check(scale)
+    c.q[:] = 0
+    c.q[..., 1] = 3e38
+    c.k[..., 1] = 0
+    for scale in (1e4, 1e10, 1e30):
+        check(scale)
