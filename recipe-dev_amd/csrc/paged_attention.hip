@@ -902,7 +902,7 @@ __global__ void __launch_bounds__(64 * many_waves(HD, F32), many_waves(HD, F32) 
     const int seq = find_seq<TM>(a.b, a.group, number);
     const int first = start_of(a.b, seq) * a.group / TM + seq;
     const Tile t = make_tile<TM>(a, seq, load_seq(a, seq), (number - first) * TM);
-    if (t.row0 >= t.rows) return;
+    if (t.row0 < 0 || t.row0 >= t.rows) return;  // (below 0: starts out of order)
     const int begin = t.first + split * t.chunk, end = min(begin + t.chunk, t.end);
     if (split && begin >= end) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

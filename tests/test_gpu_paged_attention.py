@@ -589,3 +589,34 @@ def test_factors_of_scores_at_the_ends_of_fp32(gpu, hd, nq, nkv, new):
     c.k[..., 1] = 0
     for scale in (1e4, 1e10, 1e30):
         check(scale)
+
+
+STARTS = [(128, 2, 64, True), (128, 2, 128, False), (128, 2, 256, True), (128, 2, 256, False), (64, 1, 128, True),
+          (64, 1, 64, False), (4, 2, 64, True), (2, 1, 128, False)]
+
+
+@pytest.mark.parametrize("nq,nkv,hd,f16", STARTS)
+@pytest.mark.parametrize("starts", [
+    [0, 270, 3, 4, 5, 270], [270, 200, 100, 50, 20, 0], [0, 260, 0, 260, 0, 270], [-9, 400, -9, 400, -9, 400],
+    [200, 210, 220, 230, 240, 270], [270] * 6, [-7] * 6, [2 ** 31 - 1] * 6, [0, -2 ** 31, 2 ** 31 - 1, 5, -1, 9],
+    [0, 0, 60, 60, 270, 270]])
+def test_starts_of_any_values_stay_inside_the_rows(gpu, nq, nkv, hd, f16, starts):
+    """Nothing before or behind the batch's rows is written, nor a row that no sequence could have."""
+    c = Case([(54, 100), (54, 0), (54, 300), (54, 7), (54, 64)], nq, nkv, hd, 16, f16, 54)
+    dt, bits = (np.float16, np.uint16) if f16 else (np.float32, np.uint32)
+    row, guard, size = nq * hd, 300, np.dtype(dt).itemsize
+    Q = gpu.DeviceBuffer.from_array(c.q.view(bits))
+    O = gpu.DeviceBuffer.from_array(np.full((c.rows + 2 * guard, row), 7, dt).view(bits))
+    batch = gpu.PagedBatch(5, c.rows, c.width, i32(gpu, starts), i32(gpu, c.kv_len), i32(gpu, c.table))
+    cache = gpu.PagedCache(gpu.DeviceBuffer.from_array(c.k.view(np.uint16)),
+                           gpu.DeviceBuffer.from_array(c.v.view(np.uint16)), c.blocks, 16, nkv, hd)
+    gpu.paged_attention(batch, cache, Q, 1 if f16 else 0, row, nq, O.view(guard * row * size, c.rows * row * size), row,
+                        gpu.paged_attention_workspace(batch, cache, nq))
+    gpu.synchronize()
+    out = O.download(bits).view(dt).reshape(c.rows + 2 * guard, row)
+    may = np.zeros(len(out), bool)  # rows between a start and the next one
+    for a, b in zip(starts, starts[1:]):
+        may[guard + min(max(a, 0), c.rows):guard + min(max(b, 0), c.rows)] = True
+    assert np.all(out[~may] == 7)
+    if sorted(starts) == starts and starts[0] >= 0:
+        assert np.all(out[may] != 7)
