@@ -620,3 +620,26 @@ def test_starts_of_any_values_stay_inside_the_rows(gpu, nq, nkv, hd, f16, starts
     assert np.all(out[~may] == 7)
     if sorted(starts) == starts and starts[0] >= 0:
         assert np.all(out[may] != 7)
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(128, 2, 64), (128, 2, 128), (128, 2, 256)])
+@pytest.mark.parametrize("less", [21, 23])
+def test_long_tail_of_small_weights(gpu, nq, nkv, hd, less):
+    """A first key over 40,000 equal ones of 2^-21 and 2^-23 of its weight, below fp16's normal range as the product takes
+    them: they count alike in the sum of the values and in the divisor. Their weights are whole steps of fp16
+    (the score's rounding, 23 * 2^-23, is far below half of one), and adding them to the first's loses nothing, so
+    the row is off by its output's rounding and a few of fp32."""
+    new, ctx = 270, 40000
+    c = Case([(new, ctx)], nq, nkv, hd, 256, True, 53)
+    c.q[:] = 0
+    c.q[..., 3] = 4
+    c.k[..., 3] = 0
+    c.k[c.table[0, 0], :, 0, 3] = 8
+    c.v[:] = 1
+    c.v[c.table[0, 0], :, 0] = 0
+    scale = np.float32(less * np.log(2) / 32)
+    t = np.exp(-32 * np.float64(scale))
+    n = ctx + np.arange(new)[:, None, None]
+    want = n * t / (1 + n * t)
+    got = c.run(gpu, scale=float(scale)).astype(np.float64)
+    assert np.all(np.abs(got - want) <= (2.0 ** -11 + 2.0 ** -17) * want), np.max(np.abs(got / want - 1))
