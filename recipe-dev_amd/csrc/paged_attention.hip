@@ -1002,7 +1002,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a) {
     __shared__ float4 part[SIDE > 1 ? 256 : 1];
     __shared__ float2 sums[SIDE > 1 ? SIDE : 1];
     const int heads = a.group * a.c.kv_heads;
-    const int64_t unit = (int64_t)blockIdx.x * ROWS + threadIdx.x / (TPR * SIDE);
+    const int64_t unit = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * ROWS + threadIdx.x / (TPR * SIDE);
     if (unit >= (int64_t)a.b.tokens * heads) return;  // (SIDE > 1: a row per workgroup, all of it leaves)
     const int token = (int)(unit / heads), head = (int)(unit % heads), kh = head / a.group;
     const int col = threadIdx.x % TPR, side = threadIdx.x / TPR % SIDE;
@@ -1137,7 +1137,9 @@ hipError_t launch_attention_hd(const AttnPlan& p, const AttnArgs& a, hipStream_t
     // 64: 24 us less). One row of 33 splits: 3.8 us by a workgroup, 6.3 by HD / 4 threads.
     const int64_t rows = (int64_t)a.b.tokens * a.group * a.c.kv_heads;
     constexpr int SIDE = 1024 / HD;
-    const dim3 wide((unsigned)rows), narrow((unsigned)((rows + SIDE - 1) / SIDE)), threads(256);
+    // (2^26 rows of 256 dims are 2^24 workgroups, more threads than a grid's one dimension holds)
+    const unsigned groups = (unsigned)((rows + SIDE - 1) / SIDE), across = groups < (1u << 20) ? groups : 1u << 20;
+    const dim3 wide((unsigned)rows), narrow(across, (groups - 1) / across + 1), threads(256);
     if (p.few && p.most) hipLaunchKernelGGL((paged_join_kernel<HD, SIDE, F32, true>), wide, threads, 0, stream, a);
     else if (rows <= 2048) hipLaunchKernelGGL((paged_join_kernel<HD, SIDE, F32, false>), wide, threads, 0, stream, a);
     else hipLaunchKernelGGL((paged_join_kernel<HD, 1, F32, false>), narrow, threads, 0, stream, a);

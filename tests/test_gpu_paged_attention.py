@@ -643,3 +643,32 @@ def test_long_tail_of_small_weights(gpu, nq, nkv, hd, less):
     want = n * t / (1 + n * t)
     got = c.run(gpu, scale=float(scale)).astype(np.float64)
     assert np.all(np.abs(got - want) <= (2.0 ** -11 + 2.0 ** -17) * want), np.max(np.abs(got / want - 1))
+
+
+def test_most_rows_of_256_dims(gpu):
+    """2^26 rows (token, head) of 256 dims, 32 GiB in place: the last token's keys are split, its parts joined; every
+    other token sees no key."""
+    tokens, seqs, heads, hd = 1 << 20, 8192, 64, 256
+    c = Case([(1, 271)], heads, heads, hd, 16, True, 55)
+    want = c.run(gpu)
+    row = 2 * heads * hd
+    Q = gpu.DeviceBuffer(tokens * row)
+    gpu._hip(gpu.lib().hip.hipMemset(Q.ptr, 0x3C, Q.nbytes), "hipMemset")
+    small = gpu.DeviceBuffer.from_array(c.q.view(np.uint16))
+    gpu._hip(gpu.lib().hip.hipMemcpy(Q.ptr + Q.nbytes - row, small.ptr, row, 3), "hipMemcpy")
+    start = np.minimum(np.arange(seqs + 1) * 129, tokens - 1)
+    start[-1] = tokens
+    kv = np.zeros(seqs, np.int32)
+    kv[-1] = 272
+    table = np.full((seqs, c.width), -1, np.int32)
+    table[-1] = c.table[0]
+    batch = gpu.PagedBatch(seqs, tokens, c.width, i32(gpu, start), i32(gpu, kv), i32(gpu, table))
+    cache = gpu.PagedCache(gpu.DeviceBuffer.from_array(c.k.view(np.uint16)),
+                           gpu.DeviceBuffer.from_array(c.v.view(np.uint16)), c.blocks, 16, heads, hd)
+    gpu.paged_attention(batch, cache, Q, 1, heads * hd, heads, Q, heads * hd,
+                        gpu.paged_attention_workspace(batch, cache, heads))
+    gpu.synchronize()
+    last = Q.view(Q.nbytes - 64 * row, 64 * row).download(np.uint16).reshape(64, -1)
+    assert np.array_equal(last[-1], want.view(np.uint16).reshape(-1))
+    assert not last[:-1].any()
+    Q.close()
