@@ -840,7 +840,9 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
             *reinterpret_cast<float4*>(K + q * HD * 4 + (piece ^ (q & 15)) * 16) =
                 make_float4(w.o[0][d][4 * e], w.o[0][d][4 * e + 1], w.o[0][d][4 * e + 2], w.o[0][d][4 * e + 3]);
         }
-    const float l = swap32_sum(w.l[0]);
+    float l = swap32_sum(w.l[0]);
+    // (the wave's keys and what lies between: a row that sees one of those has its weight in another wave)
+    if (l == 0.f && sees_key(a, seq, max(w.lo[0], begin + wave * KEYS), min(w.hi[0], end - 1))) l = kNoWeight;
     if (h == 0) sums[wave][q] = make_float2(w.m[0], l);
     __syncthreads();
     const int rows = min(t.rows - t.row0, TM);
@@ -861,10 +863,6 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
             v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
         }
         const int tok = (t.row0 + row) / a.group, head = kh * a.group + (t.row0 + row) % a.group;
-        if (sum == 0.f) {
-            const int pos = t.kv - t.n + tok;
-            if (sees_key(a, seq, max(a.window ? pos - a.window + 1 : 0, begin), min(pos, end - 1))) sum = kNoWeight;
-        }
         const int64_t part = a.most ? ((int64_t)item.split * a.b.tokens + t.token0 + tok) * (a.group * a.c.kv_heads) + head
                                     : part0 + row;
         if (whole) {
