@@ -110,7 +110,9 @@ class LayerTensors:
 class Sampling:
     """How a step draws its token (rqmv_sample): temperature, top_k, top_p and
     min_p, and the random number u in [0, 1) of the next step (set_random before
-    each). prob holds the drawn token's probability afterwards."""
+    each; several replays at once would draw with the same one, and are refused
+    unless the temperature is 0). prob holds the drawn token's probability
+    afterwards."""
 
     def __init__(self, vocab: int, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0):
         f32 = lambda v: DeviceBuffer.from_array(np.array([v], dtype=np.float32))  # noqa: E731
@@ -121,6 +123,10 @@ class Sampling:
 
     def set_random(self, u: float):
         self.u.upload(np.array([u], dtype=np.float32))
+
+    def draws(self) -> bool:
+        """Whether a step takes the random number: at temperature 0 it does not."""
+        return bool(self.temperature.download(np.float32, 1)[0] > 0)
 
     def read_prob(self) -> float:
         return float(self.prob.download(np.float32, 1)[0])
@@ -231,8 +237,13 @@ class DecodeModel:
         self._pos += 1
 
     def replay(self, graph: Graph, stream: Stream, times: int = 1):
-        """`times` replays of a captured step; raises before any would run past the cache."""
+        """`times` replays of a captured step; raises before any would run past
+        the cache, or draw with another's random number."""
         self._room(times)
+        sampling = getattr(graph, "sampling", None)
+        if times > 1 and sampling is not None and sampling.draws():
+            raise ValueError(f"{times} replays of a step that draws its token would share one random number: "
+                             "set_random before each, one replay at a time")
         for _ in range(times):
             graph.launch(stream)
         self._pos += times

@@ -193,3 +193,32 @@ def test_decoder_draws_its_tokens(gpu, captured):
         got.append(model.read_token())
     assert got == greedy[0] and len(junk) == 4
     graph.close()
+
+
+def test_replays_of_a_drawing_step_go_one_at_a_time(gpu):
+    """Several replays at once would draw with one random number; at temperature 0 none is drawn with."""
+    shape = DecoderShape(layers=1, d=256, q_heads=4, kv_heads=2, head_dim=64, ffn=512, vocab=5000)
+    syn = synth.DecoderSynth(shape, seed=3, norm_std=0.1)
+    model = DecodeModel(shape, 32, syn.embed(), syn.out_norm(), syn.head())
+    model.set_layer(0, syn.layer(0))
+    model.set_cache(0, *syn.cache(0, 8))
+    stream = gpu.Stream()
+    tokens = []
+    for sampling in (None, model.sampling(temperature=0.0)):
+        graph = model.capture(stream, sampling)
+        model.set_position(7, 8)
+        model.replay(graph, stream, 4)
+        stream.synchronize()
+        tokens.append(model.read_token())
+        graph.close()
+    assert tokens[0] == tokens[1]
+    graph = model.capture(stream, model.sampling(temperature=0.9))
+    model.set_position(7, 8)
+    with pytest.raises(ValueError, match="one random number"):
+        model.replay(graph, stream, 2)
+    assert model.read_position() == 8
+    graph.sampling.set_random(0.5)
+    model.replay(graph, stream)
+    stream.synchronize()
+    assert model.read_token() == ref.sample(model.read_logits(), np.float32(0.5), np.float32(0.9))[0]
+    graph.close()
