@@ -686,9 +686,22 @@ class _BatchStruct(ctypes.Structure):
                 ("slots", c_void_p)]
 
 
-class PagedCache:
+class _Described:
+    """An object whose attributes named like the fields of `struct` are what calls pass: assigning one sets the field
+    too (a captured call keeps what it was captured with)."""
+
+    def __setattr__(self, name, value):
+        struct = self.__dict__.get("struct")
+        field = dict(struct._fields_).get(name) if struct is not None else None
+        if field is not None:
+            setattr(struct, name, _p(value) if field is c_void_p else value)
+        object.__setattr__(self, name, value)
+
+
+class PagedCache(_Described):
     """One layer's keys and values in pages (rqmv_paged_cache): k and v are fp16
-    [blocks, kv_heads, block_size, head_dim] on the device."""
+    [blocks, kv_heads, block_size, head_dim] on the device. Assigned attributes
+    are what later calls pass."""
 
     def __init__(self, k, v, blocks: int, block_size: int, kv_heads: int, head_dim: int):
         self.k, self.v = k, v
@@ -702,18 +715,20 @@ class PagedCache:
         return cls(DeviceBuffer(nbytes), DeviceBuffer(nbytes), blocks, block_size, kv_heads, head_dim)
 
 
-class PagedBatch:
+class PagedBatch(_Described):
     """The tables of one step (rqmv_paged_batch): `seqs` sequences with at most
     `tokens` new tokens. Buffers are int32 on the device; those that a call does
-    not read may be None. table_stride (default max_blocks) is in entries."""
+    not read may be None. table_stride (default max_blocks) is in entries.
+    Assigned attributes are what later calls pass."""
 
     def __init__(self, seqs: int, tokens: int, max_blocks: int, q_start=None, kv_len=None, block_table=None,
                  positions=None, slots=None, table_stride: int | None = None):
         self.seqs, self.tokens, self.max_blocks = seqs, tokens, max_blocks
         self.q_start, self.kv_len, self.block_table = q_start, kv_len, block_table
         self.positions, self.slots = positions, slots
-        self.struct = _BatchStruct(_p(q_start), _p(kv_len), _p(block_table), table_stride or max_blocks, max_blocks,
-                                   seqs, tokens, _p(positions), _p(slots))
+        self.table_stride = table_stride or max_blocks
+        self.struct = _BatchStruct(_p(q_start), _p(kv_len), _p(block_table), self.table_stride, max_blocks, seqs,
+                                   tokens, _p(positions), _p(slots))
         self.ref = byref(self.struct)
 
     @classmethod

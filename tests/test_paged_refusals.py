@@ -161,3 +161,35 @@ def test_sample_refuses_arguments(kw):
     refused(rqmv.sample, **a)
     if set(kw) & {"rows", "n"}:
         refused(rqmv.sample_workspace_size, a["rows"], a["n"])
+
+
+@pytest.mark.parametrize("name", ["q_start", "kv_len", "block_table", "positions", "slots"])
+def test_assigned_buffers_are_what_calls_pass(name):
+    b = batch()
+    setattr(b, name, None)
+    assert getattr(b, name) is None and getattr(b.struct, name) is None
+    refused(plan, b=b)
+    other = At(1 << 22)
+    setattr(b, name, other)
+    assert getattr(b, name) is other and getattr(b.struct, name) == 1 << 22
+
+
+def test_assigned_counts_are_what_calls_pass():
+    for name, bad in (("seqs", 8193), ("tokens", 0), ("max_blocks", 1 << 27), ("table_stride", 2)):
+        b = batch()
+        was = getattr(b, name)
+        setattr(b, name, bad)
+        assert getattr(b, name) == getattr(b.struct, name) == bad
+        refused(plan, b=b)
+        setattr(b, name, was)
+        assert getattr(b.struct, name) == was
+    for name, bad in (("k", None), ("v", At(24)), ("blocks", 0), ("block_size", 24), ("kv_heads", 0), ("head_dim", 96)):
+        c = cache()
+        setattr(c, name, bad)
+        assert getattr(c.struct, name) == (bad if isinstance(bad, int) else rqmv._p(bad))
+        refused(attend, c=c)
+    assert cache().k is A and batch(stride=7).table_stride == 7 and batch().table_stride == 3
+    c = cache()
+    with pytest.raises(TypeError):
+        c.blocks = 2.5
+    assert c.blocks == 10  # as the calls pass it
