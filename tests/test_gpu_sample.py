@@ -170,3 +170,44 @@ def test_replayed_from_a_graph(gpu):
             assert got[0][r] == ref.sample(logits[r], u[r], 1.0, [0, 0, 50, 50, 0, 0][r],
                                            np.float32([1, 0.9, 1, 0.9, 0.5, 1][r]))[0]
     graph.close()
+
+
+@pytest.mark.parametrize("n", [4500, 40000])
+@pytest.mark.parametrize("step", [0.5, 3.0])
+def test_long_rows_of_few_values(gpu, n, step):
+    """Few distinct values in rows too long for one list: every border falls among thousands of equals."""
+    rng = np.random.default_rng(13)
+    m = 12
+    logits = (np.round(rng.standard_normal((m, n)) / step) * step).astype(np.float32)
+    u = rng.random(m)
+    check(gpu, logits, u, **settings(rng, m))
+    check(gpu, logits, u, temperature=[1.0] * m, top_k=[0, 1, 30, 1000, 1025, 4000] * 2,
+          top_p=[1.0] * 6 + [0.3, 0.9, 0.5, 0.999, 0.7, 0.0], min_p=[0, 0, 0, 0.1, 0.5, 1e-3] * 2)
+
+
+@pytest.mark.parametrize("t", [1.0, 1e4])
+def test_an_outlier_above_a_narrow_rest(gpu, t):
+    """One logit far above thousands that share its bins' last ones, drawn at a high temperature."""
+    rng = np.random.default_rng(14)
+    logits = (rng.standard_normal((4, 30000)) * 1e-3).astype(np.float32)
+    logits[:, 777] = 5e3
+    check(gpu, logits, [0.2, 0.9, 0.5, 0.99], temperature=[t] * 4, top_k=[0, 100, 0, 9000], top_p=[1, 1, 0.8, 0.9],
+          min_p=[0, 0, 0.01, 0.2])
+
+
+@pytest.mark.parametrize("n", [50, 4500])
+def test_more_rows_than_one_workspace_holds(gpu, n):
+    """1,100 rows with settings of their own: the rows behind the first 1,024 give what they give alone."""
+    rng = np.random.default_rng(15)
+    m = 1100
+    logits = (rng.standard_normal((m, n)) * 2).astype(np.float32)
+    u, kw = rng.random(m), settings(rng, m)
+    tok, prob = run(gpu, logits, u, **kw)
+    part = {k: v[1000:] for k, v in kw.items()}
+    alone = run(gpu, logits[1000:], u[1000:], **part)
+    assert np.array_equal(tok[1000:], alone[0]) and np.array_equal(prob[1000:], alone[1])
+    few = np.r_[0:4, 1020:1030]
+    check(gpu, logits[few], u[few], **{k: v[few] for k, v in kw.items()})
+    check_few = [ref.sample(logits[r], np.float32(u[r]), np.float32(kw["temperature"][r]), int(kw["top_k"][r]),
+                            np.float32(kw["top_p"][r]), np.float32(kw["min_p"][r]))[0] for r in few]
+    assert list(tok[few]) == check_few
