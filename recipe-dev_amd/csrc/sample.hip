@@ -79,6 +79,11 @@ struct Masses {
         // adding 2^52 leaves the rounded whole number in the low mantissa bits (p scale <= 2^42)
         return (uint64_t)__double_as_longlong(fma(p, scale, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
     }
+    // Whether min_p keeps l: (l - top) / temperature >= log(min_p). Unlike a comparison of masses, whose rounding
+    // makes equals of neighbours, this is a border in the logits, as the bins are.
+    __device__ __forceinline__ bool keeps(float l, double least_z) const {
+        return l == top || ((double)l - dtop) * inv_t >= least_z;
+    }
 };
 // (the workgroup's barrier before the first use is the caller's)
 __device__ __forceinline__ void fill_pow2(double* pow2) {
@@ -122,15 +127,17 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs& a, int row) {
 }
 
 // What the steps compare running sums with: top_p's prefix ends at the first candidate
-// that reaches this, the draw is the first that passes this, min_p keeps masses of at least this.
+// that reaches this, the draw is the first that passes this, min_p keeps logits of at least this many
+// temperatures above the largest (< 0).
 __device__ __forceinline__ uint64_t p_target(const Settings& s, uint64_t mass) {
     return max(part_of(s.p, mass, true), (uint64_t)1);
 }
 __device__ __forceinline__ uint64_t u_target(const Settings& s, uint64_t kept) {
     return min(part_of(s.u, kept, false), kept - 1);
 }
-__device__ __forceinline__ uint64_t least_mass(const Settings& s) {
-    return (uint64_t)ceil((double)s.m * (double)(1ull << kMassBits));
+// (2^-54 less than the logarithm: an e this near to min_p is min_p in 64 bits)
+__device__ __forceinline__ double least_z(const Settings& s) {
+    return s.m > 0.f ? log((double)s.m) - 0x1p-54 : -INFINITY;
 }
 
 // ------------------------------------------------- a row by one workgroup ----
@@ -244,14 +251,14 @@ __device__ void sample_row(RowShared& sh, const float* row, int n, const Setting
                            float* prob) {
     uint64_t total = 0, large = 0;
     unsigned candidates = 0;
-    const uint64_t least = least_mass(s);
+    const double least = least_z(s);
     for (int i = threadIdx.x; i < n; i += kRowThreads) {
         const uint32_t k = key_of(row[i]);
         if (!k) continue;
         const uint64_t m = mass_of(logit_of(k));
         total += m;
         ++candidates;
-        if (m >= least) large += m;
+        if (mass_of.keeps(logit_of(k), least)) large += m;
     }
     total = block_sum(sh, total);
     large = block_sum(sh, large);
@@ -515,8 +522,9 @@ __device__ Wanted wanted_bins(const RowWork& w, int slices, const Settings& s, c
     const bool first_wave = threadIdx.x < 64;
     if (b == kBins - 1) box[0] = box[1] = box[2] = box[5] = box[6] = box[7] = upto;
     if (first_wave && s.m > 0.f) {  // the bin of the logit whose e is min_p
-        const float cut = (float)(-log((double)s.m) / s.inv_t) * bins.per;
-        if (b == 0) box[10] = cut < (float)kBins ? (int)cut : 2 * kBins;
+        // (rounded, as a bin's place is: the border lies in it or in a neighbour, for kBins in the last bin)
+        const float cut = (float)(-least_z(s) / s.inv_t) * bins.per;
+        if (b == 0) box[10] = cut < (float)(kBins + 1) ? (int)cut : 2 * kBins;
     }
     __syncthreads();
     r.total = box[0];
@@ -527,7 +535,7 @@ __device__ Wanted wanted_bins(const RowWork& w, int slices, const Settings& s, c
     }
     if (s.m > 0.f) {
         const int cut = (int)box[10], first = max(cut - 1, 0), last = min(cut + 1, kBins - 1);
-        if (cut < kBins) {  // its bin and the neighbours
+        if (cut <= kBins) {  // its bin and the neighbours
             if (m && b >= first && b <= last) r.mine = true;
             if (b == first) box[6] = r.above;
             if (b == last) box[7] = upto;
@@ -743,6 +751,7 @@ struct DrawShared {
     unsigned long long first_sum[kBins];
     unsigned first_at[kBins];
     unsigned long long part[kThreads / 64], box[3];
+    double least_z;
 };
 
 // The draw from the sorted list, PER candidates per thread: mass, running sum and rank of
@@ -783,8 +792,12 @@ __device__ void draw(const SampleArgs& a, void* ws, int slices, int r, const Set
         sh.box[0] = sh.box[1] = all;
         sh.box[2] = prefix ? 0 : w.total[1];
     }
+    if (threadIdx.x < 64) {  // (a logarithm by one wave)
+        const double z = least_z(s);
+        if (threadIdx.x == 0) sh.least_z = z;
+    }
     __syncthreads();
-    const uint64_t least = least_mass(s);
+    const double least = sh.least_z;
     uint64_t large = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
@@ -796,7 +809,7 @@ __device__ void draw(const SampleArgs& a, void* ws, int slices, int r, const Set
             rank[j] += w.before[bin] - sh.first_at[bin];
         }
         if (s.k && rank[j] == (unsigned)s.k - 1) sh.box[0] = end[j];
-        if (m[j] >= least) large = end[j];
+        if (mass_of.keeps(logit_of((uint32_t)(list[i] >> 32)), least)) large = end[j];
     }
     // (the last candidate that min_p keeps: of a wave, in the last lane that has one)
     const unsigned long long keeps = __ballot(large != 0);

@@ -211,3 +211,28 @@ def test_more_rows_than_one_workspace_holds(gpu, n):
     check_few = [ref.sample(logits[r], np.float32(u[r]), np.float32(kw["temperature"][r]), int(kw["top_k"][r]),
                             np.float32(kw["top_p"][r]), np.float32(kw["min_p"][r]))[0] for r in few]
     assert list(tok[few]) == check_few
+
+
+@pytest.mark.parametrize("n", [900, 6177, 12362, 58032])
+@pytest.mark.parametrize("t,spread", [(1.0, 1e-21), (2.0, 1e-17), (1e5, 1e-20), (1.0, 2e-16), (1e-6, 1e-20), (30.0, 1e-13)])
+def test_min_p_of_one_among_masses_that_round_to_one(gpu, n, t, spread):
+    """Logits closer than a unit of mass: their masses are equal, but an e below 1 in 64 bits is not kept."""
+    rng = np.random.default_rng(n)
+    m = 8
+    logits = (rng.standard_normal((m, n)) * spread).astype(np.float32)
+    check(gpu, logits, rng.random(m), temperature=[t] * m, top_k=[0, 0, 5000, n - 1, 1025, 50, n - 1, 0],
+          top_p=[1, 0.3, 1, 0.3, 0.9, 1, 1, 0.999], min_p=[1.0] * m)
+
+
+@pytest.mark.parametrize("n", [900, 20000])
+def test_min_p_at_the_smallest_logits(gpu, n):
+    """min_p's border between the row's last logits, where the bins end: exact to the logit."""
+    logits = (-np.arange(n) * 2.0 ** -12).astype(np.float32)[None]  # each a candidate of its own
+    for at in (n - 1, n - 2, n - 40, n // 2):
+        min_p = np.float32(np.exp(np.float64(logits[0, at])))
+        z = np.log(np.float64(min_p))
+        kept = int((logits[0].astype(np.float64) >= z).sum())
+        e = np.exp(logits[0, :kept].astype(np.float64))
+        tok, prob = run(gpu, logits, [1.0], min_p=[min_p])  # (u of 1: the last that counts)
+        assert tok[0] == kept - 1
+        assert abs(prob[0] - e[-1] / e.sum()) <= 2.0 ** -24 * prob[0] + 2.0 ** -42 * n
