@@ -57,14 +57,15 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 // f64. `pow2` holds 2^(j / 32) in LDS. (The bins of 64 rows of 128,256 take 14.6 us, with a series
 // to x^12 and no table 17.0.)
 struct Masses {
-    float top, c;
+    float top, up, c;  // up * c = 32 / (ln 2 temperature), which alone passes fp32's range below 10^-37
     double dtop, inv_t;
     const double* pow2;
     __device__ __forceinline__ Masses(float top_, double inv_t_, const double* pow2_)
-        : top(top_), c((float)(inv_t_ * 46.166241308446828)), dtop(top_), inv_t(inv_t_), pow2(pow2_) {}
+        : top(top_), up(inv_t_ > 0x1p100 ? 0x1p40f : 1.f), c((float)(inv_t_ * (46.166241308446828 / up))), dtop(top_),
+          inv_t(inv_t_), pow2(pow2_) {}
     __device__ __forceinline__ uint64_t operator()(float l) const {
         if (l == top) return 1ull << kMassBits;
-        const float m = rintf((l - top) * c);
+        const float m = rintf((l - top) * up * c);
         if (!(m > -2000.f)) return 0;  // (an infinite top leaves only its equals)
         const double x = fma((double)m, -0.021660849392498290, ((double)l - dtop) * inv_t);
         double p = 1.0 / 120.0;

@@ -236,3 +236,15 @@ def test_min_p_at_the_smallest_logits(gpu, n):
         tok, prob = run(gpu, logits, [1.0], min_p=[min_p])  # (u of 1: the last that counts)
         assert tok[0] == kept - 1
         assert abs(prob[0] - e[-1] / e.sum()) <= 2.0 ** -24 * prob[0] + 2.0 ** -42 * n
+
+
+@pytest.mark.parametrize("n", [40, 3000, 9000])
+@pytest.mark.parametrize("t", [5e-38, 1.2e-38, 1e-41, 1e-44, 1e-30])
+def test_smallest_temperatures(gpu, n, t):
+    """Temperatures whose inverse leaves fp32's range, logits a few of them apart."""
+    rng = np.random.default_rng(n)
+    m = 6
+    logits = (-rng.random((m, n)) * 20 * np.float64(np.float32(t))).astype(np.float32)
+    logits[0] = np.round(rng.standard_normal(n)) * 1e30
+    check(gpu, logits, rng.random(m), temperature=[t] * m, top_k=[0, 0, 30, 0, 2000, 0], top_p=[1, 1, 1, 0.5, 0.9, 1],
+          min_p=[0, 0, 0, 0, 0, 0.3])
