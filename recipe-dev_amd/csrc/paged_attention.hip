@@ -183,8 +183,7 @@ struct Pages {
 };
 
 // The 16 keys from `key` on of one page (id clamped into the cache) of `cache`, to LDS.
-// (FROM..TO-1: which of its instructions)
-template <int HD, bool VALUES, int FROM = 0, int TO = Lay<HD>::NI>
+template <int HD, bool VALUES>
 __device__ __forceinline__ void load_group(const __half* cache, const PagedCache& c, int kh, int id, int key,
                                            uint32_t lds) {
     typedef Lay<HD> L;
@@ -192,7 +191,7 @@ __device__ __forceinline__ void load_group(const __half* cache, const PagedCache
     const int64_t row = (((int64_t)id * c.kv_heads + kh) << c.block_shift) + (key & ((1 << c.block_shift) - 1));
     const __half* base = cache + row * HD;
 #pragma unroll
-    for (int i = FROM; i < TO; ++i) {
+    for (int i = 0; i < L::NI; ++i) {
         const int r = i * L::RPI + lane / L::PCS;
         const int piece = (lane % L::PCS) ^ (VALUES ? L::vx(r) : L::kx(r));
         load_lds(base, (uint32_t)(r * L::ROW + piece * 16), lds + i * 1024);
@@ -881,18 +880,17 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
 // TM = 32 WAVES rows a tile (prompts, chunks of prompts): bound by the matrix
 // cores and the exponentials. Each wave has 32 rows; the waves share steps of 64 keys in
 // two LDS buffers, one barrier a step. Eight waves (two per SIMD, 256 registers each), so
-// that one multiplies while the other takes exponentials; steps of 32 keys at 256 dims of
-// fp16 (fewer registers: 310 us against 368 with four waves of 64-key steps, 2048 tokens over 6,000, 8/4
-// heads), four waves at 256 dims of fp32. 2048 tokens over 14,336, 32/8 heads of 128,
-// fp16: 528 us, 976 TFLOP/s (a library product of 8192^3: 1162). Four waves of 64 rows took 1224:
-// their sums lay in accumulator registers and were moved at every step.
-constexpr int many_waves(int hd, bool f32) { return hd == 256 && f32 ? 4 : 8; }
-constexpr int many_keys(int hd, bool f32) { return hd == 256 && !f32 ? 32 : 64; }
+// that one multiplies while the other takes exponentials; at 256 dims four, which may have 512 registers
+// (fp16 takes 291, fp32 363; fp16 in 256 registers, with steps of 32 keys, spilled inside the loop, and the
+// reloads waited for the step's own loads to LDS: 2048 tokens over 6,000, 32/8 heads, 1,015 us against 659).
+// 2048 tokens over 14,336, 32/8 heads of 128, fp16: 521 us, 989 TFLOP/s (a library product of 8192^3: 1145 on
+// the same card). Four waves of 64 rows took 1,224: their sums lay in accumulator registers and were moved at every step.
+constexpr int many_waves(int hd) { return hd == 256 ? 4 : 8; }
 
 template <int HD, bool F32>
-__global__ void __launch_bounds__(64 * many_waves(HD, F32), many_waves(HD, F32) / 4) paged_many_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(64 * many_waves(HD), many_waves(HD) / 4) paged_many_kernel(AttnArgs a) {
     typedef Lay<HD> L;
-    constexpr int WAVES = many_waves(HD, F32), TM = 32 * WAVES, KEYS = many_keys(HD, F32), KT = KEYS / 32;
+    constexpr int WAVES = many_waves(HD), TM = 32 * WAVES, KEYS = 64, KT = KEYS / 32;
     constexpr int HALF = KEYS * HD * 2;
     extern __shared__ __align__(16) char lds[];
     // the last tiles first: of one sequence's they have the most keys
@@ -910,8 +908,7 @@ __global__ void __launch_bounds__(64 * many_waves(HD, F32), many_waves(HD, F32) 
     Rows<HD, 1, F32> w;
 
     // Step i is in buffer i % 2, keys before values. Of eight waves, four load 16 rows of keys each and
-    // four of values (in steps of 32 keys half of 16 rows each); of four, each loads both. Returns which
-    // groups are absent.
+    // four of values; of four, each loads both. Returns which groups are absent.
     auto load = [&](int key0, int buffer) -> unsigned {
         pages.need(key0 >> pages.shift, (key0 + KEYS - 16) >> pages.shift);
         unsigned bad = 0;
@@ -920,17 +917,8 @@ __global__ void __launch_bounds__(64 * many_waves(HD, F32), many_waves(HD, F32) 
         const int g = wave % (KEYS / 16), key = key0 + 16 * g, id = pages.at(key >> pages.shift);
         const int page = pages.absent(id) ? 0 : id;
         const uint32_t at = lds0 + buffer * 2 * HALF + g * 16 * L::ROW;
-        if constexpr (KEYS == 64) {
-            if (WAVES == 4 || wave < 4) load_group<HD, false>(a.c.k, a.c, kh, page, key, at);
-            if (WAVES == 4 || wave >= 4) load_group<HD, true>(a.c.v, a.c, kh, page, key, at + HALF);
-        } else {
-            constexpr int NI = L::NI;
-            const int part = wave >> 1;  // halves of keys' and of values' groups
-            if (part == 0) load_group<HD, false, 0, NI / 2>(a.c.k, a.c, kh, page, key, at);
-            else if (part == 1) load_group<HD, false, NI / 2, NI>(a.c.k, a.c, kh, page, key, at);
-            else if (part == 2) load_group<HD, true, 0, NI / 2>(a.c.v, a.c, kh, page, key, at + HALF);
-            else load_group<HD, true, NI / 2, NI>(a.c.v, a.c, kh, page, key, at + HALF);
-        }
+        if (WAVES == 4 || wave < 4) load_group<HD, false>(a.c.k, a.c, kh, page, key, at);
+        if (WAVES == 4 || wave >= 4) load_group<HD, true>(a.c.v, a.c, kh, page, key, at + HALF);
         return bad;
     };
     // the keys that any of the wave's rows sees
@@ -1057,7 +1045,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(AttnArgs a) {
 // ------------------------------------------------------------------ launches ----
 
 constexpr int few_lds(int hd) { return 4 * 2 * 32 * hd * 2; }
-constexpr int many_lds(int hd, bool f32) { return 2 * 2 * many_keys(hd, f32) * hd * 2; }
+constexpr int many_lds(int hd) { return 2 * 2 * 64 * hd * 2; }
 
 struct AttnPlan {
     bool few, join, items;
@@ -1072,7 +1060,7 @@ AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int gro
     // the large tiles leave CUs idle: tiles of 32 rows over all heads up to 4 a CU (64 and 256 dims, fp16),
     // 2 (128 dims; 64, fp32) or a half (256, fp32, whose large tiles have 128 rows). Over 222
     // batches of 1 to 16 sequences, 64 to 1024 new tokens and 0 to 6,000 cached ones the choice takes 0.5 to
-    // 4.5 % more than the better form. Few against many, 32/8 heads of 128, fp16, us: 32 sequences of 128
+    // 4.5 % more than the better form (256 dims of fp16: 11 % over 131 batches). Few against many, 32/8 heads of 128, fp16, us: 32 sequences of 128
     // rows over 6,000 positions 238 / 341, of 256 398 / 350; one of 1024 rows over 1,000 23 / 27; four of 2048
     // over 6,000 350 / 221.
     p.tiles = (int64_t)tokens * group / 32 + seqs;
@@ -1096,7 +1084,7 @@ AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int gro
         if (!p.join || (int64_t)tokens * heads * p.most * hd * 4 > kEarlyBytes) p.most = 0;
         else p.parts = (int64_t)tokens * heads * p.most;
     } else {
-        p.tiles = (int64_t)tokens * group / (32 * many_waves(hd, f32)) + seqs;
+        p.tiles = (int64_t)tokens * group / (32 * many_waves(hd)) + seqs;
         // Keys are split where the tiles take at most half of the CUs (at less, a split's uneven second part
         // costs more than it gives: eight sequences of 300 tokens, 8/4 heads of 256, 41 us split, 25 whole).
         p.min_chunk = 128;
@@ -1122,13 +1110,13 @@ hipError_t launch_attention_hd(const AttnPlan& p, const AttnArgs& a, hipStream_t
     const dim3 grid((unsigned)((p.tiles + (p.few ? p.splits : 0)) * a.c.kv_heads), p.few ? 1 : p.splits);
     const void* f = p.few ? reinterpret_cast<const void*>(paged_few_kernel<HD, F32>)
                           : reinterpret_cast<const void*>(paged_many_kernel<HD, F32>);
-    const int lds = p.few ? few_lds(HD) : many_lds(HD, F32);
+    const int lds = p.few ? few_lds(HD) : many_lds(HD);
     if (lds > 48 * 1024) {
         const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
     }
     if (p.few) hipLaunchKernelGGL((paged_few_kernel<HD, F32>), grid, dim3(256), lds, stream, a);
-    else hipLaunchKernelGGL((paged_many_kernel<HD, F32>), grid, dim3(64 * many_waves(HD, F32)), lds, stream, a);
+    else hipLaunchKernelGGL((paged_many_kernel<HD, F32>), grid, dim3(64 * many_waves(HD)), lds, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || !p.join) return e;
     // A workgroup per row for few of them, for 1024 / HD rows of many (eight sequences of 300 tokens, 16 heads of
