@@ -354,20 +354,24 @@ int rqmv_qk_norm_rope(const rqmv_paged_batch* batch, const rqmv_paged_cache* cac
  * whose pages are present, in kv head h / (q_heads / kv_heads); zeros where there is
  * none. The new tokens' own keys and values are in the cache already
  * (rqmv_qk_norm_rope). out has the dtype of q: fp32 rows are computed to fp32 accuracy,
- * fp16 rows with the softmax weights rounded to fp16; sums and statistics are fp32 in
- * both. A position that is not attended to never touches the result, whatever its key
- * and value hold. A NaN or an infinity in a query or in a value attended to, and a NaN in
- * a key attended to, make their rows non-finite. So does an infinity in a key where the
- * score is +infinity or NaN; where it is -infinity the key weighs nothing beside finite scores
- * (fp32 rows may be NaN instead), and a row all of whose scores are -infinity is NaN.
- * Rows of no sequence are not written. q_heads is a multiple
- * of kv_heads, both at most 1024; scale is positive; ldq and ldo are multiples of 16
- * bytes, q and out 16-byte aligned; out is q itself (ldo = ldq) or spans none of its
- * memory. Reads q_start, kv_len, block_table of the batch. One launch, one more where
- * the keys are split over workgroups and one above 256 sequences: then the workspace
- * (16-byte aligned, rqmv_paged_attention_workspace_size bytes for this batch's counts,
- * cache and q_heads on the current device; 0: may be NULL) holds partial results, and
- * calls that share it must not overlap. */
+ * fp16 rows with the softmax weights rounded to fp16 (to zero below 2^-31 of the
+ * largest); sums and statistics are fp32 in both. A position that is not attended to
+ * never touches the result, whatever its key and value hold. A NaN or an infinity in a
+ * query or in a value attended to, and a NaN in a key attended to, make their rows
+ * non-finite. So does an infinity in a key where the score is +infinity or NaN; where
+ * it is -infinity the key weighs nothing beside finite scores (fp32 rows may be NaN
+ * instead), and a row all of whose scores are -infinity is NaN. Rows of no sequence are
+ * not written. q_heads is a multiple of kv_heads, both at most 1024; scale is positive;
+ * ldq and ldo are multiples of 16 bytes, q and out 16-byte aligned; out is q itself
+ * (ldo = ldq) or spans none of its memory. Reads q_start, kv_len, block_table of the
+ * batch. One launch, one more where the keys are split over workgroups and one above
+ * 256 sequences: then the workspace (16-byte aligned,
+ * rqmv_paged_attention_workspace_size bytes for this batch's counts, cache and q_heads
+ * on the current device; 0: may be NULL) holds partial results, and calls that share it
+ * must not overlap. tokens * q_heads is at most 2^26, and (tokens * q_heads / kv_heads
+ * / 32 + seqs) * kv_heads at most 2^23. The counts choose one form for the whole batch:
+ * a long prompt beside a hundred decoding requests takes less time in a batch of its
+ * own over the same cache. */
 int rqmv_paged_attention_workspace_size(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, int q_heads,
                                         size_t* bytes);
 int rqmv_paged_attention(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, const void* q, int dtype,
@@ -399,10 +403,12 @@ int rqmv_argmax(const float* values, int n, int* out, void* workspace, size_t wo
  * choice). A row without candidates gives -1, with probability 0. Sums are exact sums
  * of e in whole units of 2^-42, so a row's token does not depend on the other rows or
  * on scheduling, and a candidate whose e rounds to 0 units (below 2^-43) is never
- * drawn. n is at most 2^20, rows at most 2^20. The workspace is 16-byte aligned
- * (rqmv_sample_workspace_size bytes on the current device; 0: may be NULL); calls
- * sharing it must not overlap. No counterpart in the reference's kernels (its driver
- * samples on the host, recipe.rs:20286-20296). */
+ * drawn; min_p compares e in 64 bits. A row with more than 4,096 candidates around one
+ * of its borders (as many equal logits, or one far above a narrow rest) is right but
+ * slow: 0.4 to 3 ms at 128,256 logits, instead of 25 us. n is at most 2^20, rows at
+ * most 2^20. The workspace is 16-byte aligned (rqmv_sample_workspace_size bytes on the
+ * current device; 0: may be NULL); calls sharing it must not overlap. No counterpart in
+ * the reference's kernels (its driver samples on the host, recipe.rs:20286-20296). */
 int rqmv_sample_workspace_size(int rows, int n, size_t* bytes);
 int rqmv_sample(const float* logits, int rows, int n, int64_t ld, const float* u, const float* temperature,
                 const int* top_k, const float* top_p, const float* min_p, int* tokens, float* probs, void* workspace,

@@ -228,8 +228,8 @@ struct RawRows {
 // Requests the wave's rows, with the first page ids on their way. `arrived` waits for them: the compiler
 // would wait for them at their first use in the loop, in every step, and for the step's own loads, which it does not
 // count, with them. fp32 rows are asked for before the first step's loads to LDS and become operands while these
-// are on their way (one token over 4,096: 13.9 -> 13.3 us; fp16 rows, which are operands already, come
-// behind those loads: 32 sequences 39.9 -> 39.6).
+// are on their way (one token over 4,096: 4 % less); fp16 rows, which are operands already, come
+// behind those loads (32 sequences: 1 % less).
 template <int HD, bool F32>
 __device__ __forceinline__ void load_rows(const AttnArgs& a, const Tile& t, int kh, int row, Rows<HD, 1, F32>& w,
                                           RawRows<HD, F32>& raw) {
@@ -332,7 +332,7 @@ __device__ __forceinline__ void scores(const char* K, const Rows<HD, QT, F32>& w
                     s[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, w.q[i][k][p], s[i][t], 0, 0, 0);
         }
     if constexpr (HD == 128 && KT == 2) {
-        // four key operands ahead of their products (2048 tokens over 14,336, fp16: 537 -> 529 us; heads of 64
+        // four key operands ahead of their products (2048 tokens over 14,336, fp16: 533 us, without 549; heads of 64
         // and 256 lose 3 % and 1 % so)
         constexpr int READS = HD / 16 * KT, EACH = QT * Rows<HD, QT, F32>::QP;
         __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
@@ -416,15 +416,15 @@ __device__ __forceinline__ void weights(Rows<HD, QT, F32>& w, f16_t (&s)[QT][KT]
     // instruction less and below the weights' own rounding.
     // fp16, up to 128 dims: the sum of the rounded weights, two at a time. What a large weight's rounding adds
     // to the row it adds to the divisor too, so a row of one large weight is off by its output's rounding alone
-    // (2048 tokens over 14,336: 507 -> 504 us; 6,000, 8/4 heads of 256: 204 -> 213 us, so there the weights
-    // are added before they are rounded).
+    // (2048 tokens over 14,336: 533 us, with the weights added before they are rounded 538; 4,096 over 6,000, 8/4
+    // heads of 256: 492 and 484, so there they are added before).
     constexpr bool PAIRS = !F32 && HD <= 128;
 #pragma unroll
     for (int i = 0; i < QT; ++i) {
         float ref = w.m[i] == -INFINITY ? 0.f : w.m[i] - (F32 ? 0.f : 6.f), c = w.c[i];
         // Scores of 2^20 and more: the reference is a rounded product, and the exact ones may lie so far from it
         // that every weight leaves fp16's range. Then products are rounded before the difference. (The branch
-        // takes 5 % at 64 and 4 % at 256 dims of fp16, nothing at 128.)
+        // takes 5 % at 64 and 3 % at 256 dims of fp16, nothing at 128.)
         if (__any(fabsf(w.m[i]) > 0x1p20f && w.m[i] > -INFINITY)) {
 #pragma clang fp contract(off)
             ref = w.m[i] == -INFINITY ? 0.f : w.m[i];
@@ -883,8 +883,9 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
 // that one multiplies while the other takes exponentials; at 256 dims four, which may have 512 registers
 // (fp16 takes 291, fp32 363; fp16 in 256 registers, with steps of 32 keys, spilled inside the loop, and the
 // reloads waited for the step's own loads to LDS: 2048 tokens over 6,000, 32/8 heads, 1,015 us against 659).
-// 2048 tokens over 14,336, 32/8 heads of 128, fp16: 521 us, 989 TFLOP/s (a library product of 8192^3: 1145 on
-// the same card). Four waves of 64 rows took 1,224: their sums lay in accumulator registers and were moved at every step.
+// 2048 tokens over 14,336, 32/8 heads of 128, fp16: 521 to 533 us by the card, 989 TFLOP/s at 521 (a library product
+// of 8192^3: 1145 on that one). Four waves of 64 rows took 1,224: their sums lay in accumulator registers and were
+// moved at every step.
 constexpr int many_waves(int hd) { return hd == 256 ? 4 : 8; }
 
 template <int HD, bool F32>
@@ -1060,25 +1061,26 @@ AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int gro
     // the large tiles leave CUs idle: tiles of 32 rows over all heads up to 4 a CU (64 and 256 dims, fp16),
     // 2 (128 dims; 64, fp32) or a half (256, fp32, whose large tiles have 128 rows). Over 222
     // batches of 1 to 16 sequences, 64 to 1024 new tokens and 0 to 6,000 cached ones the choice takes 0.5 to
-    // 4.5 % more than the better form (256 dims of fp16: 11 % over 131 batches). Few against many, 32/8 heads of 128, fp16, us: 32 sequences of 128
-    // rows over 6,000 positions 238 / 341, of 256 398 / 350; one of 1024 rows over 1,000 23 / 27; four of 2048
-    // over 6,000 350 / 221.
+    // 4.5 % more than the better form; at 256 dims of fp16 11 % over 131 batches. Few against many, 32/8 heads of 128,
+    // fp16, us: 32 sequences of 128 rows over 6,000 positions 238 / 341, of 256 398 / 350; one of 1024 rows over 1,000
+    // 23 / 27; four of 2048 over 6,000 350 / 221. One form takes the whole batch: 100 decoding requests over 2,000 beside
+    // 2048 tokens over 6,000 take 494 (few), as two batches 157 + 255; 32 beside them 298 (many), 53 + 255.
     p.tiles = (int64_t)tokens * group / 32 + seqs;
     const int64_t few_tiles = hd == 128 ? 2 * cus : hd == 64 ? (f32 ? 2 : 4) * cus : f32 ? cus / 2 : 4 * cus;
     p.few = (int64_t)tokens * group <= (int64_t)128 * seqs || (int64_t)tokens * heads / 32 <= few_tiles;
     p.items = p.few && seqs > kItemSeqs;
     if (p.few) {
-        // Two items per CU over the whole batch (32 requests of 60 to 8,192 positions: 35.1 us; one
-        // per CU 37.6, four 37.6), of two steps for each wave at least (one request at 4,097: 10.5 us; of
-        // one step 12.4, of four 12.3).
+        // Two items per CU over the whole batch (32 requests of 60 to 8,192 positions, with the join: 39.1 us; one
+        // per CU 41.2, four 41.3), of two steps for each wave at least (one request at 4,097: 12.4 us; of
+        // one step 14.8, of four 14.6; the 32 requests with a window of 1,024 24.3, of four 20.3).
         p.min_chunk = 256;
         const int64_t want = 2 * cus / kv_heads, most = p.tiles * ((cap + p.min_chunk - 1) / p.min_chunk);
         p.splits = (int)(most < want ? most : want < 1 ? 1 : want);
         p.join = cap > p.min_chunk;
         p.parts = p.join ? (int64_t)2 * p.splits * kv_heads * 32 : 0;
         // Parts have fixed places where all that there could be take up to 1 MiB: the join then asks for them before
-        // it knows which there are (one token over 4,096, 0.3 MB: 13.4 -> 12.9 us; 40 over up to 3,000, 2 MB:
-        // 13.1 -> 13.4).
+        // it knows which there are (one token over 4,096, 0.3 MB: 12.4 us, otherwise 13.0; 40 over up to 3,000, 8 MB:
+        // 26.4 so, 25.8 otherwise).
         const int64_t all = (cap + p.min_chunk - 1) / p.min_chunk;
         p.most = (int)(all < kMaxSplits ? all : kMaxSplits);
         if (!p.join || (int64_t)tokens * heads * p.most * hd * 4 > kEarlyBytes) p.most = 0;
