@@ -883,8 +883,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_few_kernel(AttnA
 // that one multiplies while the other takes exponentials; at 256 dims four, which may have 512 registers
 // (fp16 takes 291, fp32 363; fp16 in 256 registers, with steps of 32 keys, spilled inside the loop, and the
 // reloads waited for the step's own loads to LDS: 2048 tokens over 6,000, 32/8 heads, 1,015 us against 659).
-// 2048 tokens over 14,336, 32/8 heads of 128, fp16: 521 to 533 us by the card, 989 TFLOP/s at 521 (a library product
-// of 8192^3: 1145 on that one). Four waves of 64 rows took 1,224: their sums lay in accumulator registers and were
+// 2048 tokens over 14,336, 32/8 heads of 128, fp16: 509 to 533 us by the card, 1,012 to 967 TFLOP/s (a library product
+// of 8192^3: 1,162 to 1,145). Four waves of 64 rows took 1,224 us: their sums lay in accumulator registers and were
 // moved at every step.
 constexpr int many_waves(int hd) { return hd == 256 ? 4 : 8; }
 
