@@ -291,7 +291,7 @@ def prepare(case, seed):
 def _exponent(a):
     """The smallest e in LOW..HIGH at which a / 2^e rounds to a code (a < 127.5 * 2^e)."""
     m, e = torch.frexp(a.double())
-    return torch.clamp(e - 7 + (m * 128.0 >= 127.5).int(), LOW, HIGH)
+    return torch.where(a > 0, torch.clamp(e - 7 + (m * 128.0 >= 127.5).int(), LOW, HIGH), LOW)
 
 
 def _values(codes, scale):
