@@ -378,6 +378,52 @@ int rqmv_paged_attention(const rqmv_paged_batch* batch, const rqmv_paged_cache* 
                          int64_t ldq, int q_heads, float scale, int window, void* workspace, size_t workspace_bytes,
                          void* out, int64_t ldo, void* stream);
 
+/* Pages of 8 bits: half of the bytes that attention reads in a decode step. `pages`
+ * is as above, but its k and v hold int8 codes (-127..127) of the same shape,
+ * 16-byte aligned, and each group of 16 rows of a block and kv head (rows 16 g ..
+ * 16 g + 15 of a block) has one scale byte b in k_scale and v_scale
+ * [blocks][kv_heads][block_size / 16]: a value is its code times 2^(b - 127), b in
+ * 103..136 (bytes outside count as the nearest), or NaN where b is 255. Every value
+ * is an fp16 number. rqmv_paged_plan takes &cache.pages. */
+typedef struct {
+    rqmv_paged_cache pages;
+    uint8_t* k_scale;
+    uint8_t* v_scale;
+} rqmv_paged_cache_q8;
+
+/* rqmv_qk_norm_rope with 8-bit pages; queries come out the same. The rows whose
+ * slots lie in one group are to stand within 32 rows of the call (a plan's follow each
+ * other) and their slots to be distinct; then, for keys and values of each kv head by themselves, with a the largest
+ * magnitude among the group's new rows and e(a) the smallest exponent of -24..9
+ * with a < 127.5 * 2^e(a), the group's scale becomes 2^e,
+ *   e = e(a) where its first row is among them: the group starts anew, and its
+ *       other rows become 0;
+ *   e = the larger of e(a) and its exponent before otherwise: the codes of its
+ *       other rows are divided by the power of two that it grew by and rounded;
+ * and a new row's codes are its values divided by 2^e and rounded, all to nearest,
+ * ties to even. Keys are computed in 64 bits, so that their codes are those of the exact keys whatever the step
+ * they came in. A row is within 2^e of what was stored, however often the group grows (within half of that where
+ * it does not). A NaN, an infinity or a magnitude of 65,280 or more makes the group's
+ * scale NaN, until the group starts anew. One launch. */
+int rqmv_qk_norm_rope_q8(const rqmv_paged_batch* batch, const rqmv_paged_cache_q8* cache, const void* qkv, int x_dtype,
+                         int64_t ld, int q_heads, const float* q_norm, const float* k_norm, float eps,
+                         const float* rope_table, int rot_dim, int rope_rows, void* q_out, int q_dtype, int64_t ldq,
+                         void* stream);
+
+/* Every value of 8-bit pages (those of no sequence too) into fp16 pages of the same
+ * shape, exactly. The values' memory overlaps neither codes nor scales. One launch. */
+int rqmv_paged_values_q8(const rqmv_paged_cache_q8* cache, const rqmv_paged_cache* out, void* stream);
+
+/* rqmv_paged_attention over 8-bit pages: the values that codes and scales stand for,
+ * computed as over fp16 pages of the same values (fp32 rows to fp32 accuracy, their
+ * softmax weights to within 2^-40 of the largest). All that is said there holds; a key or value can be NaN (its whole group then is), never
+ * infinite. The workspace is rqmv_paged_attention_q8_workspace_size bytes. */
+int rqmv_paged_attention_q8_workspace_size(const rqmv_paged_batch* batch, const rqmv_paged_cache_q8* cache, int q_heads,
+                                           size_t* bytes);
+int rqmv_paged_attention_q8(const rqmv_paged_batch* batch, const rqmv_paged_cache_q8* cache, const void* q, int dtype,
+                            int64_t ldq, int q_heads, float scale, int window, void* workspace, size_t workspace_bytes,
+                            void* out, int64_t ldo, void* stream);
+
 /* out[i] = silu(gate_up[i]) * gate_up[n + i]. */
 int rqmv_silu_mul(const float* gate_up, int n, float* out, void* stream);
 

@@ -2,7 +2,8 @@
 
 Written from the definitions, one sequence, head or row at a time: plan() the
 step's tables, qk_norm_rope() the norms, rotation and append, attention() a
-sequence's new tokens over its pages, sample() the next token.
+sequence's new tokens over its pages, sample() the next token; store_q8() the append to
+8-bit pages and values_q8() what they stand for.
 """
 from __future__ import annotations
 
@@ -93,6 +94,48 @@ def attention(q, k, v, q_start, kv_len, table, max_blocks, scale, window=0):
                     e = np.exp(sc - sc.max(-1, keepdims=True))
                     out[row, h] = (e / e.sum(-1, keepdims=True)) @ values[live, g]
     return out
+
+
+def values_q8(codes, scale):
+    """[blocks, nkv, block, hd] in 64 bits; scale bytes are [blocks, nkv, block / 16]."""
+    b = np.clip(scale.astype(np.int64), 103, 136)
+    s = np.where(scale == 255, np.nan, 2.0 ** (b - 127.0))
+    return codes.astype(np.float64) * np.repeat(s, 16, axis=2)[..., None]
+
+
+def exponent_q8(a):
+    """The smallest e of -24..9 with a < 127.5 * 2^e; None: there is none."""
+    return next((e for e in range(-24, 10) if a < 127.5 * 2.0 ** e), None)
+
+
+def store_q8(codes, scale, y, slots):
+    """(codes, scale) with rows y [tokens, nkv, hd] (64 bits) stored at their slots; -1 and slots past the cache: none."""
+    codes, scale = codes.copy(), scale.copy()
+    blocks, nkv, block, hd = codes.shape
+    groups = {}
+    for t, s in enumerate(slots):
+        if 0 <= s < blocks * block:
+            groups.setdefault(int(s) // 16, []).append(t)
+    for g, rows in groups.items():
+        b, first = g * 16 // block, g * 16 % block
+        at = [int(slots[t]) % block for t in rows]
+        for h in range(nkv):
+            new = np.asarray([y[t][h] for t in rows], np.float64)
+            old = scale[b, h, first // 16]
+            e = None if np.isnan(new).any() else exponent_q8(np.abs(new).max())
+            part = codes[b, h, first:first + 16]
+            if first in at:
+                part[:] = 0
+                scale[b, h, first // 16] = 255 if e is None else e + 127
+            else:
+                e_old = int(np.clip(int(old) - 127, -24, 9))
+                e = e if e is None else max(e, e_old)
+                if e is not None:
+                    part[:] = np.rint(part * 2.0 ** (e_old - e))
+                scale[b, h, first // 16] = 255 if e is None or old == 255 else e + 127
+            if e is not None:
+                codes[b, h, at] = np.rint(new * 2.0 ** -e)
+    return codes, scale
 
 
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):

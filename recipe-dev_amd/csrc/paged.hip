@@ -5,6 +5,7 @@
 #include <limits.h>
 
 #include "lanes.h"
+#include "paged_rows.h"
 
 namespace rq {
 
@@ -190,35 +191,6 @@ hipError_t launch_paged_plan(const PagedBatch& b, int blocks, int block_shift, c
 
 // -------------------------------------- norms, rotation and the append ----
 
-// y = x / sqrt(mean(x^2) + eps) * w per q and k head, then pair (i, i + rot / 2)
-// turns by its position's (cos, sin). A head is taken by HD / 8 lanes of eight
-// values: lane u < rot / 8 holds the pairs 4u..4u+3 (four values of each half, so
-// both partners are at hand), a lane past them eight values that do not
-// turn; a value head's lanes hold eight values in a row.
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float* v);
-template <>
-__device__ __forceinline__ void load4<float>(const float* p, float* v) {
-    const float4 a = *reinterpret_cast<const float4*>(p);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-}
-template <>
-__device__ __forceinline__ void load4<__half>(const __half* p, float* v) {
-    const uint2 a = *reinterpret_cast<const uint2*>(p);
-    const __half2 lo = __builtin_bit_cast(__half2, a.x), hi = __builtin_bit_cast(__half2, a.y);
-    v[0] = __low2float(lo), v[1] = __high2float(lo), v[2] = __low2float(hi), v[3] = __high2float(hi);
-}
-
-__device__ __forceinline__ void store4(float* p, const float* v) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-}
-__device__ __forceinline__ void store4(__half* p, const float* v) {
-    uint2 a;
-    a.x = __builtin_bit_cast(uint32_t, __floats2half2_rn(v[0], v[1]));
-    a.y = __builtin_bit_cast(uint32_t, __floats2half2_rn(v[2], v[3]));
-    *reinterpret_cast<uint2*>(p) = a;
-}
-
 template <int HD, typename X, typename Q>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(PagedBatch b, PagedCache c, QkNormRope p) {
     constexpr int LPH = HD / 8;  // lanes per head
@@ -227,40 +199,13 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(PagedBatch b, PagedCa
     const int u = threadIdx.x % LPH;
     if (head >= p.q_heads + 2 * c.kv_heads) return;  // (whole lane groups leave)
     const bool value = head >= p.q_heads + c.kv_heads;
-    const bool turns = !value && u < p.rot_dim / 8;
-    const int lo = turns ? 4 * u : 8 * u, hi = lo + (turns ? p.rot_dim / 2 : 4);
+    const HeadPlace at = head_place<HD>(p, value, u);
+    const int lo = at.lo, hi = at.hi;
     float x[8];
     const X* src = static_cast<const X*>(p.qkv) + (int64_t)token * p.ld + head * HD;
     load4<X>(src + lo, x);
     load4<X>(src + hi, x + 4);
-    if (!value) {
-        const float* norm = head < p.q_heads ? p.q_norm : p.k_norm;
-        if (norm) {
-            float w[8], ss = 0.f;
-            load4<float>(norm + lo, w);
-            load4<float>(norm + hi, w + 4);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-            for (int d = 1; d < LPH; d <<= 1) ss += __shfl_xor(ss, d);
-            const float scale = 1.0f / sqrtf(ss / (float)HD + p.eps);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = x[e] * scale * w[e];
-        }
-        if (turns) {
-            const int pos = min(max(b.positions[token], 0), p.rope_rows - 1);
-            const float* cs = reinterpret_cast<const float*>(p.rope + (int64_t)pos * (p.rot_dim / 2) + 4 * u);
-            float t[8];
-            load4<float>(cs, t);
-            load4<float>(cs + 4, t + 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float a = x[e], d = x[e + 4];
-                x[e] = a * t[2 * e] - d * t[2 * e + 1];
-                x[e + 4] = d * t[2 * e] + a * t[2 * e + 1];
-            }
-        }
-    }
+    if (!value) norm_and_turn<HD>(b, p, head < p.q_heads ? p.q_norm : p.k_norm, at, token, u, x);
     if (head < p.q_heads) {
         Q* dst = static_cast<Q*>(p.q_out) + (int64_t)token * p.ldq + head * HD;
         store4(dst + lo, x);

@@ -1,0 +1,286 @@
+// Attention over 8-bit pages (rqmv_paged_attention_q8): the mathematics, tiles,
+// splits and joins of paged_attention.h, over codes and scales.
+//
+// Codes go from the pages into registers, 16 keys of one page at a time (one
+// scale), a step ahead, and from there to LDS as the fp16 numbers that they stand for,
+// which is exact (q8.h). From then on the kernels are those of fp16 pages, and
+// their rows have the bits that the same values in fp16 pages give where both take
+// the same form and splits.
+#include "paged_attention.h"
+#include "q8.h"
+
+namespace rq {
+
+namespace {
+
+// How a wave takes 16 rows of codes: contiguous, 1024 bytes an instruction.
+template <int HD>
+struct Lay8 {
+    static constexpr int PCS = HD / 16;   // 16-byte pieces per row
+    static constexpr int RPI = 64 / PCS;  // rows per load instruction
+    static constexpr int NI = HD / 64;    // instructions per 16 keys
+};
+
+// 16 keys of one page, on their way.
+template <int HD>
+struct Keys16 {
+    uint4 x[Lay8<HD>::NI];
+    unsigned scale;
+};
+
+template <int HD>
+__device__ __forceinline__ void fetch16(const int8_t* codes, const uint8_t* scales, const PagedCache& c, int kh, int id,
+                                        int key, Keys16<HD>& to) {
+    const int64_t row = (((int64_t)id * c.kv_heads + kh) << c.block_shift) + (key & ((1 << c.block_shift) - 1));
+    const uint4* from = reinterpret_cast<const uint4*>(codes + row * HD) + (threadIdx.x & 63);
+#pragma unroll
+    for (int i = 0; i < Lay8<HD>::NI; ++i) to.x[i] = from[i * 64];
+    to.scale = scales[row >> 4];
+}
+
+// To 16 rows of fp16 in LDS.
+template <int HD, bool VALUES>
+__device__ __forceinline__ void put16(const Keys16<HD>& from, char* lds) {
+    typedef Lay<HD> L;
+    typedef Lay8<HD> L8;
+    const int lane = threadIdx.x & 63, c = lane % L8::PCS;
+    const uint32_t s = scale_pair(from.scale);
+#pragma unroll
+    for (int i = 0; i < L8::NI; ++i) {
+        const int r = i * L8::RPI + lane / L8::PCS, x = VALUES ? L::vx(r) : L::kx(r);
+        const uint4 w = from.x[i];
+        *reinterpret_cast<uint4*>(lds + r * L::ROW + ((2 * c) ^ x) * 16) = codes_to_h(make_uint2(w.x, w.y), s);
+        *reinterpret_cast<uint4*>(lds + r * L::ROW + ((2 * c + 1) ^ x) * 16) = codes_to_h(make_uint2(w.z, w.w), s);
+    }
+}
+
+// Four values of a row of the cache.
+template <int HD>
+struct Q8Values {
+    const int8_t* v;
+    const uint8_t* scale;
+    __device__ __forceinline__ h4_t operator()(int64_t row, int dim) const {
+        uint32_t o[2];
+        bytes_to_h(*reinterpret_cast<const uint32_t*>(v + row * HD + dim), o[0], o[1]);
+        const hv2_t s = __builtin_bit_cast(hv2_t, scale_pair(scale[row >> 4]));
+        const hv2_t a = __builtin_bit_cast(hv2_t, o[0]) * s, b = __builtin_bit_cast(hv2_t, o[1]) * s;
+        return h4_t{a[0], a[1], b[0], b[1]};
+    }
+};
+
+// Few rows: four waves, each with every fourth step of 32 keys in LDS of its own; a step's codes are asked for as
+// soon as the registers of the step before are free.
+template <int HD, bool F32>
+__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_q8_few(AttnArgs a, PagedCodes codes) {
+    typedef Lay<HD> L;
+    constexpr int TM = 32, KEYS = 32, HALF = KEYS * HD * 2;  // HALF: bytes of a wave's K (and V) buffer
+    extern __shared__ __align__(16) char lds[];
+    const int kh = blockIdx.x % a.c.kv_heads;
+    Item item;
+    if (!find_item<TM>(a, blockIdx.x / a.c.kv_heads, &item)) return;
+    // (starts out of order may count past what the workspace holds)
+    const bool whole = item.live <= 1;
+    const int64_t part0 = ((int64_t)item.part * a.c.kv_heads + kh) * TM;
+    if (!whole && (a.most ? item.split >= a.most : part0 < 0 || part0 + TM > a.parts)) return;
+    const int seq = item.seq;
+    const Tile t = make_tile<TM>(a, seq, item.of, item.tile * TM);
+    const int begin = item.first + item.split * item.chunk, end = min(begin + item.chunk, t.end);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    char* K = lds + wave * 2 * HALF;
+    char* V = K + HALF;
+    Pages pages{a.b.table + seq * a.b.table_stride, a.b.max_blocks - 1, a.c.blocks, a.c.block_shift, INT_MIN / 2, 0};
+    Rows<HD, 1, F32> w;
+
+    int id[2], next[2];
+    Keys16<HD> k[2], v[2];
+    auto look = [&](int key0, int (&ids)[2]) {  // the page ids of keys key0.. and key0 + 16..
+        const int p0 = key0 >> pages.shift, p1 = (key0 + 16) >> pages.shift;
+        pages.need(p0, p1);
+        ids[0] = pages.at(p0);
+        ids[1] = pages.at(p1);
+    };
+    auto fetch = [&](const int8_t* from, const uint8_t* scales, int key0, const int (&ids)[2], Keys16<HD> (&to)[2]) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+            fetch16<HD>(from, scales, a.c, kh, pages.absent(ids[g]) ? 0 : ids[g], key0 + 16 * g, to[g]);
+    };
+    int key0 = begin + wave * KEYS;
+    bool odd = false;
+    if (key0 < end) pages.fetch(key0 >> pages.shift);
+    RawRows<HD, F32> raw;
+    load_rows<HD, F32>(a, t, kh, t.row0, w, raw);
+    arrived(w, raw);
+    if (key0 < end) {
+        look(key0, id);
+        fetch(codes.k, codes.k_scale, key0, id, k);
+        fetch(codes.v, codes.v_scale, key0, id, v);
+    }
+    start_rows(a, w, raw);
+    while (key0 < end) {
+        const int after = key0 + 4 * KEYS;
+        const bool more = after < end;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) put16<HD, false>(k[g], K + g * 16 * L::ROW);
+        if (more) {
+            look(after, next);
+            fetch(codes.k, codes.k_scale, after, next, k);
+        }
+        f16_t s[1][1];
+        scores<HD, 1, 1, F32>(K, w, s);
+        const unsigned bad = (pages.absent(id[0]) ? 1 : 0) | (pages.absent(id[1]) ? 2 : 0);
+        const bool masked = key0 < t.all_from || key0 + KEYS > t.all_to || bad;
+        if (masked) mask_scores<HD, 1, 1, F32>(w, s, key0, bad);
+        float top[1];
+        largest<1, 1>(s, top);
+        move_references<HD, 1, F32>(w, top);
+        h8_t p[1][2][F32 ? 2 : 1];
+        weights<HD, 1, 1, F32>(w, s, p);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) put16<HD, true>(v[g], V + g * 16 * L::ROW);
+        if (more) {
+            fetch(codes.v, codes.v_scale, after, next, v);
+            id[0] = next[0], id[1] = next[1];
+        }
+        if (masked && __any(zero_dead<HD, KEYS>(V, key0, t.end, bad, lane, 64))) odd = true;
+        add_values<HD, 1, 1, F32>(V, w, p);
+        key0 = after;
+    }
+    if (odd) {  // (the wave's own steps; what unmasked ones let through is there already, and stays)
+        for (int k0 = begin + wave * KEYS; k0 < end; k0 += 4 * KEYS)
+            add_odd<HD, 1, F32>(a, t, kh, k0, min(k0 + KEYS, t.end), w, Q8Values<HD>{codes.v, codes.v_scale});
+    }
+    finish_few<HD, F32, KEYS>(a, t, item, kh, begin, end, part0, w, lds);
+}
+
+// Many rows: the waves share steps of 64 keys in two LDS buffers, one barrier a step. At a step's beginning the next
+// one's codes, which have been on their way for a step, go to the other buffer, and those after it are asked for.
+template <int HD, bool F32>
+__global__ void __launch_bounds__(64 * many_waves(HD), many_waves(HD) / 4) paged_q8_many(AttnArgs a, PagedCodes codes) {
+    typedef Lay<HD> L;
+    constexpr int WAVES = many_waves(HD), TM = 32 * WAVES, KEYS = 64, KT = KEYS / 32;
+    constexpr int HALF = KEYS * HD * 2;
+    constexpr bool BOTH = WAVES == 4;  // each wave loads keys and values; of eight, four load each
+    extern __shared__ __align__(16) char lds[];
+    // the last tiles first: of one sequence's they have the most keys
+    const int kh = blockIdx.x % a.c.kv_heads, number = a.tiles - 1 - blockIdx.x / a.c.kv_heads, split = blockIdx.y;
+    const int seq = find_seq<TM>(a.b, a.group, number);
+    const int first = start_of(a.b, seq) * a.group / TM + seq;
+    const Tile t = make_tile<TM>(a, seq, load_seq(a, seq), (number - first) * TM);
+    if (t.row0 < 0 || t.row0 >= t.rows) return;  // (below 0: starts out of order)
+    const int begin = t.first + split * t.chunk, end = min(begin + t.chunk, t.end);
+    if (split && begin >= end) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = t.row0 + 32 * wave;
+    Pages pages{a.b.table + seq * a.b.table_stride, a.b.max_blocks - 1, a.c.blocks, a.c.block_shift, INT_MIN / 2, 0};
+    Rows<HD, 1, F32> w;
+
+    const int g = wave % (KEYS / 16);
+    Keys16<HD> one, two;  // BOTH: keys, values; else what the wave loads
+    // Asks for the wave's part of a step; returns which groups are absent.
+    auto fetch = [&](int key0) -> unsigned {
+        pages.need(key0 >> pages.shift, (key0 + KEYS - 16) >> pages.shift);
+        unsigned bad = 0;
+#pragma unroll
+        for (int i = 0; i < KEYS / 16; ++i) bad |= pages.absent(pages.at((key0 + 16 * i) >> pages.shift)) ? 1u << i : 0u;
+        const int key = key0 + 16 * g, id = pages.at(key >> pages.shift);
+        const int page = pages.absent(id) ? 0 : id;
+        const bool keys = BOTH || wave < 4;
+        fetch16<HD>(keys ? codes.k : codes.v, keys ? codes.k_scale : codes.v_scale, a.c, kh, page, key, one);
+        if (BOTH) fetch16<HD>(codes.v, codes.v_scale, a.c, kh, page, key, two);
+        return bad;
+    };
+    auto put = [&](int buffer) {
+        char* at = lds + buffer * 2 * HALF + g * 16 * L::ROW;
+        if (BOTH || wave < 4) put16<HD, false>(one, at);
+        if (BOTH) put16<HD, true>(two, at + HALF);
+        else if (wave >= 4) put16<HD, true>(one, at + HALF);
+    };
+    // the keys that any of the wave's rows sees
+    const int p0 = t.kv - t.n + row / a.group, p1 = t.kv - t.n + (min(row + 32, t.rows) - 1) / a.group;
+    const int wave_to = row < t.rows ? p1 + 1 : 0, wave_from = a.window ? p0 - a.window + 1 : 0;
+    unsigned bad = 0, bad1 = 0, bad2 = 0;
+    int buffer = 0;
+    bool odd = false;
+    if (begin < end) pages.fetch(begin >> pages.shift);
+    RawRows<HD, F32> raw;
+    load_rows<HD, F32>(a, t, kh, row, w, raw);
+    arrived(w, raw);
+    if (begin < end) bad = fetch(begin);
+    start_rows(a, w, raw);
+    if (begin < end) {
+        put(0);
+        if (begin + KEYS < end) bad1 = fetch(begin + KEYS);
+    }
+    for (int key0 = begin; key0 < end; key0 += KEYS) {
+        __syncthreads();  // the step is in LDS, and the other buffer is free
+        if (key0 + KEYS < end) put(buffer ^ 1);
+        if (key0 + 2 * KEYS < end) bad2 = fetch(key0 + 2 * KEYS);
+        char* K = lds + buffer * 2 * HALF;
+        char* V = K + HALF;
+        const bool masked = key0 < t.all_from || key0 + KEYS > t.all_to || bad;
+        if (masked && __syncthreads_or(zero_dead<HD, KEYS>(V, key0, t.end, bad, threadIdx.x, 64 * WAVES))) odd = true;
+        if (key0 < wave_to && key0 + KEYS > wave_from) {  // (a wave whose rows see none of the step only loads)
+            f16_t s[1][KT];
+            scores<HD, 1, KT, F32>(K, w, s);
+            if (masked) mask_scores<HD, 1, KT, F32>(w, s, key0, bad);
+            float top[1];
+            largest<1, KT>(s, top);
+            move_references<HD, 1, F32>(w, top);
+            h8_t p[1][2 * KT][F32 ? 2 : 1];
+            weights<HD, 1, KT, F32>(w, s, p);
+            add_values<HD, 1, KT, F32>(V, w, p);
+        }
+        bad = bad1;
+        bad1 = bad2;
+        buffer ^= 1;
+    }
+    if (odd) add_odd<HD, 1, F32>(a, t, kh, begin, end, w, Q8Values<HD>{codes.v, codes.v_scale});
+    finish_many<HD, F32>(a, t, kh, split, begin, end, row, w);
+}
+
+template <int HD, bool F32>
+hipError_t launch_hd(const AttnPlan& p, const AttnArgs& a, const PagedCodes& codes, hipStream_t stream) {
+    const void* f = p.few ? reinterpret_cast<const void*>(paged_q8_few<HD, F32>)
+                          : reinterpret_cast<const void*>(paged_q8_many<HD, F32>);
+    const int lds = p.few ? few_lds(HD) : many_lds(HD);
+    if (lds > 48 * 1024) {
+        const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+    }
+    if (p.few) hipLaunchKernelGGL((paged_q8_few<HD, F32>), attention_grid(p, a), dim3(256), lds, stream, a, codes);
+    else hipLaunchKernelGGL((paged_q8_many<HD, F32>), attention_grid(p, a), dim3(64 * many_waves(HD)), lds, stream, a, codes);
+    return hipGetLastError();
+}
+
+AttnPlan plan_q8(const PagedBatch& b, const PagedCache& c, int q_heads, bool f32, int cus) {
+    return plan_attention(b.tokens, b.seqs, (int64_t)b.max_blocks << c.block_shift, c.kv_heads, q_heads / c.kv_heads,
+                          c.head_dim, f32, cus);
+}
+
+}  // namespace
+
+size_t paged_attention_q8_workspace(const PagedBatch& b, const PagedCache& c, int q_heads, int cus) {
+    size_t most = 0;
+    for (const bool f32 : {false, true}) {  // (one workspace serves both types)
+        const size_t bytes = attention_workspace_bytes(plan_q8(b, c, q_heads, f32, cus), b.tokens, b.seqs,
+                                                       q_heads / c.kv_heads, c.head_dim);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
+}
+
+hipError_t launch_paged_attention_q8(const PagedBatch& b, const PagedCache& c, const PagedCodes& codes, const void* q, bool f32,
+                                     int64_t ldq, int q_heads, float scale, int window, void* workspace, void* out,
+                                     int64_t ldo, int cus, hipStream_t stream) {
+    const AttnPlan p = plan_q8(b, c, q_heads, f32, cus);
+    AttnArgs a;
+    hipError_t e = attention_args(p, b, c, q, ldq, q_heads, scale, window, workspace, out, ldo, stream, &a);
+    if (e != hipSuccess) return e;
+    if (c.head_dim == 64) e = f32 ? launch_hd<64, true>(p, a, codes, stream) : launch_hd<64, false>(p, a, codes, stream);
+    else if (c.head_dim == 128)
+        e = f32 ? launch_hd<128, true>(p, a, codes, stream) : launch_hd<128, false>(p, a, codes, stream);
+    else e = f32 ? launch_hd<256, true>(p, a, codes, stream) : launch_hd<256, false>(p, a, codes, stream);
+    return e == hipSuccess ? launch_attention_join(p, a, f32, stream) : e;
+}
+
+}  // namespace rq

@@ -288,6 +288,15 @@ int check_paged_cache(const rqmv_paged_cache* c, const char* what, rq::PagedCach
     return RQMV_OK;
 }
 
+int check_paged_cache_q8(const rqmv_paged_cache_q8* c, const char* what, rq::PagedCache* out, rq::PagedCodes* codes) {
+    const int rc = check_paged_cache(c ? &c->pages : nullptr, what, out);
+    if (rc != RQMV_OK) return rc;
+    if (!c->k_scale || !c->v_scale) return fail(RQMV_EINVAL, std::string(what) + ": the scales must not be NULL");
+    out->k = out->v = nullptr;
+    *codes = rq::PagedCodes{static_cast<int8_t*>(c->pages.k), static_cast<int8_t*>(c->pages.v), c->k_scale, c->v_scale};
+    return RQMV_OK;
+}
+
 int check_paged_batch(const rqmv_paged_batch* b, const char* what) {
     if (!b) return fail(RQMV_EINVAL, std::string(what) + ": batch is NULL");
     if (b->seqs < 1 || b->seqs > rq::kPagedMaxSeqs || b->tokens < 1 || b->tokens > kPagedMaxTokens)
@@ -828,63 +837,133 @@ int rqmv_paged_plan(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache
     return e == hipSuccess ? RQMV_OK : hip_fail(e, "paged_plan launch");
 }
 
+// The arguments that both forms of the norms and rotation take, past their cache `c`.
+static int qk_norm_rope_args(const char* what, const rqmv_paged_batch* batch, const rq::PagedCache& c, const void* qkv,
+                             int x_dtype, int64_t ld, int q_heads, const float* q_norm, const float* k_norm, float eps,
+                             const float* rope_table, int rot_dim, int rope_rows, void* q_out, int q_dtype, int64_t ldq,
+                             rq::QkNormRope* p) {
+    const int rc = check_paged_batch(batch, what);
+    if (rc != RQMV_OK) return rc;
+    if (!batch->positions || !batch->slots || !qkv || !rope_table || !q_out || q_heads <= 0 || rope_rows <= 0 ||
+        !q_norm != !k_norm || (q_norm && !(eps >= 0.f)))
+        return fail(RQMV_EINVAL, std::string(what) + ": bad arguments");
+    if ((x_dtype != RQMV_DTYPE_F16 && x_dtype != RQMV_DTYPE_F32) || (q_dtype != RQMV_DTYPE_F16 && q_dtype != RQMV_DTYPE_F32))
+        return fail(RQMV_EINVAL, std::string(what) + ": dtypes must be F16 or F32");
+    if (q_heads > kPagedMaxHeads || c.kv_heads > kPagedMaxHeads)
+        return fail(RQMV_EINVAL, std::string(what) + ": at most 1024 heads of a kind");
+    if (rot_dim <= 0 || rot_dim % 8 || rot_dim > c.head_dim)
+        return fail(RQMV_EINVAL, std::string(what) + ": rot_dim must be a multiple of 8 up to head_dim");
+    const int64_t xs = x_dtype == RQMV_DTYPE_F16 ? 2 : 4, qs = q_dtype == RQMV_DTYPE_F16 ? 2 : 4;
+    const int64_t xrow = (int64_t)(q_heads + 2 * c.kv_heads) * c.head_dim, qrow = (int64_t)q_heads * c.head_dim;
+    const int64_t t1 = batch->tokens - 1;
+    if (t1 && (ld < xrow || ldq < qrow || ld > kPagedMaxStride || ldq > kPagedMaxStride || ld * xs % 16 || ldq * qs % 16))
+        return fail(RQMV_EINVAL, std::string(what) + ": ld or ldq is too small, too large or no multiple of 16 bytes");
+    if (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)rope_table) & 15)
+        return fail(RQMV_EINVAL, std::string(what) + ": qkv, q_out, the norms and the table must be 16-byte aligned");
+    const uintptr_t x0 = (uintptr_t)qkv, x1 = x0 + (uintptr_t)((t1 ? t1 * ld : 0) + xrow) * xs;
+    const uintptr_t q0 = (uintptr_t)q_out, q1 = q0 + (uintptr_t)((t1 ? t1 * ldq : 0) + qrow) * qs;
+    const bool same = q0 == x0 && x_dtype == q_dtype && (!t1 || ld == ldq);
+    if (!same && q0 < x1 && x0 < q1)
+        return fail(RQMV_EINVAL, std::string(what) + ": q_out must be qkv itself or lie outside it");
+    p->qkv = qkv;
+    p->ld = ld;
+    p->q_heads = q_heads;
+    p->q_norm = q_norm;
+    p->k_norm = k_norm;
+    p->eps = eps;
+    p->rope = reinterpret_cast<const float2*>(rope_table);
+    p->rot_dim = rot_dim;
+    p->rope_rows = rope_rows;
+    p->q_out = q_out;
+    p->ldq = ldq;
+    return RQMV_OK;
+}
+
 int rqmv_qk_norm_rope(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, const void* qkv, int x_dtype,
                       int64_t ld, int q_heads, const float* q_norm, const float* k_norm, float eps,
                       const float* rope_table, int rot_dim, int rope_rows, void* q_out, int q_dtype, int64_t ldq,
                       void* stream) {
     rq::PagedCache c;
-    int rc = check_paged_cache(cache, "qk_norm_rope", &c);
-    if (rc == RQMV_OK) rc = check_paged_batch(batch, "qk_norm_rope");
-    if (rc != RQMV_OK) return rc;
-    if (!batch->positions || !batch->slots || !qkv || !rope_table || !q_out || q_heads <= 0 || rope_rows <= 0 ||
-        !q_norm != !k_norm || (q_norm && !(eps >= 0.f)))
-        return fail(RQMV_EINVAL, "qk_norm_rope: bad arguments");
-    if ((x_dtype != RQMV_DTYPE_F16 && x_dtype != RQMV_DTYPE_F32) || (q_dtype != RQMV_DTYPE_F16 && q_dtype != RQMV_DTYPE_F32))
-        return fail(RQMV_EINVAL, "qk_norm_rope: dtypes must be F16 or F32");
-    if (q_heads > kPagedMaxHeads || c.kv_heads > kPagedMaxHeads)
-        return fail(RQMV_EINVAL, "qk_norm_rope: at most 1024 heads of a kind");
-    if (rot_dim <= 0 || rot_dim % 8 || rot_dim > c.head_dim)
-        return fail(RQMV_EINVAL, "qk_norm_rope: rot_dim must be a multiple of 8 up to head_dim");
-    const int64_t xs = x_dtype == RQMV_DTYPE_F16 ? 2 : 4, qs = q_dtype == RQMV_DTYPE_F16 ? 2 : 4;
-    const int64_t xrow = (int64_t)(q_heads + 2 * c.kv_heads) * c.head_dim, qrow = (int64_t)q_heads * c.head_dim;
-    const int64_t t1 = batch->tokens - 1;
-    if (t1 && (ld < xrow || ldq < qrow || ld > kPagedMaxStride || ldq > kPagedMaxStride || ld * xs % 16 || ldq * qs % 16))
-        return fail(RQMV_EINVAL, "qk_norm_rope: ld or ldq is too small, too large or no multiple of 16 bytes");
-    if (((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)q_norm | (uintptr_t)k_norm | (uintptr_t)rope_table) & 15)
-        return fail(RQMV_EINVAL, "qk_norm_rope: qkv, q_out, the norms and the table must be 16-byte aligned");
-    const uintptr_t x0 = (uintptr_t)qkv, x1 = x0 + (uintptr_t)((t1 ? t1 * ld : 0) + xrow) * xs;
-    const uintptr_t q0 = (uintptr_t)q_out, q1 = q0 + (uintptr_t)((t1 ? t1 * ldq : 0) + qrow) * qs;
-    const bool same = q0 == x0 && x_dtype == q_dtype && (!t1 || ld == ldq);
-    if (!same && q0 < x1 && x0 < q1)
-        return fail(RQMV_EINVAL, "qk_norm_rope: q_out must be qkv itself or lie outside it");
     rq::QkNormRope p;
-    p.qkv = qkv;
-    p.ld = ld;
-    p.q_heads = q_heads;
-    p.q_norm = q_norm;
-    p.k_norm = k_norm;
-    p.eps = eps;
-    p.rope = reinterpret_cast<const float2*>(rope_table);
-    p.rot_dim = rot_dim;
-    p.rope_rows = rope_rows;
-    p.q_out = q_out;
-    p.ldq = ldq;
+    int rc = check_paged_cache(cache, "qk_norm_rope", &c);
+    if (rc == RQMV_OK)
+        rc = qk_norm_rope_args("qk_norm_rope", batch, c, qkv, x_dtype, ld, q_heads, q_norm, k_norm, eps, rope_table, rot_dim,
+                               rope_rows, q_out, q_dtype, ldq, &p);
+    if (rc != RQMV_OK) return rc;
     hipError_t e = rq::launch_qk_norm_rope(paged_batch(batch), c, p, x_dtype == RQMV_DTYPE_F16,
                                            q_dtype == RQMV_DTYPE_F16, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? RQMV_OK : hip_fail(e, "qk_norm_rope launch");
 }
 
-static int paged_attention_check(const rqmv_paged_batch* batch, const rqmv_paged_cache* cache, int q_heads,
-                                 rq::PagedCache* c) {
-    int rc = check_paged_cache(cache, "paged_attention", c);
-    if (rc == RQMV_OK) rc = check_paged_batch(batch, "paged_attention");
-    if (rc == RQMV_OK) rc = check_paged_table(batch, c->block_shift, "paged_attention");
+int rqmv_qk_norm_rope_q8(const rqmv_paged_batch* batch, const rqmv_paged_cache_q8* cache, const void* qkv, int x_dtype,
+                         int64_t ld, int q_heads, const float* q_norm, const float* k_norm, float eps,
+                         const float* rope_table, int rot_dim, int rope_rows, void* q_out, int q_dtype, int64_t ldq,
+                         void* stream) {
+    rq::PagedCache c;
+    rq::PagedCodes codes;
+    rq::QkNormRope p;
+    int rc = check_paged_cache_q8(cache, "qk_norm_rope_q8", &c, &codes);
+    if (rc == RQMV_OK)
+        rc = qk_norm_rope_args("qk_norm_rope_q8", batch, c, qkv, x_dtype, ld, q_heads, q_norm, k_norm, eps, rope_table,
+                               rot_dim, rope_rows, q_out, q_dtype, ldq, &p);
     if (rc != RQMV_OK) return rc;
-    if (q_heads <= 0 || q_heads > kPagedMaxHeads || q_heads % c->kv_heads)
-        return fail(RQMV_EINVAL, "paged_attention: q_heads must be a multiple of kv_heads, at most 1024");
-    if (!rq::paged_attention_fits(paged_batch(batch), *c, q_heads))
-        return fail(RQMV_EINVAL, "paged_attention: tokens * q_heads must be at most 2^26, and (tokens * q_heads / kv_heads "
-                                 "/ 32 + seqs) * kv_heads at most 2^23");
+    hipError_t e = rq::launch_qk_norm_rope_q8(paged_batch(batch), c, codes, p, x_dtype == RQMV_DTYPE_F16,
+                                              q_dtype == RQMV_DTYPE_F16, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? RQMV_OK : hip_fail(e, "qk_norm_rope_q8 launch");
+}
+
+int rqmv_paged_values_q8(const rqmv_paged_cache_q8* cache, const rqmv_paged_cache* out, void* stream) {
+    rq::PagedCache c, o;
+    rq::PagedCodes codes;
+    int rc = check_paged_cache_q8(cache, "paged_values_q8", &c, &codes);
+    if (rc == RQMV_OK) rc = check_paged_cache(out, "paged_values_q8", &o);
+    if (rc != RQMV_OK) return rc;
+    if (o.blocks != c.blocks || o.block_shift != c.block_shift || o.kv_heads != c.kv_heads || o.head_dim != c.head_dim)
+        return fail(RQMV_EINVAL, "paged_values_q8: the caches differ in shape");
+    const uintptr_t size = (((uintptr_t)c.blocks * c.kv_heads) << c.block_shift) * c.head_dim;  // codes of each cache
+    const uintptr_t from[] = {(uintptr_t)codes.k, (uintptr_t)codes.v, (uintptr_t)codes.k_scale, (uintptr_t)codes.v_scale};
+    const uintptr_t to[] = {(uintptr_t)o.k, (uintptr_t)o.v};
+    const uintptr_t scales = size / c.head_dim / 16;
+    for (int i = 0; i < 2; ++i)
+        for (int k = 0; k < 4; ++k)
+            if (to[i] < from[k] + (k < 2 ? size : scales) && from[k] < to[i] + 2 * size)
+                return fail(RQMV_EINVAL, "paged_values_q8: the values must lie outside the codes and scales");
+    if (to[0] < to[1] + 2 * size && to[1] < to[0] + 2 * size)
+        return fail(RQMV_EINVAL, "paged_values_q8: the keys' and the values' memory overlap");
+    hipError_t e = rq::launch_paged_values_q8(c, codes, o.k, o.v, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? RQMV_OK : hip_fail(e, "paged_values_q8 launch");
+}
+
+static int paged_attention_check(const char* what, const rqmv_paged_batch* batch, const rq::PagedCache& c,
+                                 int q_heads) {
+    int rc = check_paged_batch(batch, what);
+    if (rc == RQMV_OK) rc = check_paged_table(batch, c.block_shift, what);
+    if (rc != RQMV_OK) return rc;
+    if (q_heads <= 0 || q_heads > kPagedMaxHeads || q_heads % c.kv_heads)
+        return fail(RQMV_EINVAL, std::string(what) + ": q_heads must be a multiple of kv_heads, at most 1024");
+    if (!rq::paged_attention_fits(paged_batch(batch), c, q_heads))
+        return fail(RQMV_EINVAL, std::string(what) + ": tokens * q_heads must be at most 2^26, and (tokens * q_heads / kv_heads "
+                                        "/ 32 + seqs) * kv_heads at most 2^23");
+    return RQMV_OK;
+}
+
+// The rest of what both forms of attention over pages take, past paged_attention_check.
+static int paged_attention_args(const char* what, const rqmv_paged_batch* batch, const rq::PagedCache& c,
+                                const void* q, int dtype, int64_t ldq, int q_heads, const void* workspace, const void* out,
+                                int64_t ldo) {
+    if (!batch->q_start || !batch->kv_len || !batch->block_table)
+        return fail(RQMV_EINVAL, std::string(what) + ": q_start, kv_len and block_table are needed");
+    const int64_t size = dtype == RQMV_DTYPE_F16 ? 2 : 4, row = (int64_t)q_heads * c.head_dim;
+    if (batch->tokens > 1 && (ldq < row || ldo < row || ldq > kPagedMaxStride || ldo > kPagedMaxStride ||
+                              ldq * size % 16 || ldo * size % 16))
+        return fail(RQMV_EINVAL, std::string(what) + ": ldq or ldo is too small, too large or no multiple of 16 bytes");
+    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15)
+        return fail(RQMV_EINVAL, std::string(what) + ": q, out and the workspace must be 16-byte aligned");
+    const uintptr_t span = (uintptr_t)((batch->tokens > 1 ? (batch->tokens - 1) * ldq : 0) + row) * size;
+    const uintptr_t out_span = (uintptr_t)((batch->tokens > 1 ? (batch->tokens - 1) * ldo : 0) + row) * size;
+    const bool same = q == out && (batch->tokens == 1 || ldq == ldo);
+    if (!same && (uintptr_t)q < (uintptr_t)out + out_span && (uintptr_t)out < (uintptr_t)q + span)
+        return fail(RQMV_EINVAL, std::string(what) + ": out must be q itself or lie outside it");
     return RQMV_OK;
 }
 
@@ -893,11 +972,27 @@ int rqmv_paged_attention_workspace_size(const rqmv_paged_batch* batch, const rqm
     if (!bytes) return fail(RQMV_EINVAL, "paged_attention: NULL size");
     rq::PagedCache c;
     DeviceInfo info;
-    const int rc = paged_attention_check(batch, cache, q_heads, &c);
+    int rc = check_paged_cache(cache, "paged_attention", &c);
+    if (rc == RQMV_OK) rc = paged_attention_check("paged_attention", batch, c, q_heads);
     if (rc != RQMV_OK) return rc;
     const int dev = current_device(&info);
     if (dev < 0) return dev;
     *bytes = rq::paged_attention_workspace(paged_batch(batch), c, q_heads, info.cus);
+    return RQMV_OK;
+}
+
+int rqmv_paged_attention_q8_workspace_size(const rqmv_paged_batch* batch, const rqmv_paged_cache_q8* cache, int q_heads,
+                                           size_t* bytes) {
+    if (!bytes) return fail(RQMV_EINVAL, "paged_attention_q8: NULL size");
+    rq::PagedCache c;
+    rq::PagedCodes codes;
+    DeviceInfo info;
+    int rc = check_paged_cache_q8(cache, "paged_attention_q8", &c, &codes);
+    if (rc == RQMV_OK) rc = paged_attention_check("paged_attention_q8", batch, c, q_heads);
+    if (rc != RQMV_OK) return rc;
+    const int dev = current_device(&info);
+    if (dev < 0) return dev;
+    *bytes = rq::paged_attention_q8_workspace(paged_batch(batch), c, q_heads, info.cus);
     return RQMV_OK;
 }
 
@@ -908,21 +1003,10 @@ int rqmv_paged_attention(const rqmv_paged_batch* batch, const rqmv_paged_cache* 
         return fail(RQMV_EINVAL, "paged_attention: bad arguments");
     rq::PagedCache c;
     DeviceInfo info;
-    const int rc = paged_attention_check(batch, cache, q_heads, &c);
+    int rc = check_paged_cache(cache, "paged_attention", &c);
+    if (rc == RQMV_OK) rc = paged_attention_check("paged_attention", batch, c, q_heads);
+    if (rc == RQMV_OK) rc = paged_attention_args("paged_attention", batch, c, q, dtype, ldq, q_heads, workspace, out, ldo);
     if (rc != RQMV_OK) return rc;
-    if (!batch->q_start || !batch->kv_len || !batch->block_table)
-        return fail(RQMV_EINVAL, "paged_attention: q_start, kv_len and block_table are needed");
-    const int64_t size = dtype == RQMV_DTYPE_F16 ? 2 : 4, row = (int64_t)q_heads * c.head_dim;
-    if (batch->tokens > 1 && (ldq < row || ldo < row || ldq > kPagedMaxStride || ldo > kPagedMaxStride ||
-                              ldq * size % 16 || ldo * size % 16))
-        return fail(RQMV_EINVAL, "paged_attention: ldq or ldo is too small, too large or no multiple of 16 bytes");
-    if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15)
-        return fail(RQMV_EINVAL, "paged_attention: q, out and the workspace must be 16-byte aligned");
-    const uintptr_t span = (uintptr_t)((batch->tokens > 1 ? (batch->tokens - 1) * ldq : 0) + row) * size;
-    const uintptr_t out_span = (uintptr_t)((batch->tokens > 1 ? (batch->tokens - 1) * ldo : 0) + row) * size;
-    const bool same = q == out && (batch->tokens == 1 || ldq == ldo);
-    if (!same && (uintptr_t)q < (uintptr_t)out + out_span && (uintptr_t)out < (uintptr_t)q + span)
-        return fail(RQMV_EINVAL, "paged_attention: out must be q itself or lie outside it");
     const int dev = current_device(&info);
     if (dev < 0) return dev;
     const size_t need = rq::paged_attention_workspace(paged_batch(batch), c, q_heads, info.cus);
@@ -930,6 +1014,29 @@ int rqmv_paged_attention(const rqmv_paged_batch* batch, const rqmv_paged_cache* 
     hipError_t e = rq::launch_paged_attention(paged_batch(batch), c, q, dtype == RQMV_DTYPE_F32, ldq, q_heads, scale,
                                               window, workspace, out, ldo, info.cus, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? RQMV_OK : hip_fail(e, "paged_attention launch");
+}
+
+int rqmv_paged_attention_q8(const rqmv_paged_batch* batch, const rqmv_paged_cache_q8* cache, const void* q, int dtype,
+                            int64_t ldq, int q_heads, float scale, int window, void* workspace, size_t workspace_bytes,
+                            void* out, int64_t ldo, void* stream) {
+    if (!q || !out || (dtype != RQMV_DTYPE_F16 && dtype != RQMV_DTYPE_F32) || !(scale > 0.f) || scale > 1e30f || window < 0)
+        return fail(RQMV_EINVAL, "paged_attention_q8: bad arguments");
+    rq::PagedCache c;
+    rq::PagedCodes codes;
+    DeviceInfo info;
+    const char* what = "paged_attention_q8";
+    int rc = check_paged_cache_q8(cache, what, &c, &codes);
+    if (rc == RQMV_OK) rc = paged_attention_check(what, batch, c, q_heads);
+    if (rc == RQMV_OK) rc = paged_attention_args(what, batch, c, q, dtype, ldq, q_heads, workspace, out, ldo);
+    if (rc != RQMV_OK) return rc;
+    const int dev = current_device(&info);
+    if (dev < 0) return dev;
+    const size_t need = rq::paged_attention_q8_workspace(paged_batch(batch), c, q_heads, info.cus);
+    if (workspace_bytes < need || (need && !workspace)) return fail(RQMV_EINVAL, "paged_attention_q8: workspace too small");
+    hipError_t e = rq::launch_paged_attention_q8(paged_batch(batch), c, codes, q, dtype == RQMV_DTYPE_F32, ldq, q_heads,
+                                                 scale, window, workspace, out, ldo, info.cus,
+                                                 static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? RQMV_OK : hip_fail(e, "paged_attention_q8 launch");
 }
 
 int rqmv_silu_mul(const float* gate_up, int n, float* out, void* stream) {

@@ -102,6 +102,10 @@ class _Lib:
         L.rqmv_paged_attention_workspace_size.argtypes = [c_void_p, c_void_p, c_int, POINTER(c_size_t)]
         L.rqmv_paged_attention.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_float, c_int, c_void_p,
                                            c_size_t, c_void_p, c_int64, c_void_p]
+        L.rqmv_qk_norm_rope_q8.argtypes = L.rqmv_qk_norm_rope.argtypes
+        L.rqmv_paged_values_q8.argtypes = [c_void_p, c_void_p, c_void_p]
+        L.rqmv_paged_attention_q8_workspace_size.argtypes = L.rqmv_paged_attention_workspace_size.argtypes
+        L.rqmv_paged_attention_q8.argtypes = L.rqmv_paged_attention.argtypes
         L.rqmv_sample_workspace_size.argtypes = [c_int, c_int, POINTER(c_size_t)]
         L.rqmv_sample.argtypes = [c_void_p, c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
@@ -715,6 +719,31 @@ class PagedCache(_Described):
         return cls(DeviceBuffer(nbytes), DeviceBuffer(nbytes), blocks, block_size, kv_heads, head_dim)
 
 
+class _CacheQ8Struct(ctypes.Structure):
+    # (rqmv_paged_cache_q8: its `pages` first, whose fields these are, so that a call that reads an rqmv_paged_cache
+    # takes a reference to it too)
+    _fields_ = _CacheStruct._fields_ + [("k_scale", c_void_p), ("v_scale", c_void_p)]
+
+
+class PagedCacheQ8(_Described):
+    """One layer's keys and values in pages of 8 bits (rqmv_paged_cache_q8): k and v
+    are int8 codes [blocks, kv_heads, block_size, head_dim] on the device, k_scale and
+    v_scale bytes [blocks, kv_heads, block_size / 16]. paged_plan takes it as well.
+    Assigned attributes are what later calls pass."""
+
+    def __init__(self, k, v, k_scale, v_scale, blocks: int, block_size: int, kv_heads: int, head_dim: int):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.blocks, self.block_size, self.kv_heads, self.head_dim = blocks, block_size, kv_heads, head_dim
+        self.struct = _CacheQ8Struct(_p(k), _p(v), blocks, block_size, kv_heads, head_dim, _p(k_scale), _p(v_scale))
+        self.ref = byref(self.struct)
+
+    @classmethod
+    def allocate(cls, blocks: int, block_size: int, kv_heads: int, head_dim: int) -> "PagedCacheQ8":
+        codes, scales = blocks * block_size * kv_heads * head_dim, blocks * block_size * kv_heads // 16
+        return cls(DeviceBuffer(codes), DeviceBuffer(codes), DeviceBuffer(scales), DeviceBuffer(scales), blocks,
+                   block_size, kv_heads, head_dim)
+
+
 class PagedBatch(_Described):
     """The tables of one step (rqmv_paged_batch): `seqs` sequences with at most
     `tokens` new tokens. Buffers are int32 on the device; those that a call does
@@ -778,6 +807,40 @@ def paged_attention(batch: PagedBatch, cache: PagedCache, q, dtype: int, ldq: in
                                           cache.head_dim ** -0.5 if scale is None else scale, window, _p(workspace),
                                           workspace.nbytes if workspace is not None else 0, out.ptr, ldo, _sh(stream)),
            "rqmv_paged_attention")
+
+
+def qk_norm_rope_q8(batch: PagedBatch, cache: PagedCacheQ8, qkv, x_dtype: int, ld: int, q_heads: int, table,
+                    rope_rows: int, q_out, q_dtype: int, ldq: int, q_norm=None, k_norm=None, eps: float = 1e-6,
+                    rot_dim: int | None = None, stream: Stream | None = None):
+    """qk_norm_rope with pages of 8 bits (rqmv_qk_norm_rope_q8): the rows of one group of 16 slots stand within 32 rows."""
+    _check(lib().lib.rqmv_qk_norm_rope_q8(batch.ref, cache.ref, qkv.ptr, x_dtype, ld, q_heads, _p(q_norm), _p(k_norm),
+                                          eps, table.ptr, cache.head_dim if rot_dim is None else rot_dim, rope_rows,
+                                          q_out.ptr, q_dtype, ldq, _sh(stream)), "rqmv_qk_norm_rope_q8")
+
+
+def paged_values_q8(cache: PagedCacheQ8, out: PagedCache, stream: Stream | None = None):
+    """The values of 8-bit pages into fp16 pages of the same shape (rqmv_paged_values_q8)."""
+    _check(lib().lib.rqmv_paged_values_q8(cache.ref, out.ref, _sh(stream)), "rqmv_paged_values_q8")
+
+
+def paged_attention_q8_workspace_size(batch: PagedBatch, cache: PagedCacheQ8, q_heads: int) -> int:
+    n = c_size_t()
+    _check(lib().lib.rqmv_paged_attention_q8_workspace_size(batch.ref, cache.ref, q_heads, byref(n)),
+           "rqmv_paged_attention_q8_workspace_size")
+    return n.value
+
+
+def paged_attention_q8_workspace(batch: PagedBatch, cache: PagedCacheQ8, q_heads: int) -> DeviceBuffer:
+    return DeviceBuffer(paged_attention_q8_workspace_size(batch, cache, q_heads))
+
+
+def paged_attention_q8(batch: PagedBatch, cache: PagedCacheQ8, q, dtype: int, ldq: int, q_heads: int, out, ldo: int,
+                       workspace=None, scale: float | None = None, window: int = 0, stream: Stream | None = None):
+    """paged_attention over pages of 8 bits (rqmv_paged_attention_q8)."""
+    _check(lib().lib.rqmv_paged_attention_q8(batch.ref, cache.ref, q.ptr, dtype, ldq, q_heads,
+                                             cache.head_dim ** -0.5 if scale is None else scale, window, _p(workspace),
+                                             workspace.nbytes if workspace is not None else 0, out.ptr, ldo,
+                                             _sh(stream)), "rqmv_paged_attention_q8")
 
 
 def sample_workspace_size(rows: int, n: int) -> int:
