@@ -226,6 +226,21 @@ int rqmv_moe_batch_noalloc(const rqmv_moe_params* params, const void* x_dev, int
 /* x += delta (delta may be NULL); out = x / sqrt(mean(x^2) + eps) * weight. */
 int rqmv_add_rmsnorm(float* x, const float* delta, const float* weight, int n, float eps, float* out, void* stream);
 
+/* The norms between two blocks of many rows (a serving step's or a prompt's), with the gate
+ * and the residual stream between them; row r of each at its pointer + r * its stride:
+ *   d = delta / sqrt(mean(delta^2) + eps) * post_norm   (post_norm NULL: d = delta)
+ *   u = x + scale * gate * d                            (gate NULL: 1; delta NULL: u = x)
+ *   x_out = u                                           (NULL: not written)
+ *   out = u / sqrt(mean(u^2) + eps) * pre_norm          (both NULL: not written)
+ * out has out_dtype, everything else is fp32, as is the arithmetic. gate has a row for each (ldg >=
+ * n) or one for all (ldg = 0). n is a multiple of 4 up to 32768, rows 1..2^20; pointers
+ * are 16-byte aligned, strides multiples of 4 (values). x_out may be x itself; otherwise outputs lie
+ * outside the inputs and each other. A NaN or an infinity stays in its row. One launch. With rows = 1, post_norm and gate
+ * NULL and scale 1 it is rqmv_add_rmsnorm (recipe's residual add and Normalize, recipe.rs:23190-23210). */
+int rqmv_block_norm(const float* x, int64_t ldx, const float* delta, int64_t ldd, int rows, int n, const float* post_norm,
+                    const float* gate, int64_t ldg, float scale, const float* pre_norm, float eps, float* x_out,
+                    int64_t ldxo, void* out, int out_dtype, int64_t ldo, void* stream);
+
 /* NeoX rotary on the q and k heads of qkv ([q | k | v] heads of head_dim, in
  * place; pair i turns by pos * base^(-2i/head_dim)), then the rotated keys and
  * the values are stored in the caches at pos (nothing is stored when pos is
@@ -459,6 +474,25 @@ int rqmv_sample_workspace_size(int rows, int n, size_t* bytes);
 int rqmv_sample(const float* logits, int rows, int n, int64_t ld, const float* u, const float* temperature,
                 const int* top_k, const float* top_p, const float* min_p, int* tokens, float* probs, void* workspace,
                 size_t workspace_bytes, void* stream);
+
+/* What drawn or given tokens are reported with, of `rows` rows of n logits (row r at
+ * logits + r * ld), before any temperature: with p = softmax of the row,
+ *   logprob[r] = log p(tokens[r]), tokens given (-1 and others outside 0..n-1: -infinity);
+ *   entropy[r] = -sum p log p;
+ *   the `top` (0..32, at most n) likeliest tokens in order, the lowest index first among
+ *   equals, top_tokens[r * top + i] and their log probabilities top_logprobs[r * top + i].
+ * Each output may be NULL (tokens and logprob go together). NaN and -infinity logits are
+ * no candidates (probability 0); a row without any has entropy 0, -1 for its top tokens and
+ * -infinity for its log probabilities, and so have the last places of one with fewer
+ * than `top`. Logits of +infinity share the row evenly (finite ones stand behind them
+ * with -infinity). Sums are fp32 about the largest
+ * logit. n is at most 2^20, rows at most 2^20. One launch up to 4,096 logits, two above (from some 500
+ * rows on: up to 16,384). The workspace is 16-byte aligned
+ * (rqmv_logprobs_workspace_size bytes on the current device; 0: may be NULL); calls sharing it must not
+ * overlap. No counterpart in the reference. */
+int rqmv_logprobs_workspace_size(int rows, int n, int top, size_t* bytes);
+int rqmv_logprobs(const float* logits, int rows, int n, int64_t ld, const int* tokens, float* logprob, float* entropy,
+                  int top, int* top_tokens, float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);
 
 /* out = table[token mod rows] (rows x n fp32): the next token's embedding. */
 int rqmv_embed_row(const float* table, int rows, int n, const int* token, float* out, void* stream);

@@ -3,7 +3,8 @@
 Written from the definitions, one sequence, head or row at a time: plan() the
 step's tables, qk_norm_rope() the norms, rotation and append, attention() a
 sequence's new tokens over its pages, sample() the next token; store_q8() the append to
-8-bit pages and values_q8() what they stand for.
+8-bit pages and values_q8() what they stand for, logprobs() what a token is reported
+with, block_norm() the norms between two blocks.
 """
 from __future__ import annotations
 
@@ -167,3 +168,32 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
             return order[i], w / total
     last = max(i for i, w in enumerate(e) if w > 0)
     return order[last], e[last] / total
+
+
+def logprobs(logits, token=None, top=0):
+    """(log p(token), entropy, top tokens, their log probabilities) of one row."""
+    x = np.asarray(logits, np.float64)
+    x = np.where(np.isnan(x), -np.inf, x)
+    none = np.full(len(x), -np.inf)
+    if not (x > -np.inf).any():
+        lp, entropy = none, 0.0
+    else:
+        d = np.where(x == np.inf, 0.0, -np.inf) if x.max() == np.inf else x - x.max()
+        lp = d - math.log(math.fsum(np.exp(d)))
+        p = np.exp(lp)
+        entropy = -math.fsum(p[p > 0] * lp[p > 0])
+    order = [int(i) for i in np.argsort(-x, kind="stable")[:top] if x[i] > -np.inf]
+    best = [float(lp[i]) for i in order] + [-math.inf] * (top - len(order))
+    given = None if token is None else float(lp[token]) if 0 <= token < len(x) else -math.inf
+    return given, entropy, order + [-1] * (top - len(order)), best
+
+
+def block_norm(x, delta=None, post=None, gate=None, scale=1.0, pre=None, eps=0.0):
+    """(u, out) of rows [rows, n] in 64 bits; out is None without `pre`."""
+    u = np.asarray(x, np.float64)
+    if delta is not None:
+        d = np.asarray(delta, np.float64)
+        if post is not None:
+            d = d / np.sqrt((d ** 2).mean(-1, keepdims=True) + eps) * np.asarray(post, np.float64)
+        u = u + scale * (1.0 if gate is None else np.asarray(gate, np.float64)) * d
+    return u, None if pre is None else u / np.sqrt((u ** 2).mean(-1, keepdims=True) + eps) * np.asarray(pre, np.float64)

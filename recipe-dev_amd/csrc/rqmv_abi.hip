@@ -11,8 +11,10 @@
 #include "../../include/rqmv.h"
 #include "act.h"
 #include "kernels.h"
+#include "block_norm.h"
 #include "decode.h"
 #include "gguf.h"
+#include "logprobs.h"
 #include "moe.h"
 #include "paged.h"
 #include "repack.h"
@@ -1122,6 +1124,83 @@ int rqmv_sample(const float* logits, int rows, int n, int64_t ld, const float* u
     const rq::SampleArgs a{logits, ld, rows, n, u, temperature, top_k, top_p, min_p, tokens, probs};
     hipError_t e = rq::launch_sample(a, workspace, info.cus, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? RQMV_OK : hip_fail(e, "sample launch");
+}
+
+static int logprobs_check(int rows, int n, int top, DeviceInfo* info) {
+    if (rows <= 0 || rows > (1 << 20) || n <= 0 || n > rq::kLogprobMaxN)
+        return fail(RQMV_EINVAL, "logprobs: rows and n must be 1..2^20");
+    if (top < 0 || top > rq::kLogprobMaxTop || top > n) return fail(RQMV_EINVAL, "logprobs: top must be 0..32, at most n");
+    const int dev = current_device(info);
+    return dev < 0 ? dev : RQMV_OK;
+}
+
+int rqmv_logprobs_workspace_size(int rows, int n, int top, size_t* bytes) {
+    if (!bytes) return fail(RQMV_EINVAL, "logprobs: NULL size");
+    DeviceInfo info;
+    const int rc = logprobs_check(rows, n, top, &info);
+    if (rc != RQMV_OK) return rc;
+    *bytes = rq::logprobs_workspace(rows, n, top, info.cus);
+    return RQMV_OK;
+}
+
+int rqmv_logprobs(const float* logits, int rows, int n, int64_t ld, const int* tokens, float* logprob, float* entropy,
+                  int top, int* top_tokens, float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!logits || !tokens != !logprob || (!logprob && !entropy && !top)) return fail(RQMV_EINVAL, "logprobs: bad arguments");
+    if (top > 0 && !top_tokens && !top_logprobs) return fail(RQMV_EINVAL, "logprobs: the top tokens have no output");
+    if (rows > 1 && (ld < n || ld > kPagedMaxStride)) return fail(RQMV_EINVAL, "logprobs: ld must be at least n");
+    DeviceInfo info;
+    const int rc = logprobs_check(rows, n, top, &info);
+    if (rc != RQMV_OK) return rc;
+    if ((uintptr_t)workspace & 15) return fail(RQMV_EINVAL, "logprobs: the workspace must be 16-byte aligned");
+    const size_t need = rq::logprobs_workspace(rows, n, top, info.cus);
+    if (workspace_bytes < need || (need && !workspace)) return fail(RQMV_EINVAL, "logprobs: workspace too small");
+    const rq::LogprobArgs a{logits, ld, rows, n, tokens, top, logprob, entropy, top_tokens, top_logprobs};
+    hipError_t e = rq::launch_logprobs(a, workspace, info.cus, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? RQMV_OK : hip_fail(e, "logprobs launch");
+}
+
+int rqmv_block_norm(const float* x, int64_t ldx, const float* delta, int64_t ldd, int rows, int n, const float* post_norm,
+                    const float* gate, int64_t ldg, float scale, const float* pre_norm, float eps, float* x_out,
+                    int64_t ldxo, void* out, int out_dtype, int64_t ldo, void* stream) {
+    if (!x || (!x_out && !out) || !out != !pre_norm || (!delta && (post_norm || gate)))
+        return fail(RQMV_EINVAL, "block_norm: bad arguments");
+    if (rows <= 0 || rows > (1 << 20) || n <= 0 || n > rq::kBlockNormMaxN || n % 4)
+        return fail(RQMV_EINVAL, "block_norm: rows must be 1..2^20 and n a multiple of 4 up to 32768");
+    if (out && out_dtype != RQMV_DTYPE_F16 && out_dtype != RQMV_DTYPE_F32)
+        return fail(RQMV_EINVAL, "block_norm: out_dtype must be F16 or F32");
+    if (!(eps >= 0.f) || !(scale == scale)) return fail(RQMV_EINVAL, "block_norm: eps must not be below 0, eps and scale no NaN");
+    struct Span {
+        const void* at;
+        int64_t ld;
+        int size;
+    };
+    const int os = out_dtype == RQMV_DTYPE_F16 ? 2 : 4;
+    const Span in[] = {{x, ldx, 4}, {delta, ldd, 4}, {gate, ldg, 4}, {post_norm, 0, 4}, {pre_norm, 0, 4}};
+    const Span made[] = {{x_out, ldxo, 4}, {out, ldo, os}};
+    auto bad = [&](const Span& s, bool shared) {
+        if (!s.at) return false;
+        if ((uintptr_t)s.at & 15) return true;
+        if (rows == 1 || (shared && s.ld == 0)) return false;
+        return s.ld < n || s.ld > kPagedMaxStride || s.ld % 4 != 0;
+    };
+    if (bad(in[0], false) || bad(in[1], false) || bad(in[2], true) || bad(in[3], true) || bad(in[4], true) ||
+        bad(made[0], false) || bad(made[1], false))
+        return fail(RQMV_EINVAL, "block_norm: pointers must be 16-byte aligned, strides at least n and multiples of 4");
+    auto end = [&](const Span& s) { return (uintptr_t)s.at + ((rows - 1) * (rows > 1 ? s.ld : 0) + n) * s.size; };
+    auto meet = [&](const Span& a, const Span& b) {
+        return a.at && b.at && (uintptr_t)a.at < end(b) && (uintptr_t)b.at < end(a);
+    };
+    for (const Span& o : made)
+        for (const Span& i : in)
+            if (meet(o, i) && !(o.at == x_out && x_out == x && &i == in && (rows == 1 || ldxo == ldx)))
+                return fail(RQMV_EINVAL, "block_norm: outputs must lie outside the inputs (x_out may be x itself)");
+    if (meet(made[0], made[1])) return fail(RQMV_EINVAL, "block_norm: x_out and out overlap");
+    rq::BlockNorm p{x, ldx, delta, ldd, rows, n, post_norm, gate, ldg, scale, pre_norm, eps, x_out, ldxo, out, ldo};
+    DeviceInfo info;
+    const int dev = current_device(&info);
+    if (dev < 0) return dev;
+    hipError_t e = rq::launch_block_norm(p, out_dtype == RQMV_DTYPE_F16, info.cus, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? RQMV_OK : hip_fail(e, "block_norm launch");
 }
 
 int rqmv_embed_row(const float* table, int rows, int n, const int* token, float* out, void* stream) {

@@ -109,6 +109,11 @@ class _Lib:
         L.rqmv_sample_workspace_size.argtypes = [c_int, c_int, POINTER(c_size_t)]
         L.rqmv_sample.argtypes = [c_void_p, c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+        L.rqmv_logprobs_workspace_size.argtypes = [c_int, c_int, c_int, POINTER(c_size_t)]
+        L.rqmv_logprobs.argtypes = [c_void_p, c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                    c_void_p, c_void_p, c_size_t, c_void_p]
+        L.rqmv_block_norm.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int64,
+                                      c_float, c_void_p, c_float, c_void_p, c_int64, c_void_p, c_int, c_int64, c_void_p]
         L.rqmv_glu_weight_create.argtypes = [c_int, c_int64, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]
         L.rqmv_matvec_fused.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
         L.rqmv_layout_bytes.argtypes = [c_int, c_int64, c_int64, POINTER(c_size_t)]
@@ -860,6 +865,38 @@ def sample(logits, rows: int, n: int, ld: int, u, tokens, workspace=None, temper
     _check(lib().lib.rqmv_sample(logits.ptr, rows, n, ld, u.ptr, _p(temperature), _p(top_k), _p(top_p), _p(min_p),
                                  tokens.ptr, _p(prob), _p(workspace), workspace.nbytes if workspace is not None else 0,
                                  _sh(stream)), "rqmv_sample")
+
+
+def logprobs_workspace_size(rows: int, n: int, top: int = 0) -> int:
+    size = c_size_t()
+    _check(lib().lib.rqmv_logprobs_workspace_size(rows, n, top, byref(size)), "rqmv_logprobs_workspace_size")
+    return size.value
+
+
+def logprobs_workspace(rows: int, n: int, top: int = 0) -> DeviceBuffer:
+    return DeviceBuffer(logprobs_workspace_size(rows, n, top))
+
+
+def logprobs(logits, rows: int, n: int, ld: int, tokens=None, logprob=None, entropy=None, top: int = 0, top_tokens=None,
+             top_logprobs=None, workspace=None, stream: Stream | None = None):
+    """Log probabilities of given tokens, entropies and the `top` likeliest tokens of
+    each row of logits (rqmv_logprobs); outputs that are None are not made."""
+    _check(lib().lib.rqmv_logprobs(logits.ptr, rows, n, ld, _p(tokens), _p(logprob), _p(entropy), top, _p(top_tokens),
+                                   _p(top_logprobs), _p(workspace), workspace.nbytes if workspace is not None else 0,
+                                   _sh(stream)), "rqmv_logprobs")
+
+
+def block_norm(x, rows: int, n: int, delta=None, post_norm=None, gate=None, scale: float = 1.0, pre_norm=None,
+               eps: float = 1e-6, x_out=None, out=None, out_dtype: int = DTYPE_F32, ldx: int | None = None,
+               ldd: int | None = None, ldg: int = 0, ldxo: int | None = None, ldo: int | None = None,
+               stream: Stream | None = None):
+    """The norm after a block, its gate and the residual stream, the norm before the
+    next, of many rows (rqmv_block_norm); strides default to n, the gate's to one row
+    for all."""
+    ld = [n if v is None else v for v in (ldx, ldd, ldxo, ldo)]
+    _check(lib().lib.rqmv_block_norm(x.ptr, ld[0], _p(delta), ld[1], rows, n, _p(post_norm), _p(gate), ldg, scale,
+                                     _p(pre_norm), eps, _p(x_out), ld[2], _p(out), out_dtype, ld[3], _sh(stream)),
+           "rqmv_block_norm")
 
 
 # ------------------------------------------------------- fused products ----
