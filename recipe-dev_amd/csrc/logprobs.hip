@@ -9,18 +9,17 @@
 //     s' = e^(m - m') s,   t' = e^(m - m') (t + (m - m') s).
 // A row of one slice is finished where it is read.
 //
-// The largest of a wave's logits: at least `top` of its lanes have their own
-// largest at or above the top-th largest of the lanes' largest ones, T, so what lies below T is
-// out. T is found by bisection over its upper bits (a ballot each), which
-// may leave it a little low; some 1.2 to 1.4 times `top` logits remain, are put into
-// a list in LDS and ranked by comparing each with all (the lowest index first among equals).
-// Where many are equal the list overflows; then the wave bisects for the exact top-th
-// largest of all its logits and takes the equal ones by their index.
+// The largest of a workgroup's logits: if `top` lanes of a wave have their own largest at or above T, what
+// lies below T is out. A wave finds its largest such T by bisection over its upper bits
+// (ballots), which may leave it a little low, and the workgroup takes the largest of its four. What
+// remains goes into a list in LDS and is ranked by comparing each with all (the
+// lowest index first among equals). Where many are equal a wave's share of the list overflows;
+// then it bisects for the exact top-th largest of all its logits and takes the equal ones by their index.
 //
 // Bound: HBM, at few rows the two launches and their dependent loads.
 #include "logprobs.h"
 
-#include <float.h>
+#include <limits.h>
 
 #include "lanes.h"
 
@@ -29,7 +28,8 @@ namespace rq {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kList = 128;  // of a wave
+constexpr int kList = 128;   // entries of a wave
+constexpr int kSegment = 8;  // entries compared at once
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Stats {
@@ -50,15 +50,24 @@ __device__ __forceinline__ Stats move(Stats a, float to) {
     return Stats{to, f * a.s, f > 0.f && a.m != to ? f * fmaf(a.m - to, a.s, a.t) : f > 0.f ? a.t : 0.f};
 }
 
+// Over the wave: rows of 16 by DPP, then the lane swaps.
+template <int CTRL>
+__device__ __forceinline__ float turned(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-    return v;
+    v = fmaxf(v, turned<0x128>(v));  // row_ror:8, 4, 2, 1
+    v = fmaxf(v, turned<0x124>(v));
+    v = fmaxf(v, turned<0x122>(v));
+    v = fmaxf(v, turned<0x121>(v));
+    return swap32_max(swap16_max(v));
 }
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+    v += turned<0x128>(v);
+    v += turned<0x124>(v);
+    v += turned<0x122>(v);
+    v += turned<0x121>(v);
+    return swap32_sum(swap16_sum(v));
 }
 
 // Floats to numbers in their order and back. (No NaNs and no -0.)
@@ -91,29 +100,57 @@ __device__ __forceinline__ Stats wave_stats(const float (&v)[N], float m) {
     return a;
 }
 
-// At least the `top` first of the wave's values (value descending, index ascending) into its list, at most kList;
-// returns how many. `index(i)`: of v[i], ascending by (i / 4, lane, i % 4).
-template <int N, typename F>
-__device__ __forceinline__ int wave_top(const float (&v)[N], float lane_max, int top, F index, Entry* list) {
-    uint32_t T = 0;
+struct Shared {
+    Entry list[kWaves * kList + 2 * kSegment];
+    int rank[kWaves * kList];
+    Entry best[kLogprobMaxTop];
+    Stats stats[kWaves];
+    uint32_t least[kWaves];
+    int count;
+};
+
+__device__ __forceinline__ int before(unsigned long long mask) {  // lanes of `mask` before this one
+    return __builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0));
+}
+
+// A number that at least `top` of the wave's lanes reach with their largest value, close to the largest such.
+__device__ __forceinline__ uint32_t wave_least(float lane_max, int top) {
     const uint32_t mine = key_of(lane_max);
+    uint32_t T = 0;
 #pragma unroll 1
-    for (int b = 31; b >= 12; --b) {
-        const uint32_t up = T | 1u << b;
-        if (__popcll(__ballot(mine >= up)) >= top) T = up;
+    for (int b = 30; b >= 12; b -= 2) {  // (two bits a step: three ballots that do not wait for each other)
+        const int c1 = __popcll(__ballot(mine >= (T | 1u << b))), c2 = __popcll(__ballot(mine >= (T | 2u << b))),
+                  c3 = __popcll(__ballot(mine >= (T | 3u << b)));
+        T |= (c3 >= top ? 3u : c2 >= top ? 2u : c1 >= top ? 1u : 0u) << b;
     }
-    const float least = of_key(max(T, kLowest));
+    return T;
+}
+
+// The wave's values from `least` on into the workgroup's list; of more than kList the `top` first of the
+// wave (value descending, index ascending). `index(i)`: of v[i], ascending by (i / G, lane, i % G).
+template <int N, int G, typename F>
+__device__ __forceinline__ void wave_top(Shared& sh, const float (&v)[N], uint32_t least_key, int top, F index) {
+    const float least = of_key(max(least_key, kLowest));
+    auto base_of = [&](int count) {  // a place for `count` entries
+        int base = 0;
+        if ((threadIdx.x & 63) == 0) base = atomicAdd(&sh.count, count);
+        return __builtin_amdgcn_readfirstlane(base);
+    };
     int count = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const unsigned long long hits = __ballot(v[i] >= least);
-        if (hits) {
-            const int at = count + __builtin_amdgcn_mbcnt_hi((unsigned)(hits >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hits, 0));
-            if (v[i] >= least && at < kList) list[at] = Entry{v[i], index(i)};
-            count += __popcll(hits);
+    for (int i = 0; i < N; ++i) count += __popcll(__ballot(v[i] >= least));
+    if (count <= kList) {
+        int at = base_of(count);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const unsigned long long hits = __ballot(v[i] >= least);
+            if (hits) {
+                if (v[i] >= least) sh.list[at + before(hits)] = Entry{v[i], index(i)};
+                at += __popcll(hits);
+            }
         }
+        return;
     }
-    if (count <= kList) return count;
     // Too many: the exact border, then all above it and the first of those on it.
     uint32_t V = 0;
 #pragma unroll 1
@@ -125,61 +162,70 @@ __device__ __forceinline__ int wave_top(const float (&v)[N], float lane_max, int
         if (c >= top) V = up;
     }
     const float border = of_key(max(V, kLowest));
+    const int at = base_of(top);
     count = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const unsigned long long hits = __ballot(v[i] > border);
-        const int at = count + __builtin_amdgcn_mbcnt_hi((unsigned)(hits >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hits, 0));
-        if (v[i] > border) list[at] = Entry{v[i], index(i)};  // (fewer than `top`)
+        if (v[i] > border) sh.list[at + count + before(hits)] = Entry{v[i], index(i)};  // (fewer than `top`)
         count += __popcll(hits);
     }
 #pragma unroll
-    for (int r = 0; r < N / 4; ++r) {
+    for (int r = 0; r < N / G; ++r) {
         unsigned own = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) own += v[4 * r + j] == border ? 1 : 0;
+        for (int j = 0; j < G; ++j) own += v[G * r + j] == border ? 1 : 0;
         const unsigned upto = wave_scan(own);
-        int at = count + (int)(upto - own);
+        int k = count + (int)(upto - own);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (v[4 * r + j] == border) {
-                if (at < top) list[at] = Entry{border, index(4 * r + j)};
-                ++at;
+        for (int j = 0; j < G; ++j)
+            if (v[G * r + j] == border) {
+                if (k < top) sh.list[at + k] = Entry{border, index(G * r + j)};
+                ++k;
             }
         count = min(count + __builtin_amdgcn_readlane((int)upto, 63), top);
     }
-    return count;
 }
 
-struct Shared {
-    Entry list[kWaves * kList];
-    Entry best[kLogprobMaxTop];
-    Stats stats[kWaves];
-    int count[kWaves];
-};
-
-// The waves' lists to the workgroup's `top` first, in order, in sh.best ((-infinity, -1) past the last).
-__device__ __forceinline__ void group_top(Shared& sh, int top) {
+// The `top` first of the workgroup's values in order, in sh.best ((-infinity, -1) past the last). The waves agree on the
+// largest of their `least`s, each of which has `top` values above it; then every entry of the list is compared with
+// all, its share of them by one of two threads while there are at most 128.
+template <int N, int G, typename F>
+__device__ __forceinline__ void group_top(Shared& sh, const float (&v)[N], float lane_max, int top, F index) {
+    const uint32_t mine = wave_least(lane_max, top);
+    if ((threadIdx.x & 63) == 0) sh.least[threadIdx.x >> 6] = mine;
+    if (threadIdx.x == 0) sh.count = 0;
+    for (int i = threadIdx.x; i < kWaves * kList; i += kThreads) sh.rank[i] = 0;
     __syncthreads();
-    int total = 0;
+    uint32_t least = sh.least[0];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) total += sh.count[w];
-    for (int p = threadIdx.x; p < kWaves * kList; p += kThreads) {
-        if (p % kList >= sh.count[p / kList]) continue;
+    for (int w = 1; w < kWaves; ++w) least = max(least, sh.least[w]);
+    wave_top<N, G>(sh, v, least, top, index);
+    __syncthreads();
+    const int count = sh.count;
+    // past the last: entries that are before none
+    if (threadIdx.x < 2 * kSegment) sh.list[count + threadIdx.x] = Entry{-INFINITY, INT_MAX};
+    __syncthreads();
+    const bool halves = count <= kThreads / 2;
+    const int each = halves ? (count / 2 + kSegment) & ~(kSegment - 1) : count;
+    for (int p = halves ? threadIdx.x / 2 : threadIdx.x; p < count; p += kThreads) {
         const Entry own = sh.list[p];
+        const int from = halves ? (threadIdx.x & 1) * each : 0;
         int rank = 0;
-        for (int w = 0; w < kWaves; ++w) {
-            const int c = sh.count[w];
-#pragma unroll 4
-            for (int q = 0; q < c; ++q) {
-                const Entry o = sh.list[w * kList + q];
+        for (int q = from; q < min(from + each, count); q += kSegment) {
+#pragma unroll
+            for (int k = 0; k < kSegment; ++k) {
+                const Entry o = sh.list[q + k];
                 rank += o.v > own.v || (o.v == own.v && o.i < own.i) ? 1 : 0;
             }
         }
-        if (rank < top) sh.best[rank] = own;
+        if (halves) atomicAdd(&sh.rank[p], rank);
+        else sh.rank[p] = rank;
     }
-    if ((int)threadIdx.x < top && (int)threadIdx.x >= total) sh.best[threadIdx.x] = Entry{-INFINITY, -1};
     __syncthreads();
+    for (int p = threadIdx.x; p < count; p += kThreads)
+        if (sh.rank[p] < top) sh.best[sh.rank[p]] = sh.list[p];
+    if ((int)threadIdx.x < top && (int)threadIdx.x >= count) sh.best[threadIdx.x] = Entry{-INFINITY, -1};
 }
 
 // The waves' stats as one. (Read behind a barrier.)
@@ -245,13 +291,10 @@ __global__ void __launch_bounds__(kThreads) logprobs_slice_kernel(LogprobArgs a,
             top1 = fmaxf(top1, v[i]);
         }
         const Stats st = wave_stats(v, wave_max(top1));
-        int count = 0;
+        if (lane == 0) sh.stats[wave] = st;
         if (TOP)
-            count = wave_top(v, top1, a.top, [&](int i) { return c0 + 256 * (i / 4) + 4 * lane + i % 4; },
-                             sh.list + wave * kList);
-        if (lane == 0) sh.stats[wave] = st, sh.count[wave] = count;
-        if (TOP) group_top(sh, a.top);
-        else __syncthreads();
+            group_top<4 * R, 4>(sh, v, top1, a.top, [&](int i) { return c0 + 256 * (i / 4) + 4 * lane + i % 4; });
+        __syncthreads();
         const Stats all = group_stats(sh);
         if (!parts) {
             put_row(a, row, all, sh);
@@ -280,24 +323,22 @@ __global__ void __launch_bounds__(kThreads) logprobs_join_kernel(LogprobArgs a, 
         st = move(st, m);
         st.s = wave_sum(st.s);
         st.t = wave_sum(st.t);
-        int count = 0;
+        if (lane == 0) sh.stats[wave] = st;
         if (a.top) {
-            // entry 4 (64 r + lane) + j of the wave's is v[4 r + j]: equal values stand in the order of their indices
+            // entry 256 i + thread is v[i]: a lane's are of unlike lists, and equal values stand in the order of their indices
             const int all = slices * a.top;
             float v[N], top1 = -INFINITY;
             int id[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int e = wave * 64 * N + 256 * (i / 4) + 4 * lane + i % 4;
+                const int e = kThreads * i + threadIdx.x;
                 const Entry o = e < all ? tops[row * all + e] : Entry{-INFINITY, -1};
                 v[i] = o.v, id[i] = o.i;
                 top1 = fmaxf(top1, v[i]);
             }
-            count = wave_top(v, top1, a.top, [&](int i) { return id[i]; }, sh.list + wave * kList);
+            group_top<N, 1>(sh, v, top1, a.top, [&](int i) { return id[i]; });
         }
-        if (lane == 0) sh.stats[wave] = st, sh.count[wave] = count;
-        if (a.top) group_top(sh, a.top);
-        else __syncthreads();
+        __syncthreads();
         put_row(a, row, group_stats(sh), sh);
         __syncthreads();
     }
