@@ -43,6 +43,26 @@ __device__ __forceinline__ float swap32_max(float v) {
     return fmaxf(p.lo, p.hi);
 }
 
+// Over the wave: rows of 16 by DPP, then the lane swaps.
+template <int CTRL>
+__device__ __forceinline__ float turned(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float all_max(float v) {
+    v = fmaxf(v, turned<0x128>(v));  // row_ror:8, 4, 2, 1
+    v = fmaxf(v, turned<0x124>(v));
+    v = fmaxf(v, turned<0x122>(v));
+    v = fmaxf(v, turned<0x121>(v));
+    return swap32_max(swap16_max(v));
+}
+__device__ __forceinline__ float all_sum(float v) {
+    v += turned<0x128>(v);
+    v += turned<0x124>(v);
+    v += turned<0x122>(v);
+    v += turned<0x121>(v);
+    return swap32_sum(swap16_sum(v));
+}
+
 // v of the lane that a DPP control selects, 0 where it selects none (rows outside `ROWS` too).
 template <int CTRL, int ROWS>
 __device__ __forceinline__ unsigned dpp(unsigned v) {

@@ -50,26 +50,6 @@ __device__ __forceinline__ Stats move(Stats a, float to) {
     return Stats{to, f * a.s, f > 0.f && a.m != to ? f * fmaf(a.m - to, a.s, a.t) : f > 0.f ? a.t : 0.f};
 }
 
-// Over the wave: rows of 16 by DPP, then the lane swaps.
-template <int CTRL>
-__device__ __forceinline__ float turned(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
-}
-__device__ __forceinline__ float wave_max(float v) {
-    v = fmaxf(v, turned<0x128>(v));  // row_ror:8, 4, 2, 1
-    v = fmaxf(v, turned<0x124>(v));
-    v = fmaxf(v, turned<0x122>(v));
-    v = fmaxf(v, turned<0x121>(v));
-    return swap32_max(swap16_max(v));
-}
-__device__ __forceinline__ float wave_sum(float v) {
-    v += turned<0x128>(v);
-    v += turned<0x124>(v);
-    v += turned<0x122>(v);
-    v += turned<0x121>(v);
-    return swap32_sum(swap16_sum(v));
-}
-
 // Floats to numbers in their order and back. (No NaNs and no -0.)
 __device__ __forceinline__ uint32_t key_of(float v) {
     const uint32_t b = __builtin_bit_cast(uint32_t, v);
@@ -95,8 +75,8 @@ __device__ __forceinline__ Stats wave_stats(const float (&v)[N], float m) {
             a.t = fmaf(fmaxf(d, -1000.f), e, a.t);  // (-infinity times 0 would be NaN)
         }
     }
-    a.s = wave_sum(a.s);
-    a.t = wave_sum(a.t);
+    a.s = all_sum(a.s);
+    a.t = all_sum(a.t);
     return a;
 }
 
@@ -290,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_slice_kernel(LogprobArgs a,
             v[i] = v[i] == v[i] ? v[i] + 0.f : -INFINITY;  // (NaNs are skipped; -0 is 0)
             top1 = fmaxf(top1, v[i]);
         }
-        const Stats st = wave_stats(v, wave_max(top1));
+        const Stats st = wave_stats(v, all_max(top1));
         if (lane == 0) sh.stats[wave] = st;
         if (TOP)
             group_top<4 * R, 4>(sh, v, top1, a.top, [&](int i) { return c0 + 256 * (i / 4) + 4 * lane + i % 4; });
@@ -319,10 +299,10 @@ __global__ void __launch_bounds__(kThreads) logprobs_join_kernel(LogprobArgs a, 
             const float4 p = parts[row * slices + threadIdx.x];
             st = Stats{p.x, p.y, p.z};
         }
-        const float m = wave_max(st.m);
+        const float m = all_max(st.m);
         st = move(st, m);
-        st.s = wave_sum(st.s);
-        st.t = wave_sum(st.t);
+        st.s = all_sum(st.s);
+        st.t = all_sum(st.t);
         if (lane == 0) sh.stats[wave] = st;
         if (a.top) {
             // entry 256 i + thread is v[i]: a lane's are of unlike lists, and equal values stand in the order of their indices

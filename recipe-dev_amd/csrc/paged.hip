@@ -205,7 +205,13 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(PagedBatch b, PagedCa
     const X* src = static_cast<const X*>(p.qkv) + (int64_t)token * p.ld + head * HD;
     load4<X>(src + lo, x);
     load4<X>(src + hi, x + 4);
-    if (!value) norm_and_turn<HD>(b, p, head < p.q_heads ? p.q_norm : p.k_norm, at, token, u, x);
+    if (!value) {
+        const float* norm = head < p.q_heads ? p.q_norm : p.k_norm;
+        HeadLane h;
+        if (norm) load_norm(norm, at, h);
+        if (at.turns) load_turn(p, b.positions[token], u, h);
+        norm_and_turn<HD>(norm, at.turns, p.eps, h, x);
+    }
     if (head < p.q_heads) {
         Q* dst = static_cast<Q*>(p.q_out) + (int64_t)token * p.ldq + head * HD;
         store4(dst + lo, x);

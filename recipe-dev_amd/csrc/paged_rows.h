@@ -47,35 +47,60 @@ __device__ __forceinline__ HeadPlace head_place(const QkNormRope& p, bool value,
     const int lo = turns ? 4 * u : 8 * u;
     return HeadPlace{turns, lo, lo + (turns ? p.rot_dim / 2 : 4)};
 }
-// A q or k head's values through its norm (null: none) and the rotation, in T's arithmetic.
+// What a q or k head's lane needs besides its values: the norm's weights, and (cos, sin) of its pairs at a position.
+struct HeadLane {
+    float w[8], t[8];
+};
+__device__ __forceinline__ void load_norm(const float* norm, HeadPlace at, HeadLane& h) {
+    load4<float>(norm + at.lo, h.w);
+    load4<float>(norm + at.hi, h.w + 4);
+}
+__device__ __forceinline__ void load_turn(const QkNormRope& p, int position, int u, HeadLane& h) {
+    const int pos = min(max(position, 0), p.rope_rows - 1);
+    const float* cs = reinterpret_cast<const float*>(p.rope + (int64_t)pos * (p.rot_dim / 2) + 4 * u);
+    load4<float>(cs, h.t);
+    load4<float>(cs + 4, h.t + 4);
+}
+// The sum over a head's LPH lanes, the same in each. Partners by DPP up to 16 lanes: of quads by their lanes, of
+// halves and rows mirrored (their lanes agree by then).
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double v) {
+    const int2 w = __builtin_bit_cast(int2, v);
+    return v + __builtin_bit_cast(double, make_int2(__builtin_amdgcn_update_dpp(0, w.x, CTRL, 0xf, 0xf, false),
+                                                    __builtin_amdgcn_update_dpp(0, w.y, CTRL, 0xf, 0xf, false)));
+}
+template <int LPH, typename T>
+__device__ __forceinline__ T head_sum(T v) {
+    v = dpp_add<0xB1>(v);   // quad_perm 1, 0, 3, 2
+    v = dpp_add<0x4E>(v);   // quad_perm 2, 3, 0, 1
+    v = dpp_add<0x141>(v);  // row_half_mirror
+    if constexpr (LPH > 8) v = dpp_add<0x140>(v);  // row_mirror
+    if constexpr (LPH > 16) v += __shfl_xor(v, 16);
+    return v;
+}
+// A head's values through its norm (if it has one) and the rotation (of lanes that turn), in T's arithmetic.
 template <int HD, typename T>
-__device__ __forceinline__ void norm_and_turn(const PagedBatch& b, const QkNormRope& p, const float* norm, HeadPlace at,
-                                              int token, int u, T (&x)[8]) {
+__device__ __forceinline__ void norm_and_turn(bool norm, bool turns, float eps, const HeadLane& h, T (&x)[8]) {
     constexpr int LPH = HD / 8;
     if (norm) {
-        float w[8];
         T ss = 0;
-        load4<float>(norm + at.lo, w);
-        load4<float>(norm + at.hi, w + 4);
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fma(x[e], x[e], ss);
+        ss = head_sum<LPH>(ss);
+        const T scale = T(1) / sqrt(ss / (T)HD + (T)eps);
 #pragma unroll
-        for (int d = 1; d < LPH; d <<= 1) ss += __shfl_xor(ss, d);
-        const T scale = T(1) / sqrt(ss / (T)HD + (T)p.eps);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * scale * (T)w[e];
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * scale * (T)h.w[e];
     }
-    if (at.turns) {
-        const int pos = min(max(b.positions[token], 0), p.rope_rows - 1);
-        const float* cs = reinterpret_cast<const float*>(p.rope + (int64_t)pos * (p.rot_dim / 2) + 4 * u);
-        float t[8];
-        load4<float>(cs, t);
-        load4<float>(cs + 4, t + 4);
+    if (turns) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const T a = x[e], d = x[e + 4];
-            x[e] = a * (T)t[2 * e] - d * (T)t[2 * e + 1];
-            x[e + 4] = d * (T)t[2 * e] + a * (T)t[2 * e + 1];
+            x[e] = a * (T)h.t[2 * e] - d * (T)h.t[2 * e + 1];
+            x[e + 4] = d * (T)h.t[2 * e] + a * (T)h.t[2 * e + 1];
         }
     }
 }
