@@ -77,7 +77,8 @@ struct AttnPlan {
     int64_t tiles, parts;
 };
 
-AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus);
+// `per_cu`: few rows' items per CU over the whole batch.
+AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus, int per_cu);
 size_t attention_workspace_bytes(const AttnPlan& p, int tokens, int seqs, int group, int hd);
 // A call's arguments; where the plan has items, launches the count of them.
 hipError_t attention_args(const AttnPlan& p, const PagedBatch& b, const PagedCache& c, const void* q, int64_t ldq, int q_heads,
@@ -164,6 +165,21 @@ __device__ __forceinline__ Tile make_tile(const AttnArgs& a, int seq, const Seq&
     return t;
 }
 
+// 16 bytes per lane from `base` + `offset` (bytes) straight into LDS at `lds` +
+// 16 lane. Inline assembly, so that the compiler does not make every later LDS
+// read wait for it: the kernel waits for these loads itself. (M0 holds the LDS
+// address; a write of M0 needs one wait state before a load to LDS.)
+__device__ __forceinline__ void load_lds(const void* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(offset), "s"(base), "s"(lds)
+                 : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
 template <int HD>
 struct Lay {
     static constexpr int PCS = HD / 8;    // 16-byte pieces per row
@@ -224,23 +240,25 @@ struct RawRows {
 // count, with them. fp32 rows are asked for before the first step's loads to LDS and become operands while these
 // are on their way (one token over 4,096: 4 % less); fp16 rows, which are operands already, come
 // behind those loads (32 sequences: 1 % less).
-template <int HD, bool F32>
+// HALVES: a lane holds the row's dims h HD / 2 + 8 k .. in operand k instead of 16 k + 8 h (the sum over a row's dims may go in
+// any order, if the keys' is the same).
+template <int HD, bool F32, bool HALVES = false>
 __device__ __forceinline__ void load_rows(const AttnArgs& a, const Tile& t, int kh, int row, Rows<HD, 1, F32>& w,
                                           RawRows<HD, F32>& raw) {
     const int lane = threadIdx.x & 63, h = lane >> 5;
     const int r = min(row + (lane & 31), t.rows - 1);  // (rows past the last repeat it)
     const int tok = r / a.group, pos = t.kv - t.n + tok;
-    const int64_t at = (int64_t)(t.token0 + tok) * a.ldq + (kh * a.group + r % a.group) * HD + 8 * h;
+    const int64_t at = (int64_t)(t.token0 + tok) * a.ldq + (kh * a.group + r % a.group) * HD + (HALVES ? HD / 2 : 8) * h;
     w.hi[0] = min(pos, a.cap - 1);
     w.lo[0] = a.window ? pos - a.window + 1 : 0;
 #pragma unroll
     for (int k = 0; k < HD / 16; ++k) {
         if constexpr (F32) {
-            const float* src = static_cast<const float*>(a.q) + at + 16 * k;
+            const float* src = static_cast<const float*>(a.q) + at + (HALVES ? 8 : 16) * k;
             raw.v[k][0] = *reinterpret_cast<const float4*>(src);
             raw.v[k][1] = *reinterpret_cast<const float4*>(src + 4);
         } else {
-            w.q[0][k][0] = *reinterpret_cast<const h8_t*>(static_cast<const _Float16*>(a.q) + at + 16 * k);
+            w.q[0][k][0] = *reinterpret_cast<const h8_t*>(static_cast<const _Float16*>(a.q) + at + (HALVES ? 8 : 16) * k);
         }
     }
 }
@@ -679,59 +697,66 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* i
     return true;
 }
 
-// The waves' sums of an item (each in its own 128 HD bytes of LDS: 32 rows of HD values, pieces XORed with the row),
-// joined and written: to the output, or as the item's part. `begin`..`end`: the item's keys, of which wave i took every
-// fourth step of KEYS from begin + i KEYS on.
-template <int HD, bool F32, int KEYS>
+// The waves' sums of an item, joined and written: to the output, or as the item's part; PARTS of the row's dims
+// after each other, each wave's in its own 128 HD / PARTS bytes of LDS (32 rows, 16-byte pieces XORed with the row).
+// `begin`..`end`: the item's keys, of which wave i took every fourth step of KEYS from begin + i KEYS on.
+template <int HD, bool F32, int KEYS, int PARTS = 1>
 __device__ __forceinline__ void finish_few(const AttnArgs& a, const Tile& t, const Item& item, int kh, int begin, int end,
                                            int64_t part0, const Rows<HD, 1, F32>& w, char* lds) {
-    constexpr int TM = 32, HALF = 32 * HD * 2;
+    constexpr int TM = 32, ROW = HD / PARTS * 4, PCS = ROW / 16, X = PCS < 16 ? PCS - 1 : 15, BYTES = TM * ROW;
     __shared__ float2 sums[4][32];
     const bool whole = item.live <= 1;
     const int seq = item.seq, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    char* K = lds + wave * 2 * HALF;
+    char* K = lds + wave * BYTES;
     const int q = lane & 31, h = lane >> 5;
-#pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int piece = (32 * d + 8 * e + 4 * h) / 4;
-            *reinterpret_cast<float4*>(K + q * HD * 4 + (piece ^ (q & 15)) * 16) =
-                make_float4(w.o[0][d][4 * e], w.o[0][d][4 * e + 1], w.o[0][d][4 * e + 2], w.o[0][d][4 * e + 3]);
-        }
-    float l = swap32_sum(w.l[0]);
-    // (the wave's keys and what lies between: a row that sees one of those has its weight in another wave)
-    if (l == 0.f && sees_key(a, seq, max(w.lo[0], begin + wave * KEYS), min(w.hi[0], end - 1))) l = kNoWeight;
-    if (h == 0) sums[wave][q] = make_float2(w.m[0], l);
-    __syncthreads();
+    float l = 0.f;
     const int rows = min(t.rows - t.row0, TM);
-    if (a.info && kh == 0 && item.split == 0)
-        for (int u = threadIdx.x; u < rows; u += 256)
-            a.info[(int64_t)t.token0 * a.group + t.row0 + u] = make_int2(item.live, item.part << 5 | u);
-    for (int u = threadIdx.x; u < rows * (HD / 4); u += 256) {
-        const int row = u / (HD / 4), piece = u % (HD / 4);
-        float m = sums[0][row].x, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 1; i < 4; ++i) m = fmaxf(m, sums[i][row].x);
+    for (int p = 0; p < PARTS; ++p) {
+        if (p) __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 ml = sums[i][row];
-            const float f = part_weight(ml.x, ml.y, m);
-            const float4 x = *reinterpret_cast<const float4*>(lds + i * 2 * HALF + row * HD * 4 + (piece ^ (row & 15)) * 16);
-            sum = fmaf(f, ml.y, sum);
-            v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
+        for (int d = 0; d < HD / 32 / PARTS; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int piece = (32 * d + 8 * e + 4 * h) / 4, at = p * (HD / 32 / PARTS) + d;
+                *reinterpret_cast<float4*>(K + q * ROW + (piece ^ (q & X)) * 16) =
+                    make_float4(w.o[0][at][4 * e], w.o[0][at][4 * e + 1], w.o[0][at][4 * e + 2], w.o[0][at][4 * e + 3]);
+            }
+        if (p == 0) {
+            l = swap32_sum(w.l[0]);
+            // (the wave's keys and what lies between: a row that sees one of those has its weight in another wave)
+            if (l == 0.f && sees_key(a, seq, max(w.lo[0], begin + wave * KEYS), min(w.hi[0], end - 1))) l = kNoWeight;
+            if (h == 0) sums[wave][q] = make_float2(w.m[0], l);
         }
-        const int tok = (t.row0 + row) / a.group, head = kh * a.group + (t.row0 + row) % a.group;
-        const int64_t part = a.most ? ((int64_t)item.split * a.b.tokens + t.token0 + tok) * (a.group * a.c.kv_heads) + head
-                                    : part0 + row;
-        if (whole) {
-            const float inv = reciprocal(sum);
+        __syncthreads();
+        if (p == 0 && a.info && kh == 0 && item.split == 0)
+            for (int u = threadIdx.x; u < rows; u += 256)
+                a.info[(int64_t)t.token0 * a.group + t.row0 + u] = make_int2(item.live, item.part << 5 | u);
+        for (int u = threadIdx.x; u < rows * PCS; u += 256) {
+            const int row = u / PCS, piece = u % PCS;
+            float m = sums[0][row].x, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] *= inv;
-        } else if (piece == 0) {
-            a.ml[part] = make_float2(m, sum);
+            for (int i = 1; i < 4; ++i) m = fmaxf(m, sums[i][row].x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 ml = sums[i][row];
+                const float f = part_weight(ml.x, ml.y, m);
+                const float4 x = *reinterpret_cast<const float4*>(lds + i * BYTES + row * ROW + (piece ^ (row & X)) * 16);
+                sum = fmaf(f, ml.y, sum);
+                v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
+            }
+            const int tok = (t.row0 + row) / a.group, head = kh * a.group + (t.row0 + row) % a.group;
+            const int64_t part = a.most ? ((int64_t)item.split * a.b.tokens + t.token0 + tok) * (a.group * a.c.kv_heads) + head
+                                        : part0 + row;
+            if (whole) {
+                const float inv = reciprocal(sum);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] *= inv;
+            } else if (p == 0 && piece == 0) {
+                a.ml[part] = make_float2(m, sum);
+            }
+            put4(a, !F32, whole, part, t.token0 + tok, head, HD, p * (HD / PARTS) + 4 * piece, v);
         }
-        put4(a, !F32, whole, part, t.token0 + tok, head, HD, 4 * piece, v);
     }
 }
 

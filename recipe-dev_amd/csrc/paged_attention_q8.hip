@@ -1,17 +1,18 @@
 // Attention over 8-bit pages (rqmv_paged_attention_q8): the mathematics, tiles,
 // splits and joins of paged_attention.h, over codes and scales.
 //
-// Codes go from the pages into registers, 16 keys of one page at a time (one
-// scale), a step ahead, and from there to LDS as the fp16 numbers that they stand for,
-// which is exact (q8.h). From then on the kernels are those of fp16 pages, and
-// their rows have the bits that the same values in fp16 pages give where both take
-// the same form and splits.
+// Codes become the fp16 numbers that they stand for on their way to the matrix
+// cores, which is exact (q8.h); from then on the arithmetic is that of fp16 pages.
 #include "paged_attention.h"
 #include "q8.h"
 
 namespace rq {
 
 namespace {
+
+#ifndef Q8_ITEMS
+#define Q8_ITEMS 2
+#endif
 
 // How a wave takes 16 rows of codes: contiguous, 1024 bytes an instruction.
 template <int HD>
@@ -44,7 +45,7 @@ __device__ __forceinline__ void put16(const Keys16<HD>& from, char* lds) {
     typedef Lay<HD> L;
     typedef Lay8<HD> L8;
     const int lane = threadIdx.x & 63, c = lane % L8::PCS;
-    const uint32_t s = scale_pair(from.scale);
+    const Scale s = scale_of(__builtin_amdgcn_readfirstlane(from.scale));
 #pragma unroll
     for (int i = 0; i < L8::NI; ++i) {
         const int r = i * L8::RPI + lane / L8::PCS, x = VALUES ? L::vx(r) : L::kx(r);
@@ -60,20 +61,98 @@ struct Q8Values {
     const int8_t* v;
     const uint8_t* scale;
     __device__ __forceinline__ h4_t operator()(int64_t row, int dim) const {
-        uint32_t o[2];
-        bytes_to_h(*reinterpret_cast<const uint32_t*>(v + row * HD + dim), o[0], o[1]);
-        const hv2_t s = __builtin_bit_cast(hv2_t, scale_pair(scale[row >> 4]));
-        const hv2_t a = __builtin_bit_cast(hv2_t, o[0]) * s, b = __builtin_bit_cast(hv2_t, o[1]) * s;
+        const uint32_t c = *reinterpret_cast<const uint32_t*>(v + row * HD + dim);
+        const uint4 o = codes_to_h(make_uint2(c, 0), scale_of(scale[row >> 4]));
+        const hv2_t a = __builtin_bit_cast(hv2_t, o.x), b = __builtin_bit_cast(hv2_t, o.y);
         return h4_t{a[0], a[1], b[0], b[1]};
     }
 };
 
-// Few rows: four waves, each with every fourth step of 32 keys in LDS of its own; a step's codes are asked for as
-// soon as the registers of the step before are free.
+// ------------------------------------------- few rows: keys over the waves ----
+
+// Four waves take every fourth step of 32 keys, without barriers. A step's keys go from the pages into registers,
+// where they become operands of the first product without a detour: a lane takes half of a row's dims (h HD / 2 ..,
+// and the queries' operands hold theirs in that order). The values go straight to LDS as codes, two
+// buffers a wave, and are read transposed (ds_read_b64_tr_b8); the next step's keys and values are asked for
+// once the scores are done. Codes lie in LDS as rows of HD bytes, 16-byte pieces XORed so that a read of
+// two pieces of sixteen rows hits every bank alike.
+template <int HD>
+__device__ constexpr int code_xor(int row) {
+    return HD == 64 ? ((row >> 2) & 1) << 1 : HD == 128 ? ((row >> 1) & 3) << 1 : (row & 7) << 1;
+}
+
+// A lane's half of row lane % 32 of a step of 32 keys, and the row's scale byte.
+template <int HD>
+struct KeyHalf {
+    uint4 x[HD / 32];
+    unsigned scale;
+};
+template <int HD>
+__device__ __forceinline__ void fetch_keys(const PagedCodes& codes, const PagedCache& c, int kh, const int (&ids)[2], int key0,
+                                           KeyHalf<HD>& to) {
+    const int lane = threadIdx.x & 63, r = lane & 31;
+    const int id = r < 16 ? ids[0] : ids[1];
+    const int64_t row = (((int64_t)id * c.kv_heads + kh) << c.block_shift) + ((key0 + r) & ((1 << c.block_shift) - 1));
+    const uint4* from = reinterpret_cast<const uint4*>(codes.k + row * HD + (lane >> 5) * (HD / 2));
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) to.x[i] = from[i];
+    to.scale = codes.k_scale[row >> 4];
+}
+
+// S^T of 32 keys, as scores() of paged_attention.h leaves it, but for their scales' `more`.
 template <int HD, bool F32>
-__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_q8_few(AttnArgs a, PagedCodes codes) {
-    typedef Lay<HD> L;
-    constexpr int TM = 32, KEYS = 32, HALF = KEYS * HD * 2;  // HALF: bytes of a wave's K (and V) buffer
+__device__ __forceinline__ void scores_of_codes(const KeyHalf<HD>& keys, const Scale& scale, const Rows<HD, 1, F32>& w,
+                                                f16_t& s) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < HD / 16; ++k) {
+        const uint4 x = keys.x[k / 2];
+        const h8_t key = __builtin_bit_cast(h8_t, codes_to_low(k % 2 ? make_uint2(x.z, x.w) : make_uint2(x.x, x.y), scale));
+#pragma unroll
+        for (int p = 0; p < Rows<HD, 1, F32>::QP; ++p) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(key, w.q[0][k][p], s, 0, 0, 0);
+    }
+}
+
+// O^T += V^T P^T over a step's 32 keys, whose scale bytes are v_scale. (A scale above 2^5 is 2^5, as often as it takes.)
+template <int HD, bool F32>
+__device__ __forceinline__ void add_codes(const char* V, const unsigned (&v_scale)[2], Rows<HD, 1, F32>& w,
+                                          const h8_t (&p)[2][F32 ? 2 : 1]) {
+    typedef int i2_t __attribute__((ext_vector_type(2)));
+    typedef __attribute__((address_space(3))) i2_t lds2;
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    // 16 lanes read 16 dims of eight keys, two lanes a key: 4 h .. 4 h + 3 and 8 + 4 h ..
+    const int i = (lane & 15) >> 1, r = (i < 4 ? 0 : 4) + 4 * h + i;
+    const char* at = V + r * HD + (lane & 1) * 8;
+    i2_t x[2][HD / 32];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int d = 0; d < HD / 32; ++d)
+            x[b][d] = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                (lds2*)(at + 16 * b * HD + ((2 * d + ((lane >> 4) & 1)) ^ code_xor<HD>(r)) * 16));
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        const Scale scale = scale_of(v_scale[b]);
+        int again = 1 << scale.more;
+        do {
+#pragma unroll
+            for (int d = 0; d < HD / 32; ++d) {
+                const h8_t v = __builtin_bit_cast(h8_t, codes_to_low(make_uint2(x[b][d][0], x[b][d][1]), scale));
+#pragma unroll
+                for (int part = 0; part < (F32 ? 2 : 1); ++part)
+                    w.o[0][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p[b][part], w.o[0][d], 0, 0, 0);
+            }
+        } while (--again);
+    }
+}
+
+constexpr int q8_few_lds(int hd) { return 4 * 2 * 32 * hd; }
+constexpr int q8_few_wgs(int hd, bool f32) { return hd == 256 ? 1 : 2; }
+
+template <int HD, bool F32>
+__global__ void __launch_bounds__(256, q8_few_wgs(HD, F32)) paged_q8_few(AttnArgs a, PagedCodes codes) {
+    constexpr int TM = 32, KEYS = 32, STEP = KEYS * HD;  // STEP: bytes of a step's values
     extern __shared__ __align__(16) char lds[];
     const int kh = blockIdx.x % a.c.kv_heads;
     Item item;
@@ -86,48 +165,65 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_q8_few(AttnArgs 
     const Tile t = make_tile<TM>(a, seq, item.of, item.tile * TM);
     const int begin = item.first + item.split * item.chunk, end = min(begin + item.chunk, t.end);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    char* K = lds + wave * 2 * HALF;
-    char* V = K + HALF;
+    char* V = lds + wave * 2 * STEP;
+    const uint32_t v_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)V;
     Pages pages{a.b.table + seq * a.b.table_stride, a.b.max_blocks - 1, a.c.blocks, a.c.block_shift, INT_MIN / 2, 0};
     Rows<HD, 1, F32> w;
 
-    int id[2], next[2];
-    Keys16<HD> k[2], v[2];
-    auto look = [&](int key0, int (&ids)[2]) {  // the page ids of keys key0.. and key0 + 16..
+    KeyHalf<HD> keys;
+    unsigned v_scale[2], v_next[2];
+    unsigned bad = 0, bad_next = 0;  // which 16 keys of the step are in no page
+    int buffer = 0;
+    auto fetch = [&](int key0, int to) {
         const int p0 = key0 >> pages.shift, p1 = (key0 + 16) >> pages.shift;
         pages.need(p0, p1);
-        ids[0] = pages.at(p0);
-        ids[1] = pages.at(p1);
-    };
-    auto fetch = [&](const int8_t* from, const uint8_t* scales, int key0, const int (&ids)[2], Keys16<HD> (&to)[2]) {
+        int ids[2] = {pages.at(p0), pages.at(p1)};
+        bad_next = (pages.absent(ids[0]) ? 1 : 0) | (pages.absent(ids[1]) ? 2 : 0);
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
-            fetch16<HD>(from, scales, a.c, kh, pages.absent(ids[g]) ? 0 : ids[g], key0 + 16 * g, to[g]);
+        for (int g = 0; g < 2; ++g) {
+            if (pages.absent(ids[g])) ids[g] = 0;
+            const int key = key0 + 16 * g;
+            const int64_t row = (((int64_t)ids[g] * a.c.kv_heads + kh) << a.c.block_shift) + (key & ((1 << a.c.block_shift) - 1));
+            v_next[g] = codes.v_scale[row >> 4];
+#pragma unroll
+            for (int i = 0; i < Lay8<HD>::NI; ++i) {
+                const int r = i * Lay8<HD>::RPI + lane / Lay8<HD>::PCS;
+                const int piece = (lane % Lay8<HD>::PCS) ^ code_xor<HD>(r);
+                load_lds(codes.v + row * HD, (uint32_t)(r * HD + piece * 16), v_lds + to * STEP + g * 16 * HD + i * 1024);
+            }
+        }
+        fetch_keys<HD>(codes, a.c, kh, ids, key0, keys);
     };
     int key0 = begin + wave * KEYS;
     bool odd = false;
     if (key0 < end) pages.fetch(key0 >> pages.shift);
     RawRows<HD, F32> raw;
-    load_rows<HD, F32>(a, t, kh, t.row0, w, raw);
+    load_rows<HD, F32, true>(a, t, kh, t.row0, w, raw);
     arrived(w, raw);
-    if (key0 < end) {
-        look(key0, id);
-        fetch(codes.k, codes.k_scale, key0, id, k);
-        fetch(codes.v, codes.v_scale, key0, id, v);
-    }
+    if (key0 < end) fetch(key0, 0);
     start_rows(a, w, raw);
     while (key0 < end) {
         const int after = key0 + 4 * KEYS;
-        const bool more = after < end;
+        bad = bad_next;
+        wait_loads<0>();
+        const Scale scale = scale_of(keys.scale);
 #pragma unroll
-        for (int g = 0; g < 2; ++g) put16<HD, false>(k[g], K + g * 16 * L::ROW);
-        if (more) {
-            look(after, next);
-            fetch(codes.k, codes.k_scale, after, next, k);
-        }
+        for (int g = 0; g < 2; ++g) v_scale[g] = __builtin_amdgcn_readfirstlane(v_next[g]);
         f16_t s[1][1];
-        scores<HD, 1, 1, F32>(K, w, s);
-        const unsigned bad = (pages.absent(id[0]) ? 1 : 0) | (pages.absent(id[1]) ? 2 : 0);
+        scores_of_codes<HD, F32>(keys, scale, w, s[0][0]);
+        if (__any(scale.more)) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const float by = (float)(1 << __builtin_amdgcn_readlane(scale.more, 16 * g));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[0][0][8 * g + e] *= by;
+            }
+        }
+        if (after < end) {
+            // (the reads of the other buffer have returned: their products are behind)
+            asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(s[0][0]) : : "memory");
+            fetch(after, buffer ^ 1);
+        }
         const bool masked = key0 < t.all_from || key0 + KEYS > t.all_to || bad;
         if (masked) mask_scores<HD, 1, 1, F32>(w, s, key0, bad);
         float top[1];
@@ -135,24 +231,31 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) paged_q8_few(AttnArgs 
         move_references<HD, 1, F32>(w, top);
         h8_t p[1][2][F32 ? 2 : 1];
         weights<HD, 1, 1, F32>(w, s, p);
+        if (masked) {
+            // A NaN scale must not meet a weight of 0: groups that no row sees count as 0, and NaN groups too, which come
+            // to the rows that see them at the end (add_odd).
 #pragma unroll
-        for (int g = 0; g < 2; ++g) put16<HD, true>(v[g], V + g * 16 * L::ROW);
-        if (more) {
-            fetch(codes.v, codes.v_scale, after, next, v);
-            id[0] = next[0], id[1] = next[1];
+            for (int b = 0; b < 2; ++b) {
+                const bool dead = ((bad >> b) & 1) || key0 + 16 * b >= t.end, nan = v_scale[b] == kScaleNan;
+                odd |= nan && !dead;
+                if (dead || nan) v_scale[b] = 0;
+            }
         }
-        if (masked && __any(zero_dead<HD, KEYS>(V, key0, t.end, bad, lane, 64))) odd = true;
-        add_values<HD, 1, 1, F32>(V, w, p);
+        add_codes<HD, F32>(V + buffer * STEP, v_scale, w, p[0]);
+        buffer ^= 1;
         key0 = after;
     }
     if (odd) {  // (the wave's own steps; what unmasked ones let through is there already, and stays)
         for (int k0 = begin + wave * KEYS; k0 < end; k0 += 4 * KEYS)
             add_odd<HD, 1, F32>(a, t, kh, k0, min(k0 + KEYS, t.end), w, Q8Values<HD>{codes.v, codes.v_scale});
     }
-    finish_few<HD, F32, KEYS>(a, t, item, kh, begin, end, part0, w, lds);
+    finish_few<HD, F32, KEYS, 2>(a, t, item, kh, begin, end, part0, w, lds);
 }
 
-// Many rows: the waves share steps of 64 keys in two LDS buffers, one barrier a step. At a step's beginning the next
+// --------------------------------------------- many rows: rows over the waves ----
+
+// The waves share steps of 64 keys in two LDS buffers, one barrier a step. Codes go from the pages into registers, 16
+// keys of one page at a time (one scale), and from there to LDS as fp16. At a step's beginning the next
 // one's codes, which have been on their way for a step, go to the other buffer, and those after it are asked for.
 template <int HD, bool F32>
 __global__ void __launch_bounds__(64 * many_waves(HD), many_waves(HD) / 4) paged_q8_many(AttnArgs a, PagedCodes codes) {
@@ -242,7 +345,7 @@ template <int HD, bool F32>
 hipError_t launch_hd(const AttnPlan& p, const AttnArgs& a, const PagedCodes& codes, hipStream_t stream) {
     const void* f = p.few ? reinterpret_cast<const void*>(paged_q8_few<HD, F32>)
                           : reinterpret_cast<const void*>(paged_q8_many<HD, F32>);
-    const int lds = p.few ? few_lds(HD) : many_lds(HD);
+    const int lds = p.few ? q8_few_lds(HD) : many_lds(HD);
     if (lds > 48 * 1024) {
         const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
@@ -254,7 +357,7 @@ hipError_t launch_hd(const AttnPlan& p, const AttnArgs& a, const PagedCodes& cod
 
 AttnPlan plan_q8(const PagedBatch& b, const PagedCache& c, int q_heads, bool f32, int cus) {
     return plan_attention(b.tokens, b.seqs, (int64_t)b.max_blocks << c.block_shift, c.kv_heads, q_heads / c.kv_heads,
-                          c.head_dim, f32, cus);
+                          c.head_dim, f32, cus, Q8_ITEMS);
 }
 
 }  // namespace

@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(256) values_q8_kernel(PagedCodes codes, __half
     __half* to = blockIdx.y ? v : k;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
         const uint4 x = reinterpret_cast<const uint4*>(from)[i];
-        const uint32_t s = scale_pair(scale[i >> (row_shift + 4)]);
+        const Scale s = scale_of(scale[i >> (row_shift + 4)]);
         uint4* out = reinterpret_cast<uint4*>(to) + 2 * i;
         out[0] = codes_to_h(make_uint2(x.x, x.y), s);
         out[1] = codes_to_h(make_uint2(x.z, x.w), s);

@@ -326,7 +326,8 @@ class Case8(Case):
             self.codes[name], self.codes[name + "_scale"] = codes, scale
             setattr(self, name, ref.values_q8(codes, scale).astype(np.float16))
 
-    def check(self, gpu, scale=None, window=0, **kw):
+    def check(self, gpu, scale=None, window=0, adds=1, **kw):
+        """`adds`: how often a value is added (the few-rows form adds those of scales above 2^5 up to 16 times)."""
         got = self.run(gpu, scale, window, **kw)
         out, size = self.want(scale, window)
         live = int(self.q_start[-1])
@@ -341,7 +342,7 @@ class Case8(Case):
         if not self.f16:
             e = e + sc * q.max(-1, keepdims=True) * 2.0 ** -21 * kmax * self.hd
         n = max(self.kv_len, default=0)
-        sums = (n / 16 + 40) * 2.0 ** -24
+        sums = (n / 16 * adds + 40) * 2.0 ** -24
         bar = (np.expm1(2 * e) + (2.0 ** -11 if self.f16 else 2.0 ** -21) + sums) * size
         bar = bar + max(n, 0) * vmax * (2.0 ** -31 if self.f16 else 2.0 ** -40)
         if self.f16:
@@ -450,6 +451,22 @@ def test_masked_places_never_touch_the_result(gpu, nq, nkv, hd, new, ctx, f16):
         hurt[max(last // 16 * 16 - ctx, 0):new, rows] = True
         got = c.run(gpu)
         assert np.array_equal(got[~hurt], clean[~hurt]) and np.isnan(got[hurt]).all()
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("nq,nkv,hd,new,ctx", [(4, 2, 64, 1, 200), (4, 2, 128, 5, 219), (4, 2, 256, 3, 90),
+                                               (128, 2, 64, 270, 45), (128, 2, 128, 270, 45), (128, 2, 256, 270, 45)])
+def test_scales_from_the_smallest_to_the_largest(gpu, nq, nkv, hd, new, ctx, f16):
+    """Groups of keys and values of every size that a scale reaches, side by side."""
+    c = Case8([(new, ctx)], nq, nkv, hd, 16, f16, 12)
+    rng = np.random.default_rng(hd)
+    for x, lo in ((c.k, 0), (c.v, -20)):
+        size = np.exp2(rng.integers(lo, 14, (c.blocks, nkv, 1, 1)))
+        x[:] = np.clip(x.astype(np.float64) * size, -65000, 65000).astype(np.float16)
+    c.k[:, :, :, hd // 2:] = c.k[:, :, :, hd // 2:] * np.float16(0.25)
+    c.encode()
+    assert max(c.codes[n].max() for n in ("k_scale", "v_scale")) >= 134 and c.codes["v_scale"].min() < 110
+    c.check(gpu, scale=1e-5, adds=16)
 
 
 @pytest.mark.parametrize("f16", [False, True])
