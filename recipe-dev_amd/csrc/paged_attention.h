@@ -77,8 +77,7 @@ struct AttnPlan {
     int64_t tiles, parts;
 };
 
-// `per_cu`: few rows' items per CU over the whole batch.
-AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus, int per_cu);
+AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus);
 size_t attention_workspace_bytes(const AttnPlan& p, int tokens, int seqs, int group, int hd);
 // A call's arguments; where the plan has items, launches the count of them.
 hipError_t attention_args(const AttnPlan& p, const PagedBatch& b, const PagedCache& c, const void* q, int64_t ldq, int q_heads,
@@ -645,7 +644,9 @@ __device__ __forceinline__ unsigned long long both_counts(int items, int live) {
 // 1370 us, by every workgroup 4840; 512 sequences 95, 107).
 constexpr int kItemSeqs = 256;
 
-template <int TM>
+// LONG_FIRST (of at most kItemSeqs sequences): the last item of each tile, which is shorter than the others, comes after
+// all those; a CU that is done with its long ones then finds short ones to fill the rest.
+template <int TM, bool LONG_FIRST = false>
 __device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* item) {
     int tiles = 0, first = 0, keys = 0, chunk, live;
     if (a.items) {
@@ -672,14 +673,38 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* i
         if (lane == 0) totals[wave] = own_total;
         __syncthreads();
         const int items = seq_items<TM>(a, totals[0] + totals[1] + totals[2] + totals[3], tiles, keys, &chunk, &live);
-        const unsigned long long own = both_counts(items, live), upto = wave_scan(own);
-        if (lane == 63) upto_of[wave] = upto;
-        __syncthreads();
-        unsigned long long from = upto - own;
-        for (int w = 0; w < 3; ++w) from += w < wave ? upto_of[w] : 0;
-        const int at = number - (int)(unsigned)from;
-        if (at >= 0 && at < items)
-            found = Item{t, at / live, at % live, first, chunk * 64, live, (int)(from >> 32) + at, of};
+        if constexpr (LONG_FIRST) {
+            __shared__ unsigned parts_of[4];
+            // short items in the upper half, long ones in the lower
+            const unsigned long long own = (unsigned long long)(unsigned)tiles << 32 | (unsigned)(tiles * (live - 1));
+            const unsigned own_parts = live > 1 ? items : 0;
+            const unsigned long long upto = wave_scan(own);
+            const unsigned upto_parts = wave_scan(own_parts);
+            if (lane == 63) upto_of[wave] = upto, parts_of[wave] = upto_parts;
+            __syncthreads();
+            unsigned long long from = upto - own;
+            unsigned part = upto_parts - own_parts, longs = 0;
+            for (int w = 0; w < 4; ++w) {
+                from += w < wave ? upto_of[w] : 0;
+                part += w < wave ? parts_of[w] : 0;
+                longs += (unsigned)upto_of[w];
+            }
+            const bool is_long = (unsigned)number < longs;
+            const int at = is_long ? number - (int)(unsigned)from : number - (int)longs - (int)(from >> 32);
+            if (at >= 0 && at < (is_long ? tiles * (live - 1) : tiles)) {
+                const int tile = is_long ? at / (live - 1) : at, split = is_long ? at % (live - 1) : live - 1;
+                found = Item{t, tile, split, first, chunk * 64, live, (int)part + tile * live + split, of};
+            }
+        } else {
+            const unsigned long long own = both_counts(items, live), upto = wave_scan(own);
+            if (lane == 63) upto_of[wave] = upto;
+            __syncthreads();
+            unsigned long long from = upto - own;
+            for (int w = 0; w < 3; ++w) from += w < wave ? upto_of[w] : 0;
+            const int at = number - (int)(unsigned)from;
+            if (at >= 0 && at < items)
+                found = Item{t, at / live, at % live, first, chunk * 64, live, (int)(from >> 32) + at, of};
+        }
         __syncthreads();
         if (found.seq < 0) return false;
         *item = found;

@@ -10,7 +10,6 @@ namespace rq {
 
 namespace {
 
-constexpr int kItemsPerCu = 2;
 constexpr int64_t kEarlyBytes = int64_t(1) << 20;  // of parts that a join may ask for unseen
 
 // The 16 keys from `key` on of one page (id clamped into the cache) of `cache`, to LDS.
@@ -370,7 +369,7 @@ hipError_t launch_attention_hd(const AttnPlan& p, const AttnArgs& a, hipStream_t
 
 }  // namespace
 
-AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus, int per_cu) {
+AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus) {
     AttnPlan p;
     const int heads = kv_heads * group;
     // The few-rows form up to 128 rows a sequence and kv head on average, or where there are so few that
@@ -386,11 +385,11 @@ AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int gro
     p.few = (int64_t)tokens * group <= (int64_t)128 * seqs || (int64_t)tokens * heads / 32 <= few_tiles;
     p.items = p.few && seqs > kItemSeqs;
     if (p.few) {
-        // kItemsPerCu over the whole batch (32 requests of 60 to 8,192 positions, with the join: 39.1 us; one
+        // Two items per CU over the whole batch (32 requests of 60 to 8,192 positions, with the join: 39.1 us; one
         // per CU 41.2, four 41.3), of two steps for each wave at least (one request at 4,097: 12.4 us; of
         // one step 14.8, of four 14.6; the 32 requests with a window of 1,024 24.3, of four 20.3).
         p.min_chunk = 256;
-        const int64_t want = per_cu * cus / kv_heads, most = p.tiles * ((cap + p.min_chunk - 1) / p.min_chunk);
+        const int64_t want = 2 * cus / kv_heads, most = p.tiles * ((cap + p.min_chunk - 1) / p.min_chunk);
         p.splits = (int)(most < want ? most : want < 1 ? 1 : want);
         p.join = cap > p.min_chunk;
         p.parts = p.join ? (int64_t)2 * p.splits * kv_heads * 32 : 0;
@@ -440,7 +439,7 @@ size_t paged_attention_workspace(const PagedBatch& b, const PagedCache& c, int q
     const int64_t cap = (int64_t)b.max_blocks << c.block_shift;
     size_t most = 0;
     for (const bool f32 : {false, true}) {  // (one workspace serves both types)
-        const AttnPlan p = plan_attention(b.tokens, b.seqs, cap, c.kv_heads, group, c.head_dim, f32, cus, kItemsPerCu);
+        const AttnPlan p = plan_attention(b.tokens, b.seqs, cap, c.kv_heads, group, c.head_dim, f32, cus);
         const size_t bytes = attention_workspace_bytes(p, b.tokens, b.seqs, group, c.head_dim);
         most = bytes > most ? bytes : most;
     }
@@ -485,7 +484,7 @@ hipError_t launch_paged_attention(const PagedBatch& b, const PagedCache& c, cons
                                   int q_heads, float scale, int window, void* workspace, void* out, int64_t ldo, int cus,
                                   hipStream_t stream) {
     const AttnPlan p = plan_attention(b.tokens, b.seqs, (int64_t)b.max_blocks << c.block_shift, c.kv_heads,
-                                      q_heads / c.kv_heads, c.head_dim, f32, cus, kItemsPerCu);
+                                      q_heads / c.kv_heads, c.head_dim, f32, cus);
     AttnArgs a;
     const hipError_t e = attention_args(p, b, c, q, ldq, q_heads, scale, window, workspace, out, ldo, stream, &a);
     if (e != hipSuccess) return e;

@@ -10,10 +10,6 @@ namespace rq {
 
 namespace {
 
-#ifndef Q8_ITEMS
-#define Q8_ITEMS 2
-#endif
-
 // How a wave takes 16 rows of codes: contiguous, 1024 bytes an instruction.
 template <int HD>
 struct Lay8 {
@@ -156,7 +152,7 @@ __global__ void __launch_bounds__(256, q8_few_wgs(HD, F32)) paged_q8_few(AttnArg
     extern __shared__ __align__(16) char lds[];
     const int kh = blockIdx.x % a.c.kv_heads;
     Item item;
-    if (!find_item<TM>(a, blockIdx.x / a.c.kv_heads, &item)) return;
+    if (!find_item<TM, true>(a, blockIdx.x / a.c.kv_heads, &item)) return;
     // (starts out of order may count past what the workspace holds)
     const bool whole = item.live <= 1;
     const int64_t part0 = ((int64_t)item.part * a.c.kv_heads + kh) * TM;
@@ -357,7 +353,7 @@ hipError_t launch_hd(const AttnPlan& p, const AttnArgs& a, const PagedCodes& cod
 
 AttnPlan plan_q8(const PagedBatch& b, const PagedCache& c, int q_heads, bool f32, int cus) {
     return plan_attention(b.tokens, b.seqs, (int64_t)b.max_blocks << c.block_shift, c.kv_heads, q_heads / c.kv_heads,
-                          c.head_dim, f32, cus, Q8_ITEMS);
+                          c.head_dim, f32, cus);
 }
 
 }  // namespace
