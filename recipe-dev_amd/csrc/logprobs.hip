@@ -3,18 +3,18 @@
 //
 // With m the largest logit of a row, s = sum e^(x - m) and t = sum (x - m) e^(x - m):
 //     log p(i) = x_i - m - log s,      entropy = log s - t / s.
-// Rows are read once, in slices of 1024 R logits, a workgroup each, kept in
-// registers: (m, s, t) about the slice's own largest logit, and the slice's `top` largest
-// logits. A second launch joins a row's slices: s and t move to another reference m' by
+// Rows are read once, 256 R logits a wave, kept in its registers: (m, s, t) about its own largest
+// logit, and a list of at least its `top` largest ones. s and t move to another reference m' by
 //     s' = e^(m - m') s,   t' = e^(m - m') (t + (m - m') s).
-// A row of one slice is finished where it is read.
+// A row of up to 1024 R logits is finished by its workgroup; otherwise waves leave both in the workspace, on their
+// own, and a second launch joins a row's.
 //
-// The largest of a workgroup's logits: if `top` lanes of a wave have their own largest at or above T, what
-// lies below T is out. A wave finds its largest such T by bisection over its upper bits
-// (ballots), which may leave it a little low, and the workgroup takes the largest of its four. What
-// remains goes into a list in LDS and is ranked by comparing each with all (the
-// lowest index first among equals). Where many are equal a wave's share of the list overflows;
-// then it bisects for the exact top-th largest of all its logits and takes the equal ones by their index.
+// The largest of a wave's logits: if `top` of its lanes have their own largest at or above T, what lies below T is
+// out. The wave finds its largest such T by bisection over its upper bits (ballots), which may leave it
+// a little low, and lists what remains (some 1.2 to 1.4 times `top`). Where that is more than the list
+// holds (many equal logits), it bisects for the exact top-th largest, and for the indices of the equal ones that belong
+// to the first. At the end a workgroup takes the largest of its waves' T, and ranks
+// what remains by comparing each with all (the lowest index first among equals).
 //
 // Bound: HBM, at few rows the two launches and their dependent loads.
 #include "logprobs.h"
@@ -28,7 +28,7 @@ namespace rq {
 namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kList = 128;   // entries of a wave
+constexpr int kList = 64;    // entries of a wave
 constexpr int kSegment = 8;  // entries compared at once
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -106,72 +106,67 @@ __device__ __forceinline__ uint32_t wave_least(float lane_max, int top) {
     return T;
 }
 
-// The wave's values from `least` on into the workgroup's list; of more than kList the `top` first of the
-// wave (value descending, index ascending). `index(i)`: of v[i], ascending by (i / G, lane, i % G).
-template <int N, int G, typename F>
-__device__ __forceinline__ void wave_top(Shared& sh, const float (&v)[N], uint32_t least_key, int top, F index) {
-    const float least = of_key(max(least_key, kLowest));
-    auto base_of = [&](int count) {  // a place for `count` entries
-        int base = 0;
-        if ((threadIdx.x & 63) == 0) base = atomicAdd(&sh.count, count);
-        return __builtin_amdgcn_readfirstlane(base);
-    };
+// The wave's values from `least` on, or where these are more than kList the `top` first of the wave (value
+// descending, index ascending): put(place, value, index), places from base(count) on. index.of(i): v[i]'s,
+// index.below(i, x): whether it is below x.
+template <int N, typename F, typename B, typename P>
+__device__ __forceinline__ void wave_top(const float (&v)[N], uint32_t least_key, int top, const F& index, B base, P put) {
+    float least = of_key(max(least_key, kLowest));
     int count = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) count += __popcll(__ballot(v[i] >= least));
     if (count <= kList) {
-        int at = base_of(count);
+        int at = base(count);
+        asm volatile("" : "+v"(least));  // (the comparisons again, not N kept masks)
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const unsigned long long hits = __ballot(v[i] >= least);
             if (hits) {
-                if (v[i] >= least) sh.list[at + before(hits)] = Entry{v[i], index(i)};
+                if (v[i] >= least) put(at + before(hits), v[i], index.of(i));
                 at += __popcll(hits);
             }
         }
         return;
     }
-    // Too many: the exact border, then all above it and the first of those on it.
+    // the largest key that `top` values reach
     uint32_t V = 0;
 #pragma unroll 1
     for (int b = 31; b >= 0; --b) {
-        const uint32_t up = V | 1u << b;
+        const float up = of_key(V | 1u << b);  // (NaN beyond the infinities: no value reaches it)
         int c = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) c += __popcll(__ballot(key_of(v[i]) >= up));
-        if (c >= top) V = up;
+        for (int i = 0; i < N; ++i) c += __popcll(__ballot(v[i] >= up));
+        if (c >= top) V |= 1u << b;
     }
     const float border = of_key(max(V, kLowest));
-    const int at = base_of(top);
-    count = 0;
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) above += __popcll(__ballot(v[i] > border));
+    // of those on the border as many as there is room for: the ones below index X
+    int X = 0;
+#pragma unroll 1
+    for (int b = 20; b >= 0; --b) {
+        const int up = X | 1 << b;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) c += __popcll(__ballot(v[i] == border && index.below(i, up)));
+        if (above + c <= top) X = up;
+    }
+    int at = base(top);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const unsigned long long hits = __ballot(v[i] > border);
-        if (v[i] > border) sh.list[at + count + before(hits)] = Entry{v[i], index(i)};  // (fewer than `top`)
-        count += __popcll(hits);
-    }
-#pragma unroll
-    for (int r = 0; r < N / G; ++r) {
-        unsigned own = 0;
-#pragma unroll
-        for (int j = 0; j < G; ++j) own += v[G * r + j] == border ? 1 : 0;
-        const unsigned upto = wave_scan(own);
-        int k = count + (int)(upto - own);
-#pragma unroll
-        for (int j = 0; j < G; ++j)
-            if (v[G * r + j] == border) {
-                if (k < top) sh.list[at + k] = Entry{border, index(G * r + j)};
-                ++k;
-            }
-        count = min(count + __builtin_amdgcn_readlane((int)upto, 63), top);
+        const bool take = v[i] > border || (v[i] == border && index.below(i, X));
+        const unsigned long long hits = __ballot(take);
+        if (take) put(at + before(hits), v[i], index.of(i));
+        at += __popcll(hits);
     }
 }
 
 // The `top` first of the workgroup's values in order, in sh.best ((-infinity, -1) past the last). The waves agree on the
 // largest of their `least`s, each of which has `top` values above it; then every entry of the list is compared with
 // all, its share of them by one of two threads while there are at most 128.
-template <int N, int G, typename F>
-__device__ __forceinline__ void group_top(Shared& sh, const float (&v)[N], float lane_max, int top, F index) {
+template <int N, typename F>
+__device__ __forceinline__ void group_top(Shared& sh, const float (&v)[N], float lane_max, int top, const F& index) {
     const uint32_t mine = wave_least(lane_max, top);
     if ((threadIdx.x & 63) == 0) sh.least[threadIdx.x >> 6] = mine;
     if (threadIdx.x == 0) sh.count = 0;
@@ -180,7 +175,14 @@ __device__ __forceinline__ void group_top(Shared& sh, const float (&v)[N], float
     uint32_t least = sh.least[0];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) least = max(least, sh.least[w]);
-    wave_top<N, G>(sh, v, least, top, index);
+    wave_top(
+        v, least, top, index,
+        [&](int count) {  // (a place in the workgroup's list)
+            int base = 0;
+            if ((threadIdx.x & 63) == 0) base = atomicAdd(&sh.count, count);
+            return __builtin_amdgcn_readfirstlane(base);
+        },
+        [&](int at, float x, int i) { sh.list[at] = Entry{x, i}; });
     __syncthreads();
     const int count = sh.count;
     // past the last: entries that are before none
@@ -227,8 +229,16 @@ __device__ __forceinline__ float log_prob(float x, const Stats& a, float log_s) 
     return x == a.m ? -log_s : (x - a.m) - log_s;
 }
 
+// The logit of the row's token, asked for before it is needed (thread kGiven has it).
+constexpr int kGiven = 128;
+__device__ __forceinline__ float given_logit(const LogprobArgs& a, int64_t row) {
+    if (threadIdx.x != kGiven || !a.logprob) return -INFINITY;
+    const int token = a.tokens[row];
+    return (unsigned)token < (unsigned)a.n ? a.logits[row * a.ld + token] : -INFINITY;
+}
+
 // A row's outputs from its stats, sh.best and the token's logit.
-__device__ __forceinline__ void put_row(const LogprobArgs& a, int64_t row, const Stats& st, const Shared& sh) {
+__device__ __forceinline__ void put_row(const LogprobArgs& a, int64_t row, const Stats& st, const Shared& sh, float given) {
     const int t = threadIdx.x;
     const float log_s = st.m > -INFINITY ? logf(st.s) : 0.f;
     if (t < a.top) {
@@ -237,125 +247,196 @@ __device__ __forceinline__ void put_row(const LogprobArgs& a, int64_t row, const
         if (a.top_logprobs) a.top_logprobs[row * a.top + t] = log_prob(e.v, st, log_s);
     } else if (t == 64) {
         if (a.entropy) a.entropy[row] = st.m > -INFINITY ? log_s - st.t / st.s : 0.f;
-    } else if (t == 128 && a.logprob) {
-        const int token = a.tokens[row];
-        a.logprob[row] = log_prob((unsigned)token < (unsigned)a.n ? a.logits[row * a.ld + token] : -INFINITY, st, log_s);
+    } else if (t == kGiven) {
+        if (a.logprob) a.logprob[row] = log_prob(given, st, log_s);
     }
 }
 
-// A slice of 1024 R logits: to the outputs where the row has no other (parts null), or to the workspace.
+// The indices of a wave's logits from c0 on, as load_logits puts them into its registers.
+struct SliceIndex {
+    int c0;
+    __device__ __forceinline__ int of(int i) const { return c0 + 256 * (i / 4) + i % 4 + 4 * (int)(threadIdx.x & 63); }
+    __device__ __forceinline__ bool below(int i, int x) const {
+        return 4 * (int)(threadIdx.x & 63) < x - (c0 + 256 * (i / 4) + i % 4);
+    }
+};
+
+// A wave's 256 R logits from c0 on, NaNs as -infinity and -0 as 0, and the lane's largest. (16 bytes a lane, aligned to 4
+// or more.)
+template <int R>
+__device__ __forceinline__ float load_logits(const LogprobArgs& a, int64_t row, int c0, float (&v)[4 * R]) {
+    const int lane = threadIdx.x & 63;
+    const float* x = a.logits + row * a.ld + c0 + 4 * lane;
+    if (c0 + 256 * R <= a.n) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * r + j] = x[256 * r + j];
+    } else {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * r + j] = c0 + 256 * r + 4 * lane + j < a.n ? x[256 * r + j] : -INFINITY;
+    }
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4 * R; ++i) {
+        v[i] = v[i] == v[i] ? v[i] + 0.f : -INFINITY;
+        most = fmaxf(most, v[i]);
+    }
+    return most;
+}
+
+// Rows of at most 1024 R logits.
 template <int R, bool TOP>
-__global__ void __launch_bounds__(kThreads) logprobs_slice_kernel(LogprobArgs a, float4* parts, Entry* tops) {
+__global__ void __launch_bounds__(kThreads) logprobs_row_kernel(LogprobArgs a) {
     __shared__ Shared sh;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c0 = (blockIdx.x * kWaves + wave) * 256 * R;
-    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
-        const float* x = a.logits + row * a.ld + c0 + 4 * lane;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = wave * 256 * R;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const float given = given_logit(a, row);
         float v[4 * R];
-        if (c0 + 256 * R <= a.n) {
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[4 * r + j] = x[256 * r + j];  // (16 bytes a lane, aligned to 4 or more)
-        } else {
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    v[4 * r + j] = c0 + 256 * r + 4 * lane + j < a.n ? x[256 * r + j] : -INFINITY;
-        }
-        float top1 = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4 * R; ++i) {
-            v[i] = v[i] == v[i] ? v[i] + 0.f : -INFINITY;  // (NaNs are skipped; -0 is 0)
-            top1 = fmaxf(top1, v[i]);
-        }
-        const Stats st = wave_stats(v, all_max(top1));
+        const float most = load_logits<R>(a, row, c0, v);
+        const Stats st = wave_stats(v, all_max(most));
         if (lane == 0) sh.stats[wave] = st;
-        if (TOP)
-            group_top<4 * R, 4>(sh, v, top1, a.top, [&](int i) { return c0 + 256 * (i / 4) + 4 * lane + i % 4; });
+        if (TOP) group_top(sh, v, most, a.top, SliceIndex{c0});
         __syncthreads();
-        const Stats all = group_stats(sh);
-        if (!parts) {
-            put_row(a, row, all, sh);
-        } else {
-            const int64_t at = row * gridDim.x + blockIdx.x;
-            if (threadIdx.x == 0) parts[at] = make_float4(all.m, all.s, all.t, 0.f);
-            if (TOP && (int)threadIdx.x < a.top) tops[at * a.top + threadIdx.x] = sh.best[threadIdx.x];
-        }
+        put_row(a, row, group_stats(sh), sh, given);
         __syncthreads();
     }
 }
 
-// A row's slices (at most 256), and their lists of `top` entries: at most 64 N kWaves.
-template <int N>
-__global__ void __launch_bounds__(kThreads) logprobs_join_kernel(LogprobArgs a, const float4* parts, const Entry* tops,
-                                                                 int slices) {
-    __shared__ Shared sh;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        Stats st{-INFINITY, 0.f, 0.f};
-        if ((int)threadIdx.x < slices) {
-            const float4 p = parts[row * slices + threadIdx.x];
-            st = Stats{p.x, p.y, p.z};
+// What the waves leave of longer rows: of each (m, s, t, entries in its list), and the lists, [row][place][wave].
+struct Parts {
+    float4* stats;
+    Entry* lists;
+    int slices;  // waves of a row
+};
+
+template <int R, bool TOP>
+__global__ void __launch_bounds__(kThreads) logprobs_slice_kernel(LogprobArgs a, Parts parts) {
+    const int lane = threadIdx.x & 63;
+    const int slice = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = slice * 256 * R;
+    if (slice >= parts.slices) return;
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        float v[4 * R];
+        const float most = load_logits<R>(a, row, c0, v);
+        const Stats st = wave_stats(v, all_max(most));
+        int listed = 0;
+        if (TOP) {
+            Entry* list = parts.lists + row * kList * parts.slices + slice;
+            wave_top(
+                v, wave_least(most, a.top), a.top, SliceIndex{c0}, [&](int count) { return listed = count, 0; },
+                [&](int at, float x, int i) { list[at * parts.slices] = Entry{x, i}; });
         }
+        if (lane == 0) parts.stats[row * parts.slices + slice] = make_float4(st.m, st.s, st.t, __builtin_bit_cast(float, listed));
+    }
+}
+
+// The waves of a row, at most SLOTS (64, 128 or 256) of them. A thread has every (256 / SLOTS)-th place of one wave's
+// list; the first half of the places is asked for before it is known which are taken.
+template <int SLOTS>
+__global__ void __launch_bounds__(kThreads) logprobs_join_kernel(LogprobArgs a, Parts parts) {
+    constexpr int SIDE = kThreads / SLOTS, N = kList / SIDE;
+    __shared__ Shared sh;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slices = parts.slices;
+    const int slice = threadIdx.x % SLOTS, side = threadIdx.x / SLOTS;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const float given = given_logit(a, row);
+        float4 p = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+        if (slice < slices) p = parts.stats[row * slices + slice];
+        const Entry* list = parts.lists + row * kList * slices + min(slice, slices - 1);
+        Entry e[N];
+        if (a.top) {
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i) e[i] = list[(i * SIDE + side) * slices];
+        }
+        const int listed = __builtin_bit_cast(int, p.w);
+        Stats st = side == 0 ? Stats{p.x, p.y, p.z} : Stats{-INFINITY, 0.f, 0.f};
         const float m = all_max(st.m);
         st = move(st, m);
         st.s = all_sum(st.s);
         st.t = all_sum(st.t);
         if (lane == 0) sh.stats[wave] = st;
         if (a.top) {
-            // entry 256 i + thread is v[i]: a lane's are of unlike lists, and equal values stand in the order of their indices
-            const int all = slices * a.top;
-            float v[N], top1 = -INFINITY;
-            int id[N];
+            struct Ids {
+                int id[N];
+                __device__ __forceinline__ int of(int i) const { return id[i]; }
+                __device__ __forceinline__ bool below(int i, int x) const { return id[i] < x; }
+            } ids;
+            float v[N], most = -INFINITY;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int e = kThreads * i + threadIdx.x;
-                const Entry o = e < all ? tops[row * all + e] : Entry{-INFINITY, -1};
-                v[i] = o.v, id[i] = o.i;
-                top1 = fmaxf(top1, v[i]);
+                const bool taken = i * SIDE + side < listed;
+                if (i >= N / 2) {
+                    e[i] = Entry{-INFINITY, -1};
+                    if (taken) e[i] = list[(i * SIDE + side) * slices];
+                }
+                v[i] = taken ? e[i].v : -INFINITY;
+                ids.id[i] = e[i].i;
+                most = fmaxf(most, v[i]);
             }
-            group_top<N, 1>(sh, v, top1, a.top, [&](int i) { return id[i]; });
+            group_top(sh, v, most, a.top, ids);
         }
         __syncthreads();
-        put_row(a, row, group_stats(sh), sh);
+        put_row(a, row, group_stats(sh), sh, given);
         __syncthreads();
     }
 }
 
 struct LogprobPlan {
-    int r, slices;
+    int r;
+    bool whole;  // a row by its workgroup
+    Parts parts;
 };
-LogprobPlan plan_logprobs(int rows, int n, int cus) {
-    // Slices of 16,384 logits where that gives two workgroups a CU, else of 4,096.
-    const int64_t large = (n + 16383) / 16384;
-    const int r = large * rows >= 2 * cus ? 16 : 4;
-    return LogprobPlan{r, (n + 1024 * r - 1) / (1024 * r)};
+LogprobPlan plan_logprobs(int rows, int n, int top, int cus) {
+    // Long slices where these are enough for two workgroups a CU: 4096 logits a wave, with lists 2048 (1500 rows of
+    // 128,256, twenty alternatives: 202 us, of 4096 246, of 1024 205); else 1024. A row is 256 waves' at most.
+    const bool many = (int64_t)((n + 16383) / 16384) * rows >= 2 * cus;
+    int r = !many ? 4 : top ? 8 : 16;
+    while (n > 256 * r * kThreads) r *= 2;
+    LogprobPlan p;
+    p.r = r;
+    p.whole = n <= 1024 * r;
+    p.parts.slices = (n + 256 * r - 1) / (256 * r);
+    return p;
+}
+
+template <int R, bool TOP>
+void launch_slices(const LogprobArgs& a, const LogprobPlan& p, hipStream_t stream) {
+    if (p.whole) {
+        hipLaunchKernelGGL((logprobs_row_kernel<R, TOP>), dim3(a.rows), dim3(kThreads), 0, stream, a);
+    } else {
+        const dim3 grid((p.parts.slices + kWaves - 1) / kWaves, a.rows < 65535 ? a.rows : 65535);
+        hipLaunchKernelGGL((logprobs_slice_kernel<R, TOP>), grid, dim3(kThreads), 0, stream, a, p.parts);
+    }
 }
 
 }  // namespace
 
 size_t logprobs_workspace(int rows, int n, int top, int cus) {
-    const LogprobPlan p = plan_logprobs(rows, n, cus);
-    return p.slices > 1 ? (size_t)rows * p.slices * (sizeof(float4) + top * sizeof(Entry)) : 0;
+    const LogprobPlan p = plan_logprobs(rows, n, top, cus);
+    return p.whole ? 0 : (size_t)rows * p.parts.slices * (sizeof(float4) + (top ? kList * sizeof(Entry) : 0));
 }
 
 hipError_t launch_logprobs(const LogprobArgs& a, void* workspace, int cus, hipStream_t stream) {
-    const LogprobPlan p = plan_logprobs(a.rows, a.n, cus);
-    float4* parts = p.slices > 1 ? static_cast<float4*>(workspace) : nullptr;
-    Entry* tops = p.slices > 1 ? reinterpret_cast<Entry*>(parts + (int64_t)a.rows * p.slices) : nullptr;
-    const dim3 grid(p.slices, a.rows < 65535 ? a.rows : 65535), threads(kThreads);
-    if (p.r == 16 && a.top) hipLaunchKernelGGL((logprobs_slice_kernel<16, true>), grid, threads, 0, stream, a, parts, tops);
-    else if (p.r == 16) hipLaunchKernelGGL((logprobs_slice_kernel<16, false>), grid, threads, 0, stream, a, parts, tops);
-    else if (a.top) hipLaunchKernelGGL((logprobs_slice_kernel<4, true>), grid, threads, 0, stream, a, parts, tops);
-    else hipLaunchKernelGGL((logprobs_slice_kernel<4, false>), grid, threads, 0, stream, a, parts, tops);
+    LogprobPlan p = plan_logprobs(a.rows, a.n, a.top, cus);
+    p.parts.stats = static_cast<float4*>(workspace);
+    p.parts.lists = reinterpret_cast<Entry*>(p.parts.stats + (int64_t)a.rows * p.parts.slices);
+    if (a.top) {
+        if (p.r == 4) launch_slices<4, true>(a, p, stream);
+        else if (p.r == 8) launch_slices<8, true>(a, p, stream);
+        else launch_slices<16, true>(a, p, stream);
+    } else {
+        if (p.r == 4) launch_slices<4, false>(a, p, stream);
+        else if (p.r == 8) launch_slices<8, false>(a, p, stream);
+        else launch_slices<16, false>(a, p, stream);
+    }
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.slices == 1) return e;
-    const dim3 rows(a.rows < (1 << 20) ? a.rows : 1 << 20);
-    const int entries = p.slices * a.top;
-    if (entries <= 1024) hipLaunchKernelGGL(logprobs_join_kernel<4>, rows, threads, 0, stream, a, parts, tops, p.slices);
-    else hipLaunchKernelGGL(logprobs_join_kernel<32>, rows, threads, 0, stream, a, parts, tops, p.slices);
+    if (e != hipSuccess || p.whole) return e;
+    const dim3 rows(a.rows), threads(kThreads);
+    if (p.parts.slices <= 64) hipLaunchKernelGGL(logprobs_join_kernel<64>, rows, threads, 0, stream, a, p.parts);
+    else if (p.parts.slices <= 128) hipLaunchKernelGGL(logprobs_join_kernel<128>, rows, threads, 0, stream, a, p.parts);
+    else hipLaunchKernelGGL(logprobs_join_kernel<256>, rows, threads, 0, stream, a, p.parts);
     return hipGetLastError();
 }
 
