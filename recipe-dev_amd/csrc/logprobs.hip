@@ -262,7 +262,7 @@ struct SliceIndex {
 };
 
 // A wave's 256 R logits from c0 on, NaNs as -infinity and -0 as 0, and the lane's largest. (16 bytes a lane, aligned to 4
-// or more.)
+// or more; read once, so not kept in the caches: 1500 rows of 128,256 without alternatives 121 us, otherwise 134.)
 template <int R>
 __device__ __forceinline__ float load_logits(const LogprobArgs& a, int64_t row, int c0, float (&v)[4 * R]) {
     const int lane = threadIdx.x & 63;
@@ -271,7 +271,7 @@ __device__ __forceinline__ float load_logits(const LogprobArgs& a, int64_t row, 
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * r + j] = x[256 * r + j];
+            for (int j = 0; j < 4; ++j) v[4 * r + j] = __builtin_nontemporal_load(x + 256 * r + j);
     } else {
 #pragma unroll
         for (int r = 0; r < R; ++r)

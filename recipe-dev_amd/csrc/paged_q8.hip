@@ -20,17 +20,35 @@ namespace rq {
 // rest was made faster.)
 //
 // A run's sixteen rows are shared by four waves, which join their exponents through LDS. Runs are looked for among the
-// WINDOW rows that a workgroup has; workgroups of runs come before those of queries (mixed, they
+// window of rows that a workgroup has; workgroups of runs come before those of queries (mixed, they
 // wait for each other's loads: 85 us).
 //
-// Bound: at prefill HBM (4000 rows of 32/8 heads of 128, fp32 to fp16: 31.5 us, 4.4 TB/s; the form over fp16 pages
-// 30.7 for 4096), at decode the chain of loads slots -> rows -> codes (24 requests: 4.1 us).
+// Bound: at prefill HBM (4000 rows of 32/8 heads of 128, fp32 to fp16: 28.3 us, 4.9 TB/s; the form over fp16 pages
+// 30.7 for 4096), at decode the chain of loads slots -> rows -> codes (24 requests: 4.3 us).
 constexpr int kWaves = 4;
+
+// Queries and the values of pages pass by the caches (4000 rows, 32/8 heads of 128, with the values: 38.2 us, so 33.3).
+typedef uint32_t nt2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t nt4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void stream4(float* p, const float* v) {
+    __builtin_nontemporal_store(nt4_t{__builtin_bit_cast(uint32_t, v[0]), __builtin_bit_cast(uint32_t, v[1]),
+                                      __builtin_bit_cast(uint32_t, v[2]), __builtin_bit_cast(uint32_t, v[3])},
+                                reinterpret_cast<nt4_t*>(p));
+}
+__device__ __forceinline__ void stream4(__half* p, const float* v) {
+    __builtin_nontemporal_store(nt2_t{__builtin_bit_cast(uint32_t, __floats2half2_rn(v[0], v[1])),
+                                      __builtin_bit_cast(uint32_t, __floats2half2_rn(v[2], v[3]))},
+                                reinterpret_cast<nt2_t*>(p));
+}
+__device__ __forceinline__ void stream4(uint4* p, uint4 v) {
+    __builtin_nontemporal_store(nt4_t{v.x, v.y, v.z, v.w}, reinterpret_cast<nt4_t*>(p));
+}
+
 constexpr int kRunRows = 32;  // rows that a run's rows lie within
-// Windows of 16 rows where a call has many (4000 rows of prompts, 32/8 heads of 128: 31.5 us, of 4 rows 38), of 4 for
-// few, whose runs are short and would wait for each other (300 decoding requests, with the values' launch: 18.7 us, of 16
-// rows 34.2; one prompt of 300 9.0 and 8.8; 1000 requests 51.9 and 56.3, a prompt of 1000 15.0 and 13.3).
-constexpr int kFewRows = 512;
+// Windows of 16 rows where a call has many (a prompt's 1000 rows of 32/8 heads of 128, with the values: 13.3 us, of 4 rows
+// 15.0; 4000 rows 38 and 45), of 4 for some, whose runs are short and would wait for each other (300 requests 18.7, of 16
+// rows 34.2), of one for few (24 requests 8.7, of 4 rows 10.4; but a prompt of 128 takes 10.7 so, of 4 rows 8.6).
+constexpr int kFewRows = 64, kSomeRows = 512;
 
 // The slots around a window: of rows base - 31 .. base + 32 (`a`) and the sixteen after these (`b`); -1: none.
 struct Slots {
@@ -169,10 +187,11 @@ __device__ __forceinline__ void store_run(const PagedBatch& b, const PagedCache&
     }
 }
 
-// Workgroups y < kv_groups take runs (by number: item by item, for each the windows of WINDOW rows), the others queries.
-template <int HD, int WINDOW, typename X, typename Q>
+// Workgroups y < kv_groups take runs (by number: item by item, for each the windows of `few` or 16 rows), the others queries.
+template <int HD, bool MANY, typename X, typename Q>
 __global__ void __launch_bounds__(64 * kWaves) qk_q8_kernel(PagedBatch b, PagedCache c, PagedCodes codes, QkNormRope p,
-                                                            int kv_groups) {
+                                                            int kv_groups, int few) {
+    const int window = MANY ? 16 : few;
     constexpr int LPH = HD / 8, HPB = 64 * kWaves / LPH;  // lanes per head, heads per workgroup
     auto load8 = [&](int t, int head, HeadPlace at, float (&x)[8]) {
         const X* src = static_cast<const X*>(p.qkv) + (int64_t)t * p.ld + head * HD;
@@ -182,8 +201,8 @@ __global__ void __launch_bounds__(64 * kWaves) qk_q8_kernel(PagedBatch b, PagedC
     if ((int)blockIdx.y < kv_groups) {
         __shared__ float exponents[2][kWaves];
         const int64_t number = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-        const int windows = (b.tokens - 1) / WINDOW + 1, item = (int)(number / windows);
-        const int base = (int)(number % windows) * WINDOW, lane = threadIdx.x & 63;
+        const int windows = (b.tokens - 1) / window + 1, item = (int)(number / windows);
+        const int base = (int)(number % windows) * window, lane = threadIdx.x & 63;
         if (item >= 2 * c.kv_heads) return;
         const int64_t size = (int64_t)c.blocks << c.block_shift;
         auto slot_of = [&](int row) {
@@ -199,7 +218,7 @@ __global__ void __launch_bounds__(64 * kWaves) qk_q8_kernel(PagedBatch b, PagedC
         // (a row of the group of the row before it starts no run)
         const int before = __shfl_up(slots.a, 1);
         unsigned long long starts = __ballot(slots.a >= 0 && (before < 0 || (before >> 4) != (slots.a >> 4))) >> (kRunRows - 1);
-        starts &= (1ull << WINDOW) - 1;
+        starts &= (1ull << window) - 1;
         int turn = 0;
         for (; starts; starts &= starts - 1) {
             const int at = __builtin_ctzll(starts);
@@ -220,31 +239,29 @@ __global__ void __launch_bounds__(64 * kWaves) qk_q8_kernel(PagedBatch b, PagedC
     if (at.turns) load_turn(p, b.positions[token], u, h);
     norm_and_turn<HD>(p.q_norm, at.turns, p.eps, h, x);
     Q* dst = static_cast<Q*>(p.q_out) + (int64_t)token * p.ldq + head * HD;
-    store4(dst + at.lo, x);
-    store4(dst + at.hi, x + 4);
+    stream4(dst + at.lo, x);
+    stream4(dst + at.hi, x + 4);
 }
 
-template <int HD, int WINDOW, typename X>
+template <int HD, typename X>
 static void launch_x(const PagedBatch& b, const PagedCache& c, const PagedCodes& codes, const QkNormRope& p, bool q_f16,
                      hipStream_t stream) {
     constexpr int HPB = 64 * kWaves / (HD / 8);
-    const int64_t runs = (int64_t)((b.tokens - 1) / WINDOW + 1) * 2 * c.kv_heads;
+    const bool many = b.tokens > kSomeRows;
+    const int few = b.tokens <= kFewRows ? 1 : 4, window = many ? 16 : few;
+    const int64_t runs = (int64_t)((b.tokens - 1) / window + 1) * 2 * c.kv_heads;
     const int kv_groups = (int)((runs - 1) / b.tokens + 1);
     const dim3 grid(b.tokens, kv_groups + (p.q_heads + HPB - 1) / HPB), threads(64 * kWaves);
-    if (q_f16) hipLaunchKernelGGL((qk_q8_kernel<HD, WINDOW, X, __half>), grid, threads, 0, stream, b, c, codes, p, kv_groups);
-    else hipLaunchKernelGGL((qk_q8_kernel<HD, WINDOW, X, float>), grid, threads, 0, stream, b, c, codes, p, kv_groups);
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, threads, 0, stream, b, c, codes, p, kv_groups, few); };
+    if (many) q_f16 ? launch(qk_q8_kernel<HD, true, X, __half>) : launch(qk_q8_kernel<HD, true, X, float>);
+    else q_f16 ? launch(qk_q8_kernel<HD, false, X, __half>) : launch(qk_q8_kernel<HD, false, X, float>);
 }
 
 template <int HD>
 static void launch_hd(const PagedBatch& b, const PagedCache& c, const PagedCodes& codes, const QkNormRope& p, bool x_f16,
                       bool q_f16, hipStream_t stream) {
-    if (b.tokens <= kFewRows) {
-        if (x_f16) launch_x<HD, 4, __half>(b, c, codes, p, q_f16, stream);
-        else launch_x<HD, 4, float>(b, c, codes, p, q_f16, stream);
-    } else {
-        if (x_f16) launch_x<HD, 16, __half>(b, c, codes, p, q_f16, stream);
-        else launch_x<HD, 16, float>(b, c, codes, p, q_f16, stream);
-    }
+    if (x_f16) launch_x<HD, __half>(b, c, codes, p, q_f16, stream);
+    else launch_x<HD, float>(b, c, codes, p, q_f16, stream);
 }
 
 hipError_t launch_qk_norm_rope_q8(const PagedBatch& b, const PagedCache& c, const PagedCodes& codes, const QkNormRope& p,
@@ -267,8 +284,8 @@ __global__ void __launch_bounds__(256) values_q8_kernel(PagedCodes codes, __half
         const uint4 x = reinterpret_cast<const uint4*>(from)[i];
         const Scale s = scale_of(scale[i >> (row_shift + 4)]);
         uint4* out = reinterpret_cast<uint4*>(to) + 2 * i;
-        out[0] = codes_to_h(make_uint2(x.x, x.y), s);
-        out[1] = codes_to_h(make_uint2(x.z, x.w), s);
+        stream4(out, codes_to_h(make_uint2(x.x, x.y), s));
+        stream4(out + 1, codes_to_h(make_uint2(x.z, x.w), s));
     }
 }
 
