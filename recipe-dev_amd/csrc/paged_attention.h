@@ -77,7 +77,9 @@ struct AttnPlan {
     int64_t tiles, parts;
 };
 
-AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus);
+// `few_tiles`: tiles of 32 rows over all heads up to which few rows are assumed.
+AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus,
+                        int64_t few_tiles);
 size_t attention_workspace_bytes(const AttnPlan& p, int tokens, int seqs, int group, int hd);
 // A call's arguments; where the plan has items, launches the count of them.
 hipError_t attention_args(const AttnPlan& p, const PagedBatch& b, const PagedCache& c, const void* q, int64_t ldq, int q_heads,

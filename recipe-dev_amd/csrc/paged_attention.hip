@@ -367,21 +367,27 @@ hipError_t launch_attention_hd(const AttnPlan& p, const AttnArgs& a, hipStream_t
     return join_hd<HD, F32>(p, a, stream);
 }
 
+// Tiles of 32 rows over all heads up to which few rows are assumed: 4 a CU (64 and 256 dims, fp16),
+// 2 (128 dims; 64, fp32) or a half (256, fp32, whose large tiles have 128 rows). Over 222
+// batches of 1 to 16 sequences, 64 to 1024 new tokens and 0 to 6,000 cached ones the choice takes 0.5 to
+// 4.5 % more than the better form; at 256 dims of fp16 11 % over 131 batches. Few against many, 32/8 heads of 128,
+// fp16, us: 32 sequences of 128 rows over 6,000 positions 238 / 341, of 256 398 / 350; one of 1024 rows over 1,000
+// 23 / 27; four of 2048 over 6,000 350 / 221.
+int64_t few_tiles(int hd, bool f32, int cus) {
+    return hd == 128 ? 2 * cus : hd == 64 ? (f32 ? 2 : 4) * cus : f32 ? cus / 2 : 4 * cus;
+}
+
 }  // namespace
 
-AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus) {
+AttnPlan plan_attention(int tokens, int seqs, int64_t cap, int kv_heads, int group, int hd, bool f32, int cus,
+                        int64_t few_tiles) {
     AttnPlan p;
     const int heads = kv_heads * group;
     // The few-rows form up to 128 rows a sequence and kv head on average, or where there are so few that
-    // the large tiles leave CUs idle: tiles of 32 rows over all heads up to 4 a CU (64 and 256 dims, fp16),
-    // 2 (128 dims; 64, fp32) or a half (256, fp32, whose large tiles have 128 rows). Over 222
-    // batches of 1 to 16 sequences, 64 to 1024 new tokens and 0 to 6,000 cached ones the choice takes 0.5 to
-    // 4.5 % more than the better form; at 256 dims of fp16 11 % over 131 batches. Few against many, 32/8 heads of 128,
-    // fp16, us: 32 sequences of 128 rows over 6,000 positions 238 / 341, of 256 398 / 350; one of 1024 rows over 1,000
-    // 23 / 27; four of 2048 over 6,000 350 / 221. One form takes the whole batch: 100 decoding requests over 2,000 beside
-    // 2048 tokens over 6,000 take 494 (few), as two batches 157 + 255; 32 beside them 298 (many), 53 + 255.
+    // the large tiles leave CUs idle. One form takes the whole batch: 100 decoding requests over 2,000 beside
+    // 2048 tokens over 6,000 take 494 us (few, fp16 pages, 32/8 heads of 128), as two batches 157 + 255; 32 beside them 298
+    // (many), 53 + 255.
     p.tiles = (int64_t)tokens * group / 32 + seqs;
-    const int64_t few_tiles = hd == 128 ? 2 * cus : hd == 64 ? (f32 ? 2 : 4) * cus : f32 ? cus / 2 : 4 * cus;
     p.few = (int64_t)tokens * group <= (int64_t)128 * seqs || (int64_t)tokens * heads / 32 <= few_tiles;
     p.items = p.few && seqs > kItemSeqs;
     if (p.few) {
@@ -439,7 +445,8 @@ size_t paged_attention_workspace(const PagedBatch& b, const PagedCache& c, int q
     const int64_t cap = (int64_t)b.max_blocks << c.block_shift;
     size_t most = 0;
     for (const bool f32 : {false, true}) {  // (one workspace serves both types)
-        const AttnPlan p = plan_attention(b.tokens, b.seqs, cap, c.kv_heads, group, c.head_dim, f32, cus);
+        const AttnPlan p = plan_attention(b.tokens, b.seqs, cap, c.kv_heads, group, c.head_dim, f32, cus,
+                                          few_tiles(c.head_dim, f32, cus));
         const size_t bytes = attention_workspace_bytes(p, b.tokens, b.seqs, group, c.head_dim);
         most = bytes > most ? bytes : most;
     }
@@ -484,7 +491,7 @@ hipError_t launch_paged_attention(const PagedBatch& b, const PagedCache& c, cons
                                   int q_heads, float scale, int window, void* workspace, void* out, int64_t ldo, int cus,
                                   hipStream_t stream) {
     const AttnPlan p = plan_attention(b.tokens, b.seqs, (int64_t)b.max_blocks << c.block_shift, c.kv_heads,
-                                      q_heads / c.kv_heads, c.head_dim, f32, cus);
+                                      q_heads / c.kv_heads, c.head_dim, f32, cus, few_tiles(c.head_dim, f32, cus));
     AttnArgs a;
     const hipError_t e = attention_args(p, b, c, q, ldq, q_heads, scale, window, workspace, out, ldo, stream, &a);
     if (e != hipSuccess) return e;
