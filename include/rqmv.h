@@ -419,7 +419,8 @@ typedef struct {
  * ties to even. Keys are computed in 64 bits, so that their codes are those of the exact keys whatever the step
  * they came in. A row is within 2^e of what was stored, however often the group grows (within half of that where
  * it does not). A NaN, an infinity or a magnitude of 65,280 or more makes the group's
- * scale NaN, until the group starts anew. One launch. */
+ * scale NaN, until the group starts anew. (A group whose first row is never stored keeps the scale
+ * that its byte has: set that to 0 where it holds nothing.) One launch. */
 int rqmv_qk_norm_rope_q8(const rqmv_paged_batch* batch, const rqmv_paged_cache_q8* cache, const void* qkv, int x_dtype,
                          int64_t ld, int q_heads, const float* q_norm, const float* k_norm, float eps,
                          const float* rope_table, int rot_dim, int rope_rows, void* q_out, int q_dtype, int64_t ldq,

@@ -744,9 +744,17 @@ class PagedCacheQ8(_Described):
 
     @classmethod
     def allocate(cls, blocks: int, block_size: int, kv_heads: int, head_dim: int) -> "PagedCacheQ8":
-        codes, scales = blocks * block_size * kv_heads * head_dim, blocks * block_size * kv_heads // 16
-        return cls(DeviceBuffer(codes), DeviceBuffer(codes), DeviceBuffer(scales), DeviceBuffer(scales), blocks,
-                   block_size, kv_heads, head_dim)
+        """Pages whose groups hold nothing yet (scale bytes 0, the smallest scale)."""
+        codes, none = blocks * block_size * kv_heads * head_dim, np.zeros(blocks * block_size * kv_heads // 16, np.uint8)
+        return cls(DeviceBuffer(codes), DeviceBuffer(codes), DeviceBuffer.from_array(none), DeviceBuffer.from_array(none),
+                   blocks, block_size, kv_heads, head_dim)
+
+
+def _pages(cache, q8: bool):
+    """The reference that a call over 8-bit (or fp16) pages passes; the other kind's memory would be read past its end."""
+    if isinstance(cache, PagedCacheQ8) != q8:
+        raise TypeError(f"pages of {8 if q8 else 16} bits are needed, not {type(cache).__name__}")
+    return cache.ref
 
 
 class PagedBatch(_Described):
@@ -787,7 +795,7 @@ def qk_norm_rope(batch: PagedBatch, cache: PagedCache, qkv, x_dtype: int, ld: in
                  rot_dim: int | None = None, stream: Stream | None = None):
     """Per-head norms and rotation of queries and keys, the append to the paged
     cache (rqmv_qk_norm_rope); rot_dim defaults to the whole head."""
-    _check(lib().lib.rqmv_qk_norm_rope(batch.ref, cache.ref, qkv.ptr, x_dtype, ld, q_heads,
+    _check(lib().lib.rqmv_qk_norm_rope(batch.ref, _pages(cache, False), qkv.ptr, x_dtype, ld, q_heads,
                                        _p(q_norm), _p(k_norm), eps, table.ptr,
                                        cache.head_dim if rot_dim is None else rot_dim, rope_rows, q_out.ptr, q_dtype,
                                        ldq, _sh(stream)), "rqmv_qk_norm_rope")
@@ -795,7 +803,7 @@ def qk_norm_rope(batch: PagedBatch, cache: PagedCache, qkv, x_dtype: int, ld: in
 
 def paged_attention_workspace_size(batch: PagedBatch, cache: PagedCache, q_heads: int) -> int:
     n = c_size_t()
-    _check(lib().lib.rqmv_paged_attention_workspace_size(batch.ref, cache.ref, q_heads, byref(n)),
+    _check(lib().lib.rqmv_paged_attention_workspace_size(batch.ref, _pages(cache, False), q_heads, byref(n)),
            "rqmv_paged_attention_workspace_size")
     return n.value
 
@@ -808,7 +816,7 @@ def paged_attention(batch: PagedBatch, cache: PagedCache, q, dtype: int, ldq: in
                     workspace=None, scale: float | None = None, window: int = 0, stream: Stream | None = None):
     """The new tokens' attention over their pages (rqmv_paged_attention); scale
     defaults to 1 / sqrt(head_dim)."""
-    _check(lib().lib.rqmv_paged_attention(batch.ref, cache.ref, q.ptr, dtype, ldq, q_heads,
+    _check(lib().lib.rqmv_paged_attention(batch.ref, _pages(cache, False), q.ptr, dtype, ldq, q_heads,
                                           cache.head_dim ** -0.5 if scale is None else scale, window, _p(workspace),
                                           workspace.nbytes if workspace is not None else 0, out.ptr, ldo, _sh(stream)),
            "rqmv_paged_attention")
@@ -818,19 +826,19 @@ def qk_norm_rope_q8(batch: PagedBatch, cache: PagedCacheQ8, qkv, x_dtype: int, l
                     rope_rows: int, q_out, q_dtype: int, ldq: int, q_norm=None, k_norm=None, eps: float = 1e-6,
                     rot_dim: int | None = None, stream: Stream | None = None):
     """qk_norm_rope with pages of 8 bits (rqmv_qk_norm_rope_q8): the rows of one group of 16 slots stand within 32 rows."""
-    _check(lib().lib.rqmv_qk_norm_rope_q8(batch.ref, cache.ref, qkv.ptr, x_dtype, ld, q_heads, _p(q_norm), _p(k_norm),
+    _check(lib().lib.rqmv_qk_norm_rope_q8(batch.ref, _pages(cache, True), qkv.ptr, x_dtype, ld, q_heads, _p(q_norm), _p(k_norm),
                                           eps, table.ptr, cache.head_dim if rot_dim is None else rot_dim, rope_rows,
                                           q_out.ptr, q_dtype, ldq, _sh(stream)), "rqmv_qk_norm_rope_q8")
 
 
 def paged_values_q8(cache: PagedCacheQ8, out: PagedCache, stream: Stream | None = None):
     """The values of 8-bit pages into fp16 pages of the same shape (rqmv_paged_values_q8)."""
-    _check(lib().lib.rqmv_paged_values_q8(cache.ref, out.ref, _sh(stream)), "rqmv_paged_values_q8")
+    _check(lib().lib.rqmv_paged_values_q8(_pages(cache, True), _pages(out, False), _sh(stream)), "rqmv_paged_values_q8")
 
 
 def paged_attention_q8_workspace_size(batch: PagedBatch, cache: PagedCacheQ8, q_heads: int) -> int:
     n = c_size_t()
-    _check(lib().lib.rqmv_paged_attention_q8_workspace_size(batch.ref, cache.ref, q_heads, byref(n)),
+    _check(lib().lib.rqmv_paged_attention_q8_workspace_size(batch.ref, _pages(cache, True), q_heads, byref(n)),
            "rqmv_paged_attention_q8_workspace_size")
     return n.value
 
@@ -842,7 +850,7 @@ def paged_attention_q8_workspace(batch: PagedBatch, cache: PagedCacheQ8, q_heads
 def paged_attention_q8(batch: PagedBatch, cache: PagedCacheQ8, q, dtype: int, ldq: int, q_heads: int, out, ldo: int,
                        workspace=None, scale: float | None = None, window: int = 0, stream: Stream | None = None):
     """paged_attention over pages of 8 bits (rqmv_paged_attention_q8)."""
-    _check(lib().lib.rqmv_paged_attention_q8(batch.ref, cache.ref, q.ptr, dtype, ldq, q_heads,
+    _check(lib().lib.rqmv_paged_attention_q8(batch.ref, _pages(cache, True), q.ptr, dtype, ldq, q_heads,
                                              cache.head_dim ** -0.5 if scale is None else scale, window, _p(workspace),
                                              workspace.nbytes if workspace is not None else 0, out.ptr, ldo,
                                              _sh(stream)), "rqmv_paged_attention_q8")

@@ -111,3 +111,19 @@ def test_assigned_buffers_are_what_calls_pass():
     refused(qk, c=c)
     c.k_scale = A
     assert c.struct.k_scale == A.ptr
+
+
+def test_each_kind_of_pages_has_its_calls():
+    """Codes read as fp16 would end past their memory, and fp16 pages have no scales."""
+    from tests.test_paged_refusals import attend as attend16, cache as cache16, qk as qk16
+
+    for call, c in ((qk, cache16()), (attend, cache16()), (qk16, cache()), (attend16, cache())):
+        with pytest.raises(TypeError, match="pages of"):
+            call(c=c)
+    for args in ((cache16(), cache16()), (cache(), cache())):
+        with pytest.raises(TypeError, match="pages of"):
+            rqmv.paged_values_q8(*args)
+    with pytest.raises(TypeError):
+        rqmv.paged_attention_workspace_size(batch(), cache(), 4)
+    with pytest.raises(TypeError):
+        rqmv.paged_attention_q8_workspace_size(batch(), cache16(), 4)
