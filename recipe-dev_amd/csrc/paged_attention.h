@@ -671,8 +671,8 @@ __device__ __forceinline__ bool find_item(const AttnArgs& a, int number, Item* i
             seq_size<TM>(a, of, &tiles, &first, &keys);
         }
         if (t == 0) found.seq = -1;
-        const int64_t own_total = sum_wave((int64_t)tiles * ((keys + 63) >> 6));
-        if (lane == 0) totals[wave] = own_total;
+        const unsigned long long upto_total = wave_scan((unsigned long long)tiles * (unsigned)((keys + 63) >> 6));
+        if (lane == 63) totals[wave] = (int64_t)upto_total;
         __syncthreads();
         const int items = seq_items<TM>(a, totals[0] + totals[1] + totals[2] + totals[3], tiles, keys, &chunk, &live);
         if constexpr (LONG_FIRST) {
