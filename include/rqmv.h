@@ -487,8 +487,8 @@ int rqmv_sample(const float* logits, int rows, int n, int64_t ld, const float* u
  * -infinity for its log probabilities, and so have the last places of one with fewer
  * than `top`. Logits of +infinity share the row evenly (finite ones stand behind them
  * with -infinity). Sums are fp32 about the largest
- * logit. n is at most 2^20, rows at most 2^20. One launch up to 4,096
- * logits, two above. The workspace is 16-byte aligned
+ * logit. n is at most 2^20, rows at most 2^20. One launch up to 4,096 logits (8,192 without
+ * alternatives), two above. The workspace is 16-byte aligned
  * (rqmv_logprobs_workspace_size bytes on the current device; 0: may be NULL); calls sharing it must not
  * overlap. No counterpart in the reference. */
 int rqmv_logprobs_workspace_size(int rows, int n, int top, size_t* bytes);

@@ -6,7 +6,7 @@
 // Rows are read once, 256 R logits a wave, kept in its registers: (m, s, t) about its own largest
 // logit, and a list of at least its `top` largest ones. s and t move to another reference m' by
 //     s' = e^(m - m') s,   t' = e^(m - m') (t + (m - m') s).
-// A row of up to 1024 R logits is finished by its workgroup; otherwise waves leave both in the workspace, on their
+// A short row is finished by its workgroup; otherwise waves leave both in the workspace, on their
 // own, and a second launch joins a row's.
 //
 // The largest of a wave's logits: if `top` of its lanes have their own largest at or above T, what lies below T is
@@ -16,7 +16,8 @@
 // to the first. At the end a workgroup takes the largest of its waves' T, and ranks
 // what remains by comparing each with all (the lowest index first among equals).
 //
-// Bound: HBM, at few rows the two launches and their dependent loads.
+// Bound: HBM (1500 rows of 128,256 121 us, 6.4 TB/s read; with twenty alternatives 184); at few rows the two
+// launches and the ranking's chain through LDS (17 rows, twenty alternatives: 16.7 us, of them 5.9 and 10.8).
 #include "logprobs.h"
 
 #include <limits.h>
@@ -287,7 +288,7 @@ __device__ __forceinline__ float load_logits(const LogprobArgs& a, int64_t row, 
     return most;
 }
 
-// Rows of at most 1024 R logits.
+// Rows of at most 1024 R logits: one launch, no workspace. Bound: the chain of the load and the joins.
 template <int R, bool TOP>
 __global__ void __launch_bounds__(kThreads) logprobs_row_kernel(LogprobArgs a) {
     __shared__ Shared sh;
@@ -332,8 +333,11 @@ __global__ void __launch_bounds__(kThreads) logprobs_slice_kernel(LogprobArgs a,
     }
 }
 
-// The waves of a row, at most SLOTS (64, 128 or 256) of them. A thread has every (256 / SLOTS)-th place of one wave's
-// list; the first half of the places is asked for before it is known which are taken.
+// The waves of a row, more than SLOTS / 2 and at most SLOTS of them (8 to 256). A thread has every (256 / SLOTS)-th place
+// of one wave's list; the first half of the places is asked for before it is known which are taken. So a workgroup's
+// wave has at least 32 lanes with entries (where lists hold `top`), and its T leaves few. (With a lane for each of 16 slices
+// T was 0, and all went through the exact bisection: 17 rows of 16,000 with twenty alternatives 27.7 us, so 12.6; 1500
+// of 32,000 98, so 58.)
 template <int SLOTS>
 __global__ void __launch_bounds__(kThreads) logprobs_join_kernel(LogprobArgs a, Parts parts) {
     constexpr int SIDE = kThreads / SLOTS, N = kList / SIDE;
@@ -389,26 +393,25 @@ struct LogprobPlan {
     Parts parts;
 };
 LogprobPlan plan_logprobs(int rows, int n, int top, int cus) {
-    // Long slices where these are enough for two workgroups a CU: 4096 logits a wave, with lists 2048 (1500 rows of
-    // 128,256, twenty alternatives: 202 us, of 4096 246, of 1024 205); else 1024. A row is 256 waves' at most.
+    // Without alternatives: rows of up to 8192 logits at once (17 rows of 8,000 4.6 us, by slices 6.4; 1500 12.3 and 14.3;
+    // of 16,000 it would be 6.9 and 7.8, but 26.7 and 20.5), else 1024 logits a wave (100 rows of 128,256 13.5, of 4096
+    // 15.6; 1500 121 and 119; 1500 of 32,000 34.3 and 38.9). With them: rows of up to 4096 at once (of 8,000, 17 rows, 32
+    // alternatives, by slices 14.7, at once 21.4; 1500 rows, twenty 25.5 and 29.4); 1024 logits a wave, but 2048 where
+    // these are enough for two workgroups a CU (twenty alternatives, 100 and 1500 rows of 128,256 25.5 and 184, of 1024
+    // 27.1 and 205; 400 and 1500 of 32,000 26.1 and 58.2, 25.5 and 57.8). A row is 256 waves' at most.
     const bool many = (int64_t)((n + 16383) / 16384) * rows >= 2 * cus;
-    int r = !many ? 4 : top ? 8 : 16;
-    while (n > 256 * r * kThreads) r *= 2;
     LogprobPlan p;
-    p.r = r;
-    p.whole = n <= 1024 * r;
-    p.parts.slices = (n + 256 * r - 1) / (256 * r);
+    p.whole = n <= (top ? 4096 : 8192);
+    p.r = p.whole ? (n <= 4096 ? 4 : 8) : top && many && n > 8192 ? 8 : 4;
+    while (n > 256 * p.r * kThreads) p.r *= 2;
+    p.parts.slices = (n + 256 * p.r - 1) / (256 * p.r);
     return p;
 }
 
 template <int R, bool TOP>
 void launch_slices(const LogprobArgs& a, const LogprobPlan& p, hipStream_t stream) {
-    if (p.whole) {
-        hipLaunchKernelGGL((logprobs_row_kernel<R, TOP>), dim3(a.rows), dim3(kThreads), 0, stream, a);
-    } else {
-        const dim3 grid((p.parts.slices + kWaves - 1) / kWaves, a.rows < 65535 ? a.rows : 65535);
-        hipLaunchKernelGGL((logprobs_slice_kernel<R, TOP>), grid, dim3(kThreads), 0, stream, a, p.parts);
-    }
+    const dim3 grid((p.parts.slices + kWaves - 1) / kWaves, a.rows < 65535 ? a.rows : 65535);
+    hipLaunchKernelGGL((logprobs_slice_kernel<R, TOP>), grid, dim3(kThreads), 0, stream, a, p.parts);
 }
 
 }  // namespace
@@ -422,6 +425,14 @@ hipError_t launch_logprobs(const LogprobArgs& a, void* workspace, int cus, hipSt
     LogprobPlan p = plan_logprobs(a.rows, a.n, a.top, cus);
     p.parts.stats = static_cast<float4*>(workspace);
     p.parts.lists = reinterpret_cast<Entry*>(p.parts.stats + (int64_t)a.rows * p.parts.slices);
+    const dim3 rows(a.rows), threads(kThreads);
+    if (p.whole) {
+        const auto row = a.top      ? logprobs_row_kernel<4, true>
+                         : p.r == 4 ? logprobs_row_kernel<4, false>
+                                    : logprobs_row_kernel<8, false>;
+        hipLaunchKernelGGL(row, rows, threads, 0, stream, a);
+        return hipGetLastError();
+    }
     if (a.top) {
         if (p.r == 4) launch_slices<4, true>(a, p, stream);
         else if (p.r == 8) launch_slices<8, true>(a, p, stream);
@@ -432,11 +443,14 @@ hipError_t launch_logprobs(const LogprobArgs& a, void* workspace, int cus, hipSt
         else launch_slices<16, false>(a, p, stream);
     }
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.whole) return e;
-    const dim3 rows(a.rows), threads(kThreads);
-    if (p.parts.slices <= 64) hipLaunchKernelGGL(logprobs_join_kernel<64>, rows, threads, 0, stream, a, p.parts);
-    else if (p.parts.slices <= 128) hipLaunchKernelGGL(logprobs_join_kernel<128>, rows, threads, 0, stream, a, p.parts);
-    else hipLaunchKernelGGL(logprobs_join_kernel<256>, rows, threads, 0, stream, a, p.parts);
+    if (e != hipSuccess) return e;
+    const auto join = p.parts.slices <= 8     ? logprobs_join_kernel<8>
+                      : p.parts.slices <= 16  ? logprobs_join_kernel<16>
+                      : p.parts.slices <= 32  ? logprobs_join_kernel<32>
+                      : p.parts.slices <= 64  ? logprobs_join_kernel<64>
+                      : p.parts.slices <= 128 ? logprobs_join_kernel<128>
+                                              : logprobs_join_kernel<256>;
+    hipLaunchKernelGGL(join, rows, threads, 0, stream, a, p.parts);
     return hipGetLastError();
 }
 

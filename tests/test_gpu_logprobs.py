@@ -189,6 +189,26 @@ def test_replayed_from_a_graph(gpu, rows, n, top):
     graph.close()
 
 
+@pytest.mark.parametrize("slices", [5, 8, 9, 16, 17, 32, 33, 64, 65, 128, 129, 256])
+@pytest.mark.parametrize("top", [1, 31, 32])
+def test_joins_of_any_number_of_slices(gpu, slices, top):
+    """Slices of 1024 logits, the last of one, a few or all; the likeliest tokens all in one slice, or far apart."""
+    rng = np.random.default_rng(slices)
+    for n in (1024 * slices - 1023, 1024 * slices - 1000, 1024 * slices):
+        x = rng.standard_normal((3, n)).astype(np.float32)
+        x[1, -40 if n % 1024 == 0 else 2048 - 40:][:40] += 10
+        x[2, ::max(n // 20, 1)] = 7  # (equal ones)
+        check(gpu, x, rng.integers(0, n, 3), top)
+
+
+@pytest.mark.parametrize("rows,n", [(4, 8191), (4, 8192), (4, 8193), (520, 8192), (520, 8193), (600, 16000), (300, 32000)])
+@pytest.mark.parametrize("top", [0, 32])
+def test_rows_next_to_the_borders_of_the_forms(gpu, rows, n, top):
+    rng = np.random.default_rng(n)
+    x = rng.standard_normal((rows, n)).astype(np.float32) * 3
+    check(gpu, x, rng.integers(0, n, rows), top)
+
+
 def test_the_largest_row(gpu):
     rng = np.random.default_rng(6)
     x = rng.standard_normal((1, 1 << 20)).astype(np.float32)
