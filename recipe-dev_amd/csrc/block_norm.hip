@@ -6,8 +6,8 @@
 //     out = u / sqrt(mean(u^2) + eps) * pre            (the norm before the next)
 // A row lies in the registers of T threads (V float4 each), so that it is read
 // and written once, whatever of the three a call asks for; its two sums of squares are two joins
-// over the T threads. Bound: HBM at prefill; at a few rows the chain of loads, two joins and
-// stores, for which T is 1024.
+// over the T threads. Bound: HBM at prefill (4096 rows of 4,096 with one gate, fp16 out: 41.2 us, 5.7 TB/s); at a few rows the
+// chain of loads, two joins and stores, for which T is 1024 (5 rows of 5,120: 5.6 us, 4.5 in a trace).
 #include "block_norm.h"
 
 #include <hip/hip_fp16.h>
@@ -132,10 +132,14 @@ void launch(const BlockNorm& p, bool out_f16, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_block_norm(const BlockNorm& p, bool out_f16, int cus, hipStream_t stream) {
+    // 1024 threads a row while all rows are resident at once, two a CU (500 rows of 4,096 6.3 us, of 256 threads 7.7; of
+    // 8,192 10.0 and 12.4); past that 256, whose rows end and begin at different times (750 rows of 4,096 8.8 us, of 1024
+    // threads 9.6; 4096 rows 40.7 and 45.6), from 4,097 values on, where these have fewer rows a CU, for more than
+    // four (1100 of 5,120 13.8 and 16.0; 1000 of 8,192 equal).
     const int n4 = p.n / 4;
     if (n4 <= 64) launch<64, 1>(p, out_f16, stream);
     else if (n4 <= 256) launch<64, 4>(p, out_f16, stream);
-    else if (p.rows > 4 * cus && n4 <= 1024) launch<256, 4>(p, out_f16, stream);
+    else if (p.rows > 2 * cus && n4 <= 1024) launch<256, 4>(p, out_f16, stream);
     else if (p.rows > 4 * cus && n4 <= 2048) launch<256, 8>(p, out_f16, stream);
     else if (n4 <= 1024) launch<1024, 1>(p, out_f16, stream);
     else if (n4 <= 2048) launch<1024, 2>(p, out_f16, stream);

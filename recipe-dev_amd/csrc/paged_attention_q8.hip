@@ -71,7 +71,11 @@ struct Q8Values {
 // and the queries' operands hold theirs in that order). The values go straight to LDS as codes, two
 // buffers a wave, and are read transposed (ds_read_b64_tr_b8); the next step's keys and values are asked for
 // once the scores are done. Codes lie in LDS as rows of HD bytes, 16-byte pieces XORed so that a read of
-// two pieces of sixteen rows hits every bank alike.
+// two pieces of sixteen rows hits every bank alike. (Keys through LDS, as over fp16 pages, 101.9 us for the first size
+// below, so 86.4; then a tile's last item behind all longer ones 77.5.)
+// Bound: HBM (32/8 heads of 128, fp16, with the join: 48 requests of 100 to 12,000 positions 77 us, 4.4 TB/s, over fp16
+// pages 142; 200 of 1,000 to 3,000 148, 5.1 TB/s); for one sequence the chain lengths -> table -> keys and the
+// join (one token over 8,000, fp32: 12.8 us, of which 10.8 and 3.8 in a trace).
 template <int HD>
 __device__ constexpr int code_xor(int row) {
     return HD == 64 ? ((row >> 2) & 1) << 1 : HD == 128 ? ((row >> 1) & 3) << 1 : (row & 7) << 1;
@@ -251,7 +255,9 @@ __global__ void __launch_bounds__(256, q8_few_wgs(HD, F32)) paged_q8_few(AttnArg
 // --------------------------------------------- many rows: rows over the waves ----
 
 // The waves share steps of 64 keys in two LDS buffers, one barrier a step. Codes go from the pages into registers, 16
-// keys of one page at a time (one scale), and from there, a step later, to LDS as fp16.
+// keys of one page at a time (one scale), and from there, a step later, to LDS as fp16. Bound: matrix cores and VALU in
+// turn (2000 tokens over 12,000, 32/8 heads of 128, fp16: 456 us, 935 TFLOP/s; over fp16 pages 432, as there is no
+// conversion).
 template <int HD, bool F32>
 __global__ void __launch_bounds__(64 * many_waves(HD), many_waves(HD) / 4) paged_q8_many(AttnArgs a, PagedCodes codes) {
     typedef Lay<HD> L;

@@ -23,11 +23,11 @@ namespace rq {
 // window of rows that a workgroup has; workgroups of runs come before those of queries (mixed, they
 // wait for each other's loads: 85 us).
 //
-// Bound: at prefill HBM (4000 rows of 32/8 heads of 128, fp32 to fp16: 28.3 us, 4.9 TB/s; the form over fp16 pages
-// 30.7 for 4096), at decode the chain of loads slots -> rows -> codes (24 requests: 4.3 us).
+// Bound: at prefill HBM (4000 rows of 32/8 heads of 128, fp32 to fp16: 27.5 us in a trace; the form over fp16 pages
+// 30.7 for 4096), at decode the chain of loads slots -> rows -> codes (24 requests: 4.4 us in a trace).
 constexpr int kWaves = 4;
 
-// Queries and the values of pages pass by the caches (4000 rows, 32/8 heads of 128, with the values: 38.2 us, so 33.3).
+// Queries and the values of pages pass by the caches (4000 rows, 32/8 heads of 128, with the values: 38.2 us, so 35.1).
 typedef uint32_t nt2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t nt4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void stream4(float* p, const float* v) {
@@ -274,7 +274,7 @@ hipError_t launch_qk_norm_rope_q8(const PagedBatch& b, const PagedCache& c, cons
 
 // ------------------------------------------------------------- the values ----
 
-// Sixteen codes a thread; keys and values by blockIdx.y. Bound: HBM.
+// Sixteen codes a thread; keys and values by blockIdx.y. Bound: HBM (the pages behind the step of 4000 rows: 8.7 us in a trace).
 __global__ void __launch_bounds__(256) values_q8_kernel(PagedCodes codes, __half* k, __half* v, int64_t pieces,
                                                         int row_shift) {
     const int8_t* from = blockIdx.y ? codes.v : codes.k;
