@@ -486,11 +486,11 @@ int rqmv_sample(const float* logits, int rows, int n, int64_t ld, const float* u
  * no candidates (probability 0); a row without any has entropy 0, -1 for its top tokens and
  * -infinity for its log probabilities, and so have the last places of one with fewer
  * than `top`. Logits of +infinity share the row evenly (finite ones stand behind them
- * with -infinity). Sums are fp32 about the largest
- * logit. n is at most 2^20, rows at most 2^20. One launch up to 4,096 logits (8,192 without
- * alternatives), two above. The workspace is 16-byte aligned
- * (rqmv_logprobs_workspace_size bytes on the current device; 0: may be NULL); calls sharing it must not
- * overlap. No counterpart in the reference. */
+ * with -infinity). Sums are fp32 about the largest logit, whose own term stays apart: log
+ * probabilities next to 0 and small entropies keep their digits. n is at most 2^20, rows at most
+ * 2^20. One launch up to 4,096 logits (8,192 without alternatives), two above. The workspace is
+ * 16-byte aligned (rqmv_logprobs_workspace_size bytes on the current device; 0: may be NULL);
+ * calls sharing it must not overlap. No counterpart in the reference. */
 int rqmv_logprobs_workspace_size(int rows, int n, int top, size_t* bytes);
 int rqmv_logprobs(const float* logits, int rows, int n, int64_t ld, const int* tokens, float* logprob, float* entropy,
                   int top, int* top_tokens, float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);

@@ -1,11 +1,15 @@
 // Log probabilities of given tokens, entropies and the likeliest tokens of rows
 // of logits (rqmv_logprobs).
 //
-// With m the largest logit of a row, s = sum e^(x - m) and t = sum (x - m) e^(x - m):
-//     log p(i) = x_i - m - log s,      entropy = log s - t / s.
+// With m the largest logit of a row, 1 + s = sum e^(x - m) and t = sum (x - m) e^(x - m):
+//     log p(i) = x_i - m - log(1 + s),      entropy = log(1 + s) - t / (1 + s).
+// The 1 is the term of one largest logit. It stays out of the sum: a token of probability 1 - 10^-8 has log probability
+// -10^-8, which a sum of 1 + 10^-8 in fp32 does not hold. (With it in the sum 1500 rows of 128,256 take as long, with twenty
+// alternatives 184 us instead of 186, of 32,000 58 instead of 61.)
 // Rows are read once, 256 R logits a wave, kept in its registers: (m, s, t) about its own largest
-// logit, and a list of at least its `top` largest ones. s and t move to another reference m' by
-//     s' = e^(m - m') s,   t' = e^(m - m') (t + (m - m') s).
+// logit, and a list of at least its `top` largest ones. Of parts (m, s, t) the first with the largest m keeps its s, others
+// with that m add 1 + s and t, and the rest move to the reference m' = that m:
+//     e^(m - m') (1 + s),   e^(m - m') (t + (m - m') (1 + s)).
 // A short row is finished by its workgroup; otherwise waves leave both in the workspace, on their
 // own, and a second launch joins a row's.
 //
@@ -16,7 +20,7 @@
 // to the first. At the end a workgroup takes the largest of its waves' T, and ranks
 // what remains by comparing each with all (the lowest index first among equals).
 //
-// Bound: HBM (1500 rows of 128,256 121 us, 6.4 TB/s read; with twenty alternatives 184); at few rows the two
+// Bound: HBM (1500 rows of 128,256 121 us, 6.4 TB/s read; with twenty alternatives 186); at few rows the two
 // launches and the ranking's chain through LDS (17 rows, twenty alternatives: 16.7 us, of them 5.9 and 10.8).
 #include "logprobs.h"
 
@@ -34,21 +38,18 @@ constexpr int kSegment = 8;  // entries compared at once
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Stats {
-    float m, s, t;
+    float m, s, t;  // (no candidate: -infinity, 0, 0)
 };
 struct Entry {
     float v;
     int i;
 };
 
-// e^(from - to) for to >= from, or to = -infinity (then 0).
-__device__ __forceinline__ float moved(float from, float to) {
-    return from == to ? (to == -INFINITY ? 0.f : 1.f) : __builtin_amdgcn_exp2f((from - to) * kLog2e);
-}
-// `a` about the reference `to`.
-__device__ __forceinline__ Stats move(Stats a, float to) {
-    const float f = moved(a.m, to);
-    return Stats{to, f * a.s, f > 0.f && a.m != to ? f * fmaf(a.m - to, a.s, a.t) : f > 0.f ? a.t : 0.f};
+// What `a` adds to the sums about `to` >= a.m; `first`: the 1 of these is its own.
+__device__ __forceinline__ Stats move(Stats a, float to, bool first) {
+    if (a.m == to) return Stats{to, first || to == -INFINITY ? a.s : 1.f + a.s, a.t};
+    const float f = __builtin_amdgcn_exp2f((a.m - to) * kLog2e), s = 1.f + a.s;
+    return f > 0.f ? Stats{to, f * s, f * fmaf(a.m - to, s, a.t)} : Stats{to, 0.f, 0.f};
 }
 
 // Floats to numbers in their order and back. (No NaNs and no -0.)
@@ -61,21 +62,35 @@ __device__ __forceinline__ float of_key(uint32_t k) {
 }
 constexpr uint32_t kLowest = 0x00800000u;  // key_of(-FLT_MAX): what is below is no candidate
 
+// log(1 + s), s >= 0, to within two roundings: the logarithm of the rounded 1 + s and, to first order, of what its
+// rounding left out.
+__device__ __forceinline__ float log_of_one_and(float s) {
+    const float u = 1.f + s;
+    return logf(u) + (s - (u - 1.f)) * __builtin_amdgcn_rcpf(u);
+}
+
 // What a wave's registers hold.
 template <int N>
 __device__ __forceinline__ Stats wave_stats(const float (&v)[N], float m) {
     Stats a{m, 0.f, 0.f};
+    float ones = 0.f;  // of the lane's terms
     if (m == INFINITY) {  // these alone count, all alike
 #pragma unroll
-        for (int i = 0; i < N; ++i) a.s += v[i] == INFINITY ? 1.f : 0.f;
+        for (int i = 0; i < N; ++i) ones += v[i] == INFINITY ? 1.f : 0.f;
     } else if (m > -INFINITY) {
+        // A lane adds up its terms below 1 by themselves; what all add up to says how many the others are.
+        float all = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float d = v[i] - m, e = __builtin_amdgcn_exp2f(d * kLog2e);
-            a.s += e;
+            all += e;
+            a.s += __builtin_amdgcn_fractf(e);
             a.t = fmaf(fmaxf(d, -1000.f), e, a.t);  // (-infinity times 0 would be NaN)
         }
+        ones = rintf(all - a.s);
     }
+    const unsigned long long has = __ballot(ones > 0.f);
+    a.s += ones - ((int)(threadIdx.x & 63) == (has ? __builtin_ctzll(has) : 64) ? 1.f : 0.f);
     a.s = all_sum(a.s);
     a.t = all_sum(a.t);
     return a;
@@ -217,9 +232,11 @@ __device__ __forceinline__ Stats group_stats(const Shared& sh) {
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) m = fmaxf(m, sh.stats[w].m);
     Stats a{m, 0.f, 0.f};
+    bool first = true;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-        const Stats b = move(sh.stats[w], m);
+        const Stats b = move(sh.stats[w], m, first);
+        first = first && sh.stats[w].m != m;
         a.s += b.s, a.t += b.t;
     }
     return a;
@@ -227,7 +244,7 @@ __device__ __forceinline__ Stats group_stats(const Shared& sh) {
 
 __device__ __forceinline__ float log_prob(float x, const Stats& a, float log_s) {
     if (!(x > -INFINITY) || a.m == -INFINITY) return -INFINITY;
-    return x == a.m ? -log_s : (x - a.m) - log_s;
+    return (x == a.m ? 0.f : x - a.m) - log_s;
 }
 
 // The logit of the row's token, asked for before it is needed (thread kGiven has it).
@@ -241,13 +258,13 @@ __device__ __forceinline__ float given_logit(const LogprobArgs& a, int64_t row) 
 // A row's outputs from its stats, sh.best and the token's logit.
 __device__ __forceinline__ void put_row(const LogprobArgs& a, int64_t row, const Stats& st, const Shared& sh, float given) {
     const int t = threadIdx.x;
-    const float log_s = st.m > -INFINITY ? logf(st.s) : 0.f;
+    const float log_s = st.m > -INFINITY ? log_of_one_and(st.s) : 0.f;
     if (t < a.top) {
         const Entry e = sh.best[t];
         if (a.top_tokens) a.top_tokens[row * a.top + t] = e.i;
         if (a.top_logprobs) a.top_logprobs[row * a.top + t] = log_prob(e.v, st, log_s);
     } else if (t == 64) {
-        if (a.entropy) a.entropy[row] = st.m > -INFINITY ? log_s - st.t / st.s : 0.f;
+        if (a.entropy) a.entropy[row] = st.m > -INFINITY ? log_s - st.t / (1.f + st.s) : 0.f;
     } else if (t == kGiven) {
         if (a.logprob) a.logprob[row] = log_prob(given, st, log_s);
     }
@@ -337,7 +354,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_slice_kernel(LogprobArgs a,
 // of one wave's list; the first half of the places is asked for before it is known which are taken. So a workgroup's
 // wave has at least 32 lanes with entries (where lists hold `top`), and its T leaves few. (With a lane for each of 16 slices
 // T was 0, and all went through the exact bisection: 17 rows of 16,000 with twenty alternatives 27.7 us, so 12.6; 1500
-// of 32,000 98, so 58.)
+// of 32,000 98, so 58, now 61.)
 template <int SLOTS>
 __global__ void __launch_bounds__(kThreads) logprobs_join_kernel(LogprobArgs a, Parts parts) {
     constexpr int SIDE = kThreads / SLOTS, N = kList / SIDE;
@@ -357,7 +374,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_join_kernel(LogprobArgs a, 
         const int listed = __builtin_bit_cast(int, p.w);
         Stats st = side == 0 ? Stats{p.x, p.y, p.z} : Stats{-INFINITY, 0.f, 0.f};
         const float m = all_max(st.m);
-        st = move(st, m);
+        st = move(st, m, lane == __builtin_ctzll(__ballot(st.m == m)));
         st.s = all_sum(st.s);
         st.t = all_sum(st.t);
         if (lane == 0) sh.stats[wave] = st;
