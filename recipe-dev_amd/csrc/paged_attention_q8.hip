@@ -366,7 +366,8 @@ hipError_t launch_hd(const AttnPlan& p, const AttnArgs& a, const PagedCodes& cod
 // Tiles of 32 rows over all heads up to which few rows are assumed: 4 a CU, of fp16 rows of 128 dims 2. Over 380 batches
 // of 1 to 32 sequences, 16 to 1024 new tokens and 0 to 6,000 cached ones, of seven combinations of heads and type, the
 // choice takes 2 to 5 % more than the better form on average (32/8 heads of 128, fp16, few against many, us: 32
-// sequences of 16 tokens over 6,000 115 / 148, of 64 370 / 390; 4 of 512 356 / 224).
+// sequences of 16 tokens over 6,000 115 / 148, of 64 370 / 390; 4 of 512 356 / 224). At 4 a CU the fewest rows that take
+// the form for many have tiles for more than half of the CUs, so it splits keys at fp16 rows of 128 dims alone.
 AttnPlan plan_q8(const PagedBatch& b, const PagedCache& c, int q_heads, bool f32, int cus) {
     return plan_attention(b.tokens, b.seqs, (int64_t)b.max_blocks << c.block_shift, c.kv_heads, q_heads / c.kv_heads,
                           c.head_dim, f32, cus, (c.head_dim == 128 && !f32 ? 2 : 4) * cus);
