@@ -20,8 +20,9 @@
 // to the first. At the end a workgroup takes the largest of its waves' T, and ranks
 // what remains by comparing each with all (the lowest index first among equals).
 //
-// Bound: HBM (1500 rows of 128,256 121 us, 6.4 TB/s read; with twenty alternatives 186); at few rows the two
-// launches and the ranking's chain through LDS (17 rows, twenty alternatives: 16.7 us, of them 5.9 and 10.8).
+// Bound: HBM, with the VALU as busy (1500 rows of 128,256 122 us, 6.3 TB/s read; with twenty alternatives 186); at few
+// rows the two launches and the ranking's chain through LDS (17 rows, twenty alternatives: 16.7 us, 6.5 and 10.6 in a
+// trace; 32 alternatives 26.5, 6.9 and 19.7).
 #include "logprobs.h"
 
 #include <limits.h>
@@ -353,8 +354,8 @@ __global__ void __launch_bounds__(kThreads) logprobs_slice_kernel(LogprobArgs a,
 // The waves of a row, more than SLOTS / 2 and at most SLOTS of them (8 to 256). A thread has every (256 / SLOTS)-th place
 // of one wave's list; the first half of the places is asked for before it is known which are taken. So a workgroup's
 // wave has at least 32 lanes with entries (where lists hold `top`), and its T leaves few. (With a lane for each of 16 slices
-// T was 0, and all went through the exact bisection: 17 rows of 16,000 with twenty alternatives 27.7 us, so 12.6; 1500
-// of 32,000 98, so 58, now 61.)
+// T was 0, and all went through the exact bisection: 17 rows of 16,000 with twenty alternatives 27.7 us, so 12.7; 1500
+// of 32,000 98, so 61.)
 template <int SLOTS>
 __global__ void __launch_bounds__(kThreads) logprobs_join_kernel(LogprobArgs a, Parts parts) {
     constexpr int SIDE = kThreads / SLOTS, N = kList / SIDE;
@@ -410,12 +411,12 @@ struct LogprobPlan {
     Parts parts;
 };
 LogprobPlan plan_logprobs(int rows, int n, int top, int cus) {
-    // Without alternatives: rows of up to 8192 logits at once (17 rows of 8,000 4.6 us, by slices 6.4; 1500 12.3 and 14.3;
-    // of 16,000 it would be 6.9 and 7.8, but 26.7 and 20.5), else 1024 logits a wave (100 rows of 128,256 13.5, of 4096
-    // 15.6; 1500 121 and 119; 1500 of 32,000 34.3 and 38.9). With them: rows of up to 4096 at once (of 8,000, 17 rows, 32
-    // alternatives, by slices 14.7, at once 21.4; 1500 rows, twenty 25.5 and 29.4); 1024 logits a wave, but 2048 where
-    // these are enough for two workgroups a CU (twenty alternatives, 100 and 1500 rows of 128,256 25.5 and 184, of 1024
-    // 27.1 and 205; 400 and 1500 of 32,000 26.1 and 58.2, 25.5 and 57.8). A row is 256 waves' at most.
+    // Without alternatives: rows of up to 8192 logits at once (17 rows of 8,000 4.8 us, by slices 8.0; 1500 12.5 and 14.5;
+    // of 16,000 it would be 6.9 and 7.7, but 26.8 and 20.7), else 1024 logits a wave (100 rows of 128,256 13.8, of 4096
+    // 16.3; 1500 122 and 122; 1500 of 32,000 34.6 and 39.7). With them: rows of up to 4096 at once (of 8,000, 17 rows, 32
+    // alternatives, by slices 14.7, at once 21.0; 1500 rows, twenty 25.8 and 29.4); 1024 logits a wave, but 2048 where
+    // these are enough for two workgroups a CU (twenty alternatives, 100 and 1500 rows of 128,256 25.7 and 186, of 1024
+    // 27.2 and 204; 400 and 1500 of 32,000 26.7 and 60.6, 25.8 and 58.5). A row is 256 waves' at most.
     const bool many = (int64_t)((n + 16383) / 16384) * rows >= 2 * cus;
     LogprobPlan p;
     p.whole = n <= (top ? 4096 : 8192);

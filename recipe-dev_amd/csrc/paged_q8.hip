@@ -16,18 +16,19 @@ namespace rq {
 // are c -> rint(c * 2^(e - e')) and the run's rint(y * 2^-e').
 //
 // A code is a whole number next to its borders, so keys are computed in 64 bits: a key's codes are those of the
-// exact key, whatever the step it came in. (With keys in fp32 the prefill step of 4000 rows took 4 us less of 48, before the
+// exact key, whatever the step it came in. (With keys in fp32 a prefill step of 3,480 rows took 4 us less of 48, before the
 // rest was made faster.)
 //
 // A run's sixteen rows are shared by four waves, which join their exponents through LDS. Runs are looked for among the
 // window of rows that a workgroup has; workgroups of runs come before those of queries (mixed, they
 // wait for each other's loads: 85 us).
 //
-// Bound: at prefill HBM (4000 rows of 32/8 heads of 128, fp32 to fp16: 27.5 us in a trace; the form over fp16 pages
-// 30.7 for 4096), at decode the chain of loads slots -> rows -> codes (24 requests: 4.4 us in a trace).
+// Bound: at prefill HBM (3,480 rows of 32/8 heads of 128, fp32 to fp16: 27.3 us in a trace, the form over fp16 pages
+// 25.5), at decode the chain of loads slots -> rows -> codes (24 requests: 4.3 us in a trace).
 constexpr int kWaves = 4;
 
-// Queries and the values of pages pass by the caches (4000 rows, 32/8 heads of 128, with the values: 38.2 us, so 35.1).
+// Queries and the values of pages pass by the caches (3,480 rows, 32/8 heads of 128, with the values: 38.2 us, so 35.1;
+// attention behind the append takes as long as after plain stores).
 typedef uint32_t nt2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t nt4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void stream4(float* p, const float* v) {
@@ -46,8 +47,10 @@ __device__ __forceinline__ void stream4(uint4* p, uint4 v) {
 
 constexpr int kRunRows = 32;  // rows that a run's rows lie within
 // Windows of 16 rows where a call has many (a prompt's 1000 rows of 32/8 heads of 128, with the values: 13.3 us, of 4 rows
-// 15.0; 4000 rows 38 and 45), of 4 for some, whose runs are short and would wait for each other (300 requests 18.7, of 16
-// rows 34.2), of one for few (24 requests 8.7, of 4 rows 10.4; but a prompt of 128 takes 10.7 so, of 4 rows 8.6).
+// 15.0; 3,480 rows 38 and 45), of 4 for some, whose runs are short and would wait for each other (300 requests 18.7, of 16
+// rows 34.2), of one for few (24 requests 8.7, of 4 rows 10.4; but a prompt of 128 takes 10.7 so, of 4 rows 8.6). The number of
+// rows alone decides, so more than 512 requests of one token go by windows of 16 too: 1000 take 28.6 us by themselves, a
+// prompt of 1000 rows 9.6, either over fp16 pages 9.3 and 8.3.
 constexpr int kFewRows = 64, kSomeRows = 512;
 
 // The slots around a window: of rows base - 31 .. base + 32 (`a`) and the sixteen after these (`b`); -1: none.
@@ -274,7 +277,7 @@ hipError_t launch_qk_norm_rope_q8(const PagedBatch& b, const PagedCache& c, cons
 
 // ------------------------------------------------------------- the values ----
 
-// Sixteen codes a thread; keys and values by blockIdx.y. Bound: HBM (the pages behind the step of 4000 rows: 8.7 us in a trace).
+// Sixteen codes a thread; keys and values by blockIdx.y. Bound: HBM (the pages behind the step of 3,480 rows: 8.6 us in a trace).
 __global__ void __launch_bounds__(256) values_q8_kernel(PagedCodes codes, __half* k, __half* v, int64_t pieces,
                                                         int row_shift) {
     const int8_t* from = blockIdx.y ? codes.v : codes.k;
